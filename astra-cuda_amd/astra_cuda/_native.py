@@ -46,6 +46,19 @@ PROTOTYPES = {
     "astra_high_low_trade_scratch": (_c_int, [_vp, _vp, _vp]),
     "astra_high_low_observation": (_c_int, [_vp, _vp]),
     "astra_high_low_rewards": (_c_int, [_vp, ctypes.c_int64, _c_i32, _c_i32, _vp, _vp]),
+    "astra_short_conv_forward": (_c_int, [_vp, _vp]),
+    "astra_short_conv_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
+    "astra_short_conv_backward": (_c_int, [_vp, _vp]),
+    "astra_short_conv_step": (_c_int, [_vp, _vp]),
+    "astra_state_scan_chunk_states": (_c_int, [_vp, ctypes.POINTER(_sz)]),
+    "astra_state_scan_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
+    "astra_state_scan_forward": (_c_int, [_vp, _vp]),
+    "astra_state_scan_grad_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
+    "astra_state_scan_backward": (_c_int, [_vp, _vp]),
+    "astra_state_scan_step": (_c_int, [_vp, _vp]),
+    "astra_join_norm_forward": (_c_int, [_vp, _vp]),
+    "astra_join_norm_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
+    "astra_join_norm_backward": (_c_int, [_vp, _vp]),
 }
 
 
@@ -70,6 +83,63 @@ class HLObservation(ctypes.Structure):
         "best_bid_sizes", "best_ask_sizes", "last_prices")] + [(n, _c_i32) for n in (
         "num_envs", "players", "steps_per_player", "player", "current_round")] + [
         (n, ctypes.c_float) for n in ("player_sin", "player_cos", "round_fraction")]
+
+
+def _fields(pointers: str, sizes: str, ints: str) -> list:
+    return [(n, _vp) for n in pointers.split()] + [(n, ctypes.c_int64) for n in sizes.split()] + [
+        (n, _c_i32) for n in ints.split()]
+
+
+class ShortConv(ctypes.Structure):
+    """astra_short_conv (include/astra_sequence.h)."""
+    _fields_ = _fields("x weight bias window lengths y last", "batch length x_stride_b x_stride_t",
+                       "width taps type activation")
+
+
+class ShortConvGrad(ctypes.Structure):
+    """astra_short_conv_grad (include/astra_sequence.h)."""
+    _fields_ = [("f", ShortConv)] + _fields("dy dlast dx dwindow dweight dbias workspace", "", "") + [
+        ("workspace_bytes", _sz)]
+
+
+class ShortConvOne(ctypes.Structure):
+    """astra_short_conv_one (include/astra_sequence.h)."""
+    _fields_ = _fields("x weight bias window y", "batch x_stride_b", "width taps type activation")
+
+
+class StateScan(ctypes.Structure):
+    """astra_state_scan (include/astra_sequence.h)."""
+    _fields_ = _fields("x dt b c A D dt_bias initial lengths y final_state chunk_states",
+                       "batch length x_stride_b x_stride_t x_stride_h dt_stride_b dt_stride_t dt_stride_h "
+                       "b_stride_b b_stride_t b_stride_g c_stride_b c_stride_t c_stride_g",
+                       "heads dim groups state type") + [("workspace", _vp), ("workspace_bytes", _sz)]
+
+
+class StateScanGrad(ctypes.Structure):
+    """astra_state_scan_grad (include/astra_sequence.h)."""
+    _fields_ = [("f", StateScan)] + _fields("dy dfinal dx ddt db dc dA dD ddt_bias dinitial workspace", "", "") + [
+        ("workspace_bytes", _sz)]
+
+
+class StateScanOne(ctypes.Structure):
+    """astra_state_scan_one (include/astra_sequence.h)."""
+    _fields_ = _fields("x dt b c A D dt_bias h y",
+                       "batch x_stride_b x_stride_h dt_stride_b dt_stride_h b_stride_b b_stride_g c_stride_b "
+                       "c_stride_g", "heads dim groups state type")
+
+
+class JoinNorm(ctypes.Structure):
+    """astra_join_norm (include/astra_sequence.h)."""
+    _fields_ = _fields("residual block gate post next scale joined normed rstd",
+                       "rows residual_stride block_stride gate_stride",
+                       "width gate_width scale_width type residual_type") + [("eps", ctypes.c_float)]
+
+
+class JoinNormGrad(ctypes.Structure):
+    """astra_join_norm_grad (include/astra_sequence.h)."""
+    _fields_ = [("f", JoinNorm)] + _fields("djoined dnormed dresidual dblock dgate dpost dnext dscale workspace",
+                                           "", "") + [("workspace_bytes", _sz)]
+
 
 _lib = None
 

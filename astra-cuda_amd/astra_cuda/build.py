@@ -1,7 +1,8 @@
 """Builds ``libastra_market.so`` (the HIP engine + C ABI) in-tree for gfx950.
 
-Sources: ``csrc/market.hip`` (the VecMarket engine, include/astra_market.h) and
-``csrc/high_low.hip`` (the high-low game's move kernels, include/astra_high_low.h).
+Sources: ``csrc/market.hip`` (the VecMarket engine, include/astra_market.h),
+``csrc/high_low.hip`` (the high-low game's move kernels, include/astra_high_low.h) and
+``csrc/sequence_*.hip`` (the policies' sequence operators, include/astra_sequence.h).
 
 Usage: ``python astra-cuda_amd/astra_cuda/build.py`` or ``astra_cuda.build.build()``.
 The library links the HIP runtime by its SONAME (libamdhip64.so.7); imported after
@@ -22,7 +23,8 @@ CSRC = os.path.join(os.path.dirname(PKG_DIR), "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB_NAME = "libastra_market.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = [os.path.join(CSRC, "market.hip"), os.path.join(CSRC, "high_low.hip")]
+SOURCES = [os.path.join(CSRC, f) for f in ("market.hip", "high_low.hip", "sequence_conv.hip", "sequence_join.hip",
+                                           "sequence_scan.hip")]
 
 ARCH = os.environ.get("ASTRA_OFFLOAD_ARCH", "gfx950")
 
@@ -30,7 +32,8 @@ ARCH = os.environ.get("ASTRA_OFFLOAD_ARCH", "gfx950")
 # for each, and one for the entry points, compiled side by side.
 UNITS = [("market", SOURCES[0], ["-DASTRA_W_UNITS"])] + \
         [(f"market_w{w}", SOURCES[0], [f"-DASTRA_W={w}"]) for w in (16, 8, 4, 2, 1)] + \
-        [("high_low", SOURCES[1], [])]
+        [("high_low", SOURCES[1], [])] + \
+        [(os.path.basename(s)[:-len(".hip")], s, []) for s in SOURCES[2:]]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
