@@ -38,6 +38,7 @@ MAX_TAPS = 4        # ASTRA_SEQ_MAX_TAPS
 MAX_STATE = 128     # ASTRA_SEQ_MAX_STATE
 MAX_NORM_WIDTH = 16384  # ASTRA_SEQ_MAX_NORM_WIDTH
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}  # ASTRA_SEQ_F32, ASTRA_SEQ_BF16
 _ACTIVATIONS = {None: 0, "silu": 1}             # ASTRA_SEQ_LINEAR, ASTRA_SEQ_SILU
 
@@ -49,6 +50,10 @@ def _need(cond: bool, what: str) -> None:
 
 def _data(name: str, t, like=None, shape=None):
     """A float32 or bfloat16 tensor on a HIP device, of ``like``'s type and device."""
+    if type(t) in _PLAIN and t.is_cuda and (
+            t.dtype in _TYPES if like is None else t.dtype is like.dtype and t.device == like.device) and (
+            shape is None or t.shape == shape):
+        return t
     _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
     _need(t.is_cuda, f"{name} must be on a HIP device, got {t.device}")
     _need(t.dtype in _TYPES, f"{name} must be float32 or bfloat16, got {t.dtype}")
@@ -64,6 +69,9 @@ def _param(name: str, t, like, shape):
     """A parameter or state as a contiguous float32 tensor (None stays None)."""
     if t is None:
         return None
+    if type(t) in _PLAIN and t.dtype is torch.float32 and t.shape == shape and t.device == like.device \
+            and t.is_contiguous():
+        return t
     _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
     _need(t.device == like.device, f"{name} must be on {like.device}, got {t.device}")
     _need(t.dtype.is_floating_point, f"{name} must be a floating point tensor, got {t.dtype}")
@@ -89,6 +97,14 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+def _with_grad(*tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _call(fn, struct, device) -> None:
     if torch.cuda.current_device() == device.index:
         rc = fn(ctypes.addressof(struct), _raw_stream(device.index))
@@ -110,28 +126,31 @@ def _workspace(nbytes: int, device):
 
 
 def _no_grad(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if _with_grad(*tensors):
         _fatal(f"sequence.py {name} moves its state on in place and has no gradient; "
                "call it under torch.no_grad(), or use the whole-sequence operator")
 
 
 # ------------------------------------------------------------------------ short_conv
 
+def _conv_forward(x, weight, bias, window, lengths, activation, want_last):
+    B, T, D = x.shape
+    K = weight.shape[1]
+    y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+    last = torch.empty((B, K - 1, D), dtype=x.dtype, device=x.device) if want_last else None
+    f = _native.ShortConv(_p(x), _p(weight), _p(bias), _p(window), _p(lengths), _p(y), _p(last), B, T,
+                          x.stride(0), x.stride(1), D, K, _TYPES[x.dtype], activation)
+    _call(_native.lib().astra_short_conv_forward, f, x.device)
+    return y, last
+
+
 class _ShortConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, window, lengths, activation, want_last):
-        B, T, D = x.shape
-        K = weight.shape[1]
-        x = _rows(x)
-        y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
-        last = torch.empty((B, K - 1, D), dtype=x.dtype, device=x.device) if want_last else None
-        f = _native.ShortConv(_p(x), _p(weight), _p(bias), _p(window), _p(lengths), _p(y), _p(last), B, T,
-                              x.stride(0), x.stride(1), D, K, _TYPES[x.dtype], activation)
-        _call(_native.lib().astra_short_conv_forward, f, x.device)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, weight, bias, window, lengths)
         ctx.activation = activation
-        return y, last
+        return _conv_forward(x, weight, bias, window, lengths, activation, want_last)
 
     @staticmethod
     @once_differentiable
@@ -182,8 +201,8 @@ def short_conv(x, weight, bias=None, *, activation="silu", initial_state=None, l
     K, w, b = _conv_checks(x, weight, bias, activation, D)
     if initial_state is not None:
         initial_state = _data("initial_state", initial_state, x, (B, K - 1, D)).contiguous()
-    y, last = _ShortConv.apply(x, w, b, initial_state, _lengths(lengths, x, B), _ACTIVATIONS[activation],
-                               bool(return_state))
+    run = _ShortConv.apply if _with_grad(x, w, b, initial_state) else _conv_forward
+    y, last = run(_rows(x), w, b, initial_state, _lengths(lengths, x, B), _ACTIVATIONS[activation], bool(return_state))
     return (y, last) if return_state else y
 
 
@@ -216,23 +235,27 @@ def _scan_struct(x, dt, A, B, C, D, dt_bias, initial, lengths, y, final, states,
         x.shape[3], B.shape[2], B.shape[3], _TYPES[x.dtype], _p(ws), ws.numel() if ws is not None else 0)
 
 
+def _scan_forward(x, dt, A, B, C, D, dt_bias, initial, lengths, want_state, grad=False):
+    lib = _native.lib()
+    batch, _, H, P = x.shape
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    final = torch.empty((batch, H, P, B.shape[3]), dtype=torch.float32, device=x.device) if want_state else None
+    f = _scan_struct(x, dt, A, B, C, D, dt_bias, initial, lengths, y, final, None, None)
+    ws = _workspace(_size(lib.astra_state_scan_workspace_size, f), x.device)
+    states = None
+    if grad:
+        n = _size(lib.astra_state_scan_chunk_states, f)
+        states = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
+    f.chunk_states, f.workspace = _p(states), _p(ws)
+    f.workspace_bytes = ws.numel() if ws is not None else 0
+    _call(lib.astra_state_scan_forward, f, x.device)
+    return (y, final, states) if grad else (y, final)
+
+
 class _StateScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, dt_bias, initial, lengths, want_state):
-        x, B, C = _rows(x), _rows(B), _rows(C)
-        lib = _native.lib()
-        batch, _, H, P = x.shape
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        final = torch.empty((batch, H, P, B.shape[3]), dtype=torch.float32, device=x.device) if want_state else None
-        f = _scan_struct(x, dt, A, B, C, D, dt_bias, initial, lengths, y, final, None, None)
-        ws = _workspace(_size(lib.astra_state_scan_workspace_size, f), x.device)
-        states = None
-        if any(ctx.needs_input_grad):
-            n = _size(lib.astra_state_scan_chunk_states, f)
-            states = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
-        f.chunk_states, f.workspace = _p(states), _p(ws)
-        f.workspace_bytes = ws.numel() if ws is not None else 0
-        _call(lib.astra_state_scan_forward, f, x.device)
+        y, final, states = _scan_forward(x, dt, A, B, C, D, dt_bias, initial, lengths, want_state, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, dt, A, B, C, D, dt_bias, initial, lengths, states)
         return y, final
@@ -299,8 +322,9 @@ def state_scan(x, dt, A, B, C, D=None, *, dt_bias=None, initial_state=None, leng
     A, D, dt_bias = _scan_checks(x, dt, A, B, C, D, dt_bias, 2)
     batch, _, H, P = x.shape
     initial_state = _param("initial_state", initial_state, x, (batch, H, P, B.shape[3]))
-    y, state = _StateScan.apply(x, dt, A, B, C, D, dt_bias, initial_state, _lengths(lengths, x, batch),
-                                bool(return_state))
+    run = _StateScan.apply if _with_grad(x, dt, A, B, C, D, dt_bias, initial_state) else _scan_forward
+    y, state = run(_rows(x), dt, A, _rows(B), _rows(C), D, dt_bias, initial_state, _lengths(lengths, x, batch),
+                   bool(return_state))
     return (y, state) if return_state else y
 
 
@@ -328,33 +352,34 @@ def state_scan_step(x, dt, A, B, C, state, D=None, *, dt_bias=None):
 
 # ------------------------------------------------------------------------- join_norm
 
+def _join_struct(residual, block, post, nxt, gate, scale, joined, normed, rstd, eps):
+    like = residual if block is None else block
+    return _native.JoinNorm(
+        _p(residual), _p(block), _p(gate), _p(post), _p(nxt), _p(scale), _p(joined), _p(normed), _p(rstd),
+        residual.shape[0], residual.stride(0), like.stride(0), 0 if gate is None else gate.stride(0),
+        residual.shape[1], 0 if gate is None else gate.shape[1], 0 if scale is None else scale.shape[0],
+        _TYPES[like.dtype], _TYPES[residual.dtype], eps)
+
+
+def _join_forward(residual, block, post, nxt, gate, scale, eps, rstd=None):
+    # every tensor is 2-D here, [rows, width]
+    like = residual if block is None else block
+    joined = torch.empty(residual.shape, dtype=residual.dtype, device=like.device) if block is not None else None
+    normed = torch.empty(residual.shape, dtype=like.dtype, device=like.device) if nxt is not None else None
+    if residual.shape[0]:
+        f = _join_struct(residual, block, post, nxt, gate, scale, joined, normed, rstd, eps)
+        _call(_native.lib().astra_join_norm_forward, f, like.device)
+    return joined, normed
+
+
 class _JoinNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, residual, block, post, nxt, gate, scale, eps):
-        # every tensor is 2-D here, [rows, width]
-        R, D = residual.shape
-        residual, block, gate = (None if t is None else _rows(t) for t in (residual, block, gate))
-        like = residual if block is None else block
-        joined = torch.empty((R, D), dtype=residual.dtype, device=residual.device) if block is not None else None
-        normed = torch.empty((R, D), dtype=like.dtype, device=residual.device) if nxt is not None else None
-        grad = any(ctx.needs_input_grad)
-        rstd = torch.empty((R, 2), dtype=torch.float32, device=residual.device) if grad else None
-        f = _JoinNorm.struct(residual, block, post, nxt, gate, scale, joined, normed, rstd, eps)
-        if R:
-            _call(_native.lib().astra_join_norm_forward, f, residual.device)
+        rstd = torch.empty((residual.shape[0], 2), dtype=torch.float32, device=residual.device)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(residual, block, post, nxt, gate, scale, rstd)
         ctx.eps = eps
-        return joined, normed
-
-    @staticmethod
-    def struct(residual, block, post, nxt, gate, scale, joined, normed, rstd, eps):
-        like = residual if block is None else block
-        return _native.JoinNorm(
-            _p(residual), _p(block), _p(gate), _p(post), _p(nxt), _p(scale), _p(joined), _p(normed), _p(rstd),
-            residual.shape[0], residual.stride(0), like.stride(0), 0 if gate is None else gate.stride(0),
-            residual.shape[1], 0 if gate is None else gate.shape[1], 0 if scale is None else scale.shape[0],
-            _TYPES[like.dtype], _TYPES[residual.dtype], eps)
+        return _join_forward(residual, block, post, nxt, gate, scale, eps, rstd)
 
     @staticmethod
     @once_differentiable
@@ -364,7 +389,7 @@ class _JoinNorm(torch.autograd.Function):
             return (None,) * 7
         need = ctx.needs_input_grad
         djoined, dnormed = (None if t is None else t.contiguous() for t in (djoined, dnormed))
-        f = _JoinNorm.struct(residual, block, post, nxt, gate, scale, None, None, rstd, ctx.eps)
+        f = _join_struct(residual, block, post, nxt, gate, scale, None, None, rstd, ctx.eps)
 
         def like(i, t):
             return torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and need[i] else None
@@ -384,8 +409,14 @@ class _JoinNorm(torch.autograd.Function):
 
 
 def _flat(t):
-    """[..., D] as [rows, D] (a view where the strides allow it)."""
-    return t.reshape(-1, t.shape[-1])
+    """[..., D] as [rows, D] (a view where the strides allow it) with contiguous rows."""
+    return _rows(t) if t.dim() == 2 else _rows(t.reshape(-1, t.shape[-1]))
+
+
+def _join(residual, block, post, nxt, gate, scale, eps):
+    run = _JoinNorm.apply if _with_grad(residual, block, post, nxt, gate, scale) else _join_forward
+    return run(_flat(residual), None if block is None else _flat(block), post, nxt,
+               None if gate is None else _flat(gate), scale, float(eps))
 
 
 def join_norm(residual, block, post_weight, next_weight, *, gate=None, scale=None, eps=1e-6):
@@ -411,15 +442,13 @@ def join_norm(residual, block, post_weight, next_weight, *, gate=None, scale=Non
         _data("gate", gate, block)
         _need(gate.shape in (block.shape, block.shape[:-1] + (1,)),
               f"gate must have shape {list(block.shape)} or {list(block.shape[:-1]) + [1]}, got {list(gate.shape)}")
-        gate = _flat(gate)
     if scale is not None:
         _need(isinstance(scale, torch.Tensor) and tuple(scale.shape) in ((D,), (1,)),
               f"scale must be a tensor of shape [{D}] or [1]")
         scale = _param("scale", scale, block, scale.shape)
     post = _param("post_weight", post_weight, block, (D,))
     _need(post is not None, "post_weight must be a tensor")
-    joined, normed = _JoinNorm.apply(_flat(residual), _flat(block), post, _param("next_weight", next_weight, block, (D,)),
-                                     gate, scale, float(eps))
+    joined, normed = _join(residual, block, post, _param("next_weight", next_weight, block, (D,)), gate, scale, eps)
     return joined.view(block.shape), None if normed is None else normed.view(block.shape)
 
 
@@ -432,4 +461,4 @@ def rms_norm(x, weight, *, eps=1e-6):
     _need(1 <= D <= MAX_NORM_WIDTH, f"the width must be 1 to {MAX_NORM_WIDTH}, got {D}")
     weight = _param("weight", weight, x, (D,))
     _need(weight is not None, "weight must be a tensor")
-    return _JoinNorm.apply(_flat(x), None, None, weight, None, None, float(eps))[1].view(x.shape)
+    return _join(x, None, None, weight, None, None, eps)[1].view(x.shape)

@@ -43,18 +43,20 @@ struct Vec<T, 1> {
   static __device__ __forceinline__ void store(T *p, const float (&v)[1]) { *p = (T)v[0]; }
 };
 
-// The sum over the 64 lanes, in every lane.
-__device__ __forceinline__ float wave_sum(float v) {
+// The sum over N neighbouring lanes, in each of them.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, kWave);
+  for (int m = N / 2; m; m >>= 1) v += __shfl_xor(v, m, kWave);
   return v;
 }
+__device__ __forceinline__ float wave_sum(float v) { return lanes_sum<kWave>(v); }
 
-// The sum over TPR threads (a wavefront, or a whole workgroup through `lds`, TPR / 64
-// words that nothing else uses; two calls in a row need two such areas).
+// The sum over TPR threads (part of a wavefront, or a whole workgroup through `lds`,
+// TPR / 64 words that nothing else uses; two calls in a row need two such areas).
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float *lds) {
-  v = wave_sum(v);
+  v = lanes_sum<(TPR < kWave ? TPR : kWave)>(v);
   if constexpr (TPR > kWave) {
     constexpr int W = TPR / kWave;
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -66,7 +68,10 @@ __device__ __forceinline__ float row_sum(float v, float *lds) {
   return v;
 }
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + __expf(-v)); }
+// 1 / (1 + exp(-v)): the hardware's exp2 and reciprocal are each good to 1 ulp.
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
+}
 
 __device__ __forceinline__ int row_length(const int32_t *lengths, int64_t b, int64_t T) {
   if (!lengths) return (int)T;
@@ -74,29 +79,34 @@ __device__ __forceinline__ int row_length(const int32_t *lengths, int64_t b, int
   return n < 0 ? 0 : n > T ? (int)T : n;
 }
 
-// The sum of part[r, j] over the rows r, in a fixed order: called by a workgroup of four
-// wavefronts for the 64 columns from 64 * blockIdx.x on, each taking a quarter of the rows.
-// True in the one thread that has the sum of column j.
+// The sum of part[r, j] over the rows r, in a fixed order: called by a workgroup of
+// kSumThreads for the kSumCols columns from kSumCols * blockIdx.x on. 64 threads a column,
+// so that a thousand rows are 16 loads a thread. True in the one thread that has the sum
+// of column j.
+constexpr int kSumCols = 16, kSumThreads = 1024;
 __device__ __forceinline__ bool sum_rows(const float *part, int64_t rows, int64_t cols, int64_t *col, float *sum) {
-  __shared__ float lds[4][kWave];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t j = (int64_t)blockIdx.x * kWave + lane;
-  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+  constexpr int kSlots = kSumThreads / kSumCols;
+  __shared__ float lds[kSlots][kSumCols];
+  const int c = threadIdx.x % kSumCols, slot = threadIdx.x / kSumCols;
+  const int64_t j = (int64_t)blockIdx.x * kSumCols + c;
+  float s[8] = {};
   if (j < cols) {
-    int64_t r = w;
-    for (; r + 12 < rows; r += 16) {
-      s0 += part[r * cols + j];
-      s1 += part[(r + 4) * cols + j];
-      s2 += part[(r + 8) * cols + j];
-      s3 += part[(r + 12) * cols + j];
-    }
-    for (; r < rows; r += 4) s0 += part[r * cols + j];
+    int64_t r = slot;
+    for (; r + 7 * kSlots < rows; r += 8 * kSlots)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += part[(r + i * kSlots) * cols + j];
+    for (; r < rows; r += kSlots) s[0] += part[r * cols + j];
   }
-  lds[w][lane] = (s0 + s1) + (s2 + s3);
+  lds[slot][c] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   __syncthreads();
+#pragma unroll
+  for (int h = kSlots / 2; h; h /= 2) {
+    if (slot < h) lds[slot][c] += lds[slot + h][c];
+    __syncthreads();
+  }
   *col = j;
-  *sum = (lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]);
-  return w == 0 && j < cols;
+  *sum = lds[0][c];
+  return slot == 0 && j < cols;
 }
 
 inline bool aligned(const void *p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

@@ -28,8 +28,10 @@ __device__ __forceinline__ void load_taps(const ConvArgs &a, int d, float (&w)[K
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     b[i] = a.bias ? a.bias[d + i] : 0.f;
+    float taps[K];
+    __builtin_memcpy(taps, a.weight + (int64_t)(d + i) * K, sizeof(taps));
 #pragma unroll
-    for (int k = 0; k < K; ++k) w[k][i] = a.weight[(int64_t)(d + i) * K + k];
+    for (int k = 0; k < K; ++k) w[k][i] = taps[k];
   }
 }
 
@@ -102,11 +104,12 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a) {
 // g[t] = dy[t] act'(p[t]); dx[t] = sum_k w[k] g[t+K-1-k]; dw[k] = sum_t g[t] x[t-K+1+k].
 // A workgroup: CX groups of V channels by 256 / CX rows; a row of threads walks runs of
 // positions, `gridDim.y` rows of workgroups apart, and keeps its part of dw and dbias in
-// registers. A run recomputes the K-1 values of g after its end.
+// registers. A run recomputes the K-1 values of g after its end. U positions at a time, so
+// that their loads are in flight together and the windows of x and g need no moves.
 constexpr int kConvCols = 16;
 template <class T, int K, int V>
 __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
-  constexpr int CX = kConvCols, IY = 256 / CX;
+  constexpr int CX = kConvCols, IY = 256 / CX, U = 4;
   const int cx = threadIdx.x % CX, iy = threadIdx.x / CX;
   const int groups = a.D / V;
   const int cg = blockIdx.x * CX + cx;
@@ -126,57 +129,60 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
     const int64_t t0 = (row - b * a.runs) * a.run;
     const int64_t t1 = t0 + a.run < a.T ? t0 + a.run : a.T;
     const int len = row_length(a.lengths, b, a.T);
-    float in[K][V], g[K][V];  // in[K-1] = x[t], g[0] = g[t], g[k] = g[t-k]
+    float in[K - 1 + U][V], g[K - 1 + U][V];  // entry K-1+u is position t+u
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) load_input<T, K, V>(a, b, t0 - (K - 1) + k, len, d, in[k + 1]);
-#pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K - 1; ++k) {
+      load_input<T, K, V>(a, b, t0 - (K - 1) + k, len, d, in[k]);
+      // the g before a run are another run's, but no output of this one takes them: it
+      // writes dx[t - (K-1)] for t in [t0 + K-1, t1 + K-1), and the window
 #pragma unroll
       for (int i = 0; i < V; ++i) g[k][i] = 0.f;
-    // the g before a run are another run's, but they take part in no output of this one:
-    // what this run writes is x[t - (K-1)] for t in [t0 + K-1, t1 + K-1), and the window
-    for (int64_t t = t0; t < t1 + K - 1; ++t) {
-      float dy[V];
+    }
+    for (int64_t t = t0; t < t1 + K - 1; t += U) {
+      float dy[U][V];
 #pragma unroll
-      for (int k = 0; k < K - 1; ++k)
+      for (int u = 0; u < U; ++u) {
+        load_input<T, K, V>(a, b, t + u, len, d, in[K - 1 + u]);
+        if (t + u < len)
+          Vec<T, V>::load((const T *)a.dy + (b * a.T + t + u) * a.D + d, dy[u]);
+        else
 #pragma unroll
-        for (int i = 0; i < V; ++i) in[k][i] = in[k + 1][i];
-      load_input<T, K, V>(a, b, t, len, d, in[K - 1]);
-      if (t < len)
-        Vec<T, V>::load((const T *)a.dy + (b * a.T + t) * a.D + d, dy);
-      else
-#pragma unroll
-        for (int i = 0; i < V; ++i) dy[i] = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float p = bias[i];
-#pragma unroll
-        for (int k = 0; k < K; ++k) p += w[k][i] * in[k][i];
-        const float s = sigmoid(p);
-        const float gt = a.silu ? dy[i] * s * (1.f + p * (1.f - s)) : dy[i];
-#pragma unroll
-        for (int k = K - 1; k > 0; --k) g[k][i] = g[k - 1][i];
-        g[0][i] = t < len ? gt : 0.f;
-        if (t < t1) {
-          db[i] += g[0][i];
-#pragma unroll
-          for (int k = 0; k < K; ++k) dw[k][i] += g[0][i] * in[k][i];
-        }
+          for (int i = 0; i < V; ++i) dy[u][i] = 0.f;
       }
-      // the gradient of the input at t - (K-1); before 0 it is the window's
-      const int64_t at = t - (K - 1);
-      if (at >= t0 || t0 == 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool mine = t + u < t1;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float v = dy[u][i];
+          if (a.silu) {
+            float p = bias[i];
+#pragma unroll
+            for (int k = 0; k < K; ++k) p += w[k][i] * in[u + k][i];
+            const float s = sigmoid(p);
+            v *= s * (1.f + p * (1.f - s));
+          }
+          v = t + u < len ? v : 0.f;
+          g[K - 1 + u][i] = v;
+          const float own = mine ? v : 0.f;
+          db[i] += own;
+#pragma unroll
+          for (int k = 0; k < K; ++k) dw[k][i] += own * in[u + k][i];
+        }
+        // the gradient of the input at t + u - (K-1); before 0 it is the window's
+        const int64_t at = t + u - (K - 1);
+        if (t + u >= t1 + K - 1 || (at < t0 && t0 > 0)) continue;
         float o[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           o[i] = 0.f;
 #pragma unroll
-          for (int k = 0; k < K; ++k) o[i] += w[k][i] * g[k][i];
+          for (int k = 0; k < K; ++k) o[i] += w[k][i] * g[K - 1 + u - k][i];
         }
         // position len - (K-1) + k is row k of `last`
-        if (a.dlast && at < len && t >= len) {
+        if (a.dlast && at < len && t + u >= len) {
           float e[V];
-          Vec<T, V>::load((const T *)a.dlast + (b * (K - 1) + (t - len)) * a.D + d, e);
+          Vec<T, V>::load((const T *)a.dlast + (b * (K - 1) + (t + u - len)) * a.D + d, e);
 #pragma unroll
           for (int i = 0; i < V; ++i) o[i] += e[i];
         }
@@ -188,9 +194,16 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
             Vec<T, V>::store((T *)a.dx + (b * a.T + at) * a.D + d, o);
           }
         } else if (a.dwindow) {
-          Vec<T, V>::store((T *)a.dwindow + (b * (K - 1) + t) * a.D + d, o);
+          Vec<T, V>::store((T *)a.dwindow + (b * (K - 1) + t + u) * a.D + d, o);
         }
       }
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          in[k][i] = in[k + U][i];
+          g[k][i] = g[k + U][i];
+        }
     }
   }
   if (!a.part) return;
@@ -219,7 +232,7 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
 
 // dweight and dbias from the partial rows [parts, D, K + 1].
 template <int K>
-__global__ __launch_bounds__(256) void conv_weights_kernel(const float *part, int64_t parts, int32_t D, float *dw,
+__global__ __launch_bounds__(kSumThreads) void conv_weights_kernel(const float *part, int64_t parts, int32_t D, float *dw,
                                                            float *db) {
   int64_t j;
   float s;
@@ -301,19 +314,23 @@ void set_runs(ConvArgs &a, int64_t threads_per_position) {
   if (a.runs < 1) a.runs = 1;
 }
 
-// 16-byte accesses where every row starts on one.
-template <class T>
+// Accesses of V elements where every row starts on one.
+template <class T, int V>
 int wide(const ConvArgs &a, std::initializer_list<const void *> ptrs) {
-  constexpr int V = 16 / sizeof(T);
   if (a.D % V || a.xsb % V || a.xst % V) return 1;
   for (const void *p : ptrs)
-    if (!aligned(p, 16)) return 1;
+    if (!aligned(p, V * sizeof(T))) return 1;
   return V;
 }
 
-#define CONV_DISPATCH(T, KERNEL, grid)                                                        \
+// Channels of a thread: 16 bytes forwards; backwards, where 11 values of each are in
+// registers, 4.
+template <class T>
+constexpr int kForward = 16 / sizeof(T);
+constexpr int kBackward = 4;
+
+#define CONV_DISPATCH(T, KERNEL, VW, grid)                                                    \
   do {                                                                                        \
-    constexpr int VW = 16 / sizeof(T);                                                        \
     if (v == 1) {                                                                             \
       if (taps == 2) hipLaunchKernelGGL((KERNEL<T, 2, 1>), grid, dim3(256), 0, st, a);        \
       if (taps == 3) hipLaunchKernelGGL((KERNEL<T, 3, 1>), grid, dim3(256), 0, st, a);        \
@@ -328,11 +345,11 @@ int wide(const ConvArgs &a, std::initializer_list<const void *> ptrs) {
 template <class T>
 int forward(const astra_short_conv &f, hipStream_t st) {
   ConvArgs a = args_of(f);
-  const int v = wide<T>(a, {a.x, a.window, a.y, a.last}), taps = f.taps;
+  const int v = wide<T, kForward<T>>(a, {a.x, a.window, a.y, a.last}), taps = f.taps;
   set_runs(a, a.D / v);
   const int64_t blocks = cdiv(a.B * a.runs * (a.D / v), 256);
   ASTRA_ABI_CHECK(blocks, <, 2147483648ll);
-  CONV_DISPATCH(T, conv_forward_kernel, dim3((unsigned)blocks));
+  CONV_DISPATCH(T, conv_forward_kernel, kForward<T>, dim3((unsigned)blocks));
   ASTRA_HIP_CHECK(rt_last_error(), "conv_forward_kernel launch");
   return ASTRA_OK;
 }
@@ -353,7 +370,7 @@ int backward(const astra_short_conv_grad &g, hipStream_t st) {
   a.dlast = g.dlast;
   a.dx = g.dx;
   a.dwindow = g.dwindow;
-  const int v = wide<T>(a, {a.x, a.window, a.dy, a.dlast, a.dx, a.dwindow}), taps = g.f.taps;
+  const int v = wide<T, kBackward>(a, {a.x, a.window, a.dy, a.dlast, a.dx, a.dwindow}), taps = g.f.taps;
   set_runs(a, a.D / v);
   const int64_t rows = backward_rows(a, v);
   const bool sums = g.dweight || g.dbias;
@@ -362,13 +379,13 @@ int backward(const astra_short_conv_grad &g, hipStream_t st) {
     ASTRA_ABI_CHECK((int64_t)g.workspace_bytes, >=, (int64_t)(rows * a.D * (taps + 1) * sizeof(float)));
     a.part = (float *)g.workspace;
   }
-  CONV_DISPATCH(T, conv_backward_kernel, dim3((unsigned)cdiv(a.D / v, kConvCols), (unsigned)rows));
+  CONV_DISPATCH(T, conv_backward_kernel, kBackward, dim3((unsigned)cdiv(a.D / v, kConvCols), (unsigned)rows));
   ASTRA_HIP_CHECK(rt_last_error(), "conv_backward_kernel launch");
   if (sums) {
-    const dim3 grid((unsigned)cdiv((int64_t)a.D * (taps + 1), kWave));
-    if (taps == 2) hipLaunchKernelGGL(conv_weights_kernel<2>, grid, dim3(256), 0, st, a.part, rows, a.D, g.dweight, g.dbias);
-    if (taps == 3) hipLaunchKernelGGL(conv_weights_kernel<3>, grid, dim3(256), 0, st, a.part, rows, a.D, g.dweight, g.dbias);
-    if (taps == 4) hipLaunchKernelGGL(conv_weights_kernel<4>, grid, dim3(256), 0, st, a.part, rows, a.D, g.dweight, g.dbias);
+    const dim3 grid((unsigned)cdiv((int64_t)a.D * (taps + 1), kSumCols));
+    if (taps == 2) hipLaunchKernelGGL(conv_weights_kernel<2>, grid, dim3(kSumThreads), 0, st, a.part, rows, a.D, g.dweight, g.dbias);
+    if (taps == 3) hipLaunchKernelGGL(conv_weights_kernel<3>, grid, dim3(kSumThreads), 0, st, a.part, rows, a.D, g.dweight, g.dbias);
+    if (taps == 4) hipLaunchKernelGGL(conv_weights_kernel<4>, grid, dim3(kSumThreads), 0, st, a.part, rows, a.D, g.dweight, g.dbias);
     ASTRA_HIP_CHECK(rt_last_error(), "conv_weights_kernel launch");
   }
   return ASTRA_OK;
@@ -386,10 +403,10 @@ int step(const astra_short_conv_one &o, hipStream_t st) {
   a.xsb = o.x_stride_b;
   a.D = o.width;
   a.silu = o.activation == ASTRA_SEQ_SILU;
-  const int v = wide<T>(a, {a.x, a.dwindow, a.y}), taps = o.taps;
+  const int v = wide<T, kForward<T>>(a, {a.x, a.dwindow, a.y}), taps = o.taps;
   const int64_t blocks = cdiv(a.B * (a.D / v), 256);
   ASTRA_ABI_CHECK(blocks, <, 2147483648ll);
-  CONV_DISPATCH(T, conv_step_kernel, dim3((unsigned)blocks));
+  CONV_DISPATCH(T, conv_step_kernel, kForward<T>, dim3((unsigned)blocks));
   ASTRA_HIP_CHECK(rt_last_error(), "conv_step_kernel launch");
   return ASTRA_OK;
 }
@@ -420,7 +437,7 @@ int astra_short_conv_workspace_size(const astra_short_conv *f, size_t *bytes) {
   // the most partial rows that any alignment leads to
   ConvArgs a = args_of(*f);
   int64_t rows = 1;
-  for (int v : {1, f->type == ASTRA_SEQ_BF16 ? 8 : 4}) {
+  for (int v : {1, kBackward}) {
     if (a.D % v) continue;
     set_runs(a, a.D / v);
     const int64_t r = backward_rows(a, v);

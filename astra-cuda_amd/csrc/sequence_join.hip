@@ -134,8 +134,8 @@ __global__ __launch_bounds__(block_of<TPR>) void join_forward_kernel(JoinArgs a)
 //   dsg = dr c hat,  dhat = dr sg c,  du = i1 dhat - u i1^3 mean(dhat u)
 //   q   = sum over rows of dr sg hat: dpost = q scale, dscale = q post;  dnext = sum dn r' i2
 // With a single column the two terms of a norm's gradient cancel but for eps i^3.
-// A thread keeps q and dnext of its columns over its rows; a workgroup's are row
-// blockIdx.x * RPB + sub of part [gridDim.x * RPB, 2, D].
+// A thread keeps q and dnext of its columns over its rows; a workgroup's are row blockIdx.x
+// of part [gridDim.x, 2, D].
 template <class TR, class T, int V, int NV, int TPR>
 __global__ __launch_bounds__(block_of<TPR>) void join_backward_kernel(JoinArgs a) {
   constexpr int RPB = block_of<TPR> / TPR;
@@ -232,21 +232,44 @@ __global__ __launch_bounds__(block_of<TPR>) void join_backward_kernel(JoinArgs a
     if constexpr (TPR > kWave) __syncthreads();
   }
   if (!a.part) return;
-  float *part = a.part + ((int64_t)blockIdx.x * RPB + sub) * a.D * 2;
+  float *part = a.part + (int64_t)blockIdx.x * a.D * 2;
+  if constexpr (RPB == 1) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (j * TPR + t) * V + i;
-      if (c < a.D) {
-        part[c] = q[j][i];
-        part[a.D + c] = dnw[j][i];
+      for (int i = 0; i < V; ++i) {
+        const int c = (j * TPR + t) * V + i;
+        if (c < a.D) {
+          part[c] = q[j][i];
+          part[a.D + c] = dnw[j][i];
+        }
+      }
+  } else {
+    // one vector of columns of the RPB rows of threads at a time
+    __shared__ float sums[2][RPB][TPR * V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        sums[0][sub][t * V + i] = q[j][i];
+        sums[1][sub][t * V + i] = dnw[j][i];
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < 2 * TPR * V; e += block_of<TPR>) {
+        const int k = e / (TPR * V), c = e % (TPR * V);
+        if (j * TPR * V + c >= a.D) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int n = 0; n < RPB; ++n) v += sums[k][n][c];
+        part[k * a.D + j * TPR * V + c] = v;
       }
     }
+  }
 }
 
 // dpost, dnext, dscale [D] from the partial rows [parts, 2, D].
-__global__ __launch_bounds__(256) void join_weights_kernel(const float *part, int64_t parts, JoinArgs a, float *dpost,
+__global__ __launch_bounds__(kSumThreads) void join_weights_kernel(const float *part, int64_t parts, JoinArgs a, float *dpost,
                                                            float *dnext, float *dscale) {
   int64_t j;
   float s;
@@ -316,14 +339,17 @@ struct Shape {
   int rows_per_block() const { return tpr > 256 ? 1 : 256 / tpr; }
 };
 
-// 16-byte accesses of the block's type where every row allows it. Threads a row: a
-// wavefront as long as each lane has at most 4 vectors, then 256 threads, then 1024.
+// 16-byte accesses of the block's type where every row allows it. Threads a row: 16 or 32
+// lanes where that is one vector each, a wavefront as long as each lane has at most 4
+// vectors, then 256 threads, then 1024.
 Shape shape_of(const astra_join_norm &f, std::initializer_list<const void *> ptrs) {
   const int V = f.type == ASTRA_SEQ_BF16 ? 8 : 4;
   bool wide = f.width % V == 0 && f.residual_stride % V == 0 && f.block_stride % V == 0 &&
               (!f.gate || f.gate_width == 1 || f.gate_stride % V == 0);
   for (const void *p : ptrs) wide = wide && aligned(p, 16);
   Shape s{wide ? V : 1, 1, 64};
+  for (s.tpr = 16; s.tpr < 64 && s.tpr * s.v < f.width;) s.tpr *= 2;
+  if (s.tpr < 64) return s;
   for (s.tpr = 64; s.tpr < 1024 && (int64_t)s.tpr * s.v * 4 < f.width; s.tpr *= 4) {
   }
   while ((int64_t)s.tpr * s.v * s.nv < f.width) s.nv *= 2;
@@ -342,6 +368,8 @@ Shape shape_of(const astra_join_norm &f, std::initializer_list<const void *> ptr
 template <class TR, class T>
 void launch(bool backward, const Shape &s, dim3 grid, hipStream_t st, const JoinArgs &a) {
   constexpr int VW = 16 / sizeof(T);
+  JOIN_ONE(VW, 1, 16)
+  JOIN_ONE(VW, 1, 32)
   JOIN_ONE(VW, 1, 64)
   JOIN_ONE(VW, 2, 64)
   JOIN_ONE(VW, 4, 64)
@@ -351,6 +379,8 @@ void launch(bool backward, const Shape &s, dim3 grid, hipStream_t st, const Join
   if constexpr (VW == 4) {
     JOIN_ONE(VW, 4, 1024)
   }
+  JOIN_ONE(1, 1, 16)
+  JOIN_ONE(1, 1, 32)
   JOIN_ONE(1, 1, 64)
   JOIN_ONE(1, 2, 64)
   JOIN_ONE(1, 4, 64)
@@ -362,16 +392,17 @@ void launch(bool backward, const Shape &s, dim3 grid, hipStream_t st, const Join
   JOIN_ONE(1, 16, 1024)
 }
 
-// Workgroups: enough to fill the CUs, few enough that the weights and (backward) the
-// partial sums are little beside the rows.
-int64_t blocks_of(const astra_join_norm &f, const Shape &s) {
+// Workgroups: enough to fill the CUs (8 wavefronts a SIMD forwards, 4 backwards, whose
+// threads hold more), few enough that the weights and the partial sums are little beside
+// the rows.
+int64_t blocks_of(const astra_join_norm &f, const Shape &s, bool backward) {
   const int64_t need = cdiv(f.rows, s.rows_per_block());
-  const int64_t most = s.tpr > 256 ? 512 : 1024;
+  const int64_t most = s.tpr > 256 ? 512 : backward ? 1024 : 2048;
   return need < most ? (need > 0 ? need : 1) : most;
 }
 
 void dispatch(const astra_join_norm &f, bool backward, const Shape &s, hipStream_t st, const JoinArgs &a) {
-  const dim3 grid((unsigned)blocks_of(f, s));
+  const dim3 grid((unsigned)blocks_of(f, s, backward));
   if (f.type == ASTRA_SEQ_F32)
     launch<float, float>(backward, s, grid, st, a);
   else if (f.residual_type == ASTRA_SEQ_F32)
@@ -402,10 +433,9 @@ int astra_join_norm_forward(const astra_join_norm *f, void *stream) {
 int astra_join_norm_workspace_size(const astra_join_norm *f, size_t *bytes) {
   if (int rc = check(f)) return rc;
   ASTRA_SEQ_POINTER(bytes);
-  // partial rows of the layout with the most of them, and the sum for a single scale
-  *bytes = ((size_t)1024 * 4 * 2 + 1) * f->width * sizeof(float);
-  const int64_t rows = f->rows > 0 ? f->rows : 1;
-  if (rows < 4096) *bytes = ((size_t)cdiv(rows, 4) * 4 * 2 + 1) * f->width * sizeof(float);
+  // as many partial rows as any layout has, and the sum for a single scale
+  const int64_t rows = f->rows < 1024 ? (f->rows > 0 ? f->rows : 1) : 1024;
+  *bytes = (size_t)(rows * 2 + 1) * f->width * sizeof(float);
   return ASTRA_OK;
 }
 
@@ -430,7 +460,7 @@ int astra_join_norm_backward(const astra_join_norm_grad *g, void *stream) {
     return fail(ASTRA_ERR_INVALID_ARGUMENT, "astra_join_norm_backward: the gradient of an absent gate or scale");
   const Shape s = shape_of(f, {f.residual, f.block, f.gate_width == 1 ? nullptr : f.gate, g->djoined, g->dnormed,
                                g->dresidual, g->dblock, f.gate_width == 1 ? nullptr : g->dgate});
-  const int64_t parts = blocks_of(f, s) * s.rows_per_block();
+  const int64_t parts = blocks_of(f, s, true);
   const bool sums = g->dpost || g->dnext || g->dscale;
   const hipStream_t st = as_stream(stream);
   float *single = nullptr;
@@ -447,7 +477,7 @@ int astra_join_norm_backward(const astra_join_norm_grad *g, void *stream) {
   }
   if (sums) {
     float *dscale = g->dscale && a.scale_one ? single : g->dscale;
-    hipLaunchKernelGGL(join_weights_kernel, dim3((unsigned)cdiv(2 * (int64_t)f.width, kWave)), dim3(256), 0, st,
+    hipLaunchKernelGGL(join_weights_kernel, dim3((unsigned)cdiv(2 * (int64_t)f.width, kSumCols)), dim3(kSumThreads), 0, st,
                        a.part, parts, a, g->dpost, g->dnext, dscale);
     ASTRA_HIP_CHECK(rt_last_error(), "join_weights_kernel launch");
     if (g->dscale && a.scale_one) {

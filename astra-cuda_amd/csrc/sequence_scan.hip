@@ -984,14 +984,14 @@ __global__ __launch_bounds__(256) void scan_join_slices_kernel(ScanArgs a) {
 // dA, ddt_bias and dD from the parts of the chunks, [rows, H, 3]: a first pass leaves at
 // most kSumRows rows (grid.y of them), the second ends in the gradients.
 constexpr int kSumRows = 128;
-__global__ __launch_bounds__(256) void scan_sum_rows_kernel(const float *part, int64_t rows, int64_t cols, float *out) {
+__global__ __launch_bounds__(kSumThreads) void scan_sum_rows_kernel(const float *part, int64_t rows, int64_t cols, float *out) {
   const int64_t each = (rows + gridDim.y - 1) / gridDim.y, r0 = each * blockIdx.y;
   const int64_t n = rows - r0 < each ? rows - r0 : each;
   int64_t j;
   float s;
   if (sum_rows(part + r0 * cols, n, cols, &j, &s)) out[(int64_t)blockIdx.y * cols + j] = s;
 }
-__global__ __launch_bounds__(256) void scan_sum_heads_kernel(const float *part, int64_t rows, int32_t H, float *dA,
+__global__ __launch_bounds__(kSumThreads) void scan_sum_heads_kernel(const float *part, int64_t rows, int32_t H, float *dA,
                                                              float *dbias, float *dD) {
   int64_t j;
   float s;
@@ -1012,17 +1012,31 @@ struct StepArgs {
 };
 
 // A state is read and written once, 8 bytes an element for 5 operations. LPR lanes hold a
-// row of N (V * NJ values each); a workgroup's 256 / LPR rows at a time walk the head's P.
+// row of N (V * NJ values each); a wavefront has kStepRows / LPR rows of one head, as many
+// of them in flight at once as it has, and does the head's step size once for them.
+constexpr int kStepRows = 256;  // 4 passes of 64 / LPR rows
 template <class T, int V, int LPR, int NJ>
 __global__ __launch_bounds__(256) void scan_step_kernel(StepArgs a) {
-  const int ln = threadIdx.x % LPR, row = threadIdx.x / LPR;
-  constexpr int kRows = 256 / LPR;
-  const int64_t bh = blockIdx.x, b = bh / a.H;
-  const int h = (int)(bh - b * a.H), g = h / (a.H / a.G);
+  constexpr int kRows = 64 / LPR, U = kStepRows / 64;
+  const int lane = threadIdx.x & 63, ln = lane % LPR, row = lane / LPR;
+  const int parts = (a.P + kRows * U - 1) / (kRows * U);
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), bh = id / parts, b = bh / a.H;
+  if (b >= a.B) return;
+  const int h = (int)(bh - b * a.H), g = h / (a.H / a.G), p0 = (int)(id - bh * parts) * kRows * U + row;
+  float *hp = a.h + (bh * a.P + p0) * a.N;
+  float v[U][NJ][V], x[U], bv[NJ][V], cv[NJ][V];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    x[u] = 0.f;
+    if (p0 + u * kRows >= a.P) continue;
+    x[u] = (float)((const T *)a.x)[b * a.xsb + h * a.xsh + p0 + u * kRows];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      if ((j * LPR + ln) * V < a.N) Vec<float, V>::load(hp + (int64_t)u * kRows * a.N + (j * LPR + ln) * V, v[u][j]);
+  }
+  const T *bp = (const T *)a.b + b * a.bsb + g * a.bsg, *cp = (const T *)a.c + b * a.csb + g * a.csg;
   const float raw = (float)((const T *)a.dt)[b * a.dsb + h * a.dsh] + (a.bias ? a.bias[h] : 0.f);
   const float dt = softplus(raw), decay = expf(dt * a.A[h]), D = a.D ? a.D[h] : 0.f;
-  const T *bp = (const T *)a.b + b * a.bsb + g * a.bsg, *cp = (const T *)a.c + b * a.csb + g * a.csg;
-  float bv[NJ][V], cv[NJ][V];
 #pragma unroll
   for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -1031,26 +1045,22 @@ __global__ __launch_bounds__(256) void scan_step_kernel(StepArgs a) {
       bv[j][i] = n < a.N ? dt * (float)bp[n] : 0.f;
       cv[j][i] = n < a.N ? (float)cp[n] : 0.f;
     }
-  for (int p = row; p < a.P; p += kRows) {
-    const float x = (float)((const T *)a.x)[b * a.xsb + h * a.xsh + p];
-    float *hp = a.h + (bh * a.P + p) * a.N;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (p0 + u * kRows >= a.P) continue;
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const int n = (j * LPR + ln) * V;
-      if (n >= a.N) continue;
-      float v[V];
-      Vec<float, V>::load(hp + n, v);
+      if ((j * LPR + ln) * V >= a.N) continue;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        v[i] = decay * v[i] + x * bv[j][i];
-        s += v[i] * cv[j][i];
+        v[u][j][i] = decay * v[u][j][i] + x[u] * bv[j][i];
+        s += v[u][j][i] * cv[j][i];
       }
-      Vec<float, V>::store(hp + n, v);
+      Vec<float, V>::store(hp + (int64_t)u * kRows * a.N + (j * LPR + ln) * V, v[u][j]);
     }
-#pragma unroll
-    for (int m = LPR / 2; m; m >>= 1) s += __shfl_xor(s, m, kWave);
-    if (ln == 0) ((T *)a.y)[bh * a.P + p] = (T)(s + D * x);
+    s = lanes_sum<LPR>(s);
+    if (ln == 0) ((T *)a.y)[bh * a.P + p0 + u * kRows] = (T)(s + D * x[u]);
   }
 }
 
@@ -1226,18 +1236,21 @@ int run_backward(const astra_state_scan &f, ScanArgs &a, hipStream_t st) {
 
 template <class T>
 int step(const StepArgs &a, bool wide, hipStream_t st) {
-  const int64_t blocks = a.B * a.H;
-  ASTRA_ABI_CHECK(blocks, <, 2147483648ll);
-  const dim3 grid((unsigned)blocks), block(256);
+#define STEP_LAUNCH(V, LPR, NJ)                                                                       \
+  do {                                                                                                \
+    const int64_t blocks = cdiv(a.B * a.H * cdiv(a.P, kStepRows / LPR), 4);                           \
+    ASTRA_ABI_CHECK(blocks, <, 2147483648ll);                                                         \
+    hipLaunchKernelGGL((scan_step_kernel<T, V, LPR, NJ>), dim3((unsigned)blocks), dim3(256), 0, st, a); \
+  } while (false)
   if (wide) {
-    if (a.N <= 16) hipLaunchKernelGGL((scan_step_kernel<T, 4, 4, 1>), grid, block, 0, st, a);
-    else if (a.N <= 32) hipLaunchKernelGGL((scan_step_kernel<T, 4, 8, 1>), grid, block, 0, st, a);
-    else if (a.N <= 64) hipLaunchKernelGGL((scan_step_kernel<T, 4, 16, 1>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((scan_step_kernel<T, 4, 32, 1>), grid, block, 0, st, a);
+    if (a.N <= 16) STEP_LAUNCH(4, 4, 1);
+    else if (a.N <= 32) STEP_LAUNCH(4, 8, 1);
+    else if (a.N <= 64) STEP_LAUNCH(4, 16, 1);
+    else STEP_LAUNCH(4, 32, 1);
   } else {
-    if (a.N <= 16) hipLaunchKernelGGL((scan_step_kernel<T, 1, 16, 1>), grid, block, 0, st, a);
-    else if (a.N <= 64) hipLaunchKernelGGL((scan_step_kernel<T, 1, 64, 1>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((scan_step_kernel<T, 1, 64, 2>), grid, block, 0, st, a);
+    if (a.N <= 16) STEP_LAUNCH(1, 16, 1);
+    else if (a.N <= 64) STEP_LAUNCH(1, 64, 1);
+    else STEP_LAUNCH(1, 64, 2);
   }
   ASTRA_HIP_CHECK(rt_last_error(), "scan_step_kernel launch");
   return ASTRA_OK;
@@ -1351,15 +1364,15 @@ int astra_state_scan_backward(const astra_state_scan_grad *g, void *stream) {
   if (!g->dA && !g->dD && !g->ddt_bias) return ASTRA_OK;
   int64_t rows = a.B * a.chunks;
   const float *part = a.part;
-  const unsigned cols = (unsigned)cdiv(3 * (int64_t)a.H, kWave);
+  const unsigned cols = (unsigned)cdiv(3 * (int64_t)a.H, kSumCols);
   if (rows > 4 * kSumRows) {
     float *sums = a.part + (size_t)rows * a.H * 3;
-    hipLaunchKernelGGL(scan_sum_rows_kernel, dim3(cols, kSumRows), dim3(256), 0, st, part, rows, 3 * (int64_t)a.H, sums);
+    hipLaunchKernelGGL(scan_sum_rows_kernel, dim3(cols, kSumRows), dim3(kSumThreads), 0, st, part, rows, 3 * (int64_t)a.H, sums);
     ASTRA_HIP_CHECK(rt_last_error(), "scan_sum_rows_kernel launch");
     part = sums;
     rows = kSumRows;
   }
-  hipLaunchKernelGGL(scan_sum_heads_kernel, dim3(cols), dim3(256), 0, st, part, rows, a.H, g->dA, g->ddt_bias, g->dD);
+  hipLaunchKernelGGL(scan_sum_heads_kernel, dim3(cols), dim3(kSumThreads), 0, st, part, rows, a.H, g->dA, g->ddt_bias, g->dD);
   ASTRA_HIP_CHECK(rt_last_error(), "scan_sum_heads_kernel launch");
   return ASTRA_OK;
 }
