@@ -43,11 +43,53 @@ struct Vec<T, 1> {
   static __device__ __forceinline__ void store(T *p, const float (&v)[1]) { *p = (T)v[0]; }
 };
 
+// v of another lane by a data-parallel move, which costs a vector operation where a general
+// shuffle goes through LDS; lanes that are given none get 0.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float moved(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E;                // lane ^ 1, lane ^ 2 (quad_perm)
+constexpr int kMirror8 = 0x141, kMirror16 = 0x140;         // reversed within 8, within 16 lanes
+constexpr int kUp = 0x110, kBcast15 = 0x142, kBcast31 = 0x143;  // row_shr:n, and the last lane of the rows before
+
+// v of the even and of the odd row of 16 lanes of this lane's half, and of the lower and the
+// upper half, at this lane's place in them.
+struct Pair {
+  float first, second;
+};
+__device__ __forceinline__ Pair rows_of_half(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const unsigned first = p[0], second = p[1];  // (a bit_cast of p[1] itself reads p[0])
+  return {__builtin_bit_cast(float, first), __builtin_bit_cast(float, second)};
+}
+__device__ __forceinline__ Pair halves(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned first = p[0], second = p[1];  // (a bit_cast of p[1] itself reads p[0])
+  return {__builtin_bit_cast(float, first), __builtin_bit_cast(float, second)};
+}
+
+// The sum over the lanes with this lane's place in their rows of 16.
+__device__ __forceinline__ float rows_sum(float v) {
+  Pair p = rows_of_half(v);
+  p = halves(p.first + p.second);
+  return p.first + p.second;
+}
+
 // The sum over N neighbouring lanes, in each of them.
 template <int N>
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int m = N / 2; m; m >>= 1) v += __shfl_xor(v, m, kWave);
+  if constexpr (N >= 2) v += moved<kSwap1>(v);
+  if constexpr (N >= 4) v += moved<kSwap2>(v);
+  if constexpr (N >= 8) v += moved<kMirror8>(v);  // the other four lanes, which are alike by now
+  if constexpr (N >= 16) v += moved<kMirror16>(v);
+  if constexpr (N == 64) return rows_sum(v);
+  if constexpr (N == 32) {
+    const Pair p = rows_of_half(v);
+    return p.first + p.second;
+  }
   return v;
 }
 __device__ __forceinline__ float wave_sum(float v) { return lanes_sum<kWave>(v); }

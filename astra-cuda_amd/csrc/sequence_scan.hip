@@ -24,11 +24,16 @@
 // nothing overflows where A <= 0; s is summed in 64 bits and kept as two floats, because a
 // difference of two long sums would otherwise lose the digits that a short one has.
 //
-// Types. x, B, C and dY enter the products as they are. What is computed in between (M, Q,
-// the states, and the weighted B and C of the states' update) is in 32 bits; for bf16 inputs it
-// enters a product as the sum of two bf16 values (16 bits of significand, an error of 4e-6
-// at most), so each such product is two matrix instructions. For float inputs the
-// products use the float matrix instructions, at 1/16 of the bf16 ones' rate.
+// Types. x, B, C and dY enter the products as they are; sums and states are in 32 bits. For
+// bf16 inputs, what is computed in between enters a product as
+//   - one bf16 value in the products whose result is rounded to bf16: M and Q, and the states
+//     in y and dX. That adds 1.1e-3 (rms, of its term) to the 1.7e-3 of the result's own
+//     rounding;
+//   - the sum of two (2^-18) in those that end in float gradients: the states in U = h0^T dY
+//     and V = dh1^T x, which d(dt A) takes;
+//   - the sum of three (2^-26) in those that end in float states: w B and exp(s) C.
+// For float inputs the products use the float matrix instructions, at 1/16 of the bf16
+// ones' rate.
 //
 // A chunk is handled by wavefronts that each own 16 of its positions. A product's result
 // has its column in lane % 16 and four consecutive rows in its registers, which is the
@@ -57,8 +62,10 @@ struct ScanArgs {
   float *dbc;       // [slices, 2, B, T, G, N]: parts of db and dc, where heads are split
   int64_t B, T;
   int64_t xsb, xst, xsh, dsb, dst, dsh, bsb, bst, bsg, csb, cst, csg;
-  int32_t H, P, G, N, ptiles, chunks, seg_chunks, segs, slices;
-  int32_t xv, bv, cv, yv, nv;  // whether 4 elements of a row can be accessed at once
+  int32_t H, P, G, N, ptiles, chunks, seg_chunks, segs;
+  int32_t parts;   // forward: workgroups that share a group's heads (and their tiles of P)
+  int32_t slices;  // backward: likewise
+  bool vec;  // 4 elements of every row can be accessed at once
 };
 
 // ---------------------------------------------------------------- operands of the products
@@ -87,12 +94,23 @@ struct Ops<bf16> {
     const bf16x4 b = *reinterpret_cast<const bf16x4 *>(row + k0 + 16 + 4 * q);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
-  static __device__ __forceinline__ Split split(const float (&v)[8]) {
-    Split s;
+  struct Split3 {
+    bf16x8 hi, mid, lo;
+  };
+  static __device__ __forceinline__ Frag round(const float (&v)[8]) {
+    Frag f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (bf16)v[i];
+    return f;
+  }
+  static __device__ __forceinline__ Split3 split3(const float (&v)[8]) {
+    Split3 s;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       s.hi[i] = (bf16)v[i];
-      s.lo[i] = (bf16)(v[i] - (float)s.hi[i]);
+      const float rest = v[i] - (float)s.hi[i];
+      s.mid[i] = (bf16)rest;
+      s.lo[i] = (bf16)(rest - (float)s.mid[i]);
     }
     return s;
   }
@@ -107,9 +125,10 @@ struct Ops<bf16> {
     mma(acc, a.lo, b);
     mma(acc, a.hi, b);
   }
-  static __device__ __forceinline__ void mma(f32x4 &acc, const Frag &a, const Split &b) {
-    mma(acc, a, b.lo);
-    mma(acc, a, b.hi);
+  static __device__ __forceinline__ void mma(f32x4 &acc, const Split3 &a, const Frag &b) {
+    mma(acc, a.lo, b);
+    mma(acc, a.mid, b);
+    mma(acc, a.hi, b);
   }
 };
 
@@ -117,6 +136,7 @@ template <>
 struct Ops<float> {
   using Frag = FragF;
   using Split = FragF;
+  using Split3 = FragF;
   static __device__ __forceinline__ Frag near(const float *row, int k0, int q) {
     Frag f;
     const f32x4 a = *reinterpret_cast<const f32x4 *>(row + k0 + 8 * q);
@@ -128,12 +148,13 @@ struct Ops<float> {
     }
     return f;
   }
-  static __device__ __forceinline__ Split split(const float (&v)[8]) {
-    Split s;
+  static __device__ __forceinline__ Frag round(const float (&v)[8]) {
+    Frag s;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s.v[i] = v[i];
     return s;
   }
+  static __device__ __forceinline__ Split3 split3(const float (&v)[8]) { return round(v); }
   static __device__ __forceinline__ void expand(const Frag &f, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = f.v[i];
@@ -142,6 +163,11 @@ struct Ops<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
   }
+};
+
+template <class T>
+struct V4 {
+  typedef T type __attribute__((ext_vector_type(4)));
 };
 
 // A tile of F features by Q positions in LDS, read along its features (`rows`: position
@@ -182,15 +208,15 @@ struct Along {  // operands contracted over positions
   }
 };
 
-// A state tile [R, K] (K contracted) in LDS: two bf16 parts, or floats.
-template <class T, int R, int K>
+// A state tile [R, K] (K contracted) in LDS: one bf16 part or two, or floats.
+template <class T, int R, int K, int PARTS>
 struct StateTile {
+  static constexpr bool kTwo = sizeof(T) == 2 && PARTS == 2;
   static constexpr int kRow = K + 16 / (int)sizeof(T);
-  static constexpr size_t kPart = R * kRow * sizeof(T);
-  static constexpr size_t kBytes = (sizeof(T) == 2 ? 2 : 1) * kPart;
+  static constexpr size_t kBytes = (kTwo ? 2 : 1) * R * kRow * sizeof(T);
   T *p;
-  __device__ __forceinline__ typename Ops<T>::Split near(int r, int k0, int q) const {
-    if constexpr (sizeof(T) == 2) {
+  __device__ __forceinline__ auto near(int r, int k0, int q) const {
+    if constexpr (kTwo) {
       typename Ops<T>::Split s;
       s.hi = Ops<T>::near(p + r * kRow, k0, q);
       s.lo = Ops<T>::near(p + R * kRow + r * kRow, k0, q);
@@ -200,43 +226,42 @@ struct StateTile {
     }
   }
   // contracted over the rows instead (floats only)
-  __device__ __forceinline__ typename Ops<T>::Split across(int k, int r0, int q) const {
+  __device__ __forceinline__ FragF across(int k, int r0, int q) const {
     FragF s;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s.v[i] = p[(r0 + 8 * q + i) * kRow + k];
     return s;
   }
   __device__ __forceinline__ void put4(int r, int k, const float (&v)[4]) const {
-    if constexpr (sizeof(T) == 2) {
-      bf16x4 hi, lo;
+    typename V4<T>::type hi, lo;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        hi[i] = (bf16)v[i];
-        lo[i] = (bf16)(v[i] - (float)hi[i]);
-      }
-      *reinterpret_cast<bf16x4 *>(p + r * kRow + k) = hi;
-      *reinterpret_cast<bf16x4 *>(p + R * kRow + r * kRow + k) = lo;
-    } else {
-      f32x4 f;
+    for (int i = 0; i < 4; ++i) {
+      hi[i] = (T)v[i];
+      if constexpr (kTwo) lo[i] = (T)(v[i] - (float)hi[i]);
+    }
+    *reinterpret_cast<typename V4<T>::type *>(p + r * kRow + k) = hi;
+    if constexpr (kTwo) *reinterpret_cast<typename V4<T>::type *>(p + R * kRow + r * kRow + k) = lo;
+  }
+  // the 8 values from element i on, as floats
+  __device__ __forceinline__ void get8(int r, int k, float (&v)[8]) const {
+    Ops<T>::expand(Ops<T>::near(p + r * kRow, k, 0), v);
+    if constexpr (kTwo) {
+      float lo[8];
+      Ops<T>::expand(Ops<T>::near(p + R * kRow + r * kRow, k, 0), lo);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = v[i];
-      *reinterpret_cast<f32x4 *>(p + r * kRow + k) = f;
+      for (int i = 0; i < 8; ++i) v[i] += lo[i];
     }
   }
 };
 
 // ---------------------------------------------------------------------- global memory
 
-template <class T>
-struct V4 {
-  typedef T type __attribute__((ext_vector_type(4)));
-};
-
-// 4 elements of a row from element f on, zeros from `n` on.
-template <class T>
-__device__ __forceinline__ typename V4<T>::type load4(const T *p, int f, int n, bool vec) {
+// 4 elements of a row from element f on, zeros from `n` on. VEC: n, the rows' strides and
+// their addresses allow one access of all four.
+template <bool VEC, class T>
+__device__ __forceinline__ typename V4<T>::type load4(const T *p, int f, int n) {
   typename V4<T>::type r = {};
-  if (vec) {
+  if constexpr (VEC) {
     if (f < n) r = *reinterpret_cast<const typename V4<T>::type *>(p + f);
   } else {
 #pragma unroll
@@ -246,9 +271,9 @@ __device__ __forceinline__ typename V4<T>::type load4(const T *p, int f, int n, 
   return r;
 }
 
-template <class T>
-__device__ __forceinline__ void store4(T *p, int f, int n, bool vec, const float (&v)[4]) {
-  if (vec) {
+template <bool VEC, class T>
+__device__ __forceinline__ void store4(T *p, int f, int n, const float (&v)[4]) {
+  if constexpr (VEC) {
     typename V4<T>::type r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = (T)v[i];
@@ -263,11 +288,11 @@ __device__ __forceinline__ void store4(T *p, int f, int n, bool vec, const float
 // F features by Q positions on their way from memory to LDS: THREADS threads hold blocks of
 // 4 positions by 4 features. Positions at and after `len` and features at and after `n`
 // are zero, whatever memory holds there.
-template <class T, int F, int THREADS>
+template <class T, int F, int THREADS, bool VEC>
 struct Stage {
   static constexpr int kGroups = F / 4, kBlocks = kGroups * (Q / 4), kEach = (kBlocks + THREADS - 1) / THREADS;
   typename V4<T>::type v[kEach][4];
-  __device__ __forceinline__ void load(const T *base, int64_t stride, int64_t t0, int len, int n, bool vec, int tid) {
+  __device__ __forceinline__ void load(const T *base, int64_t stride, int64_t t0, int len, int n, int tid) {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int blk = tid + e * THREADS;
@@ -275,7 +300,7 @@ struct Stage {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         v[e][k] = {};
-        if (blk < kBlocks && t0 + t + k < len) v[e][k] = load4<T>(base + (t0 + t + k) * stride, f, n, vec);
+        if (blk < kBlocks && t0 + t + k < len) v[e][k] = load4<VEC>(base + (t0 + t + k) * stride, f, n);
       }
     }
   }
@@ -310,7 +335,9 @@ struct Times {
   float dt[Q], hi[Q], lo[Q];  // the step; log2 of the decay from the chunk's start, in two parts
   float from[Q], left[Q];     // exp(s_t), exp(s_Q - s_t)
   float into[Q];              // dt exp(s_Q - s_t): what a position's input counts after the chunk
+  float slope[Q];             // the step's derivative by dt_raw, 0 where no position counts
   float total;                // exp(s_Q)
+  float pad[3];
 };
 
 __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
@@ -321,43 +348,67 @@ __device__ __forceinline__ float raw_step(const ScanArgs &a, int64_t b, int h, i
   return (float)((const T *)a.dt)[b * a.dsb + t * a.dst + h * a.dsh] + (a.bias ? a.bias[h] : 0.f);
 }
 
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double moved64(double v) {
+  const int64_t i = __builtin_bit_cast(int64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)i, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(i >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
 // Fills `o` from this lane's raw step; returns log2 of the chunk's decay.
 __device__ __forceinline__ double make_times(Times &o, float raw, bool live, float A, int lane) {
   const float dt = live ? softplus(raw) : 0.f;
   double s = (double)dt * (double)A * 1.4426950408889634;
-#pragma unroll
-  for (int m = 1; m < Q; m *= 2) {
-    const double up = __shfl_up(s, m, kWave);
-    if (lane >= m) s += up;
-  }
-  const double total = __shfl(s, Q - 1, kWave);
+  s += moved64<kUp + 1>(s);
+  s += moved64<kUp + 2>(s);
+  s += moved64<kUp + 4>(s);
+  s += moved64<kUp + 8>(s);
+  s += moved64<kBcast15, 0xa>(s);
+  s += moved64<kBcast31, 0xc>(s);
+  const int64_t last = __builtin_bit_cast(int64_t, s);
+  const uint32_t tl = (uint32_t)__builtin_amdgcn_readlane((int)last, Q - 1);
+  const uint32_t th = (uint32_t)__builtin_amdgcn_readlane((int)(last >> 32), Q - 1);
+  const double total = __builtin_bit_cast(double, ((uint64_t)th << 32) | tl);
+  const float left = __builtin_amdgcn_exp2f((float)(total - s));
   o.dt[lane] = dt;
   o.hi[lane] = (float)s;
   o.lo[lane] = (float)(s - (double)(float)s);
-  o.from[lane] = exp2f((float)s);
-  o.left[lane] = exp2f((float)(total - s));
-  o.into[lane] = dt * o.left[lane];
-  if (lane == 0) o.total = exp2f((float)total);
+  o.from[lane] = __builtin_amdgcn_exp2f((float)s);
+  o.left[lane] = left;
+  o.into[lane] = dt * left;
+  o.slope[lane] = live ? sigmoid(raw) : 0.f;
+  if (lane == 0) o.total = __builtin_amdgcn_exp2f((float)total);
   return total;
+}
+
+// Workgroups go to the eight XCDs in turn: neighbours in this order share an XCD, and with it
+// the L2 that holds the B and C that they share.
+__device__ __forceinline__ int64_t workgroup_id() {
+  const unsigned n = gridDim.x, id = blockIdx.x;
+  return n % 8 ? id : (id % 8) * (n / 8) + id / 8;
 }
 
 // --------------------------------------------------------- the states' update over a chunk
 
-// This wavefront's part of a state [PT, NT] in registers: 16 x 16 tiles wave, wave + 4, ...
-// of [n tile, p tile]; lane (q, r) of tile (nt, pt) has n = 16 nt + 4 q + 0..3, p = 16 pt + r.
-template <int PT, int NT>
+// A wavefront's part of a state [PT, NT] in registers, WAVES of them sharing it: 16 x 16 tiles
+// wave, wave + WAVES, ... of [p tile, n tile]; lane (q, r) of tile (pt, nt) has
+// n = 16 nt + 4 q + 0..3 and p = 16 pt + r.
+template <int PT, int NT, int WAVES>
 struct Mine {
-  static constexpr int kN = NT / 16, kTiles = (PT / 16) * kN, kEach = kTiles / 4;
-  static_assert(kTiles % 4 == 0, "four wavefronts share the tiles evenly");
-  static __device__ __forceinline__ int n_of(int wave, int i, int q) { return ((wave + 4 * i) % kN) * 16 + 4 * q; }
-  static __device__ __forceinline__ int p_of(int wave, int i, int r) { return ((wave + 4 * i) / kN) * 16 + r; }
+  static constexpr int kN = NT / 16, kTiles = (PT / 16) * kN, kEach = kTiles / WAVES;
+  static constexpr bool kOneN = WAVES % kN == 0;  // one tile of n for all of a wavefront's tiles
+  static_assert(kTiles % WAVES == 0, "the wavefronts share the tiles evenly");
+  static __device__ __forceinline__ int nt_of(int wave, int i) { return (wave + WAVES * i) % kN; }
+  static __device__ __forceinline__ int n_of(int wave, int i, int q) { return nt_of(wave, i) * 16 + 4 * q; }
+  static __device__ __forceinline__ int p_of(int wave, int i, int r) { return ((wave + WAVES * i) / kN) * 16 + r; }
 };
 
 // S = total S + X^T (weight K): X over PT features, K over NT, weight a position's.
-template <class T, int PT, int NT>
-__device__ __forceinline__ void update_state(f32x4 *S, float total, const float *weight,
-                                             const Along<T, PT> &X, const Along<T, NT> &K, int wave, int q, int r) {
-  using M = Mine<PT, NT>;
+template <class T, int PT, int NT, int WAVES>
+__device__ __forceinline__ void update_state(f32x4 *S, float total, const float *weight, const Along<T, PT> &X,
+                                             const Along<T, NT> &K, int wave, int q, int r) {
+  using M = Mine<PT, NT, WAVES>;
 #pragma unroll
   for (int i = 0; i < M::kEach; ++i) S[i] *= total;
 #pragma unroll
@@ -365,172 +416,216 @@ __device__ __forceinline__ void update_state(f32x4 *S, float total, const float 
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = weight[t0 + 8 * q + e];
-    typename Ops<T>::Split kf;
+    typename Ops<T>::Split3 kf;
 #pragma unroll
     for (int i = 0; i < M::kEach; ++i) {
-      const int nt = (wave + 4 * i) % M::kN;
-      if (i == 0 || M::kN > 4) {  // with up to 4 tiles of n a wavefront has only one of them
+      if (i == 0 || !M::kOneN) {
         float v[8];
-        Ops<T>::expand(K.near(16 * nt + r, t0, q), v);
+        Ops<T>::expand(K.near(16 * M::nt_of(wave, i) + r, t0, q), v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= w[e];
-        kf = Ops<T>::split(v);
+        kf = Ops<T>::split3(v);
       }
       Ops<T>::mma(S[i], kf, X.near(M::p_of(wave, i, r), t0, q));
     }
   }
 }
 
-template <int PT, int NT>
-__device__ __forceinline__ void load_state(f32x4 *S, const float *base, const ScanArgs &a, int p0,
-                                           int wave, int q, int r) {
-  using M = Mine<PT, NT>;
+template <int PT, int NT, int WAVES, bool VEC>
+__device__ __forceinline__ void load_state(f32x4 *S, const float *base, const ScanArgs &a, int p0, int wave, int q, int r) {
+  using M = Mine<PT, NT, WAVES>;
 #pragma unroll
   for (int i = 0; i < M::kEach; ++i) {
     const int p = p0 + M::p_of(wave, i, r), n = M::n_of(wave, i, q);
     S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (base && p < a.P) S[i] = load4<float>(base + (int64_t)p * a.N, n, a.N, a.nv);
+    if (base && p < a.P) S[i] = load4<VEC>(base + (int64_t)p * a.N, n, a.N);
   }
 }
 
-template <int PT, int NT>
-__device__ __forceinline__ void store_state(const f32x4 *S, float *base, const ScanArgs &a, int p0,
-                                            int wave, int q, int r) {
-  using M = Mine<PT, NT>;
+template <int PT, int NT, int WAVES, bool VEC>
+__device__ __forceinline__ void store_state(const f32x4 *S, float *base, const ScanArgs &a, int p0, int wave, int q, int r) {
+  using M = Mine<PT, NT, WAVES>;
 #pragma unroll
   for (int i = 0; i < M::kEach; ++i) {
     const int p = p0 + M::p_of(wave, i, r), n = M::n_of(wave, i, q);
     const float v[4] = {S[i][0], S[i][1], S[i][2], S[i][3]};
-    if (p < a.P) store4<float>(base + (int64_t)p * a.N, n, a.N, a.nv, v);
+    if (p < a.P) store4<VEC>(base + (int64_t)p * a.N, n, a.N, v);
   }
 }
 
 // ------------------------------------------------------------------------ forward
 
-template <class T, int PT, int NT>
+template <class T, int PT, int NT, bool ST>
 struct ForwardLds {
   static constexpr size_t x = 0;  // along positions only
   static constexpr size_t bn = x + (sizeof(T) == 2 ? Tile<T, PT>::kColsBytes : Tile<T, PT>::kRowsBytes);
   static constexpr size_t bt = bn + Tile<T, NT>::kRowsBytes;
   static constexpr size_t cn = bt + Tile<T, NT>::kColsBytes;
   static constexpr size_t h = cn + Tile<T, NT>::kRowsBytes;
-  static constexpr size_t times = h + StateTile<T, PT, NT>::kBytes;
-  static constexpr size_t bytes = times + sizeof(Times);
+  static constexpr size_t times = h + (ST ? StateTile<T, PT, NT, 1>::kBytes : 0);
+  static constexpr size_t bytes = times + 2 * sizeof(Times);
 };
 
-// One workgroup of four wavefronts: a head's PT features over a segment of chunks, one
-// after the other, the state in registers between them.
-template <class T, int PT, int NT>
-__global__ __launch_bounds__(256) void scan_forward_kernel(ScanArgs a) {
-  using L = ForwardLds<T, PT, NT>;
-  using M = Mine<PT, NT>;
+// A workgroup of 4 PW wavefronts: a segment of chunks of one row, for some of a group's heads
+// (and tiles of PT features) in turn. Wavefront w has positions 16 (w % 4) + 0..15 and the
+// (w / 4)th part of the features. While an item (a head's chunk) is computed, the next one's
+// inputs are on their way to registers, and the first wavefront, which has the fewest pairs
+// of positions, works out its step sizes. Where the segment is a single chunk, B, C and their
+// scores are loaded and computed once for all heads. ST: whether there are states before a chunk.
+template <class T, int PT, int NT, int PW, bool ST, bool VEC>
+__global__ __launch_bounds__(256 * PW, PW == 1 ? 3 : 2) void scan_forward_kernel(ScanArgs a) {
+  using L = ForwardLds<T, PT, NT, ST>;
+  constexpr int kThreads = 256 * PW, kWaves = 4 * PW, PP = PT / PW;
+  using M = Mine<PT, NT, kWaves>;
   extern __shared__ __align__(16) char lds[];
   T *xl = (T *)(lds + L::x), *bn = (T *)(lds + L::bn), *bt = (T *)(lds + L::bt), *cn = (T *)(lds + L::cn);
-  const StateTile<T, PT, NT> hl{(T *)(lds + L::h)};
-  Times &tm = *(Times *)(lds + L::times);
+  const StateTile<T, PT, NT, 1> hl{(T *)(lds + L::h)};
+  Times *times = (Times *)(lds + L::times);
   const Along<T, PT> xa{xl, xl};
   const Along<T, NT> ba{bn, bt};
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, r = lane & 15;
-  int64_t id = blockIdx.x;
-  const int pt = (int)(id % a.ptiles);
-  id /= a.ptiles;
-  const int h = (int)(id % a.H);
-  id /= a.H;
-  const int64_t b = id % a.B;
-  const int seg = (int)(id / a.B);
-  const int g = h / (a.H / a.G), p0 = pt * PT, len = row_length(a.lengths, b, a.T);
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave & 3, f0 = (wave >> 2) * PP;
+  int64_t id = workgroup_id();
+  const int per = a.H / a.G, heads = per * a.ptiles;  // a group's heads and tiles of features
+  const int part = (int)(id % a.parts);
+  id /= a.parts;
+  const int g = (int)(id % a.G);
+  id /= a.G;
+  const int seg = (int)(id % a.segs);
+  const int64_t b = id / a.segs;
+  const int len = row_length(a.lengths, b, a.T);
   const int c0 = seg * a.seg_chunks, c1 = min(c0 + a.seg_chunks, a.chunks);
-  const float A = a.A[h], D = a.D ? a.D[h] : 0.f;
-  const T *xg = (const T *)a.x + b * a.xsb + h * a.xsh + p0;
+  const int last = (int)((int64_t)heads * (part + 1) / a.parts);
+  const int64_t pn = (int64_t)a.P * a.N;
   const T *bg = (const T *)a.b + b * a.bsb + g * a.bsg;
   const T *cg = (const T *)a.c + b * a.csb + g * a.csg;
-  const int64_t bh = b * a.H + h, pn = (int64_t)a.P * a.N;
 
-  f32x4 S[M::kEach];
-  const float *start = a.segs > 1 ? a.seg + (bh * a.segs + seg) * pn : a.initial ? a.initial + bh * pn : nullptr;
-  load_state<PT, NT>(S, start, a, p0, wave, q, r);
-  bool any = start != nullptr;  // whether the state is more than zeros
-
-  Stage<T, PT, 256> xs;
-  Stage<T, NT, 256> bs, cs;
-  for (int c = c0; c < c1; ++c) {
+  Stage<T, PT, kThreads, VEC> xs;
+  Stage<T, NT, kThreads, VEC> bs, cs;
+  float raw = 0.f;
+  int hp = (int)((int64_t)heads * part / a.parts), c = c0;  // the item that is loaded next
+  auto load = [&](bool with_bc) __attribute__((always_inline)) {
+    const int h = g * per + hp / a.ptiles, p0 = (hp % a.ptiles) * PT;
     const int64_t t0 = (int64_t)c * Q;
-    xs.load(xg, a.xst, t0, len, a.P - p0, a.xv, tid);
-    bs.load(bg, a.bst, t0, len, a.N, a.bv, tid);
-    cs.load(cg, a.cst, t0, len, a.N, a.cv, tid);
+    xs.load((const T *)a.x + b * a.xsb + h * a.xsh + p0, a.xst, t0, len, a.P - p0, tid);
+    if (with_bc) {
+      bs.load(bg, a.bst, t0, len, a.N, tid);
+      cs.load(cg, a.cst, t0, len, a.N, tid);
+    }
+    if (wave == 0) raw = raw_step<T>(a, b, h, t0 + lane, len);
+  };
+  if (hp >= last) return;
+  load(true);
+  if (wave == 0) make_times(times[0], raw, (int64_t)c * Q + lane < len, a.A[g * per + hp / a.ptiles], lane);
+
+  f32x4 S[M::kEach], sc[4];
+  bool fresh = true, any = false;
+  for (int k = 0;; ++k) {
+    const int h = g * per + hp / a.ptiles, p0 = (hp % a.ptiles) * PT;
+    const int64_t t0 = (int64_t)c * Q, bh = b * a.H + h;
+    const int cc = c;
+    const bool new_bc = fresh || c1 - c0 > 1;
+    const Times &tm = times[k & 1];
+    if (c == c0) {
+      const float *start = !ST ? nullptr : a.segs > 1 ? a.seg + (bh * a.segs + seg) * pn : a.initial ? a.initial + bh * pn : nullptr;
+      load_state<PT, NT, kWaves, VEC>(S, start, a, p0, wave, q, r);
+      any = start != nullptr;
+    }
+    if (k) __syncthreads();  // nobody reads the last item's tiles any more
     if constexpr (sizeof(T) == 2)
       xs.put(nullptr, xl, tid);
     else
       xs.put(xl, nullptr, tid);
-    bs.put(bn, bt, tid);
-    cs.put(cn, nullptr, tid);
-    if (wave == 0) make_times(tm, raw_step<T>(a, b, h, t0 + lane, len), t0 + lane < len, A, lane);
-    if (any) {
-#pragma unroll
-      for (int i = 0; i < M::kEach; ++i) {
-        const float v[4] = {S[i][0], S[i][1], S[i][2], S[i][3]};
-        hl.put4(M::p_of(wave, i, r), M::n_of(wave, i, q), v);
-      }
+    if (new_bc) {
+      bs.put(bn, bt, tid);
+      cs.put(cn, nullptr, tid);
     }
-    if (a.cs) store_state<PT, NT>(S, a.cs + (bh * a.chunks + c) * pn, a, p0, wave, q, r);
+    if constexpr (ST) {
+      if (any) {
+#pragma unroll
+        for (int i = 0; i < M::kEach; ++i) {
+          const float v[4] = {S[i][0], S[i][1], S[i][2], S[i][3]};
+          hl.put4(M::p_of(wave, i, r), M::n_of(wave, i, q), v);
+        }
+      }
+      if (a.cs) store_state<PT, NT, kWaves, VEC>(S, a.cs + (bh * a.chunks + c) * pn, a, p0, wave, q, r);
+    }
     __syncthreads();
+    if (++c == c1) {
+      c = c0;
+      ++hp;
+    }
+    const bool more = hp < last;
+    if (more) load(c1 - c0 > 1);
 
-    // this wavefront's 16 positions i = 16 wave + r: Y^T, rows the features
-    f32x4 y[PT / 16];
+    // this wavefront's 16 positions i = 16 wi + r: Y^T, rows the features
+    f32x4 y[PP / 16];
 #pragma unroll
-    for (int i = 0; i < PT / 16; ++i) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int ti = 16 * wave + r;
-    typename Ops<T>::Frag cf[NT / 32];
+    for (int i = 0; i < PP / 16; ++i) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int ti = 16 * wi + r;
+    if (new_bc || (ST && any)) {
+      typename Ops<T>::Frag cf[NT / 32];
 #pragma unroll
-    for (int k = 0; k < NT / 32; ++k) cf[k] = Ops<T>::near(cn + ti * Tile<T, NT>::kRow, 32 * k, q);
-    if (any) {
-      const float e = tm.from[ti];
+      for (int n = 0; n < NT / 32; ++n) cf[n] = Ops<T>::near(cn + ti * Tile<T, NT>::kRow, 32 * n, q);
+      if (new_bc) {
 #pragma unroll
-      for (int i = 0; i < PT / 16; ++i) {
+        for (int jt = 0; jt < 4; ++jt) {
+          sc[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (jt <= wi)
 #pragma unroll
-        for (int k = 0; k < NT / 32; ++k) Ops<T>::mma(y[i], hl.near(16 * i + r, 32 * k, q), cf[k]);
-        y[i] *= e;
+            for (int n = 0; n < NT / 32; ++n)
+              Ops<T>::mma(sc[jt], Ops<T>::near(bn + (16 * jt + r) * Tile<T, NT>::kRow, 32 * n, q), cf[n]);
+        }
+        fresh = false;
+      }
+      if constexpr (ST) {
+        if (any) {
+          const float e = tm.from[ti];
+#pragma unroll
+          for (int i = 0; i < PP / 16; ++i) {
+#pragma unroll
+            for (int n = 0; n < NT / 32; ++n) Ops<T>::mma(y[i], hl.near(f0 + 16 * i + r, 32 * n, q), cf[n]);
+            y[i] *= e;
+          }
+        }
       }
     }
-    const float hi = tm.hi[ti], lo = tm.lo[ti];
+    const float hi = tm.hi[ti], lo = tm.lo[ti], D = a.D ? a.D[h] : 0.f;
 #pragma unroll
     for (int jp = 0; jp < 2; ++jp) {  // two tiles of 16 positions j at a time
-      if (2 * jp > wave) break;
+      if (2 * jp > wi) break;
       float m[8];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int jt = 2 * jp + half;
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
-        if (jt <= wave) {
-#pragma unroll
-          for (int k = 0; k < NT / 32; ++k)
-            Ops<T>::mma(s, Ops<T>::near(bn + (16 * jt + r) * Tile<T, NT>::kRow, 32 * k, q), cf[k]);
-        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int tj = 16 * jt + 4 * q + e;
           const float f = __builtin_amdgcn_exp2f((hi - tm.hi[tj]) + (lo - tm.lo[tj])) * tm.dt[tj];
-          m[4 * half + e] = (tj <= ti ? s[e] * f : 0.f) + (tj == ti ? D : 0.f);
+          m[4 * half + e] = (tj <= ti ? sc[jt][e] * f : 0.f) + (tj == ti ? D : 0.f);
         }
       }
-      const typename Ops<T>::Split mf = Ops<T>::split(m);
+      const typename Ops<T>::Frag mf = Ops<T>::round(m);
 #pragma unroll
-      for (int i = 0; i < PT / 16; ++i) Ops<T>::mma(y[i], xa.far(16 * i + r, 32 * jp, q), mf);
+      for (int i = 0; i < PP / 16; ++i) Ops<T>::mma(y[i], xa.far(f0 + 16 * i + r, 32 * jp, q), mf);
     }
     if (t0 + ti < a.T) {
       T *yp = (T *)a.y + ((b * a.T + t0 + ti) * a.H + h) * a.P + p0;
 #pragma unroll
-      for (int i = 0; i < PT / 16; ++i) {
+      for (int i = 0; i < PP / 16; ++i) {
         const float v[4] = {y[i][0], y[i][1], y[i][2], y[i][3]};
-        store4<T>(yp, 16 * i + 4 * q, a.P - p0, a.yv, v);
+        store4<VEC>(yp, f0 + 16 * i + 4 * q, a.P - p0, v);
       }
     }
-    if (c + 1 < c1 || a.final_state) update_state<T, PT, NT>(S, tm.total, tm.into, xa, ba, wave, q, r);
-    any = true;
-    __syncthreads();
+    if (cc + 1 < c1 || a.final_state) {
+      update_state<T, PT, NT, kWaves>(S, tm.total, tm.into, xa, ba, wave, q, r);
+      any = true;
+      if (a.final_state && cc + 1 == a.chunks) store_state<PT, NT, kWaves, VEC>(S, a.final_state + bh * pn, a, p0, wave, q, r);
+    }
+    if (!more) break;
+    if (wave == 0) make_times(times[(k + 1) & 1], raw, (int64_t)c * Q + lane < len, a.A[g * per + hp / a.ptiles], lane);
   }
-  if (a.final_state && c1 == a.chunks) store_state<PT, NT>(S, a.final_state + bh * pn, a, p0, wave, q, r);
 }
 
 // ----------------------------------------------------------------- states of segments
@@ -540,30 +635,33 @@ struct StatesLds {
   static constexpr size_t x = 0;
   static constexpr size_t k = x + (sizeof(T) == 2 ? Tile<T, PT>::kColsBytes : Tile<T, PT>::kRowsBytes);
   static constexpr size_t times = k + (sizeof(T) == 2 ? Tile<T, NT>::kColsBytes : Tile<T, NT>::kRowsBytes);
-  static constexpr size_t bytes = times + sizeof(Times);
+  static constexpr size_t bytes = times + 2 * sizeof(Times);
 };
 
-// A segment's chunks without their outputs. Forwards: the state that the segment's inputs
-// leave (x, w B). Backwards (REV): the gradient of the state before it that its outputs
-// leave (dY, exp(s) C). KEEP: from what the segment starts from, writing what comes into
-// each chunk (ds); otherwise from zero, writing what comes out and the segment's decay.
-template <class T, int PT, int NT, bool REV, bool KEEP>
-__global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a) {
+// A segment's chunks of one head and PT features without their outputs. Forwards: the state
+// that the segment's inputs leave (x, w B). Backwards (REV): the gradient of the state before
+// it that its outputs leave (dY, exp(s) C). KEEP: from what the segment starts from, writing
+// what comes into each chunk (ds); otherwise from zero, writing what comes out and the
+// segment's decay. Pipelined like the forward kernel.
+template <class T, int PT, int NT, int PW, bool REV, bool KEEP, bool VEC>
+__global__ __launch_bounds__(256 * PW, PW == 1 ? 3 : 2) void scan_states_kernel(ScanArgs a) {
   using L = StatesLds<T, PT, NT>;
-  using M = Mine<PT, NT>;
+  constexpr int kThreads = 256 * PW, kWaves = 4 * PW;
+  using M = Mine<PT, NT, kWaves>;
   extern __shared__ __align__(16) char lds[];
   T *xl = (T *)(lds + L::x), *kl = (T *)(lds + L::k);
-  Times &tm = *(Times *)(lds + L::times);
+  Times *times = (Times *)(lds + L::times);
   const Along<T, PT> xa{xl, xl};
   const Along<T, NT> ka{kl, kl};
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, r = lane & 15;
-  int64_t id = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t id = workgroup_id();
   const int pt = (int)(id % a.ptiles);
   id /= a.ptiles;
   const int h = (int)(id % a.H);
   id /= a.H;
-  const int64_t b = id % a.B;
-  const int seg = (int)(id / a.B);
+  const int seg = (int)(id % a.segs);
+  const int64_t b = id / a.segs;
   const int g = h / (a.H / a.G), p0 = pt * PT, len = row_length(a.lengths, b, a.T);
   const int c0 = seg * a.seg_chunks, c1 = min(c0 + a.seg_chunks, a.chunks);
   const float A = a.A[h];
@@ -572,21 +670,32 @@ __global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a) {
   const T *kg = REV ? (const T *)a.c + b * a.csb + g * a.csg : (const T *)a.b + b * a.bsb + g * a.bsg;
   const int64_t kstride = REV ? a.cst : a.bst;
   const int64_t bh = b * a.H + h, pn = (int64_t)a.P * a.N;
+  // the last chunk that is walked: backwards, what comes out of the first one is not always wanted
+  const int n_chunks = c1 - c0 - (REV && KEEP && c0 == 0 && !a.dinitial ? 1 : 0);
   f32x4 S[M::kEach];
   const float *start = !KEEP ? nullptr : a.segs > 1 ? a.seg + (bh * a.segs + seg) * pn : a.dfinal ? a.dfinal + bh * pn : nullptr;
-  load_state<PT, NT>(S, start, a, p0, wave, q, r);
+  load_state<PT, NT, kWaves, VEC>(S, start, a, p0, wave, q, r);
   double decay = 0.;
-  Stage<T, PT, 256> xs;
-  Stage<T, NT, 256> ks;
-  for (int n = c0; n < c1; ++n) {
-    const int c = REV ? c1 - 1 - (n - c0) : n;
-    const int64_t t0 = (int64_t)c * Q;
-    if (KEEP) {
-      if (a.chunks > 1) store_state<PT, NT>(S, a.ds + (bh * a.chunks + c) * pn, a, p0, wave, q, r);
-      if (c == 0 && !a.dinitial) break;
-    }
-    xs.load(xg, xstride, t0, len, a.P - p0, REV ? a.yv : a.xv, tid);
-    ks.load(kg, kstride, t0, len, a.N, REV ? a.cv : a.bv, tid);
+  float raw = 0.f;
+  Stage<T, PT, kThreads, VEC> xs;
+  Stage<T, NT, kThreads, VEC> ks;
+  auto chunk_of = [&](int n) __attribute__((always_inline)) { return REV ? c1 - 1 - n : c0 + n; };
+  auto load = [&](int n) __attribute__((always_inline)) {
+    const int64_t t0 = (int64_t)chunk_of(n) * Q;
+    xs.load(xg, xstride, t0, len, a.P - p0, tid);
+    ks.load(kg, kstride, t0, len, a.N, tid);
+    if (wave == 0) raw = raw_step<T>(a, b, h, t0 + lane, len);
+  };
+  auto step = [&](int n) __attribute__((always_inline)) {
+    decay += make_times(times[n & 1], raw, (int64_t)chunk_of(n) * Q + lane < len, A, lane);
+  };
+  if (n_chunks > 0) {
+    load(0);
+    if (wave == 0) step(0);
+  }
+  for (int n = 0; n < n_chunks; ++n) {
+    const Times &tm = times[n & 1];
+    if (n) __syncthreads();
     if constexpr (sizeof(T) == 2) {
       xs.put(nullptr, xl, tid);
       ks.put(nullptr, kl, tid);
@@ -594,16 +703,20 @@ __global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a) {
       xs.put(xl, nullptr, tid);
       ks.put(kl, nullptr, tid);
     }
-    if (wave == 0) decay += make_times(tm, raw_step<T>(a, b, h, t0 + lane, len), t0 + lane < len, A, lane);
     __syncthreads();
-    update_state<T, PT, NT>(S, tm.total, REV ? tm.from : tm.into, xa, ka, wave, q, r);
-    __syncthreads();
+    if (n + 1 < n_chunks) load(n + 1);
+    if (KEEP && a.chunks > 1) store_state<PT, NT, kWaves, VEC>(S, a.ds + (bh * a.chunks + chunk_of(n)) * pn, a, p0, wave, q, r);
+    update_state<T, PT, NT, kWaves>(S, tm.total, REV ? tm.from : tm.into, xa, ka, wave, q, r);
+    if (wave == 0 && n + 1 < n_chunks) step(n + 1);
   }
   if (!KEEP) {
-    store_state<PT, NT>(S, a.seg + (bh * a.segs + seg) * pn, a, p0, wave, q, r);
+    store_state<PT, NT, kWaves, VEC>(S, a.seg + (bh * a.segs + seg) * pn, a, p0, wave, q, r);
     if (tid == 0 && pt == 0) a.seg_log2[bh * a.segs + seg] = (float)decay;
-  } else if (a.dinitial && c0 == 0) {
-    store_state<PT, NT>(S, a.dinitial + bh * pn, a, p0, wave, q, r);
+  } else if (c0 == 0) {
+    if (a.dinitial)
+      store_state<PT, NT, kWaves, VEC>(S, a.dinitial + bh * pn, a, p0, wave, q, r);
+    else if (a.chunks > 1)
+      store_state<PT, NT, kWaves, VEC>(S, a.ds + bh * a.chunks * pn, a, p0, wave, q, r);
   }
 }
 
@@ -626,6 +739,16 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(ScanArgs a) {
 
 // ----------------------------------------------------------------------- backward
 
+// What the wavefronts of the backward kernel leave of a head for its gradient of dt.
+struct HeadSums {
+  float uc[Q];        // exp(s_i) C_i . (h0^T dY_i)
+  float vb[Q];        // exp(s_Q - s_j) B_j . (dh1^T x_j)
+  float col[Q];       // sum over i >= j of the pairs (i, j), without dt_j
+  float cross[4][Q];  // sum of the pairs (i, j) with j < t <= i, over the j of each wavefront
+  float dot[8], diag[4];  // parts of <dh1, h0>, and of the sum of dY x
+  float pad[4];
+};
+
 template <class T, int PT, int NT, bool ST>
 struct GradLds {
   static constexpr bool two = sizeof(T) == 2;
@@ -637,19 +760,56 @@ struct GradLds {
   static constexpr size_t yn = xn + Tile<T, PT>::kRowsBytes;
   static constexpr size_t yt = yn + Tile<T, PT>::kRowsBytes;
   static constexpr size_t dh = yt + Tile<T, PT>::kColsBytes;                               // [p][n]
-  static constexpr size_t dht = dh + (ST ? StateTile<T, PT, NT>::kBytes : 0);              // [n][p]
-  static constexpr size_t h0 = dht + (ST && two ? StateTile<T, NT, PT>::kBytes : 0);       // [n][p], floats [p][n]
-  static constexpr size_t times = h0 + (!ST ? 0 : two ? StateTile<T, NT, PT>::kBytes : StateTile<T, PT, NT>::kBytes);
-  static constexpr size_t sums = times + sizeof(Times);
-  static constexpr size_t bytes = sums + (7 * Q + 2 * 8) * sizeof(float);
+  static constexpr size_t dht = dh + (ST ? StateTile<T, PT, NT, 1>::kBytes : 0);           // [n][p]
+  static constexpr size_t h0 = dht + (ST && two ? StateTile<T, NT, PT, 2>::kBytes : 0);    // [n][p], floats [p][n]
+  static constexpr size_t times = h0 + (!ST ? 0 : two ? StateTile<T, NT, PT, 2>::kBytes : StateTile<T, PT, NT, 1>::kBytes);
+  static constexpr size_t sums = times + 2 * sizeof(Times);
+  static constexpr size_t bytes = sums + 2 * sizeof(HeadSums);
+};
+
+// 4 x 4 blocks of a state [P, N] on their way from memory to LDS.
+template <int PT, int NT, int THREADS, bool VEC>
+struct StageState {
+  static constexpr int kBlocks = (PT / 4) * (NT / 4), kEach = (kBlocks + THREADS - 1) / THREADS;
+  f32x4 v[kEach][4];
+  __device__ __forceinline__ void load(const float *base, const ScanArgs &a, int p0, int tid) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int blk = tid + e * THREADS, n = (blk % (NT / 4)) * 4, p = (blk / (NT / 4)) * 4;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[e][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (base && blk < kBlocks && p0 + p + k < a.P)
+          v[e][k] = load4<VEC>(base + (int64_t)(p0 + p + k) * a.N, n, a.N);
+      }
+    }
+  }
+  template <class Rows, class Cols>
+  __device__ __forceinline__ void put(const Rows *rows, const Cols *cols, int tid) const {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int blk = tid + e * THREADS, n = (blk % (NT / 4)) * 4, p = (blk / (NT / 4)) * 4;
+      if (blk >= kBlocks) continue;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float along[4] = {v[e][k][0], v[e][k][1], v[e][k][2], v[e][k][3]};
+        const float across[4] = {v[e][0][k], v[e][1][k], v[e][2][k], v[e][3][k]};
+        if (rows) rows->put4(p + k, n, along);
+        if (cols) cols->put4(n + k, p, across);
+      }
+    }
+  }
 };
 
 // One workgroup of eight wavefronts: a chunk of one row and one group's B and C, its heads
-// one after the other, so that dB and dC are sums in registers. The first four wavefronts
-// own 16 positions j each (dX, dB), the other four 16 positions i each (dC). ST: whether
-// there are states before or after the chunk.
-template <class T, int PT, int NT, bool ST>
-__global__ __launch_bounds__(512) void scan_grad_kernel(ScanArgs a) {
+// (and their tiles of PT features) one after the other, so that dB and dC are sums in
+// registers. The first four wavefronts own 16 positions j each (dX, dB), the other four 16
+// positions i each (dC). While an item is computed the next one's inputs are on their way,
+// its step sizes are worked out by the wavefront of the first 16 i, and what the last head's
+// sums give for dt by the wavefront of the last 16 j: those have the fewest pairs. ST:
+// whether there are states before or after the chunk.
+template <class T, int PT, int NT, bool ST, bool VEC>
+__global__ __launch_bounds__(512, ST ? 2 : 4) void scan_grad_kernel(ScanArgs a) {
   using L = GradLds<T, PT, NT, ST>;
   using O = Ops<T>;
   using BC = Tile<T, NT>;
@@ -657,17 +817,17 @@ __global__ __launch_bounds__(512) void scan_grad_kernel(ScanArgs a) {
   extern __shared__ __align__(16) char lds[];
   T *bn = (T *)(lds + L::bn), *bt = (T *)(lds + L::bt), *cn = (T *)(lds + L::cn), *ct = (T *)(lds + L::ct);
   T *xn = (T *)(lds + L::xn), *yn = (T *)(lds + L::yn), *yt = (T *)(lds + L::yt);
-  const StateTile<T, PT, NT> dhl{(T *)(lds + L::dh)}, h0f{(T *)(lds + L::h0)};
-  const StateTile<T, NT, PT> dhtl{(T *)(lds + L::dht)}, h0l{(T *)(lds + L::h0)};
-  Times &tm = *(Times *)(lds + L::times);
-  // of a head: C.(h0^T dY) and B.(dh1^T x) with their decays, sum_i of the pairs (i, j), for
-  // each wavefront's j the pairs across a position, and two sums of each wavefront
-  float *uc = (float *)(lds + L::sums), *vb = uc + Q, *col = vb + Q, *cross = col + Q, *red = cross + 4 * Q;
+  const StateTile<T, PT, NT, 1> dhl{(T *)(lds + L::dh)}, h0f{(T *)(lds + L::h0)};
+  const StateTile<T, NT, PT, 2> dhtl{(T *)(lds + L::dht)}, h0l{(T *)(lds + L::h0)};
+  Times *times = (Times *)(lds + L::times);
+  HeadSums *sums = (HeadSums *)(lds + L::sums);
   const Along<T, NT> ba{bn, bt}, ca{cn, ct};
   const Along<T, PT> ya{yn, yt};
+  constexpr int kTimesWave = 4, kStepWave = 3;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, r = lane & 15;
-  int64_t id = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t id = workgroup_id();
   const int slice = (int)(id % a.slices);
   id /= a.slices;
   const int g = (int)(id % a.G);
@@ -680,274 +840,286 @@ __global__ __launch_bounds__(512) void scan_grad_kernel(ScanArgs a) {
   const int h_hi = g * per + (int)((int64_t)per * (slice + 1) / a.slices);
   const bool own_j = wave < 4;
   const int mine = wave & 3, tw = 16 * mine + r;  // this lane's position
+  const bool live = t0 + lane < len;
+
+  Stage<T, PT, 512, VEC> xs, ys;
+  StageState<PT, NT, 512, VEC> hs, ds;
+  float raw = 0.f;
+  const float *dh_next = nullptr, *h0_next = nullptr;
+  auto load = [&](int h, int pt) __attribute__((always_inline)) {
+    const int p0 = pt * PT;
+    const int64_t bh = b * a.H + h;
+    xs.load((const T *)a.x + b * a.xsb + h * a.xsh + p0, a.xst, t0, len, a.P - p0, tid);
+    ys.load((const T *)a.dy + (b * a.T * a.H + h) * a.P + p0, (int64_t)a.H * a.P, t0, len, a.P - p0, tid);
+    if constexpr (ST) {
+      h0_next = a.chunks > 1 ? a.cs + (bh * a.chunks + c) * pn : a.initial ? a.initial + bh * pn : nullptr;
+      dh_next = a.chunks > 1 ? a.ds + (bh * a.chunks + c) * pn : a.dfinal ? a.dfinal + bh * pn : nullptr;
+      hs.load(h0_next, a, p0, tid);
+      ds.load(dh_next, a, p0, tid);
+    }
+    if (pt == 0 && wave == kTimesWave) raw = raw_step<T>(a, b, h, t0 + lane, len);
+  };
+  // dt's gradient of head h from its sums, and the chunk's part of those of A, dt_bias and D
+  auto finish = [&](int h) __attribute__((always_inline)) {
+    const Times &tm = times[h & 1];
+    const HeadSums &s = sums[h & 1];
+    float dot = 0.f, diag = 0.f, cross = 0.f;
+    if constexpr (ST) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot += s.dot[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      diag += s.diag[i];
+      cross += 16 * i <= lane ? s.cross[i][lane] : 0.f;
+    }
+    const float dt = tm.dt[lane];
+    float before = 0.f, bdv = s.col[lane], after = 0.f;
+    if constexpr (ST) {
+      const float vb = s.vb[lane];
+      before = dt * vb;
+      bdv += vb;
+      after = s.uc[lane];
+#pragma unroll
+      for (int m = 1; m < Q; m *= 2) {
+        const float upper = __shfl_down(after, m, kWave);
+        if (lane + m < Q) after += upper;
+      }
+      before += moved<kUp + 1>(before);
+      before += moved<kUp + 2>(before);
+      before += moved<kUp + 4>(before);
+      before += moved<kUp + 8>(before);
+      before += moved<kBcast15, 0xa>(before);
+      before += moved<kBcast31, 0xc>(before);
+      before = __shfl_up(before, 1, kWave);
+      if (lane == 0) before = 0.f;
+    }
+    const float da = (before + after) + (cross + tm.total * dot);
+    const float ddt = (a.A[h] * da + bdv) * tm.slope[lane];
+    if (t0 + lane < a.T) ((T *)a.ddt)[(b * a.T + t0 + lane) * a.H + h] = (T)ddt;
+    const float dA = wave_sum(da * dt), dbias = wave_sum(ddt);
+    if (lane == 0) {
+      float *o = a.part + ((b * a.chunks + c) * a.H + h) * 3;
+      o[0] = dA;
+      o[1] = dbias;
+      o[2] = diag;
+    }
+  };
 
   {
-    Stage<T, NT, 512> s;
-    s.load((const T *)a.b + b * a.bsb + g * a.bsg, a.bst, t0, len, a.N, a.bv, tid);
+    Stage<T, NT, 512, VEC> s, u;
+    s.load((const T *)a.b + b * a.bsb + g * a.bsg, a.bst, t0, len, a.N, tid);
+    u.load((const T *)a.c + b * a.csb + g * a.csg, a.cst, t0, len, a.N, tid);
+    load(h_lo, 0);
     s.put(bn, bt, tid);
-    s.load((const T *)a.c + b * a.csb + g * a.csg, a.cst, t0, len, a.N, a.cv, tid);
-    s.put(cn, ct, tid);
+    u.put(cn, ct, tid);
   }
+  if (wave == kTimesWave) make_times(times[h_lo & 1], raw, live, a.A[h_lo], lane);
   f32x4 acc[NT / 16];  // dB^T (rows n, columns j), or dC^T, over the heads
 #pragma unroll
   for (int i = 0; i < NT / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float diag = 0.f, inter = 0.f, col = 0.f, dot = 0.f;
 
-  for (int h = h_lo; h < h_hi; ++h) {
-    const int64_t bh = b * a.H + h;
-    const float *h0 = !ST ? nullptr : a.chunks > 1 ? a.cs + (bh * a.chunks + c) * pn : a.initial ? a.initial + bh * pn : nullptr;
-    const float *dh = !ST ? nullptr : a.chunks > 1 ? a.ds + (bh * a.chunks + c) * pn : a.dfinal ? a.dfinal + bh * pn : nullptr;
-    const float A = a.A[h], D = a.D ? a.D[h] : 0.f;
-    const bool live = t0 + lane < len;
-    float raw = 0.f;
-    float dot = 0.f, diag = 0.f, inter = 0.f, cols = 0.f;
-    for (int pt = 0; pt < a.ptiles; ++pt) {
-      const int p0 = pt * PT;
-      if (pt == 0 && wave == 0) {
-        raw = raw_step<T>(a, b, h, t0 + lane, len);
-        make_times(tm, raw, live, A, lane);
-      }
-      {
-        Stage<T, PT, 512> s, u;
-        s.load((const T *)a.x + b * a.xsb + h * a.xsh + p0, a.xst, t0, len, a.P - p0, a.xv, tid);
-        u.load((const T *)a.dy + (b * a.T * a.H + h) * a.P + p0, (int64_t)a.H * a.P, t0, len, a.P - p0, a.yv, tid);
-        s.put(xn, nullptr, tid);
-        u.put(yn, yt, tid);
-      }
-      if constexpr (ST) {
-        constexpr int kBlocks = (PT / 4) * (NT / 4);
-        for (int blk = tid; blk < kBlocks; blk += 512) {
-          const int n = (blk % (NT / 4)) * 4, p = (blk / (NT / 4)) * 4;
-          float u[4][4], v[4][4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            f32x4 s = {0.f, 0.f, 0.f, 0.f}, w = s;
-            if (p0 + p + k < a.P) {
-              if (h0) s = load4<float>(h0 + (int64_t)(p0 + p + k) * a.N, n, a.N, a.nv);
-              if (dh) w = load4<float>(dh + (int64_t)(p0 + p + k) * a.N, n, a.N, a.nv);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              u[k][i] = s[i];
-              v[k][i] = w[i];
-              dot += s[i] * w[i];
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float ut[4] = {u[0][k], u[1][k], u[2][k], u[3][k]}, vt[4] = {v[0][k], v[1][k], v[2][k], v[3][k]};
-            dhl.put4(p + k, n, v[k]);
-            if constexpr (L::two) {
-              dhtl.put4(n + k, p, vt);
-              h0l.put4(n + k, p, ut);
-            } else {
-              h0f.put4(p + k, n, u[k]);
-            }
-          }
-        }
-      }
-      __syncthreads();
-
-      f32x4 own[NT / 16];  // this head's dB^T / dt or dC^T
-#pragma unroll
-      for (int i = 0; i < NT / 16; ++i) own[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const float hi = tm.hi[tw], lo = tm.lo[tw];
-      if (own_j) {
-        f32x4 dx[PT / 16];
-#pragma unroll
-        for (int i = 0; i < PT / 16; ++i) dx[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        typename O::Frag bf[NT / 32], xf[PT / 32];
-#pragma unroll
-        for (int k = 0; k < NT / 32; ++k) bf[k] = O::near(bn + tw * BC::kRow, 32 * k, q);
-#pragma unroll
-        for (int k = 0; k < PT / 32; ++k) xf[k] = O::near(xn + tw * XY::kRow, 32 * k, q);
-        const float left = tm.left[tw], dt = tm.dt[tw];
-        if (ST && dh) {
-#pragma unroll
-          for (int i = 0; i < PT / 16; ++i) {
-#pragma unroll
-            for (int k = 0; k < NT / 32; ++k) O::mma(dx[i], dhl.near(16 * i + r, 32 * k, q), bf[k]);
-            dx[i] *= left * dt;
-          }
-#pragma unroll
-          for (int i = 0; i < NT / 16; ++i) {
-#pragma unroll
-            for (int k = 0; k < PT / 32; ++k) {
-              if constexpr (L::two)
-                O::mma(own[i], dhtl.near(16 * i + r, 32 * k, q), xf[k]);
-              else
-                O::mma(own[i], dhl.across(16 * i + r, 32 * k, q), xf[k]);
-            }
-            own[i] *= left;
-          }
-#pragma unroll
-          for (int i = 0; i < NT / 16; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              inter += own[i][e] * (float)bn[tw * BC::kRow + 16 * i + 4 * q + e];
-        }
-        float later = 0.f;  // the pairs (i, j) of the tiles of i after this one
-#pragma unroll
-        for (int ip = 1; ip >= 0; --ip) {
-          if (2 * ip + 1 < mine) continue;
-          float m[8], s[8];
-#pragma unroll
-          for (int half = 1; half >= 0; --half) {
-            const int it = 2 * ip + half;
-            f32x4 gs = {0.f, 0.f, 0.f, 0.f}, ms = gs;
-            if (it >= mine) {
-#pragma unroll
-              for (int k = 0; k < NT / 32; ++k) O::mma(gs, O::near(cn + (16 * it + r) * BC::kRow, 32 * k, q), bf[k]);
-#pragma unroll
-              for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(yn + (16 * it + r) * XY::kRow, 32 * k, q), xf[k]);
-            }
-            float pair[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int ti = 16 * it + 4 * q + e;
-              const float f = __builtin_amdgcn_exp2f((tm.hi[ti] - hi) + (tm.lo[ti] - lo));
-              const float d = ti >= tw ? ms[e] * f : 0.f;
-              m[4 * half + e] = (ti >= tw ? gs[e] * f * dt : 0.f) + (ti == tw ? D : 0.f);
-              s[4 * half + e] = d;
-              pair[e] = d * gs[e];
-              diag += ti == tw ? ms[e] : 0.f;
-            }
-            if (it >= mine) {
-              // from each i to the chunk's end, then over the j before i
-              pair[2] += pair[3];
-              pair[1] += pair[2];
-              pair[0] += pair[1];
-              float from = pair[0], up = __shfl_down(from, 16, kWave);
-              from += q < 3 ? up : 0.f;
-              up = __shfl_down(from, 32, kWave);
-              from += q < 2 ? up : 0.f;
-              up = __shfl_down(from, 16, kWave);
-              const float after = later + (q < 3 ? up : 0.f);
-              f32x4 over;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float v = tw < 16 * it + 4 * q + e ? (pair[e] + after) * dt : 0.f;
-#pragma unroll
-                for (int d = 1; d < 16; d *= 2) v += __shfl_xor(v, d, kWave);
-                over[e] = v;
-              }
-              if (r == 0) {
-                f32x4 *o = reinterpret_cast<f32x4 *>(cross + mine * Q + 16 * it + 4 * q);
-                *o = pt ? *o + over : over;
-              }
-              later += __shfl(from, r, kWave);
-            }
-          }
-          const typename O::Split mf = O::split(m), sf = O::split(s);
-#pragma unroll
-          for (int i = 0; i < PT / 16; ++i) O::mma(dx[i], ya.far(16 * i + r, 32 * ip, q), mf);
-#pragma unroll
-          for (int i = 0; i < NT / 16; ++i) O::mma(own[i], ca.far(16 * i + r, 32 * ip, q), sf);
-        }
-        cols += later;
-        if (t0 + tw < a.T) {
-          T *xp = (T *)a.dx + ((b * a.T + t0 + tw) * a.H + h) * a.P + p0;
-#pragma unroll
-          for (int i = 0; i < PT / 16; ++i) {
-            const float v[4] = {dx[i][0], dx[i][1], dx[i][2], dx[i][3]};
-            store4<T>(xp, 16 * i + 4 * q, a.P - p0, a.yv, v);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NT / 16; ++i) acc[i] += own[i] * dt;
+  int h = h_lo, pt = 0;
+  for (bool first = true;; first = false) {
+    const int p0 = pt * PT, h_now = h, pt_now = pt;
+    const Times &tm = times[h & 1];
+    HeadSums &sum = sums[h & 1];
+    const bool dh = ST && dh_next, h0 = ST && h0_next;
+    const float D = a.D ? a.D[h] : 0.f;
+    if (!first) __syncthreads();
+    xs.put(xn, nullptr, tid);
+    ys.put(yn, yt, tid);
+    if constexpr (ST) {
+      if constexpr (L::two) {
+        hs.put((const StateTile<T, PT, NT, 1> *)nullptr, &h0l, tid);
+        ds.put(&dhl, &dhtl, tid);
       } else {
-        typename O::Frag yf[PT / 32];
-#pragma unroll
-        for (int k = 0; k < PT / 32; ++k) yf[k] = O::near(yn + tw * XY::kRow, 32 * k, q);
-        if (ST && h0) {
-          const float from = tm.from[tw];
-#pragma unroll
-          for (int i = 0; i < NT / 16; ++i) {
-#pragma unroll
-            for (int k = 0; k < PT / 32; ++k) {
-              if constexpr (L::two)
-                O::mma(own[i], h0l.near(16 * i + r, 32 * k, q), yf[k]);
-              else
-                O::mma(own[i], h0f.across(16 * i + r, 32 * k, q), yf[k]);
-            }
-            own[i] *= from;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) inter += own[i][e] * (float)cn[tw * BC::kRow + 16 * i + 4 * q + e];
-          }
-        }
-#pragma unroll
-        for (int jp = 0; jp < 2; ++jp) {
-          if (2 * jp > mine) break;
-          float s[8];
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int jt = 2 * jp + half;
-            f32x4 ms = {0.f, 0.f, 0.f, 0.f};
-            if (jt <= mine) {
-#pragma unroll
-              for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(xn + (16 * jt + r) * XY::kRow, 32 * k, q), yf[k]);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int tj = 16 * jt + 4 * q + e;
-              const float f = __builtin_amdgcn_exp2f((hi - tm.hi[tj]) + (lo - tm.lo[tj])) * tm.dt[tj];
-              s[4 * half + e] = tj <= tw ? ms[e] * f : 0.f;
-            }
-          }
-          const typename O::Split sf = O::split(s);
-#pragma unroll
-          for (int i = 0; i < NT / 16; ++i) O::mma(own[i], ba.far(16 * i + r, 32 * jp, q), sf);
-        }
-#pragma unroll
-        for (int i = 0; i < NT / 16; ++i) acc[i] += own[i];
+        hs.put(&h0f, (const StateTile<T, NT, PT, 2> *)nullptr, tid);
+        ds.put(&dhl, (const StateTile<T, NT, PT, 2> *)nullptr, tid);
       }
-      if (pt + 1 == a.ptiles) {
-        // a position's n are spread over the four lanes of one r
-        inter += __shfl_xor(inter, 16, kWave);
-        inter += __shfl_xor(inter, 32, kWave);
-        if (q == 0) {
-          (own_j ? vb : uc)[tw] = inter;
-          if (own_j) col[tw] = cols;
+      if (pt == 0) dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < hs.kEach; ++e)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dot += hs.v[e][k][i] * ds.v[e][k][i];
+    }
+    __syncthreads();
+    if (++pt == a.ptiles) {
+      pt = 0;
+      ++h;
+    }
+    const bool more = h < h_hi;
+    if (more) load(h, pt);
+    if (wave == kStepWave && pt_now == 0 && !first) finish(h_now - 1);
+    if (pt_now == 0) diag = inter = col = 0.f;
+
+    f32x4 own[NT / 16];  // this head's dB^T / dt or dC^T
+#pragma unroll
+    for (int i = 0; i < NT / 16; ++i) own[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float hi = tm.hi[tw], lo = tm.lo[tw];
+    if (own_j) {
+      f32x4 dx[PT / 16];
+#pragma unroll
+      for (int i = 0; i < PT / 16; ++i) dx[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      typename O::Frag bf[NT / 32], xf[PT / 32];
+#pragma unroll
+      for (int k = 0; k < NT / 32; ++k) bf[k] = O::near(bn + tw * BC::kRow, 32 * k, q);
+#pragma unroll
+      for (int k = 0; k < PT / 32; ++k) xf[k] = O::near(xn + tw * XY::kRow, 32 * k, q);
+      const float left = tm.left[tw], dt = tm.dt[tw];
+      if (dh) {
+        const float into = left * dt;
+#pragma unroll
+        for (int i = 0; i < PT / 16; ++i) {
+#pragma unroll
+          for (int k = 0; k < NT / 32; ++k) O::mma(dx[i], dhl.near(16 * i + r, 32 * k, q), bf[k]);
+          dx[i] *= into;
         }
-        dot = wave_sum(dot);
+#pragma unroll
+        for (int i = 0; i < NT / 16; ++i) {
+#pragma unroll
+          for (int k = 0; k < PT / 32; ++k) {
+            if constexpr (L::two)
+              O::mma(own[i], dhtl.near(16 * i + r, 32 * k, q), xf[k]);
+            else
+              O::mma(own[i], dhl.across(16 * i + r, 32 * k, q), xf[k]);
+          }
+          own[i] *= left;
+          const typename V4<T>::type bv = *reinterpret_cast<const typename V4<T>::type *>(bn + tw * BC::kRow + 16 * i + 4 * q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) inter += own[i][e] * (float)bv[e];
+        }
+      }
+      float later = 0.f;  // the pairs (i, j) of the tiles of i after this one, without dt_j
+#pragma unroll 1
+      for (int ip = 1; 2 * ip + 1 >= mine; --ip) {
+        float m[8], s[8];
+#pragma unroll
+        for (int half = 1; half >= 0; --half) {
+          const int it = 2 * ip + half;
+          f32x4 gs = {0.f, 0.f, 0.f, 0.f}, ms = gs;
+          if (it >= mine) {
+#pragma unroll
+            for (int k = 0; k < NT / 32; ++k) O::mma(gs, O::near(cn + (16 * it + r) * BC::kRow, 32 * k, q), bf[k]);
+#pragma unroll
+            for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(yn + (16 * it + r) * XY::kRow, 32 * k, q), xf[k]);
+          }
+          const f32x4 thi = *reinterpret_cast<const f32x4 *>(tm.hi + 16 * it + 4 * q);
+          const f32x4 tlo = *reinterpret_cast<const f32x4 *>(tm.lo + 16 * it + 4 * q);
+          float pair[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int ti = 16 * it + 4 * q + e;
+            const float f = __builtin_amdgcn_exp2f((thi[e] - hi) + (tlo[e] - lo));
+            const float d = ti >= tw ? ms[e] * f : 0.f, gf = ti >= tw ? gs[e] * f * dt : 0.f;
+            m[4 * half + e] = gf + (ti == tw ? D : 0.f);
+            s[4 * half + e] = d;
+            pair[e] = d * gs[e];
+            diag += ti == tw ? ms[e] : 0.f;
+          }
+          // from each i to the chunk's end, then over the j before i
+          pair[2] += pair[3];
+          pair[1] += pair[2];
+          pair[0] += pair[1];
+          const Pair rows = rows_of_half(pair[0]), both = halves(rows.first + rows.second);
+          const float after = later + (q & 1 ? 0.f : rows.second) + (q < 2 ? both.second : 0.f);
+          f32x4 over;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            over[e] = lanes_sum<16>(tw < 16 * it + 4 * q + e ? (pair[e] + after) * dt : 0.f);
+          if (r == 0 && it >= mine) {
+            f32x4 *o = reinterpret_cast<f32x4 *>(sum.cross[mine] + 16 * it + 4 * q);
+            *o = pt_now ? *o + over : over;
+          }
+          later += both.first + both.second;
+        }
+        const typename O::Frag mf = O::round(m), sf = O::round(s);
+#pragma unroll
+        for (int i = 0; i < PT / 16; ++i) O::mma(dx[i], ya.far(16 * i + r, 32 * ip, q), mf);
+#pragma unroll
+        for (int i = 0; i < NT / 16; ++i) O::mma(own[i], ca.far(16 * i + r, 32 * ip, q), sf);
+      }
+      if (t0 + tw < a.T) {
+        T *xp = (T *)a.dx + ((b * a.T + t0 + tw) * a.H + h_now) * a.P + p0;
+#pragma unroll
+        for (int i = 0; i < PT / 16; ++i) {
+          const float v[4] = {dx[i][0], dx[i][1], dx[i][2], dx[i][3]};
+          store4<VEC>(xp, 16 * i + 4 * q, a.P - p0, v);
+        }
+      }
+      col += later;
+#pragma unroll
+      for (int i = 0; i < NT / 16; ++i) acc[i] += own[i] * dt;
+    } else {
+      typename O::Frag yf[PT / 32];
+#pragma unroll
+      for (int k = 0; k < PT / 32; ++k) yf[k] = O::near(yn + tw * XY::kRow, 32 * k, q);
+      if (h0) {
+        const float from = tm.from[tw];
+#pragma unroll
+        for (int i = 0; i < NT / 16; ++i) {
+#pragma unroll
+          for (int k = 0; k < PT / 32; ++k) {
+            if constexpr (L::two)
+              O::mma(own[i], h0l.near(16 * i + r, 32 * k, q), yf[k]);
+            else
+              O::mma(own[i], h0f.across(16 * i + r, 32 * k, q), yf[k]);
+          }
+          own[i] *= from;
+          const typename V4<T>::type cv = *reinterpret_cast<const typename V4<T>::type *>(cn + tw * BC::kRow + 16 * i + 4 * q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) inter += own[i][e] * (float)cv[e];
+        }
+      }
+#pragma unroll 1
+      for (int jp = 0; 2 * jp <= mine; ++jp) {
+        float s[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int jt = 2 * jp + half;
+          f32x4 ms = {0.f, 0.f, 0.f, 0.f};
+          if (jt <= mine) {
+#pragma unroll
+            for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(xn + (16 * jt + r) * XY::kRow, 32 * k, q), yf[k]);
+          }
+          const f32x4 thi = *reinterpret_cast<const f32x4 *>(tm.hi + 16 * jt + 4 * q);
+          const f32x4 tlo = *reinterpret_cast<const f32x4 *>(tm.lo + 16 * jt + 4 * q);
+          const f32x4 tdt = *reinterpret_cast<const f32x4 *>(tm.dt + 16 * jt + 4 * q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = __builtin_amdgcn_exp2f((hi - thi[e]) + (lo - tlo[e])) * tdt[e];
+            s[4 * half + e] = 16 * jt + 4 * q + e <= tw ? ms[e] * f : 0.f;
+          }
+        }
+        const typename O::Frag sf = O::round(s);
+#pragma unroll
+        for (int i = 0; i < NT / 16; ++i) O::mma(own[i], ba.far(16 * i + r, 32 * jp, q), sf);
+      }
+#pragma unroll
+      for (int i = 0; i < NT / 16; ++i) acc[i] += own[i];
+    }
+    if (pt_now + 1 == a.ptiles) {
+      // a position's n are spread over the four lanes of one r
+      if constexpr (ST) {
+        inter = rows_sum(inter);
+        if (q == 0) (own_j ? sum.vb : sum.uc)[tw] = inter;
+        const float v = wave_sum(dot);
+        if (lane == 0) sum.dot[wave] = v;
+      }
+      if (own_j) {
         diag = wave_sum(diag);
-        if (lane == 0) {
-          red[wave] = dot;
-          red[8 + wave] = diag;
-        }
-      }
-      __syncthreads();
-    }
-    if (wave == 0) {
-      float dot_all = 0.f, diag_all = 0.f, over = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        dot_all += red[i];
-        diag_all += red[8 + i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) over += 16 * i <= lane ? cross[i * Q + lane] : 0.f;
-      const float dt = tm.dt[lane], bdv = col[lane] + vb[lane], into = dt * vb[lane];
-      float before = into, after = uc[lane];  // sums over j <= t, i >= t
-#pragma unroll
-      for (int m = 1; m < Q; m *= 2) {
-        const float lower = __shfl_up(before, m, kWave), upper = __shfl_down(after, m, kWave);
-        if (lane >= m) before += lower;
-        if (lane + m < Q) after += upper;
-      }
-      before = __shfl_up(before, 1, kWave);
-      if (lane == 0) before = 0.f;
-      const float da = (before + after) + (over + tm.total * dot_all);
-      const float ddt = live ? (A * da + bdv) / (1.f + expf(-raw)) : 0.f;
-      if (t0 + lane < a.T) ((T *)a.ddt)[(b * a.T + t0 + lane) * a.H + h] = (T)ddt;
-      const float dA = wave_sum(da * dt), dbias = wave_sum(ddt);
-      if (lane == 0) {
-        float *o = a.part + ((b * a.chunks + c) * a.H + h) * 3;
-        o[0] = dA;
-        o[1] = dbias;
-        o[2] = diag_all;
+        if (q == 0) sum.col[tw] = col;
+        if (lane == 0) sum.diag[mine] = diag;
       }
     }
+    if (!more) break;
+    if (wave == kTimesWave && pt == 0) make_times(times[h & 1], raw, live, a.A[h], lane);
   }
+  __syncthreads();
+  if (wave == kStepWave) finish(h_hi - 1);
   if (t0 + tw < a.T) {
     const int64_t row = (b * a.T + t0 + tw) * a.G + g;
     if (a.slices == 1) {
@@ -955,14 +1127,14 @@ __global__ __launch_bounds__(512) void scan_grad_kernel(ScanArgs a) {
 #pragma unroll
       for (int i = 0; i < NT / 16; ++i) {
         const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
-        store4<T>(o, 16 * i + 4 * q, a.N, a.nv, v);
+        store4<VEC>(o, 16 * i + 4 * q, a.N, v);
       }
     } else {
       float *o = a.dbc + ((int64_t)(slice * 2 + !own_j) * a.B * a.T * a.G + row) * a.N;
 #pragma unroll
       for (int i = 0; i < NT / 16; ++i) {
         const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
-        store4<float>(o, 16 * i + 4 * q, a.N, a.nv, v);
+        store4<VEC>(o, 16 * i + 4 * q, a.N, v);
       }
     }
   }
@@ -1081,19 +1253,19 @@ int check(const astra_state_scan *f) {
   return ASTRA_OK;
 }
 
-// The tile of features and of states that a call is padded to. With states over 64 the
+// The tiles of features and of states that a call is padded to, and for the forward and
+// states kernels the parts of the features that wavefronts share. With states over 64 the
 // backward kernel's tiles fit a CU's LDS for 32 features only.
 struct Tiles {
-  int p, n;
+  int p, n, pw;
 };
-Tiles tiles_of(const astra_state_scan &f) {
+Tiles tiles_of(const astra_state_scan &f, bool grad) {
   Tiles t;
   t.n = f.state <= 32 ? 32 : f.state <= 64 ? 64 : 128;
-  t.p = t.n == 128 || f.dim <= 32 ? 32 : 64;
+  t.p = f.dim <= 32 || (grad && t.n == 128) ? 32 : 64;
+  t.pw = t.n == 128 && t.p == 64 ? 2 : 1;
   return t;
 }
-
-constexpr int64_t kFull = 512;  // workgroups that fill the card
 
 ScanArgs args_of(const astra_state_scan &f) {
   ScanArgs a{};
@@ -1126,26 +1298,30 @@ ScanArgs args_of(const astra_state_scan &f) {
   a.P = f.dim;
   a.G = f.groups;
   a.N = f.state;
-  a.ptiles = (int32_t)cdiv(f.dim, tiles_of(f).p);
+  const Tiles tiles = tiles_of(f, false);
+  a.ptiles = (int32_t)cdiv(f.dim, tiles.p);
   a.chunks = (int32_t)cdiv(f.length, Q);
-  // few rows: the length is split into segments, joined by their states
+  // few rows: the length is split into segments, joined by their states; as many workgroups
+  // as are resident at once (two a CU, one of the largest tiles)
+  const int64_t resident = tiles.pw == 2 ? 256 : 512;
   const int64_t rows = a.B * a.H * a.ptiles;
   int64_t segs = 1;
-  if (rows > 0 && rows < kFull) segs = cdiv(kFull, rows);
+  if (rows > 0 && rows < resident) segs = cdiv(resident, rows);
   if (segs > a.chunks / 2) segs = a.chunks / 2;
   if (segs < 1) segs = 1;
   a.seg_chunks = (int32_t)cdiv(a.chunks, segs);
   a.segs = a.seg_chunks ? (int32_t)cdiv(a.chunks, a.seg_chunks) : 1;
+  // a workgroup walks as many of a group's heads as leave twice that many workgroups
+  const int per = a.H / a.G;
+  const int64_t shared = a.B * a.G * a.segs;
+  a.parts = shared > 0 ? (int32_t)std::min<int64_t>((int64_t)per * a.ptiles, cdiv(2 * resident, shared)) : 1;
   // few chunks: the heads of a group are split, and their parts of db and dc added up
   const int64_t items = a.B * a.chunks * a.G;
-  const int per = a.H / a.G;
-  a.slices = items > 0 && items < kFull / 2 ? (int32_t)std::min<int64_t>(per, cdiv(kFull / 2, items)) : 1;
+  a.slices = items > 0 && items < 256 ? (int32_t)std::min<int64_t>(per, cdiv(256, items)) : 1;
   const int64_t e = 4 * (int64_t)elem_size(f.type);
-  a.xv = a.P % 4 == 0 && a.xsb % 4 == 0 && a.xst % 4 == 0 && a.xsh % 4 == 0 && aligned(a.x, e);
-  a.bv = a.N % 4 == 0 && a.bsb % 4 == 0 && a.bst % 4 == 0 && a.bsg % 4 == 0 && aligned(a.b, e);
-  a.cv = a.N % 4 == 0 && a.csb % 4 == 0 && a.cst % 4 == 0 && a.csg % 4 == 0 && aligned(a.c, e);
-  a.yv = a.P % 4 == 0 && aligned(a.y, e);
-  a.nv = a.N % 4 == 0 && aligned(a.initial, 16) && aligned(a.final_state, 16);
+  a.vec = a.P % 4 == 0 && a.N % 4 == 0 && aligned(a.x, e) && aligned(a.b, e) && aligned(a.c, e) && aligned(a.y, e) &&
+          aligned(a.initial, 16) && aligned(a.final_state, 16);
+  for (int64_t stride : {a.xsb, a.xst, a.xsh, a.bsb, a.bst, a.bsg, a.csb, a.cst, a.csg}) a.vec = a.vec && stride % 4 == 0;
   return a;
 }
 
@@ -1180,34 +1356,53 @@ int allow_lds(K *kernel, size_t bytes) {
     ASTRA_HIP_CHECK(rt_last_error(), #kernel " launch");                                               \
   } while (false)
 
-template <class T, int PT, int NT>
-int forward(ScanArgs &a, hipStream_t st) {
+template <class T, int PT, int NT, int PW, bool REV, bool KEEP>
+int states(ScanArgs &a, hipStream_t st) {
   const int64_t blocks = a.B * a.H * a.ptiles * a.segs;
-  if (a.segs > 1) {
-    SCAN_LAUNCH((scan_states_kernel<T, PT, NT, false, false>), blocks, 256, (StatesLds<T, PT, NT>::bytes));
-    hipLaunchKernelGGL(scan_carry_kernel<false>, dim3((unsigned)cdiv(a.B * a.H * a.P * a.N, 256)), dim3(256), 0, st, a);
-    ASTRA_HIP_CHECK(rt_last_error(), "scan_carry_kernel launch");
-  }
-  SCAN_LAUNCH((scan_forward_kernel<T, PT, NT>), blocks, 256, (ForwardLds<T, PT, NT>::bytes));
+  if (a.vec)
+    SCAN_LAUNCH((scan_states_kernel<T, PT, NT, PW, REV, KEEP, true>), blocks, 256 * PW, (StatesLds<T, PT, NT>::bytes));
+  else
+    SCAN_LAUNCH((scan_states_kernel<T, PT, NT, PW, REV, KEEP, false>), blocks, 256 * PW, (StatesLds<T, PT, NT>::bytes));
+  if (KEEP) return ASTRA_OK;
+  hipLaunchKernelGGL(scan_carry_kernel<REV>, dim3((unsigned)cdiv(a.B * a.H * a.P * a.N, 256)), dim3(256), 0, st, a);
+  ASTRA_HIP_CHECK(rt_last_error(), "scan_carry_kernel launch");
   return ASTRA_OK;
+}
+
+template <class T, int PT, int NT, int PW>
+int forward(ScanArgs &a, hipStream_t st) {
+  if (a.segs > 1)
+    if (int rc = states<T, PT, NT, PW, false, false>(a, st)) return rc;
+  const int64_t blocks = a.B * a.G * a.segs * a.parts;
+  constexpr size_t bytes = ForwardLds<T, PT, NT, true>::bytes;
+  if (!a.vec)
+    SCAN_LAUNCH((scan_forward_kernel<T, PT, NT, PW, true, false>), blocks, 256 * PW, bytes);
+  else if (a.chunks > 1 || a.initial)
+    SCAN_LAUNCH((scan_forward_kernel<T, PT, NT, PW, true, true>), blocks, 256 * PW, bytes);
+  else
+    SCAN_LAUNCH((scan_forward_kernel<T, PT, NT, PW, false, true>), blocks, 256 * PW, (ForwardLds<T, PT, NT, false>::bytes));
+  return ASTRA_OK;
+}
+
+// The gradients of the states after the chunks.
+template <class T, int PT, int NT, int PW>
+int backward_states(ScanArgs &a, hipStream_t st) {
+  if (a.segs > 1)
+    if (int rc = states<T, PT, NT, PW, true, false>(a, st)) return rc;
+  return states<T, PT, NT, PW, true, true>(a, st);
 }
 
 template <class T, int PT, int NT>
 int backward(ScanArgs &a, hipStream_t st) {
-  if (a.chunks > 1 || a.dinitial) {
-    const int64_t blocks = a.B * a.H * a.ptiles * a.segs;
-    if (a.segs > 1) {
-      SCAN_LAUNCH((scan_states_kernel<T, PT, NT, true, false>), blocks, 256, (StatesLds<T, PT, NT>::bytes));
-      hipLaunchKernelGGL(scan_carry_kernel<true>, dim3((unsigned)cdiv(a.B * a.H * a.P * a.N, 256)), dim3(256), 0, st, a);
-      ASTRA_HIP_CHECK(rt_last_error(), "scan_carry_kernel launch");
-    }
-    SCAN_LAUNCH((scan_states_kernel<T, PT, NT, true, true>), blocks, 256, (StatesLds<T, PT, NT>::bytes));
-  }
+  a.ptiles = (int32_t)cdiv(a.P, PT);
   const int64_t blocks = a.B * a.chunks * a.G * a.slices;
-  if (a.chunks > 1 || a.initial || a.dfinal)
-    SCAN_LAUNCH((scan_grad_kernel<T, PT, NT, true>), blocks, 512, (GradLds<T, PT, NT, true>::bytes));
+  constexpr size_t bytes = GradLds<T, PT, NT, true>::bytes;
+  if (!a.vec)
+    SCAN_LAUNCH((scan_grad_kernel<T, PT, NT, true, false>), blocks, 512, bytes);
+  else if (a.chunks > 1 || a.initial || a.dfinal)
+    SCAN_LAUNCH((scan_grad_kernel<T, PT, NT, true, true>), blocks, 512, bytes);
   else
-    SCAN_LAUNCH((scan_grad_kernel<T, PT, NT, false>), blocks, 512, (GradLds<T, PT, NT, false>::bytes));
+    SCAN_LAUNCH((scan_grad_kernel<T, PT, NT, false, true>), blocks, 512, (GradLds<T, PT, NT, false>::bytes));
   if (a.slices > 1) {
     hipLaunchKernelGGL(scan_join_slices_kernel<T>, dim3((unsigned)cdiv(2 * a.B * a.T * a.G * a.N, 256)), dim3(256), 0, st, a);
     ASTRA_HIP_CHECK(rt_last_error(), "scan_join_slices_kernel launch");
@@ -1215,23 +1410,31 @@ int backward(ScanArgs &a, hipStream_t st) {
   return ASTRA_OK;
 }
 
-#define SCAN_TILES(FN)                                                    \
-  do {                                                                    \
-    const bool h = f.type == ASTRA_SEQ_BF16;                              \
-    if (t.n == 128) return h ? FN<bf16, 32, 128>(a, st) : FN<float, 32, 128>(a, st); \
-    if (t.n == 64 && t.p == 32) return h ? FN<bf16, 32, 64>(a, st) : FN<float, 32, 64>(a, st); \
-    if (t.n == 64) return h ? FN<bf16, 64, 64>(a, st) : FN<float, 64, 64>(a, st); \
-    if (t.p == 32) return h ? FN<bf16, 32, 32>(a, st) : FN<float, 32, 32>(a, st); \
-    return h ? FN<bf16, 64, 32>(a, st) : FN<float, 64, 32>(a, st);        \
+#define SCAN_BOTH(FN, ...) (h ? FN<bf16, __VA_ARGS__>(a, st) : FN<float, __VA_ARGS__>(a, st))
+#define SCAN_TILES(FN)                                              \
+  do {                                                              \
+    const Tiles t = tiles_of(f, false);                             \
+    const bool h = f.type == ASTRA_SEQ_BF16;                        \
+    if (t.n == 128 && t.p == 64) return SCAN_BOTH(FN, 64, 128, 2);  \
+    if (t.n == 128) return SCAN_BOTH(FN, 32, 128, 1);               \
+    if (t.n == 64 && t.p == 64) return SCAN_BOTH(FN, 64, 64, 1);    \
+    if (t.n == 64) return SCAN_BOTH(FN, 32, 64, 1);                 \
+    if (t.p == 64) return SCAN_BOTH(FN, 64, 32, 1);                 \
+    return SCAN_BOTH(FN, 32, 32, 1);                                \
   } while (false)
 
-int run_forward(const astra_state_scan &f, ScanArgs &a, hipStream_t st) {
-  const Tiles t = tiles_of(f);
-  SCAN_TILES(forward);
-}
+int run_forward(const astra_state_scan &f, ScanArgs &a, hipStream_t st) { SCAN_TILES(forward); }
+int run_backward_states(const astra_state_scan &f, ScanArgs &a, hipStream_t st) { SCAN_TILES(backward_states); }
 int run_backward(const astra_state_scan &f, ScanArgs &a, hipStream_t st) {
-  const Tiles t = tiles_of(f);
-  SCAN_TILES(backward);
+  if (a.chunks > 1 || a.dinitial)
+    if (int rc = run_backward_states(f, a, st)) return rc;
+  const Tiles t = tiles_of(f, true);
+  const bool h = f.type == ASTRA_SEQ_BF16;
+  if (t.n == 128) return SCAN_BOTH(backward, 32, 128);
+  if (t.n == 64 && t.p == 64) return SCAN_BOTH(backward, 64, 64);
+  if (t.n == 64) return SCAN_BOTH(backward, 32, 64);
+  if (t.p == 64) return SCAN_BOTH(backward, 64, 32);
+  return SCAN_BOTH(backward, 32, 32);
 }
 
 template <class T>
@@ -1358,8 +1561,8 @@ int astra_state_scan_backward(const astra_state_scan_grad *g, void *stream) {
   a.dbc = a.seg + round4(seg_floats(a));
   a.part = a.dbc + round4(slice_floats(a));
   const int64_t e = 4 * (int64_t)elem_size(f.type);
-  a.yv = a.P % 4 == 0 && aligned(a.dy, e) && aligned(a.dx, e);
-  a.nv = a.N % 4 == 0 && aligned(a.initial, 16) && aligned(a.dfinal, 16) && aligned(a.dinitial, 16) && aligned(a.db, e) && aligned(a.dc, e);
+  for (const void *p : {g->dy, (const void *)a.dx, (const void *)a.db, (const void *)a.dc}) a.vec = a.vec && aligned(p, e);
+  a.vec = a.vec && aligned(a.dfinal, 16) && aligned(a.dinitial, 16);
   if (int rc = run_backward(f, a, st)) return rc;
   if (!g->dA && !g->dD && !g->ddt_bias) return ASTRA_OK;
   int64_t rows = a.B * a.chunks;
