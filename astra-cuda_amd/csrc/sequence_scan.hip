@@ -256,51 +256,76 @@ struct StateTile {
 
 // ---------------------------------------------------------------------- global memory
 
-// 4 elements of a row from element f on, zeros from `n` on. VEC: n, the rows' strides and
-// their addresses allow one access of all four.
-template <bool VEC, class T>
-__device__ __forceinline__ typename V4<T>::type load4(const T *p, int f, int n) {
-  typename V4<T>::type r = {};
-  if constexpr (VEC) {
-    if (f < n) r = *reinterpret_cast<const typename V4<T>::type *>(p + f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (f + i < n) r[i] = p[f + i];
+// A matrix of rows in memory, `n` elements of each counting. VEC: four neighbouring elements
+// are one access through a buffer descriptor, whose bounds check (a byte offset of this
+// descriptor's size or more reads zeros and writes nothing) stands in for a branch per row;
+// needs n, the stride and the address to be multiples of four, and n <= stride < 2^23.
+// Otherwise elements go one by one.
+constexpr unsigned kOutside = 0x80000000u;  // beyond any descriptor, also after some rows are added
+template <class T, bool VEC>
+struct Matrix {
+  T *base;
+  int64_t stride;
+  int rows, n;
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ Matrix(const T *p, int64_t stride_, int64_t rows_, int n_)
+      : base(const_cast<T *>(p)), stride(stride_), rows(rows_ < 0 ? 0 : rows_ > 1024 ? 1024 : (int)rows_), n(n_) {
+    if constexpr (VEC)
+      rsrc = __builtin_amdgcn_make_buffer_rsrc(base, 0, rows ? ((rows - 1) * (int)stride + n) * (int)sizeof(T) : 0, 0x00020000);
   }
-  return r;
-}
-
-template <bool VEC, class T>
-__device__ __forceinline__ void store4(T *p, int f, int n, const float (&v)[4]) {
-  if constexpr (VEC) {
+  // the offset of four elements from (row, f) on, for load and store
+  __device__ __forceinline__ unsigned at(int row, int f) const {
+    return f < n ? (unsigned)(row * (int)stride + f) * (unsigned)sizeof(T) : kOutside;
+  }
+  __device__ __forceinline__ typename V4<T>::type load(int row, int f, unsigned off) const {
+    typename V4<T>::type r = {};
+    if constexpr (VEC && sizeof(T) == 2) {
+      r = __builtin_bit_cast(typename V4<T>::type, __builtin_amdgcn_raw_buffer_load_b64(rsrc, off, 0, 0));
+    } else if constexpr (VEC) {
+      r = __builtin_bit_cast(typename V4<T>::type, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (row < rows && f + i < n) r[i] = base[row * stride + f + i];
+    }
+    return r;
+  }
+  __device__ __forceinline__ typename V4<T>::type load(int row, int f) const { return load(row, f, at(row, f)); }
+  __device__ __forceinline__ void store(int row, int f, const float (&v)[4]) const {
     typename V4<T>::type r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = (T)v[i];
-    if (f < n) *reinterpret_cast<typename V4<T>::type *>(p + f) = r;
-  } else {
+    if constexpr (VEC && sizeof(T) == 2) {
+      typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, r), rsrc, at(row, f), 0, 0);
+    } else if constexpr (VEC) {
+      typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, r), rsrc, at(row, f), 0, 0);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (f + i < n) p[f + i] = (T)v[i];
+      for (int i = 0; i < 4; ++i)
+        if (row < rows && f + i < n) base[row * stride + f + i] = r[i];
+    }
   }
-}
+};
 
 // F features by Q positions on their way from memory to LDS: THREADS threads hold blocks of
-// 4 positions by 4 features. Positions at and after `len` and features at and after `n`
-// are zero, whatever memory holds there.
+// 4 positions by 4 features. What lies beyond the matrix is zero, whatever memory holds there.
 template <class T, int F, int THREADS, bool VEC>
 struct Stage {
   static constexpr int kGroups = F / 4, kBlocks = kGroups * (Q / 4), kEach = (kBlocks + THREADS - 1) / THREADS;
   typename V4<T>::type v[kEach][4];
-  __device__ __forceinline__ void load(const T *base, int64_t stride, int64_t t0, int len, int n, int tid) {
+  __device__ __forceinline__ void load(const Matrix<T, VEC> &m, int tid) {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int blk = tid + e * THREADS;
       const int f = (blk % kGroups) * 4, t = (blk / kGroups) * 4;
+      unsigned off = blk < kBlocks ? m.at(t, f) : kOutside;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         v[e][k] = {};
-        if (blk < kBlocks && t0 + t + k < len) v[e][k] = load4<VEC>(base + (t0 + t + k) * stride, f, n);
+        if (VEC || blk < kBlocks) v[e][k] = m.load(t + k, f, off);
+        off += (unsigned)m.stride * (unsigned)sizeof(T);
       }
     }
   }
@@ -308,7 +333,7 @@ struct Stage {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int blk = tid + e * THREADS;
-      if (blk >= kBlocks) continue;
+      if (kBlocks % THREADS && blk >= kBlocks) continue;
       const int f = (blk % kGroups) * 4, t = (blk / kGroups) * 4;
       if (rows) {
 #pragma unroll
@@ -327,6 +352,23 @@ struct Stage {
     }
   }
 };
+
+// A row's 8 elements from f + 8 q on (an operand that is read from memory as it is).
+template <class T, bool VEC>
+__device__ __forceinline__ typename Ops<T>::Frag load_near(const Matrix<T, VEC> &m, int row, int f, int q) {
+  const typename V4<T>::type a = m.load(row, f + 8 * q), b = m.load(row, f + 8 * q + 4);
+  typename Ops<T>::Frag r;
+  if constexpr (sizeof(T) == 2) {
+    r = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r.v[i] = a[i];
+      r.v[4 + i] = b[i];
+    }
+  }
+  return r;
+}
 
 // ------------------------------------------------------------------------- step sizes
 
@@ -431,25 +473,26 @@ __device__ __forceinline__ void update_state(f32x4 *S, float total, const float 
   }
 }
 
+// The PT features from p0 on of a state [P, N], nothing where there is none.
+template <bool VEC>
+__device__ __forceinline__ Matrix<float, VEC> state_rows(const float *base, const ScanArgs &a, int p0) {
+  return Matrix<float, VEC>(base ? base + (int64_t)p0 * a.N : nullptr, a.N, base ? a.P - p0 : 0, a.N);
+}
 template <int PT, int NT, int WAVES, bool VEC>
 __device__ __forceinline__ void load_state(f32x4 *S, const float *base, const ScanArgs &a, int p0, int wave, int q, int r) {
   using M = Mine<PT, NT, WAVES>;
+  const Matrix<float, VEC> m = state_rows<VEC>(base, a, p0);
 #pragma unroll
-  for (int i = 0; i < M::kEach; ++i) {
-    const int p = p0 + M::p_of(wave, i, r), n = M::n_of(wave, i, q);
-    S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (base && p < a.P) S[i] = load4<VEC>(base + (int64_t)p * a.N, n, a.N);
-  }
+  for (int i = 0; i < M::kEach; ++i) S[i] = m.load(M::p_of(wave, i, r), M::n_of(wave, i, q));
 }
-
 template <int PT, int NT, int WAVES, bool VEC>
 __device__ __forceinline__ void store_state(const f32x4 *S, float *base, const ScanArgs &a, int p0, int wave, int q, int r) {
   using M = Mine<PT, NT, WAVES>;
+  const Matrix<float, VEC> m = state_rows<VEC>(base, a, p0);
 #pragma unroll
   for (int i = 0; i < M::kEach; ++i) {
-    const int p = p0 + M::p_of(wave, i, r), n = M::n_of(wave, i, q);
     const float v[4] = {S[i][0], S[i][1], S[i][2], S[i][3]};
-    if (p < a.P) store4<VEC>(base + (int64_t)p * a.N, n, a.N, v);
+    m.store(M::p_of(wave, i, r), M::n_of(wave, i, q), v);
   }
 }
 
@@ -460,8 +503,7 @@ struct ForwardLds {
   static constexpr size_t x = 0;  // along positions only
   static constexpr size_t bn = x + (sizeof(T) == 2 ? Tile<T, PT>::kColsBytes : Tile<T, PT>::kRowsBytes);
   static constexpr size_t bt = bn + Tile<T, NT>::kRowsBytes;
-  static constexpr size_t cn = bt + Tile<T, NT>::kColsBytes;
-  static constexpr size_t h = cn + Tile<T, NT>::kRowsBytes;
+  static constexpr size_t h = bt + Tile<T, NT>::kColsBytes;
   static constexpr size_t times = h + (ST ? StateTile<T, PT, NT, 1>::kBytes : 0);
   static constexpr size_t bytes = times + 2 * sizeof(Times);
 };
@@ -473,12 +515,12 @@ struct ForwardLds {
 // of positions, works out its step sizes. Where the segment is a single chunk, B, C and their
 // scores are loaded and computed once for all heads. ST: whether there are states before a chunk.
 template <class T, int PT, int NT, int PW, bool ST, bool VEC>
-__global__ __launch_bounds__(256 * PW, PW == 1 ? 3 : 2) void scan_forward_kernel(ScanArgs a) {
+__global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void scan_forward_kernel(ScanArgs a) {
   using L = ForwardLds<T, PT, NT, ST>;
   constexpr int kThreads = 256 * PW, kWaves = 4 * PW, PP = PT / PW;
   using M = Mine<PT, NT, kWaves>;
   extern __shared__ __align__(16) char lds[];
-  T *xl = (T *)(lds + L::x), *bn = (T *)(lds + L::bn), *bt = (T *)(lds + L::bt), *cn = (T *)(lds + L::cn);
+  T *xl = (T *)(lds + L::x), *bn = (T *)(lds + L::bn), *bt = (T *)(lds + L::bt);
   const StateTile<T, PT, NT, 1> hl{(T *)(lds + L::h)};
   Times *times = (Times *)(lds + L::times);
   const Along<T, PT> xa{xl, xl};
@@ -486,6 +528,7 @@ __global__ __launch_bounds__(256 * PW, PW == 1 ? 3 : 2) void scan_forward_kernel
 
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, r = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave & 3, f0 = (wave >> 2) * PP;
+  const int ti = 16 * wi + r;  // this lane's position
   int64_t id = workgroup_id();
   const int per = a.H / a.G, heads = per * a.ptiles;  // a group's heads and tiles of features
   const int part = (int)(id % a.parts);
@@ -502,16 +545,19 @@ __global__ __launch_bounds__(256 * PW, PW == 1 ? 3 : 2) void scan_forward_kernel
   const T *cg = (const T *)a.c + b * a.csb + g * a.csg;
 
   Stage<T, PT, kThreads, VEC> xs;
-  Stage<T, NT, kThreads, VEC> bs, cs;
+  Stage<T, NT, kThreads, VEC> bs;
+  typename Ops<T>::Frag cf[NT / 32], cf_next[NT / 32];  // this position's C, read as it is used
   float raw = 0.f;
   int hp = (int)((int64_t)heads * part / a.parts), c = c0;  // the item that is loaded next
   auto load = [&](bool with_bc) __attribute__((always_inline)) {
     const int h = g * per + hp / a.ptiles, p0 = (hp % a.ptiles) * PT;
     const int64_t t0 = (int64_t)c * Q;
-    xs.load((const T *)a.x + b * a.xsb + h * a.xsh + p0, a.xst, t0, len, a.P - p0, tid);
+    xs.load(Matrix<T, VEC>((const T *)a.x + b * a.xsb + t0 * a.xst + h * a.xsh + p0, a.xst, len - t0, a.P - p0), tid);
     if (with_bc) {
-      bs.load(bg, a.bst, t0, len, a.N, tid);
-      cs.load(cg, a.cst, t0, len, a.N, tid);
+      bs.load(Matrix<T, VEC>(bg + t0 * a.bst, a.bst, len - t0, a.N), tid);
+      const Matrix<T, VEC> cm(cg + t0 * a.cst, a.cst, len - t0, a.N);
+#pragma unroll
+      for (int n = 0; n < NT / 32; ++n) cf_next[n] = load_near(cm, ti, 32 * n, q);
     }
     if (wave == 0) raw = raw_step<T>(a, b, h, t0 + lane, len);
   };
@@ -539,7 +585,8 @@ __global__ __launch_bounds__(256 * PW, PW == 1 ? 3 : 2) void scan_forward_kernel
       xs.put(xl, nullptr, tid);
     if (new_bc) {
       bs.put(bn, bt, tid);
-      cs.put(cn, nullptr, tid);
+#pragma unroll
+      for (int n = 0; n < NT / 32; ++n) cf[n] = cf_next[n];
     }
     if constexpr (ST) {
       if (any) {
@@ -559,64 +606,70 @@ __global__ __launch_bounds__(256 * PW, PW == 1 ? 3 : 2) void scan_forward_kernel
     const bool more = hp < last;
     if (more) load(c1 - c0 > 1);
 
-    // this wavefront's 16 positions i = 16 wi + r: Y^T, rows the features
-    f32x4 y[PP / 16];
+    // this wavefront's 16 positions i = 16 wi + r: first M^T, two tiles of j to an operand
+    auto scores = [&](int jt) __attribute__((always_inline)) {
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < PP / 16; ++i) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int ti = 16 * wi + r;
-    if (new_bc || (ST && any)) {
-      typename Ops<T>::Frag cf[NT / 32];
-#pragma unroll
-      for (int n = 0; n < NT / 32; ++n) cf[n] = Ops<T>::near(cn + ti * Tile<T, NT>::kRow, 32 * n, q);
+      for (int n = 0; n < NT / 32; ++n)
+        Ops<T>::mma(v, Ops<T>::near(bn + (16 * jt + r) * Tile<T, NT>::kRow, 32 * n, q), cf[n]);
+      return v;
+    };
+    if constexpr (!ST) {
       if (new_bc) {
 #pragma unroll
-        for (int jt = 0; jt < 4; ++jt) {
-          sc[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (jt <= wi)
-#pragma unroll
-            for (int n = 0; n < NT / 32; ++n)
-              Ops<T>::mma(sc[jt], Ops<T>::near(bn + (16 * jt + r) * Tile<T, NT>::kRow, 32 * n, q), cf[n]);
-        }
-        fresh = false;
-      }
-      if constexpr (ST) {
-        if (any) {
-          const float e = tm.from[ti];
-#pragma unroll
-          for (int i = 0; i < PP / 16; ++i) {
-#pragma unroll
-            for (int n = 0; n < NT / 32; ++n) Ops<T>::mma(y[i], hl.near(f0 + 16 * i + r, 32 * n, q), cf[n]);
-            y[i] *= e;
-          }
-        }
+        for (int jt = 0; jt < 4; ++jt)
+          if (jt <= wi) sc[jt] = scores(jt);
       }
     }
+    fresh = false;
     const float hi = tm.hi[ti], lo = tm.lo[ti], D = a.D ? a.D[h] : 0.f;
+    typename Ops<T>::Frag mf[2];
 #pragma unroll
-    for (int jp = 0; jp < 2; ++jp) {  // two tiles of 16 positions j at a time
+    for (int jp = 0; jp < 2; ++jp) {
       if (2 * jp > wi) break;
       float m[8];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int jt = 2 * jp + half;
+        if (jt > wi) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tj = 16 * jt + 4 * q + e;
-          const float f = __builtin_amdgcn_exp2f((hi - tm.hi[tj]) + (lo - tm.lo[tj])) * tm.dt[tj];
-          m[4 * half + e] = (tj <= ti ? sc[jt][e] * f : 0.f) + (tj == ti ? D : 0.f);
+          for (int e = 0; e < 4; ++e) m[4 * half + e] = 0.f;
+          continue;
+        }
+        const f32x4 thi = *reinterpret_cast<const f32x4 *>(tm.hi + 16 * jt + 4 * q);
+        const f32x4 tlo = *reinterpret_cast<const f32x4 *>(tm.lo + 16 * jt + 4 * q);
+        const f32x4 tdt = *reinterpret_cast<const f32x4 *>(tm.dt + 16 * jt + 4 * q);
+        const f32x4 g = ST ? scores(jt) : sc[jt];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          m[4 * half + e] = g[e] * (__builtin_amdgcn_exp2f((hi - thi[e]) + (lo - tlo[e])) * tdt[e]);
+        if (jt == wi) {  // the only tile with pairs j > i, and the diagonal
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int ahead = 4 * q + e - r;
+            m[4 * half + e] = ahead > 0 ? 0.f : ahead == 0 ? m[4 * half + e] + D : m[4 * half + e];
+          }
         }
       }
-      const typename Ops<T>::Frag mf = Ops<T>::round(m);
-#pragma unroll
-      for (int i = 0; i < PP / 16; ++i) Ops<T>::mma(y[i], xa.far(f0 + 16 * i + r, 32 * jp, q), mf);
+      mf[jp] = Ops<T>::round(m);
     }
-    if (t0 + ti < a.T) {
-      T *yp = (T *)a.y + ((b * a.T + t0 + ti) * a.H + h) * a.P + p0;
+    // then Y^T, 16 features at a time
+    const Matrix<T, VEC> ym((const T *)a.y + ((b * a.T + t0) * a.H + h) * a.P + p0, (int64_t)a.H * a.P, a.T - t0, a.P - p0);
+    const float from = tm.from[ti];
 #pragma unroll
-      for (int i = 0; i < PP / 16; ++i) {
-        const float v[4] = {y[i][0], y[i][1], y[i][2], y[i][3]};
-        store4<VEC>(yp, f0 + 16 * i + 4 * q, a.P - p0, v);
+    for (int i = 0; i < PP / 16; ++i) {
+      f32x4 y = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (ST) {
+        if (any) {
+#pragma unroll
+          for (int n = 0; n < NT / 32; ++n) Ops<T>::mma(y, hl.near(f0 + 16 * i + r, 32 * n, q), cf[n]);
+          y *= from;
+        }
       }
+      Ops<T>::mma(y, xa.far(f0 + 16 * i + r, 0, q), mf[0]);
+      if (wi > 1) Ops<T>::mma(y, xa.far(f0 + 16 * i + r, 32, q), mf[1]);
+      const float v[4] = {y[0], y[1], y[2], y[3]};
+      ym.store(ti, f0 + 16 * i + 4 * q, v);
     }
     if (cc + 1 < c1 || a.final_state) {
       update_state<T, PT, NT, kWaves>(S, tm.total, tm.into, xa, ba, wave, q, r);
@@ -644,7 +697,7 @@ struct StatesLds {
 // what comes into each chunk (ds); otherwise from zero, writing what comes out and the
 // segment's decay. Pipelined like the forward kernel.
 template <class T, int PT, int NT, int PW, bool REV, bool KEEP, bool VEC>
-__global__ __launch_bounds__(256 * PW, PW == 1 ? 3 : 2) void scan_states_kernel(ScanArgs a) {
+__global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs a) {
   using L = StatesLds<T, PT, NT>;
   constexpr int kThreads = 256 * PW, kWaves = 4 * PW;
   using M = Mine<PT, NT, kWaves>;
@@ -682,8 +735,8 @@ __global__ __launch_bounds__(256 * PW, PW == 1 ? 3 : 2) void scan_states_kernel(
   auto chunk_of = [&](int n) __attribute__((always_inline)) { return REV ? c1 - 1 - n : c0 + n; };
   auto load = [&](int n) __attribute__((always_inline)) {
     const int64_t t0 = (int64_t)chunk_of(n) * Q;
-    xs.load(xg, xstride, t0, len, a.P - p0, tid);
-    ks.load(kg, kstride, t0, len, a.N, tid);
+    xs.load(Matrix<T, VEC>(xg + t0 * xstride, xstride, len - t0, a.P - p0), tid);
+    ks.load(Matrix<T, VEC>(kg + t0 * kstride, kstride, len - t0, a.N), tid);
     if (wave == 0) raw = raw_step<T>(a, b, h, t0 + lane, len);
   };
   auto step = [&](int n) __attribute__((always_inline)) {
@@ -773,14 +826,14 @@ struct StageState {
   static constexpr int kBlocks = (PT / 4) * (NT / 4), kEach = (kBlocks + THREADS - 1) / THREADS;
   f32x4 v[kEach][4];
   __device__ __forceinline__ void load(const float *base, const ScanArgs &a, int p0, int tid) {
+    const Matrix<float, VEC> m = state_rows<VEC>(base, a, p0);
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int blk = tid + e * THREADS, n = (blk % (NT / 4)) * 4, p = (blk / (NT / 4)) * 4;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         v[e][k] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (base && blk < kBlocks && p0 + p + k < a.P)
-          v[e][k] = load4<VEC>(base + (int64_t)(p0 + p + k) * a.N, n, a.N);
+        if (kBlocks % THREADS == 0 || blk < kBlocks) v[e][k] = m.load(p + k, n);
       }
     }
   }
@@ -789,7 +842,7 @@ struct StageState {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int blk = tid + e * THREADS, n = (blk % (NT / 4)) * 4, p = (blk / (NT / 4)) * 4;
-      if (blk >= kBlocks) continue;
+      if (kBlocks % THREADS && blk >= kBlocks) continue;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float along[4] = {v[e][k][0], v[e][k][1], v[e][k][2], v[e][k][3]};
@@ -809,7 +862,7 @@ struct StageState {
 // sums give for dt by the wavefront of the last 16 j: those have the fewest pairs. ST:
 // whether there are states before or after the chunk.
 template <class T, int PT, int NT, bool ST, bool VEC>
-__global__ __launch_bounds__(512, ST ? 2 : 4) void scan_grad_kernel(ScanArgs a) {
+__global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_kernel(ScanArgs a) {
   using L = GradLds<T, PT, NT, ST>;
   using O = Ops<T>;
   using BC = Tile<T, NT>;
@@ -849,8 +902,8 @@ __global__ __launch_bounds__(512, ST ? 2 : 4) void scan_grad_kernel(ScanArgs a) 
   auto load = [&](int h, int pt) __attribute__((always_inline)) {
     const int p0 = pt * PT;
     const int64_t bh = b * a.H + h;
-    xs.load((const T *)a.x + b * a.xsb + h * a.xsh + p0, a.xst, t0, len, a.P - p0, tid);
-    ys.load((const T *)a.dy + (b * a.T * a.H + h) * a.P + p0, (int64_t)a.H * a.P, t0, len, a.P - p0, tid);
+    xs.load(Matrix<T, VEC>((const T *)a.x + b * a.xsb + t0 * a.xst + h * a.xsh + p0, a.xst, len - t0, a.P - p0), tid);
+    ys.load(Matrix<T, VEC>((const T *)a.dy + ((b * a.T + t0) * a.H + h) * a.P + p0, (int64_t)a.H * a.P, len - t0, a.P - p0), tid);
     if constexpr (ST) {
       h0_next = a.chunks > 1 ? a.cs + (bh * a.chunks + c) * pn : a.initial ? a.initial + bh * pn : nullptr;
       dh_next = a.chunks > 1 ? a.ds + (bh * a.chunks + c) * pn : a.dfinal ? a.dfinal + bh * pn : nullptr;
@@ -908,8 +961,8 @@ __global__ __launch_bounds__(512, ST ? 2 : 4) void scan_grad_kernel(ScanArgs a) 
 
   {
     Stage<T, NT, 512, VEC> s, u;
-    s.load((const T *)a.b + b * a.bsb + g * a.bsg, a.bst, t0, len, a.N, tid);
-    u.load((const T *)a.c + b * a.csb + g * a.csg, a.cst, t0, len, a.N, tid);
+    s.load(Matrix<T, VEC>((const T *)a.b + b * a.bsb + t0 * a.bst + g * a.bsg, a.bst, len - t0, a.N), tid);
+    u.load(Matrix<T, VEC>((const T *)a.c + b * a.csb + t0 * a.cst + g * a.csg, a.cst, len - t0, a.N), tid);
     load(h_lo, 0);
     s.put(bn, bt, tid);
     u.put(cn, ct, tid);
@@ -956,150 +1009,168 @@ __global__ __launch_bounds__(512, ST ? 2 : 4) void scan_grad_kernel(ScanArgs a) 
     if (wave == kStepWave && pt_now == 0 && !first) finish(h_now - 1);
     if (pt_now == 0) diag = inter = col = 0.f;
 
-    f32x4 own[NT / 16];  // this head's dB^T / dt or dC^T
-#pragma unroll
-    for (int i = 0; i < NT / 16; ++i) own[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float hi = tm.hi[tw], lo = tm.lo[tw];
     if (own_j) {
-      f32x4 dx[PT / 16];
-#pragma unroll
-      for (int i = 0; i < PT / 16; ++i) dx[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       typename O::Frag bf[NT / 32], xf[PT / 32];
 #pragma unroll
       for (int k = 0; k < NT / 32; ++k) bf[k] = O::near(bn + tw * BC::kRow, 32 * k, q);
 #pragma unroll
       for (int k = 0; k < PT / 32; ++k) xf[k] = O::near(xn + tw * XY::kRow, 32 * k, q);
       const float left = tm.left[tw], dt = tm.dt[tw];
-      if (dh) {
-        const float into = left * dt;
-#pragma unroll
-        for (int i = 0; i < PT / 16; ++i) {
-#pragma unroll
-          for (int k = 0; k < NT / 32; ++k) O::mma(dx[i], dhl.near(16 * i + r, 32 * k, q), bf[k]);
-          dx[i] *= into;
-        }
-#pragma unroll
-        for (int i = 0; i < NT / 16; ++i) {
-#pragma unroll
-          for (int k = 0; k < PT / 32; ++k) {
-            if constexpr (L::two)
-              O::mma(own[i], dhtl.near(16 * i + r, 32 * k, q), xf[k]);
-            else
-              O::mma(own[i], dhl.across(16 * i + r, 32 * k, q), xf[k]);
-          }
-          own[i] *= left;
-          const typename V4<T>::type bv = *reinterpret_cast<const typename V4<T>::type *>(bn + tw * BC::kRow + 16 * i + 4 * q);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) inter += own[i][e] * (float)bv[e];
-        }
-      }
       float later = 0.f;  // the pairs (i, j) of the tiles of i after this one, without dt_j
-#pragma unroll 1
-      for (int ip = 1; 2 * ip + 1 >= mine; --ip) {
+      typename O::Frag mf[2], sf[2];  // M and Q, two tiles of i to an operand
+#pragma unroll
+      for (int ip = 1; ip >= 0; --ip) {
+        if (2 * ip + 1 < mine) break;
         float m[8], s[8];
 #pragma unroll
         for (int half = 1; half >= 0; --half) {
           const int it = 2 * ip + half;
-          f32x4 gs = {0.f, 0.f, 0.f, 0.f}, ms = gs;
-          if (it >= mine) {
+          if (it < mine) {
 #pragma unroll
-            for (int k = 0; k < NT / 32; ++k) O::mma(gs, O::near(cn + (16 * it + r) * BC::kRow, 32 * k, q), bf[k]);
-#pragma unroll
-            for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(yn + (16 * it + r) * XY::kRow, 32 * k, q), xf[k]);
+            for (int e = 0; e < 4; ++e) m[4 * half + e] = s[4 * half + e] = 0.f;
+            continue;
           }
+          f32x4 gs = {0.f, 0.f, 0.f, 0.f}, ms = gs;
+#pragma unroll
+          for (int k = 0; k < NT / 32; ++k) O::mma(gs, O::near(cn + (16 * it + r) * BC::kRow, 32 * k, q), bf[k]);
+#pragma unroll
+          for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(yn + (16 * it + r) * XY::kRow, 32 * k, q), xf[k]);
           const f32x4 thi = *reinterpret_cast<const f32x4 *>(tm.hi + 16 * it + 4 * q);
           const f32x4 tlo = *reinterpret_cast<const f32x4 *>(tm.lo + 16 * it + 4 * q);
-          float pair[4];
+          float pair[4], lower[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int ti = 16 * it + 4 * q + e;
             const float f = __builtin_amdgcn_exp2f((thi[e] - hi) + (tlo[e] - lo));
-            const float d = ti >= tw ? ms[e] * f : 0.f, gf = ti >= tw ? gs[e] * f * dt : 0.f;
-            m[4 * half + e] = gf + (ti == tw ? D : 0.f);
-            s[4 * half + e] = d;
-            pair[e] = d * gs[e];
-            diag += ti == tw ? ms[e] : 0.f;
+            m[4 * half + e] = gs[e] * (f * dt);
+            s[4 * half + e] = ms[e] * f;
           }
+          if (it == mine) {  // the only tile with pairs j > i, and the diagonal
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int ahead = r - 4 * q - e;
+              m[4 * half + e] = ahead > 0 ? 0.f : ahead == 0 ? m[4 * half + e] + D : m[4 * half + e];
+              s[4 * half + e] = ahead > 0 ? 0.f : s[4 * half + e];
+              diag += ahead == 0 ? ms[e] : 0.f;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pair[e] = s[4 * half + e] * gs[e];
           // from each i to the chunk's end, then over the j before i
           pair[2] += pair[3];
           pair[1] += pair[2];
           pair[0] += pair[1];
           const Pair rows = rows_of_half(pair[0]), both = halves(rows.first + rows.second);
           const float after = later + (q & 1 ? 0.f : rows.second) + (q < 2 ? both.second : 0.f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) lower[e] = (pair[e] + after) * dt;
+          if (it == mine) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) lower[e] = r < 4 * q + e ? lower[e] : 0.f;
+          }
           f32x4 over;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            over[e] = lanes_sum<16>(tw < 16 * it + 4 * q + e ? (pair[e] + after) * dt : 0.f);
-          if (r == 0 && it >= mine) {
+          for (int e = 0; e < 4; ++e) over[e] = lanes_sum<16>(lower[e]);
+          if (r == 0) {
             f32x4 *o = reinterpret_cast<f32x4 *>(sum.cross[mine] + 16 * it + 4 * q);
             *o = pt_now ? *o + over : over;
           }
           later += both.first + both.second;
         }
-        const typename O::Frag mf = O::round(m), sf = O::round(s);
 #pragma unroll
-        for (int i = 0; i < PT / 16; ++i) O::mma(dx[i], ya.far(16 * i + r, 32 * ip, q), mf);
-#pragma unroll
-        for (int i = 0; i < NT / 16; ++i) O::mma(own[i], ca.far(16 * i + r, 32 * ip, q), sf);
-      }
-      if (t0 + tw < a.T) {
-        T *xp = (T *)a.dx + ((b * a.T + t0 + tw) * a.H + h_now) * a.P + p0;
-#pragma unroll
-        for (int i = 0; i < PT / 16; ++i) {
-          const float v[4] = {dx[i][0], dx[i][1], dx[i][2], dx[i][3]};
-          store4<VEC>(xp, 16 * i + 4 * q, a.P - p0, v);
-        }
+        for (int e = 0; e < 8; ++e) s[e] *= dt;
+        mf[ip] = O::round(m);
+        sf[ip] = O::round(s);
       }
       col += later;
+      const float into = left * dt;
+      const Matrix<T, VEC> xm((const T *)a.dx + ((b * a.T + t0) * a.H + h_now) * a.P + p0, (int64_t)a.H * a.P, a.T - t0, a.P - p0);
 #pragma unroll
-      for (int i = 0; i < NT / 16; ++i) acc[i] += own[i] * dt;
+      for (int i = 0; i < PT / 16; ++i) {
+        f32x4 dx = {0.f, 0.f, 0.f, 0.f};
+        if (dh) {
+#pragma unroll
+          for (int k = 0; k < NT / 32; ++k) O::mma(dx, dhl.near(16 * i + r, 32 * k, q), bf[k]);
+          dx *= into;
+        }
+        if (mine < 2) O::mma(dx, ya.far(16 * i + r, 0, q), mf[0]);
+        O::mma(dx, ya.far(16 * i + r, 32, q), mf[1]);
+        const float v[4] = {dx[0], dx[1], dx[2], dx[3]};
+        xm.store(tw, 16 * i + 4 * q, v);
+      }
+#pragma unroll
+      for (int i = 0; i < NT / 16; ++i) {
+        if (dh) {
+          f32x4 u = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < PT / 32; ++k) {
+            if constexpr (L::two)
+              O::mma(u, dhtl.near(16 * i + r, 32 * k, q), xf[k]);
+            else
+              O::mma(u, dhl.across(16 * i + r, 32 * k, q), xf[k]);
+          }
+          const typename V4<T>::type bv = *reinterpret_cast<const typename V4<T>::type *>(bn + tw * BC::kRow + 16 * i + 4 * q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) inter += left * u[e] * (float)bv[e];
+          acc[i] += u * into;
+        }
+        if (mine < 2) O::mma(acc[i], ca.far(16 * i + r, 0, q), sf[0]);
+        O::mma(acc[i], ca.far(16 * i + r, 32, q), sf[1]);
+      }
     } else {
       typename O::Frag yf[PT / 32];
 #pragma unroll
       for (int k = 0; k < PT / 32; ++k) yf[k] = O::near(yn + tw * XY::kRow, 32 * k, q);
-      if (h0) {
-        const float from = tm.from[tw];
+      typename O::Frag sf[2];
 #pragma unroll
-        for (int i = 0; i < NT / 16; ++i) {
-#pragma unroll
-          for (int k = 0; k < PT / 32; ++k) {
-            if constexpr (L::two)
-              O::mma(own[i], h0l.near(16 * i + r, 32 * k, q), yf[k]);
-            else
-              O::mma(own[i], h0f.across(16 * i + r, 32 * k, q), yf[k]);
-          }
-          own[i] *= from;
-          const typename V4<T>::type cv = *reinterpret_cast<const typename V4<T>::type *>(cn + tw * BC::kRow + 16 * i + 4 * q);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) inter += own[i][e] * (float)cv[e];
-        }
-      }
-#pragma unroll 1
-      for (int jp = 0; 2 * jp <= mine; ++jp) {
+      for (int jp = 0; jp < 2; ++jp) {
+        if (2 * jp > mine) break;
         float s[8];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int jt = 2 * jp + half;
-          f32x4 ms = {0.f, 0.f, 0.f, 0.f};
-          if (jt <= mine) {
+          if (jt > mine) {
 #pragma unroll
-            for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(xn + (16 * jt + r) * XY::kRow, 32 * k, q), yf[k]);
+            for (int e = 0; e < 4; ++e) s[4 * half + e] = 0.f;
+            continue;
           }
+          f32x4 ms = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(xn + (16 * jt + r) * XY::kRow, 32 * k, q), yf[k]);
           const f32x4 thi = *reinterpret_cast<const f32x4 *>(tm.hi + 16 * jt + 4 * q);
           const f32x4 tlo = *reinterpret_cast<const f32x4 *>(tm.lo + 16 * jt + 4 * q);
           const f32x4 tdt = *reinterpret_cast<const f32x4 *>(tm.dt + 16 * jt + 4 * q);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float f = __builtin_amdgcn_exp2f((hi - thi[e]) + (lo - tlo[e])) * tdt[e];
-            s[4 * half + e] = 16 * jt + 4 * q + e <= tw ? ms[e] * f : 0.f;
+          for (int e = 0; e < 4; ++e)
+            s[4 * half + e] = ms[e] * (__builtin_amdgcn_exp2f((hi - thi[e]) + (lo - tlo[e])) * tdt[e]);
+          if (jt == mine) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * half + e] = 4 * q + e <= r ? s[4 * half + e] : 0.f;
           }
         }
-        const typename O::Frag sf = O::round(s);
-#pragma unroll
-        for (int i = 0; i < NT / 16; ++i) O::mma(own[i], ba.far(16 * i + r, 32 * jp, q), sf);
+        sf[jp] = O::round(s);
       }
+      const float from = tm.from[tw];
 #pragma unroll
-      for (int i = 0; i < NT / 16; ++i) acc[i] += own[i];
+      for (int i = 0; i < NT / 16; ++i) {
+        if (h0) {
+          f32x4 u = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < PT / 32; ++k) {
+            if constexpr (L::two)
+              O::mma(u, h0l.near(16 * i + r, 32 * k, q), yf[k]);
+            else
+              O::mma(u, h0f.across(16 * i + r, 32 * k, q), yf[k]);
+          }
+          u *= from;
+          const typename V4<T>::type cv = *reinterpret_cast<const typename V4<T>::type *>(cn + tw * BC::kRow + 16 * i + 4 * q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) inter += u[e] * (float)cv[e];
+          acc[i] += u;
+        }
+        O::mma(acc[i], ba.far(16 * i + r, 0, q), sf[0]);
+        if (mine > 1) O::mma(acc[i], ba.far(16 * i + r, 32, q), sf[1]);
+      }
     }
     if (pt_now + 1 == a.ptiles) {
       // a position's n are spread over the four lanes of one r
@@ -1120,22 +1191,21 @@ __global__ __launch_bounds__(512, ST ? 2 : 4) void scan_grad_kernel(ScanArgs a) 
   }
   __syncthreads();
   if (wave == kStepWave) finish(h_hi - 1);
-  if (t0 + tw < a.T) {
-    const int64_t row = (b * a.T + t0 + tw) * a.G + g;
-    if (a.slices == 1) {
-      T *o = (T *)(own_j ? a.db : a.dc) + row * a.N;
+  const int64_t first_row = ((b * a.T + t0) * a.G + g) * a.N;
+  if (a.slices == 1) {
+    const Matrix<T, VEC> m((const T *)(own_j ? a.db : a.dc) + first_row, (int64_t)a.G * a.N, a.T - t0, a.N);
 #pragma unroll
-      for (int i = 0; i < NT / 16; ++i) {
-        const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
-        store4<VEC>(o, 16 * i + 4 * q, a.N, v);
-      }
-    } else {
-      float *o = a.dbc + ((int64_t)(slice * 2 + !own_j) * a.B * a.T * a.G + row) * a.N;
+    for (int i = 0; i < NT / 16; ++i) {
+      const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+      m.store(tw, 16 * i + 4 * q, v);
+    }
+  } else {
+    const Matrix<float, VEC> m(a.dbc + (int64_t)(slice * 2 + !own_j) * a.B * a.T * a.G * a.N + first_row, (int64_t)a.G * a.N,
+                               a.T - t0, a.N);
 #pragma unroll
-      for (int i = 0; i < NT / 16; ++i) {
-        const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
-        store4<VEC>(o, 16 * i + 4 * q, a.N, v);
-      }
+    for (int i = 0; i < NT / 16; ++i) {
+      const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+      m.store(tw, 16 * i + 4 * q, v);
     }
   }
 }
@@ -1322,6 +1392,9 @@ ScanArgs args_of(const astra_state_scan &f) {
   a.vec = a.P % 4 == 0 && a.N % 4 == 0 && aligned(a.x, e) && aligned(a.b, e) && aligned(a.c, e) && aligned(a.y, e) &&
           aligned(a.initial, 16) && aligned(a.final_state, 16);
   for (int64_t stride : {a.xsb, a.xst, a.xsh, a.bsb, a.bst, a.bsg, a.csb, a.cst, a.csg}) a.vec = a.vec && stride % 4 == 0;
+  const int64_t most = int64_t(1) << 23;  // 64 rows' bytes stay below 2^31
+  a.vec = a.vec && a.xst >= a.P && a.xst < most && a.bst >= a.N && a.bst < most && a.cst >= a.N && a.cst < most &&
+          (int64_t)a.H * a.P < most && (int64_t)a.G * a.N < most && a.P * (int64_t)a.N < most;
   return a;
 }
 
