@@ -269,9 +269,13 @@ struct Matrix {
   int rows, n;
   __amdgpu_buffer_rsrc_t rsrc;
   __device__ __forceinline__ Matrix(const T *p, int64_t stride_, int64_t rows_, int n_)
-      : base(const_cast<T *>(p)), stride(stride_), rows(rows_ < 0 ? 0 : rows_ > 1024 ? 1024 : (int)rows_), n(n_) {
-    if constexpr (VEC)
-      rsrc = __builtin_amdgcn_make_buffer_rsrc(base, 0, rows ? ((rows - 1) * (int)stride + n) * (int)sizeof(T) : 0, 0x00020000);
+      : base(const_cast<T *>(p)), stride(stride_), rows(rows_ < 0 ? 0 : rows_ > Q ? Q : (int)rows_), n(n_) {
+    if constexpr (VEC) {
+      // (the clamps are done by vector operations, although they are the same in every lane)
+      rows = __builtin_amdgcn_readfirstlane(rows);
+      const int bytes = rows ? ((rows - 1) * (int)stride + n) * (int)sizeof(T) : 0;
+      rsrc = __builtin_amdgcn_make_buffer_rsrc(base, 0, bytes, 0x00020000);
+    }
   }
   // the offset of four elements from (row, f) on, for load and store
   __device__ __forceinline__ unsigned at(int row, int f) const {
@@ -291,6 +295,16 @@ struct Matrix {
     return r;
   }
   __device__ __forceinline__ typename V4<T>::type load(int row, int f) const { return load(row, f, at(row, f)); }
+  // the first element of a row
+  __device__ __forceinline__ T load1(int row) const {
+    const unsigned off = (unsigned)(row * (int)stride) * (unsigned)sizeof(T);
+    if constexpr (VEC && sizeof(T) == 2)
+      return __builtin_bit_cast(T, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rsrc, off, 0, 0));
+    else if constexpr (VEC)
+      return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, 0));
+    else
+      return row < rows ? base[row * stride] : (T)0.f;
+  }
   __device__ __forceinline__ void store(int row, int f, const float (&v)[4]) const {
     typename V4<T>::type r;
 #pragma unroll
@@ -311,15 +325,21 @@ struct Matrix {
 
 // F features by Q positions on their way from memory to LDS: THREADS threads hold blocks of
 // 4 positions by 4 features. What lies beyond the matrix is zero, whatever memory holds there.
+// Eight neighbouring lanes have neighbouring features, the next eight the next positions:
+// 64 bytes of a row at once, and writes along the positions that meet two to a bank instead
+// of the four that whole rows of 64 features would.
 template <class T, int F, int THREADS, bool VEC>
 struct Stage {
-  static constexpr int kGroups = F / 4, kBlocks = kGroups * (Q / 4), kEach = (kBlocks + THREADS - 1) / THREADS;
+  static_assert(F % 32 == 0 && Q == 64, "eight groups of features by sixteen of positions");
+  static constexpr int kBlocks = (F / 4) * (Q / 4), kEach = (kBlocks + THREADS - 1) / THREADS;
+  static __device__ __forceinline__ int f_of(int blk) { return ((blk & 7) | (blk >> 7) << 3) * 4; }
+  static __device__ __forceinline__ int t_of(int blk) { return ((blk >> 3) & 15) * 4; }
   typename V4<T>::type v[kEach][4];
   __device__ __forceinline__ void load(const Matrix<T, VEC> &m, int tid) {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int blk = tid + e * THREADS;
-      const int f = (blk % kGroups) * 4, t = (blk / kGroups) * 4;
+      const int f = f_of(blk), t = t_of(blk);
       unsigned off = blk < kBlocks ? m.at(t, f) : kOutside;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -334,7 +354,7 @@ struct Stage {
     for (int e = 0; e < kEach; ++e) {
       const int blk = tid + e * THREADS;
       if (kBlocks % THREADS && blk >= kBlocks) continue;
-      const int f = (blk % kGroups) * 4, t = (blk / kGroups) * 4;
+      const int f = f_of(blk), t = t_of(blk);
       if (rows) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -384,10 +404,10 @@ struct Times {
 
 __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
 
-template <class T>
-__device__ __forceinline__ float raw_step(const ScanArgs &a, int64_t b, int h, int64_t t, int len) {
-  if (t >= len) return 0.f;
-  return (float)((const T *)a.dt)[b * a.dsb + t * a.dst + h * a.dsh] + (a.bias ? a.bias[h] : 0.f);
+// dt of a head's positions from t0 on, a lane a position, before its bias.
+template <class T, bool VEC>
+__device__ __forceinline__ T raw_step(const ScanArgs &a, int64_t b, int h, int64_t t0, int len, int lane) {
+  return Matrix<T, VEC>((const T *)a.dt + b * a.dsb + t0 * a.dst + h * a.dsh, a.dst, len - t0, 1).load1(lane);
 }
 
 template <int CTRL, int ROWS = 0xf>
@@ -398,9 +418,9 @@ __device__ __forceinline__ double moved64(double v) {
   return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
-// Fills `o` from this lane's raw step; returns log2 of the chunk's decay.
-__device__ __forceinline__ double make_times(Times &o, float raw, bool live, float A, int lane) {
-  const float dt = live ? softplus(raw) : 0.f;
+// Fills `o` from this lane's dt and the head's bias and A; returns log2 of the chunk's decay.
+__device__ __forceinline__ double make_times(Times &o, float dt_raw, float bias, bool live, float A, int lane) {
+  const float raw = dt_raw + bias, dt = live ? softplus(raw) : 0.f;
   double s = (double)dt * (double)A * 1.4426950408889634;
   s += moved64<kUp + 1>(s);
   s += moved64<kUp + 2>(s);
@@ -547,46 +567,55 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void
   Stage<T, PT, kThreads, VEC> xs;
   Stage<T, NT, kThreads, VEC> bs;
   typename Ops<T>::Frag cf[NT / 32], cf_next[NT / 32];  // this position's C, read as it is used
-  float raw = 0.f;
-  int hp = (int)((int64_t)heads * part / a.parts), c = c0;  // the item that is loaded next
+  T raw = (T)0.f;
+  // the item that is loaded next: a head, its tile of features and a chunk
+  int hp = (int)((int64_t)heads * part / a.parts), c = c0;
+  int h = g * per + hp / a.ptiles, pt = hp % a.ptiles;
+  const T *xg = (const T *)a.x + b * a.xsb + (int64_t)c0 * Q * a.xst;
   auto load = [&](bool with_bc) __attribute__((always_inline)) {
-    const int h = g * per + hp / a.ptiles, p0 = (hp % a.ptiles) * PT;
     const int64_t t0 = (int64_t)c * Q;
-    xs.load(Matrix<T, VEC>((const T *)a.x + b * a.xsb + t0 * a.xst + h * a.xsh + p0, a.xst, len - t0, a.P - p0), tid);
     if (with_bc) {
-      bs.load(Matrix<T, VEC>(bg + t0 * a.bst, a.bst, len - t0, a.N), tid);
       const Matrix<T, VEC> cm(cg + t0 * a.cst, a.cst, len - t0, a.N);
 #pragma unroll
       for (int n = 0; n < NT / 32; ++n) cf_next[n] = load_near(cm, ti, 32 * n, q);
     }
-    if (wave == 0) raw = raw_step<T>(a, b, h, t0 + lane, len);
+    xs.load(Matrix<T, VEC>(xg + (t0 - (int64_t)c0 * Q) * a.xst + h * a.xsh + pt * PT, a.xst, len - t0, a.P - pt * PT), tid);
+    if (with_bc) bs.load(Matrix<T, VEC>(bg + t0 * a.bst, a.bst, len - t0, a.N), tid);
+    if (wave == 0) raw = raw_step<T, VEC>(a, b, h, t0, len, lane);
+  };
+  auto step = [&](int k) __attribute__((always_inline)) {
+    make_times(times[k & 1], (float)raw, a.bias ? a.bias[h] : 0.f, (int64_t)c * Q + lane < len, a.A[h], lane);
   };
   if (hp >= last) return;
   load(true);
-  if (wave == 0) make_times(times[0], raw, (int64_t)c * Q + lane < len, a.A[g * per + hp / a.ptiles], lane);
+  if (wave == 0) step(0);
 
   f32x4 S[M::kEach], sc[4];
   bool fresh = true, any = false;
   for (int k = 0;; ++k) {
-    const int h = g * per + hp / a.ptiles, p0 = (hp % a.ptiles) * PT;
+    const int p0 = pt * PT, cc = c, h_now = h;
     const int64_t t0 = (int64_t)c * Q, bh = b * a.H + h;
-    const int cc = c;
     const bool new_bc = fresh || c1 - c0 > 1;
     const Times &tm = times[k & 1];
-    if (c == c0) {
-      const float *start = !ST ? nullptr : a.segs > 1 ? a.seg + (bh * a.segs + seg) * pn : a.initial ? a.initial + bh * pn : nullptr;
-      load_state<PT, NT, kWaves, VEC>(S, start, a, p0, wave, q, r);
-      any = start != nullptr;
-    }
     if (k) __syncthreads();  // nobody reads the last item's tiles any more
     if constexpr (sizeof(T) == 2)
       xs.put(nullptr, xl, tid);
     else
       xs.put(xl, nullptr, tid);
     if (new_bc) {
-      bs.put(bn, bt, tid);
 #pragma unroll
       for (int n = 0; n < NT / 32; ++n) cf[n] = cf_next[n];
+      bs.put(bn, bt, tid);
+    }
+    if (c == c0) {
+      const float *start = !ST ? nullptr : a.segs > 1 ? a.seg + (bh * a.segs + seg) * pn : a.initial ? a.initial + bh * pn : nullptr;
+      any = start != nullptr;
+      if (any) {
+        load_state<PT, NT, kWaves, VEC>(S, start, a, p0, wave, q, r);
+      } else {
+#pragma unroll
+        for (int i = 0; i < M::kEach; ++i) S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
     }
     if constexpr (ST) {
       if (any) {
@@ -602,6 +631,10 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void
     if (++c == c1) {
       c = c0;
       ++hp;
+      if (++pt == a.ptiles) {
+        pt = 0;
+        ++h;
+      }
     }
     const bool more = hp < last;
     if (more) load(c1 - c0 > 1);
@@ -622,7 +655,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void
       }
     }
     fresh = false;
-    const float hi = tm.hi[ti], lo = tm.lo[ti], D = a.D ? a.D[h] : 0.f;
+    const float hi = tm.hi[ti], lo = tm.lo[ti], D = a.D ? a.D[h_now] : 0.f;
     typename Ops<T>::Frag mf[2];
 #pragma unroll
     for (int jp = 0; jp < 2; ++jp) {
@@ -654,7 +687,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void
       mf[jp] = Ops<T>::round(m);
     }
     // then Y^T, 16 features at a time
-    const Matrix<T, VEC> ym((const T *)a.y + ((b * a.T + t0) * a.H + h) * a.P + p0, (int64_t)a.H * a.P, a.T - t0, a.P - p0);
+    const Matrix<T, VEC> ym((const T *)a.y + ((b * a.T + t0) * a.H + h_now) * a.P + p0, (int64_t)a.H * a.P, a.T - t0, a.P - p0);
     const float from = tm.from[ti];
 #pragma unroll
     for (int i = 0; i < PP / 16; ++i) {
@@ -677,7 +710,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void
       if (a.final_state && cc + 1 == a.chunks) store_state<PT, NT, kWaves, VEC>(S, a.final_state + bh * pn, a, p0, wave, q, r);
     }
     if (!more) break;
-    if (wave == 0) make_times(times[(k + 1) & 1], raw, (int64_t)c * Q + lane < len, a.A[g * per + hp / a.ptiles], lane);
+    if (wave == 0) step(k + 1);
   }
 }
 
@@ -717,7 +750,7 @@ __global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs a) {
   const int64_t b = id / a.segs;
   const int g = h / (a.H / a.G), p0 = pt * PT, len = row_length(a.lengths, b, a.T);
   const int c0 = seg * a.seg_chunks, c1 = min(c0 + a.seg_chunks, a.chunks);
-  const float A = a.A[h];
+  const float A = a.A[h], bias = a.bias ? a.bias[h] : 0.f;
   const T *xg = REV ? (const T *)a.dy + (b * a.T * a.H + h) * a.P + p0 : (const T *)a.x + b * a.xsb + h * a.xsh + p0;
   const int64_t xstride = REV ? (int64_t)a.H * a.P : a.xst;
   const T *kg = REV ? (const T *)a.c + b * a.csb + g * a.csg : (const T *)a.b + b * a.bsb + g * a.bsg;
@@ -729,7 +762,7 @@ __global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs a) {
   const float *start = !KEEP ? nullptr : a.segs > 1 ? a.seg + (bh * a.segs + seg) * pn : a.dfinal ? a.dfinal + bh * pn : nullptr;
   load_state<PT, NT, kWaves, VEC>(S, start, a, p0, wave, q, r);
   double decay = 0.;
-  float raw = 0.f;
+  T raw = (T)0.f;
   Stage<T, PT, kThreads, VEC> xs;
   Stage<T, NT, kThreads, VEC> ks;
   auto chunk_of = [&](int n) __attribute__((always_inline)) { return REV ? c1 - 1 - n : c0 + n; };
@@ -737,10 +770,10 @@ __global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs a) {
     const int64_t t0 = (int64_t)chunk_of(n) * Q;
     xs.load(Matrix<T, VEC>(xg + t0 * xstride, xstride, len - t0, a.P - p0), tid);
     ks.load(Matrix<T, VEC>(kg + t0 * kstride, kstride, len - t0, a.N), tid);
-    if (wave == 0) raw = raw_step<T>(a, b, h, t0 + lane, len);
+    if (wave == 0) raw = raw_step<T, VEC>(a, b, h, t0, len, lane);
   };
   auto step = [&](int n) __attribute__((always_inline)) {
-    decay += make_times(times[n & 1], raw, (int64_t)chunk_of(n) * Q + lane < len, A, lane);
+    decay += make_times(times[n & 1], (float)raw, bias, (int64_t)chunk_of(n) * Q + lane < len, A, lane);
   };
   if (n_chunks > 0) {
     load(0);
@@ -897,7 +930,7 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
 
   Stage<T, PT, 512, VEC> xs, ys;
   StageState<PT, NT, 512, VEC> hs, ds;
-  float raw = 0.f;
+  T raw = (T)0.f;
   const float *dh_next = nullptr, *h0_next = nullptr;
   auto load = [&](int h, int pt) __attribute__((always_inline)) {
     const int p0 = pt * PT;
@@ -910,7 +943,10 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
       hs.load(h0_next, a, p0, tid);
       ds.load(dh_next, a, p0, tid);
     }
-    if (pt == 0 && wave == kTimesWave) raw = raw_step<T>(a, b, h, t0 + lane, len);
+    if (pt == 0 && wave == kTimesWave) raw = raw_step<T, VEC>(a, b, h, t0, len, lane);
+  };
+  auto step = [&](int h) __attribute__((always_inline)) {
+    make_times(times[h & 1], (float)raw, a.bias ? a.bias[h] : 0.f, live, a.A[h], lane);
   };
   // dt's gradient of head h from its sums, and the chunk's part of those of A, dt_bias and D
   auto finish = [&](int h) __attribute__((always_inline)) {
@@ -967,7 +1003,7 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
     s.put(bn, bt, tid);
     u.put(cn, ct, tid);
   }
-  if (wave == kTimesWave) make_times(times[h_lo & 1], raw, live, a.A[h_lo], lane);
+  if (wave == kTimesWave) step(h_lo);
   f32x4 acc[NT / 16];  // dB^T (rows n, columns j), or dC^T, over the heads
 #pragma unroll
   for (int i = 0; i < NT / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1187,7 +1223,7 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
       }
     }
     if (!more) break;
-    if (wave == kTimesWave && pt == 0) make_times(times[h & 1], raw, live, a.A[h], lane);
+    if (wave == kTimesWave && pt == 0) step(h);
   }
   __syncthreads();
   if (wave == kStepWave) finish(h_hi - 1);
@@ -1393,7 +1429,7 @@ ScanArgs args_of(const astra_state_scan &f) {
           aligned(a.initial, 16) && aligned(a.final_state, 16);
   for (int64_t stride : {a.xsb, a.xst, a.xsh, a.bsb, a.bst, a.bsg, a.csb, a.cst, a.csg}) a.vec = a.vec && stride % 4 == 0;
   const int64_t most = int64_t(1) << 23;  // 64 rows' bytes stay below 2^31
-  a.vec = a.vec && a.xst >= a.P && a.xst < most && a.bst >= a.N && a.bst < most && a.cst >= a.N && a.cst < most &&
+  a.vec = a.vec && a.xst >= a.P && a.xst < most && a.bst >= a.N && a.bst < most && a.cst >= a.N && a.cst < most && a.dst >= 1 && a.dst < most &&
           (int64_t)a.H * a.P < most && (int64_t)a.G * a.N < most && a.P * (int64_t)a.N < most;
   return a;
 }
