@@ -535,7 +535,7 @@ struct ForwardLds {
 // of positions, works out its step sizes. Where the segment is a single chunk, B, C and their
 // scores are loaded and computed once for all heads. ST: whether there are states before a chunk.
 template <class T, int PT, int NT, int PW, bool ST, bool VEC>
-__global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void scan_forward_kernel(ScanArgs a) {
+__global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : PT == 32 && NT == 128 ? 3 : 4) void scan_forward_kernel(ScanArgs a) {
   using L = ForwardLds<T, PT, NT, ST>;
   constexpr int kThreads = 256 * PW, kWaves = 4 * PW, PP = PT / PW;
   using M = Mine<PT, NT, kWaves>;
@@ -566,7 +566,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void
 
   Stage<T, PT, kThreads, VEC> xs;
   Stage<T, NT, kThreads, VEC> bs;
-  typename Ops<T>::Frag cf[NT / 32], cf_next[NT / 32];  // this position's C, read as it is used
+  typename Ops<T>::Frag cf[NT / 32];  // this position's C, read as it is used
   T raw = (T)0.f;
   // the item that is loaded next: a head, its tile of features and a chunk
   int hp = (int)((int64_t)heads * part / a.parts), c = c0;
@@ -574,20 +574,22 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void
   const T *xg = (const T *)a.x + b * a.xsb + (int64_t)c0 * Q * a.xst;
   auto load = [&](bool with_bc) __attribute__((always_inline)) {
     const int64_t t0 = (int64_t)c * Q;
-    if (with_bc) {
-      const Matrix<T, VEC> cm(cg + t0 * a.cst, a.cst, len - t0, a.N);
-#pragma unroll
-      for (int n = 0; n < NT / 32; ++n) cf_next[n] = load_near(cm, ti, 32 * n, q);
-    }
     xs.load(Matrix<T, VEC>(xg + (t0 - (int64_t)c0 * Q) * a.xst + h * a.xsh + pt * PT, a.xst, len - t0, a.P - pt * PT), tid);
     if (with_bc) bs.load(Matrix<T, VEC>(bg + t0 * a.bst, a.bst, len - t0, a.N), tid);
     if (wave == 0) raw = raw_step<T, VEC>(a, b, h, t0, len, lane);
+  };
+  auto load_c = [&]() __attribute__((always_inline)) {
+    const int64_t t0 = (int64_t)c * Q;
+    const Matrix<T, VEC> cm(cg + t0 * a.cst, a.cst, len - t0, a.N);
+#pragma unroll
+    for (int n = 0; n < NT / 32; ++n) cf[n] = load_near(cm, ti, 32 * n, q);
   };
   auto step = [&](int k) __attribute__((always_inline)) {
     make_times(times[k & 1], (float)raw, a.bias ? a.bias[h] : 0.f, (int64_t)c * Q + lane < len, a.A[h], lane);
   };
   if (hp >= last) return;
   load(true);
+  load_c();
   if (wave == 0) step(0);
 
   f32x4 S[M::kEach], sc[4];
@@ -602,11 +604,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void
       xs.put(nullptr, xl, tid);
     else
       xs.put(xl, nullptr, tid);
-    if (new_bc) {
-#pragma unroll
-      for (int n = 0; n < NT / 32; ++n) cf[n] = cf_next[n];
-      bs.put(bn, bt, tid);
-    }
+    if (new_bc) bs.put(bn, bt, tid);
     if (c == c0) {
       const float *start = !ST ? nullptr : a.segs > 1 ? a.seg + (bh * a.segs + seg) * pn : a.initial ? a.initial + bh * pn : nullptr;
       any = start != nullptr;
@@ -704,6 +702,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 || NT == 128 ? 2 : 3) void
       const float v[4] = {y[0], y[1], y[2], y[3]};
       ym.store(ti, f0 + 16 * i + 4 * q, v);
     }
+    if (more && c1 - c0 > 1) load_c();  // this item's is done with
     if (cc + 1 < c1 || a.final_state) {
       update_state<T, PT, NT, kWaves>(S, tm.total, tm.into, xa, ba, wave, q, r);
       any = true;
@@ -1129,6 +1128,7 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
           for (int k = 0; k < NT / 32; ++k) O::mma(dx, dhl.near(16 * i + r, 32 * k, q), bf[k]);
           dx *= into;
         }
+        if (i & 1) __builtin_amdgcn_sched_barrier(0);  // (reads further ahead cost more registers than there are)
         if (mine < 2) O::mma(dx, ya.far(16 * i + r, 0, q), mf[0]);
         O::mma(dx, ya.far(16 * i + r, 32, q), mf[1]);
         const float v[4] = {dx[0], dx[1], dx[2], dx[3]};
@@ -1150,6 +1150,7 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
           for (int e = 0; e < 4; ++e) inter += left * u[e] * (float)bv[e];
           acc[i] += u * into;
         }
+        if (i & 1) __builtin_amdgcn_sched_barrier(0);
         if (mine < 2) O::mma(acc[i], ca.far(16 * i + r, 0, q), sf[0]);
         O::mma(acc[i], ca.far(16 * i + r, 32, q), sf[1]);
       }
@@ -1204,6 +1205,7 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
           for (int e = 0; e < 4; ++e) inter += u[e] * (float)cv[e];
           acc[i] += u;
         }
+        if (i & 1) __builtin_amdgcn_sched_barrier(0);
         O::mma(acc[i], ba.far(16 * i + r, 0, q), sf[0]);
         if (mine > 1) O::mma(acc[i], ba.far(16 * i + r, 32, q), sf[1]);
       }
@@ -1408,8 +1410,8 @@ ScanArgs args_of(const astra_state_scan &f) {
   a.ptiles = (int32_t)cdiv(f.dim, tiles.p);
   a.chunks = (int32_t)cdiv(f.length, Q);
   // few rows: the length is split into segments, joined by their states; as many workgroups
-  // as are resident at once (two a CU, one of the largest tiles)
-  const int64_t resident = tiles.pw == 2 ? 256 : 512;
+  // as are resident at once (two a CU)
+  const int64_t resident = 512;
   const int64_t rows = a.B * a.H * a.ptiles;
   int64_t segs = 1;
   if (rows > 0 && rows < resident) segs = cdiv(resident, rows);
