@@ -48,48 +48,60 @@ __device__ __forceinline__ void load_input(const ConvArgs &a, int64_t b, int64_t
   }
 }
 
-// One thread: V channels, `run` positions, the last K-1 inputs in registers.
+// One thread: V channels, `run` positions, the last K-1 inputs in registers. U positions at
+// a time, so that their loads are in flight together; where all of them count, without a
+// check each.
 template <class T, int K, int V>
 __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a) {
+  constexpr int U = 4;
   const int groups = a.D / V;
   const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t row = item / groups;
   const int d = (int)(item - row * groups) * V;
   const int64_t b = row / a.runs;
   if (b >= a.B) return;
-  const int64_t t0 = (row - b * a.runs) * a.run;
-  const int64_t t1 = t0 + a.run < a.T ? t0 + a.run : a.T;
+  const int t0 = (int)(row - b * a.runs) * a.run;
+  const int t1 = (int)min((int64_t)t0 + a.run, a.T);
   const int len = row_length(a.lengths, b, a.T);
-  float w[K][V], bias[V], win[K - 1][V];
+  float w[K][V], bias[V], in[K - 1 + U][V];  // entry K-1+u is position t+u
   load_taps<K, V>(a, d, w, bias);
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) load_input<T, K, V>(a, b, t0 - (K - 1) + k, len, d, win[k]);
-  T *y = (T *)a.y + (b * a.T) * a.D + d;
-  constexpr int U = 4;  // positions whose loads are in flight together
-  for (int64_t t = t0; t < t1; t += U) {
-    float in[U][V];
-#pragma unroll
-    for (int u = 0; u < U; ++u) load_input<T, K, V>(a, b, t + u, len, d, in[u]);
+  for (int k = 0; k < K - 1; ++k) load_input<T, K, V>(a, b, t0 - (K - 1) + k, len, d, in[k]);
+  const T *x = (const T *)a.x + b * a.xsb + (int64_t)t0 * a.xst + d;
+  T *y = (T *)a.y + (b * a.T + t0) * a.D + d;
+  const int64_t xst = a.xst, yst = a.D;
+  auto outputs = [&](int t, bool all) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (t + u >= t1) break;
+      if (!all && t + u >= t1) break;
       float out[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float p = bias[i];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const int at = u - (K - 1) + k;  // < 0: in the window of what came before
-          p += w[k][i] * (at < 0 ? win[at + K - 1][i] : in[at < 0 ? 0 : at][i]);
-        }
-        out[i] = t + u < len ? (a.silu ? p * sigmoid(p) : p) : 0.f;
+        for (int k = 0; k < K; ++k) p += w[k][i] * in[u + k][i];
+        out[i] = a.silu ? p * sigmoid(p) : p;
+        if (!all) out[i] = t + u < len ? out[i] : 0.f;
       }
-      Vec<T, V>::store(y + (t + u) * a.D, out);
+      Vec<T, V>::store(y + u * yst, out);
     }
 #pragma unroll
     for (int k = 0; k < K - 1; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[k][i] = in[U - (K - 1) + k][i];
+      for (int i = 0; i < V; ++i) in[k][i] = in[k + U][i];
+    x += U * xst;
+    y += U * yst;
+  };
+  int t = t0;
+  for (const int full = min(t1, len); t + U <= full; t += U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) Vec<T, V>::load(x + u * xst, in[K - 1 + u]);
+    outputs(t, true);
+  }
+  for (; t < t1; t += U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_input<T, K, V>(a, b, t + u, len, d, in[K - 1 + u]);
+    outputs(t, false);
   }
   if (a.last && t0 == 0) {
 #pragma unroll
@@ -105,7 +117,8 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a) {
 // A workgroup: CX groups of V channels by 256 / CX rows; a row of threads walks runs of
 // positions, `gridDim.y` rows of workgroups apart, and keeps its part of dw and dbias in
 // registers. A run recomputes the K-1 values of g after its end. U positions at a time, so
-// that their loads are in flight together and the windows of x and g need no moves.
+// that their loads are in flight together and the windows of x and g need few moves; inside
+// a run without a check each.
 constexpr int kConvCols = 16;
 template <class T, int K, int V>
 __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
@@ -126,8 +139,8 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
   const int64_t rows = a.B * a.runs;
   for (int64_t row = (int64_t)blockIdx.y * IY + iy; row < rows && live; row += (int64_t)gridDim.y * IY) {
     const int64_t b = row / a.runs;
-    const int64_t t0 = (row - b * a.runs) * a.run;
-    const int64_t t1 = t0 + a.run < a.T ? t0 + a.run : a.T;
+    const int t0 = (int)(row - b * a.runs) * a.run;
+    const int t1 = (int)min((int64_t)t0 + a.run, a.T);
     const int len = row_length(a.lengths, b, a.T);
     float in[K - 1 + U][V], g[K - 1 + U][V];  // entry K-1+u is position t+u
 #pragma unroll
@@ -138,20 +151,13 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) g[k][i] = 0.f;
     }
-    for (int64_t t = t0; t < t1 + K - 1; t += U) {
-      float dy[U][V];
+    const T *x = (const T *)a.x + b * a.xsb + (int64_t)t0 * a.xst + d;
+    const T *dyp = (const T *)a.dy + (b * a.T + t0) * a.D + d;
+    T *dx = (T *)a.dx + (b * a.T + t0 - (K - 1)) * a.D + d;
+    float dy[U][V];
+    auto gradients = [&](int t, bool all) __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        load_input<T, K, V>(a, b, t + u, len, d, in[K - 1 + u]);
-        if (t + u < len)
-          Vec<T, V>::load((const T *)a.dy + (b * a.T + t + u) * a.D + d, dy[u]);
-        else
-#pragma unroll
-          for (int i = 0; i < V; ++i) dy[u][i] = 0.f;
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool mine = t + u < t1;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           float v = dy[u][i];
@@ -160,24 +166,28 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
 #pragma unroll
             for (int k = 0; k < K; ++k) p += w[k][i] * in[u + k][i];
             const float s = sigmoid(p);
-            v *= s * (1.f + p * (1.f - s));
+            v *= s + p * (s - s * s);
           }
-          v = t + u < len ? v : 0.f;
+          if (!all) v = t + u < len ? v : 0.f;
           g[K - 1 + u][i] = v;
-          const float own = mine ? v : 0.f;
-          db[i] += own;
+          if (!all) v = t + u < t1 ? v : 0.f;
+          db[i] += v;
 #pragma unroll
-          for (int k = 0; k < K; ++k) dw[k][i] += own * in[u + k][i];
+          for (int k = 0; k < K; ++k) dw[k][i] += v * in[u + k][i];
         }
         // the gradient of the input at t + u - (K-1); before 0 it is the window's
-        const int64_t at = t + u - (K - 1);
-        if (t + u >= t1 + K - 1 || (at < t0 && t0 > 0)) continue;
+        const int at = t + u - (K - 1);
+        if (!all && (t + u >= t1 + K - 1 || (at < t0 && t0 > 0))) continue;
         float o[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           o[i] = 0.f;
 #pragma unroll
           for (int k = 0; k < K; ++k) o[i] += w[k][i] * g[K - 1 + u - k][i];
+        }
+        if (all) {
+          if (a.dx) Vec<T, V>::store(dx + (int64_t)u * a.D, o);
+          continue;
         }
         // position len - (K-1) + k is row k of `last`
         if (a.dlast && at < len && t + u >= len) {
@@ -191,7 +201,7 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
             if (at >= len)
 #pragma unroll
               for (int i = 0; i < V; ++i) o[i] = 0.f;
-            Vec<T, V>::store((T *)a.dx + (b * a.T + at) * a.D + d, o);
+            Vec<T, V>::store(dx + (int64_t)u * a.D, o);
           }
         } else if (a.dwindow) {
           Vec<T, V>::store((T *)a.dwindow + (b * (K - 1) + t + u) * a.D + d, o);
@@ -204,6 +214,33 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
           in[k][i] = in[k + U][i];
           g[k][i] = g[k + U][i];
         }
+      x += U * a.xst;
+      dyp += (int64_t)U * a.D;
+      dx += (int64_t)U * a.D;
+    };
+    // the first U positions write the window, or nothing; from the last ones on, some do
+    // not count
+    int t = t0;
+    for (const int full = min(t1, len); t < t1 + K - 1; t += U) {
+      if (t > t0 && t + U <= full) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          Vec<T, V>::load(x + u * a.xst, in[K - 1 + u]);
+          Vec<T, V>::load(dyp + (int64_t)u * a.D, dy[u]);
+        }
+        gradients(t, true);
+        continue;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        load_input<T, K, V>(a, b, t + u, len, d, in[K - 1 + u]);
+        if (t + u < len)
+          Vec<T, V>::load(dyp + (int64_t)u * a.D, dy[u]);
+        else
+#pragma unroll
+          for (int i = 0; i < V; ++i) dy[u][i] = 0.f;
+      }
+      gradients(t, false);
     }
   }
   if (!a.part) return;
@@ -304,14 +341,14 @@ ConvArgs args_of(const astra_short_conv &f) {
 }
 
 // Positions a thread walks: long runs reread less of their neighbours (K-1 inputs each),
-// short ones give every CU work where the batch is small.
+// short ones give every CU work where the batch is small. Runs of a row are alike, and of
+// whole groups of four positions.
 void set_runs(ConvArgs &a, int64_t threads_per_position) {
   int64_t run = 64;
   while (run > 8 && a.B * cdiv(a.T, run) * threads_per_position < 256 * 1024) run /= 2;
-  if (run > a.T) run = a.T;
-  a.run = (int32_t)(run > 0 ? run : 1);
-  a.runs = (int32_t)cdiv(a.T, a.run);
-  if (a.runs < 1) a.runs = 1;
+  const int64_t runs = a.T > 0 ? cdiv(a.T, run) : 1;
+  a.run = (int32_t)(a.T > 0 ? cdiv(cdiv(a.T, runs), 4) * 4 : 1);
+  a.runs = (int32_t)(a.T > 0 ? cdiv(a.T, a.run) : 1);
 }
 
 // Accesses of V elements where every row starts on one.

@@ -813,12 +813,22 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(ScanArgs a) {
   const int64_t bh = i / pn, e = i - bh * pn;
   const float *from = REV ? a.dfinal : a.initial;
   float carry = from ? from[i] : 0.f;
-  for (int n = 0; n < a.segs; ++n) {
-    const int s = REV ? a.segs - 1 - n : n;
-    float *p = a.seg + (bh * a.segs + s) * pn + e;
-    const float own = *p;
-    *p = carry;
-    carry = __builtin_amdgcn_exp2f(a.seg_log2[bh * a.segs + s]) * carry + own;
+  float *p = a.seg + bh * a.segs * pn + e;
+  const float *log2 = a.seg_log2 + bh * a.segs;
+  for (int n0 = 0; n0 < a.segs; n0 += 8) {  // eight loads in flight at a time
+    float own[8], decay[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int s = REV ? a.segs - 1 - n0 - k : n0 + k;
+      own[k] = n0 + k < a.segs ? p[s * pn] : 0.f;
+      decay[k] = n0 + k < a.segs ? log2[s] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (n0 + k >= a.segs) break;
+      p[(REV ? a.segs - 1 - n0 - k : n0 + k) * pn] = carry;
+      carry = __builtin_amdgcn_exp2f(decay[k]) * carry + own[k];
+    }
   }
 }
 
