@@ -54,7 +54,7 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found; the HIP engine cannot be built")
 
 
-BINDING_SRC = os.path.join(CSRC, "bindings.cpp")
+BINDING_SRCS = [os.path.join(CSRC, f) for f in ("bindings.cpp", "sequence_bindings.cpp")]
 
 
 def binding_path() -> str:
@@ -64,8 +64,9 @@ def binding_path() -> str:
 
 def build_binding(verbose: bool = False) -> str:
     """Compile the pybind11 module astra_cuda._C (csrc/bindings.cpp, the reference's
-    market_bindings.cc surface over the C ABI) against torch's headers and libraries,
-    linked to libastra_market.so in the same directory. Always recompiles."""
+    market_bindings.cc surface over the C ABI, and csrc/sequence_bindings.cpp, the compiled
+    half of astra_cuda.sequence) against torch's headers and libraries, linked to
+    libastra_market.so in the same directory. Always recompiles."""
     import sysconfig
     import torch
     tdir = os.path.dirname(torch.__file__)
@@ -74,20 +75,18 @@ def build_binding(verbose: bool = False) -> str:
     out = binding_path()
     tmp = out + ".tmp"
     cxx = os.environ.get("CXX", "g++")
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           *(f"-I{d}" for d in incs), BINDING_SRC,
-           f"-L{os.path.join(tdir, 'lib')}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
-           "-ltorch_python", f"-L{PKG_DIR}", "-l:" + LIB_NAME,
-           # the engine library next to the module, and torch's libraries
-           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{os.path.join(tdir, 'lib')}", "-o", tmp]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"{cxx} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             *(f"-I{d}" for d in incs)]
+    with tempfile.TemporaryDirectory() as d:
+        objs = [os.path.join(d, os.path.basename(s) + ".o") for s in BINDING_SRCS]
+        cmds = [[cxx, *flags, "-c", src, "-o", obj] for src, obj in zip(BINDING_SRCS, objs)]
+        with concurrent.futures.ThreadPoolExecutor(len(cmds)) as pool:
+            list(pool.map(lambda c: _run(c, verbose), cmds))
+        _run([cxx, "-shared", *objs, f"-L{os.path.join(tdir, 'lib')}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
+              "-ltorch_hip", "-ltorch_python", f"-L{PKG_DIR}", "-l:" + LIB_NAME,
+              # the engine library next to the module, and torch's libraries
+              "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{os.path.join(tdir, 'lib')}", "-o", tmp], verbose)
     os.replace(tmp, out)
     return out
 
@@ -111,7 +110,7 @@ def _run(cmd: list, verbose: bool) -> None:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
 
 
 if __name__ == "__main__":

@@ -10,7 +10,8 @@
 // Every call runs on PyTorch's current HIP stream of the market's device. The
 // book lives in a workspace tensor the market owns; FillBatch and BBOBatch hold
 // their tensors as plain fields (def_readwrite, as in the reference).
-#include <torch/extension.h>
+#include "bindings.h"
+
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -374,4 +375,5 @@ PYBIND11_MODULE(_C, m) {
   om.attr("MAX_ACTIVE_FILLS_PER_MARKET") = ASTRA_MAX_ACTIVE_FILLS_PER_MARKET;
   om.attr("NULL_INDEX") = ASTRA_NULL_INDEX;
   om.attr("MAX_CUSTOMERS") = ASTRA_MAX_CUSTOMERS;
+  bind_sequence(m);
 }
