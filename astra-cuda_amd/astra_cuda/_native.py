@@ -46,6 +46,10 @@ PROTOTYPES = {
     "astra_high_low_trade_scratch": (_c_int, [_vp, _vp, _vp]),
     "astra_high_low_observation": (_c_int, [_vp, _vp]),
     "astra_high_low_rewards": (_c_int, [_vp, ctypes.c_int64, _c_i32, _c_i32, _vp, _vp]),
+}
+
+# include/sequence/astra_sequence.h
+SEQUENCE_PROTOTYPES = {
     "astra_short_conv_forward": (_c_int, [_vp, _vp]),
     "astra_short_conv_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
     "astra_short_conv_backward": (_c_int, [_vp, _vp]),
@@ -91,24 +95,24 @@ def _fields(pointers: str, sizes: str, ints: str) -> list:
 
 
 class ShortConv(ctypes.Structure):
-    """astra_short_conv (include/astra_sequence.h)."""
+    """astra_short_conv (include/sequence/astra_sequence.h)."""
     _fields_ = _fields("x weight bias window lengths y last", "batch length x_stride_b x_stride_t",
                        "width taps type activation")
 
 
 class ShortConvGrad(ctypes.Structure):
-    """astra_short_conv_grad (include/astra_sequence.h)."""
+    """astra_short_conv_grad (include/sequence/astra_sequence.h)."""
     _fields_ = [("f", ShortConv)] + _fields("dy dlast dx dwindow dweight dbias workspace", "", "") + [
         ("workspace_bytes", _sz)]
 
 
 class ShortConvOne(ctypes.Structure):
-    """astra_short_conv_one (include/astra_sequence.h)."""
+    """astra_short_conv_one (include/sequence/astra_sequence.h)."""
     _fields_ = _fields("x weight bias window y", "batch x_stride_b", "width taps type activation")
 
 
 class StateScan(ctypes.Structure):
-    """astra_state_scan (include/astra_sequence.h)."""
+    """astra_state_scan (include/sequence/astra_sequence.h)."""
     _fields_ = _fields("x dt b c A D dt_bias initial lengths y final_state chunk_states",
                        "batch length x_stride_b x_stride_t x_stride_h dt_stride_b dt_stride_t dt_stride_h "
                        "b_stride_b b_stride_t b_stride_g c_stride_b c_stride_t c_stride_g",
@@ -116,27 +120,27 @@ class StateScan(ctypes.Structure):
 
 
 class StateScanGrad(ctypes.Structure):
-    """astra_state_scan_grad (include/astra_sequence.h)."""
+    """astra_state_scan_grad (include/sequence/astra_sequence.h)."""
     _fields_ = [("f", StateScan)] + _fields("dy dfinal dx ddt db dc dA dD ddt_bias dinitial workspace", "", "") + [
         ("workspace_bytes", _sz)]
 
 
 class StateScanOne(ctypes.Structure):
-    """astra_state_scan_one (include/astra_sequence.h)."""
+    """astra_state_scan_one (include/sequence/astra_sequence.h)."""
     _fields_ = _fields("x dt b c A D dt_bias h y",
                        "batch x_stride_b x_stride_h dt_stride_b dt_stride_h b_stride_b b_stride_g c_stride_b "
                        "c_stride_g", "heads dim groups state type")
 
 
 class JoinNorm(ctypes.Structure):
-    """astra_join_norm (include/astra_sequence.h)."""
+    """astra_join_norm (include/sequence/astra_sequence.h)."""
     _fields_ = _fields("residual block gate post next scale joined normed rstd",
                        "rows residual_stride block_stride gate_stride",
                        "width gate_width scale_width type residual_type") + [("eps", ctypes.c_float)]
 
 
 class JoinNormGrad(ctypes.Structure):
-    """astra_join_norm_grad (include/astra_sequence.h)."""
+    """astra_join_norm_grad (include/sequence/astra_sequence.h)."""
     _fields_ = [("f", JoinNorm)] + _fields("djoined dnormed dresidual dblock dgate dpost dnext dscale workspace",
                                            "", "") + [("workspace_bytes", _sz)]
 
@@ -153,7 +157,7 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build the HIP engine first "
                 "(python astra-cuda_amd/astra_cuda/build.py or __graft_entry__.build())")
         L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in PROTOTYPES.items():
+        for name, (res, args) in {**PROTOTYPES, **SEQUENCE_PROTOTYPES}.items():
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

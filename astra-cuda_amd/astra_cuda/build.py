@@ -2,7 +2,7 @@
 
 Sources: ``csrc/market.hip`` (the VecMarket engine, include/astra_market.h),
 ``csrc/high_low.hip`` (the high-low game's move kernels, include/astra_high_low.h) and
-``csrc/sequence_*.hip`` (the policies' sequence operators, include/astra_sequence.h).
+``csrc/sequence_*.hip`` (the policies' sequence operators, include/sequence/astra_sequence.h).
 
 Usage: ``python astra-cuda_amd/astra_cuda/build.py`` or ``astra_cuda.build.build()``.
 The library links the HIP runtime by its SONAME (libamdhip64.so.7); imported after

@@ -2,7 +2,7 @@
 
 A game of hidden information asks a policy to remember the moves it has seen. These
 operators are one layer of such a policy, over whole games in training and a move at a
-time in rollouts with a state of fixed size per env (include/astra_sequence.h):
+time in rollouts with a state of fixed size per env (include/sequence/astra_sequence.h):
 
 ``short_conv``       every channel filtered by its own few taps, causally, then SiLU
 ``state_scan``       a selective state space scan: per head a decaying state, with input,

@@ -3,7 +3,7 @@
 // ends every gradient of a parameter.
 #pragma once
 
-#include "astra_sequence.h"
+#include "sequence/astra_sequence.h"
 #include "runtime.h"
 
 namespace astra_seq {

@@ -1,5 +1,5 @@
 // sequence_bindings.cpp -- the compiled half of astra_cuda.sequence: argument checks, output
-// and workspace tensors, the calls of include/astra_sequence.h on PyTorch's current stream,
+// and workspace tensors, the calls of include/sequence/astra_sequence.h on PyTorch's current stream,
 // and the autograd nodes around them. In C++ because a call of one position, or a backward
 // pass on autograd's own thread, takes less time on the GPU than a Python body would.
 #include "bindings.h"
@@ -8,7 +8,7 @@
 
 #include <optional>
 
-#include "astra_sequence.h"
+#include "sequence/astra_sequence.h"
 
 namespace py = pybind11;
 
