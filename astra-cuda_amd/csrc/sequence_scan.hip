@@ -97,11 +97,18 @@ struct Ops<bf16> {
   struct Split3 {
     bf16x8 hi, mid, lo;
   };
-  static __device__ __forceinline__ Frag round(const float (&v)[8]) {
-    Frag f;
+  static __device__ __forceinline__ Split split(const float (&v)[8]) {
+    Split s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (bf16)v[i];
-    return f;
+    for (int i = 0; i < 8; ++i) {
+      s.hi[i] = (bf16)v[i];
+      s.lo[i] = (bf16)(v[i] - (float)s.hi[i]);
+    }
+    return s;
+  }
+  static __device__ __forceinline__ void mma(f32x4 &acc, const Frag &a, const Split &b) {
+    mma(acc, a, b.lo);
+    mma(acc, a, b.hi);
   }
   static __device__ __forceinline__ Split3 split3(const float (&v)[8]) {
     Split3 s;
@@ -148,13 +155,13 @@ struct Ops<float> {
     }
     return f;
   }
-  static __device__ __forceinline__ Frag round(const float (&v)[8]) {
-    Frag s;
+  static __device__ __forceinline__ Split split(const float (&v)[8]) {
+    Split s;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s.v[i] = v[i];
     return s;
   }
-  static __device__ __forceinline__ Split3 split3(const float (&v)[8]) { return round(v); }
+  static __device__ __forceinline__ Split3 split3(const float (&v)[8]) { return split(v); }
   static __device__ __forceinline__ void expand(const Frag &f, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = f.v[i];
@@ -654,7 +661,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : PT == 32 && NT == 12
     }
     fresh = false;
     const float hi = tm.hi[ti], lo = tm.lo[ti], D = a.D ? a.D[h_now] : 0.f;
-    typename Ops<T>::Frag mf[2];
+    typename Ops<T>::Split mf[2];
 #pragma unroll
     for (int jp = 0; jp < 2; ++jp) {
       if (2 * jp > wi) break;
@@ -682,7 +689,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : PT == 32 && NT == 12
           }
         }
       }
-      mf[jp] = Ops<T>::round(m);
+      mf[jp] = Ops<T>::split(m);
     }
     // then Y^T, 16 features at a time
     const Matrix<T, VEC> ym((const T *)a.y + ((b * a.T + t0) * a.H + h_now) * a.P + p0, (int64_t)a.H * a.P, a.T - t0, a.P - p0);
@@ -904,7 +911,7 @@ struct StageState {
 // sums give for dt by the wavefront of the last 16 j: those have the fewest pairs. ST:
 // whether there are states before or after the chunk.
 template <class T, int PT, int NT, bool ST, bool VEC>
-__global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_kernel(ScanArgs a) {
+__global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) void scan_grad_kernel(ScanArgs a) {
   using L = GradLds<T, PT, NT, ST>;
   using O = Ops<T>;
   using BC = Tile<T, NT>;
@@ -937,20 +944,23 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
   const int mine = wave & 3, tw = 16 * mine + r;  // this lane's position
   const bool live = t0 + lane < len;
 
-  Stage<T, PT, 512, VEC> xs, ys;
-  StageState<PT, NT, 512, VEC> hs, ds;
+  // one half of the workgroup brings x and the state, the other dY and the state's gradient
+  const bool lower = wave < 4;
+  const int ht = tid & 255;
+  Stage<T, PT, 256, VEC> xy;
+  StageState<PT, NT, 256, VEC> hd;
   T raw = (T)0.f;
   const float *dh_next = nullptr, *h0_next = nullptr;
   auto load = [&](int h, int pt) __attribute__((always_inline)) {
     const int p0 = pt * PT;
     const int64_t bh = b * a.H + h;
-    xs.load(Matrix<T, VEC>((const T *)a.x + b * a.xsb + t0 * a.xst + h * a.xsh + p0, a.xst, len - t0, a.P - p0), tid);
-    ys.load(Matrix<T, VEC>((const T *)a.dy + ((b * a.T + t0) * a.H + h) * a.P + p0, (int64_t)a.H * a.P, len - t0, a.P - p0), tid);
+    const T *row = lower ? (const T *)a.x + b * a.xsb + t0 * a.xst + h * a.xsh + p0
+                         : (const T *)a.dy + ((b * a.T + t0) * a.H + h) * a.P + p0;
+    xy.load(Matrix<T, VEC>(row, lower ? a.xst : (int64_t)a.H * a.P, len - t0, a.P - p0), ht);
     if constexpr (ST) {
       h0_next = a.chunks > 1 ? a.cs + (bh * a.chunks + c) * pn : a.initial ? a.initial + bh * pn : nullptr;
       dh_next = a.chunks > 1 ? a.ds + (bh * a.chunks + c) * pn : a.dfinal ? a.dfinal + bh * pn : nullptr;
-      hs.load(h0_next, a, p0, tid);
-      ds.load(dh_next, a, p0, tid);
+      hd.load(lower ? h0_next : dh_next, a, p0, ht);
     }
     if (pt == 0 && wave == kTimesWave) raw = raw_step<T, VEC>(a, b, h, t0, len, lane);
   };
@@ -1026,23 +1036,17 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
     const bool dh = ST && dh_next, h0 = ST && h0_next;
     const float D = a.D ? a.D[h] : 0.f;
     if (!first) __syncthreads();
-    xs.put(xn, nullptr, tid);
-    ys.put(yn, yt, tid);
+    if (lower)
+      xy.put(xn, nullptr, ht);
+    else
+      xy.put(yn, yt, ht);
     if constexpr (ST) {
-      if constexpr (L::two) {
-        hs.put((const StateTile<T, PT, NT, 1> *)nullptr, &h0l, tid);
-        ds.put(&dhl, &dhtl, tid);
-      } else {
-        hs.put(&h0f, (const StateTile<T, NT, PT, 2> *)nullptr, tid);
-        ds.put(&dhl, (const StateTile<T, NT, PT, 2> *)nullptr, tid);
-      }
-      if (pt == 0) dot = 0.f;
-#pragma unroll
-      for (int e = 0; e < hs.kEach; ++e)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dot += hs.v[e][k][i] * ds.v[e][k][i];
+      using Rows = const StateTile<T, PT, NT, 1> *;
+      using Cols = const StateTile<T, NT, PT, 2> *;
+      if (lower)
+        hd.put(L::two ? (Rows) nullptr : &h0f, L::two ? &h0l : (Cols) nullptr, ht);
+      else
+        hd.put(&dhl, L::two ? &dhtl : (Cols) nullptr, ht);
     }
     __syncthreads();
     if (++pt == a.ptiles) {
@@ -1052,7 +1056,21 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
     const bool more = h < h_hi;
     if (more) load(h, pt);
     if (wave == kStepWave && pt_now == 0 && !first) finish(h_now - 1);
-    if (pt_now == 0) diag = inter = col = 0.f;
+    if (pt_now == 0) diag = inter = col = dot = 0.f;
+    if (dh && h0) {
+      for (int i = tid; i < PT * NT / 8; i += 512) {
+        float u[8], v[8];
+        if constexpr (L::two) {
+          h0l.get8(i / (PT / 8), i % (PT / 8) * 8, u);
+          dhtl.get8(i / (PT / 8), i % (PT / 8) * 8, v);
+        } else {
+          h0f.get8(i / (NT / 8), i % (NT / 8) * 8, u);
+          dhl.get8(i / (NT / 8), i % (NT / 8) * 8, v);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot += u[e] * v[e];
+      }
+    }
 
     const float hi = tm.hi[tw], lo = tm.lo[tw];
     if (own_j) {
@@ -1063,7 +1081,7 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
       for (int k = 0; k < PT / 32; ++k) xf[k] = O::near(xn + tw * XY::kRow, 32 * k, q);
       const float left = tm.left[tw], dt = tm.dt[tw];
       float later = 0.f;  // the pairs (i, j) of the tiles of i after this one, without dt_j
-      typename O::Frag mf[2], sf[2];  // M and Q, two tiles of i to an operand
+      typename O::Split mf[2], sf[2];  // M and Q, two tiles of i to an operand
 #pragma unroll
       for (int ip = 1; ip >= 0; --ip) {
         if (2 * ip + 1 < mine) break;
@@ -1124,8 +1142,8 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] *= dt;
-        mf[ip] = O::round(m);
-        sf[ip] = O::round(s);
+        mf[ip] = O::split(m);
+        sf[ip] = O::split(s);
       }
       col += later;
       const float into = left * dt;
@@ -1168,7 +1186,7 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
       typename O::Frag yf[PT / 32];
 #pragma unroll
       for (int k = 0; k < PT / 32; ++k) yf[k] = O::near(yn + tw * XY::kRow, 32 * k, q);
-      typename O::Frag sf[2];
+      typename O::Split sf[2];
 #pragma unroll
       for (int jp = 0; jp < 2; ++jp) {
         if (2 * jp > mine) break;
@@ -1195,7 +1213,7 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 ? 2 : 4) void scan_grad_k
             for (int e = 0; e < 4; ++e) s[4 * half + e] = 4 * q + e <= r ? s[4 * half + e] : 0.f;
           }
         }
-        sf[jp] = O::round(s);
+        sf[jp] = O::split(s);
       }
       const float from = tm.from[tw];
 #pragma unroll
