@@ -405,6 +405,10 @@ struct Times {
   float from[Q], left[Q];     // exp(s_t), exp(s_Q - s_t)
   float into[Q];              // dt exp(s_Q - s_t): what a position's input counts after the chunk
   float slope[Q];             // the step's derivative by dt_raw, 0 where no position counts
+  // Between tiles of 16 positions exp(s_i - s_j) is a product by way of the end e of j's
+  // tile (both factors are at most 1 where A <= 0, and small only where the product is):
+  float past[3][Q];           // exp(s_i - s_e) for i after tile 0, 1, 2
+  float till[Q];              // exp(s_e - s_j) dt_j for j's own tile
   float total;                // exp(s_Q)
   float pad[3];
 };
@@ -435,11 +439,19 @@ __device__ __forceinline__ double make_times(Times &o, float dt_raw, float bias,
   s += moved64<kUp + 8>(s);
   s += moved64<kBcast15, 0xa>(s);
   s += moved64<kBcast31, 0xc>(s);
-  const int64_t last = __builtin_bit_cast(int64_t, s);
-  const uint32_t tl = (uint32_t)__builtin_amdgcn_readlane((int)last, Q - 1);
-  const uint32_t th = (uint32_t)__builtin_amdgcn_readlane((int)(last >> 32), Q - 1);
-  const double total = __builtin_bit_cast(double, ((uint64_t)th << 32) | tl);
+  double ends[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t at = __builtin_bit_cast(int64_t, s);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)at, 16 * i + 15);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), 16 * i + 15);
+    ends[i] = __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+    if (i < 3) o.past[i][lane] = __builtin_amdgcn_exp2f((float)(s - ends[i]));
+  }
+  const double total = ends[3];
   const float left = __builtin_amdgcn_exp2f((float)(total - s));
+  const double end = lane < 32 ? (lane < 16 ? ends[0] : ends[1]) : (lane < 48 ? ends[2] : ends[3]);
+  o.till[lane] = dt * __builtin_amdgcn_exp2f((float)(end - s));
   o.dt[lane] = dt;
   o.hi[lane] = (float)s;
   o.lo[lane] = (float)(s - (double)(float)s);
@@ -542,7 +554,7 @@ struct ForwardLds {
 // of positions, works out its step sizes. Where the segment is a single chunk, B, C and their
 // scores are loaded and computed once for all heads. ST: whether there are states before a chunk.
 template <class T, int PT, int NT, int PW, bool ST, bool VEC>
-__global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : PT == 32 && NT == 128 ? 3 : 4) void scan_forward_kernel(ScanArgs a) {
+__global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 128) || (PT == 64 && NT == 64 && !ST) ? 3 : 4) void scan_forward_kernel(ScanArgs a) {
   using L = ForwardLds<T, PT, NT, ST>;
   constexpr int kThreads = 256 * PW, kWaves = 4 * PW, PP = PT / PW;
   using M = Mine<PT, NT, kWaves>;
@@ -674,19 +686,23 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : PT == 32 && NT == 12
           for (int e = 0; e < 4; ++e) m[4 * half + e] = 0.f;
           continue;
         }
+        const f32x4 g = ST ? scores(jt) : sc[jt];
+        if (jt < wi) {
+          const float past = tm.past[jt][ti];
+          const f32x4 till = *reinterpret_cast<const f32x4 *>(tm.till + 16 * jt + 4 * q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) m[4 * half + e] = g[e] * (past * till[e]);
+          continue;
+        }
+        // the only tile with pairs j > i, and the diagonal
         const f32x4 thi = *reinterpret_cast<const f32x4 *>(tm.hi + 16 * jt + 4 * q);
         const f32x4 tlo = *reinterpret_cast<const f32x4 *>(tm.lo + 16 * jt + 4 * q);
         const f32x4 tdt = *reinterpret_cast<const f32x4 *>(tm.dt + 16 * jt + 4 * q);
-        const f32x4 g = ST ? scores(jt) : sc[jt];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          m[4 * half + e] = g[e] * (__builtin_amdgcn_exp2f((hi - thi[e]) + (lo - tlo[e])) * tdt[e]);
-        if (jt == wi) {  // the only tile with pairs j > i, and the diagonal
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int ahead = 4 * q + e - r;
-            m[4 * half + e] = ahead > 0 ? 0.f : ahead == 0 ? m[4 * half + e] + D : m[4 * half + e];
-          }
+        for (int e = 0; e < 4; ++e) {
+          const int ahead = 4 * q + e - r;
+          const float v = g[e] * (__builtin_amdgcn_exp2f((hi - thi[e]) + (lo - tlo[e])) * tdt[e]);
+          m[4 * half + e] = ahead > 0 ? 0.f : ahead == 0 ? v + D : v;
         }
       }
       mf[jp] = Ops<T>::split(m);
@@ -1080,7 +1096,8 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) voi
 #pragma unroll
       for (int k = 0; k < PT / 32; ++k) xf[k] = O::near(xn + tw * XY::kRow, 32 * k, q);
       const float left = tm.left[tw], dt = tm.dt[tw];
-      float later = 0.f;  // the pairs (i, j) of the tiles of i after this one, without dt_j
+      float later = 0.f;  // the pairs (i, j) of the tiles of i after this one
+      const float till = tm.till[tw];
       typename O::Split mf[2], sf[2];  // M and Q, two tiles of i to an operand
 #pragma unroll
       for (int ip = 1; ip >= 0; --ip) {
@@ -1099,53 +1116,52 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) voi
           for (int k = 0; k < NT / 32; ++k) O::mma(gs, O::near(cn + (16 * it + r) * BC::kRow, 32 * k, q), bf[k]);
 #pragma unroll
           for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(yn + (16 * it + r) * XY::kRow, 32 * k, q), xf[k]);
-          const f32x4 thi = *reinterpret_cast<const f32x4 *>(tm.hi + 16 * it + 4 * q);
-          const f32x4 tlo = *reinterpret_cast<const f32x4 *>(tm.lo + 16 * it + 4 * q);
-          float pair[4], lower[4];
+          float pair[4];  // with dt_j
+          if (it > mine) {
+            const f32x4 past = *reinterpret_cast<const f32x4 *>(tm.past[mine] + 16 * it + 4 * q);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float f = __builtin_amdgcn_exp2f((thi[e] - hi) + (tlo[e] - lo));
-            m[4 * half + e] = gs[e] * (f * dt);
-            s[4 * half + e] = ms[e] * f;
-          }
-          if (it == mine) {  // the only tile with pairs j > i, and the diagonal
+            for (int e = 0; e < 4; ++e) {
+              const float f = past[e] * till;
+              m[4 * half + e] = gs[e] * f;
+              s[4 * half + e] = ms[e] * f;
+              pair[e] = s[4 * half + e] * gs[e];
+            }
+          } else {  // the only tile with pairs j > i, and the diagonal
+            const f32x4 thi = *reinterpret_cast<const f32x4 *>(tm.hi + 16 * it + 4 * q);
+            const f32x4 tlo = *reinterpret_cast<const f32x4 *>(tm.lo + 16 * it + 4 * q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int ahead = r - 4 * q - e;
-              m[4 * half + e] = ahead > 0 ? 0.f : ahead == 0 ? m[4 * half + e] + D : m[4 * half + e];
-              s[4 * half + e] = ahead > 0 ? 0.f : s[4 * half + e];
+              const float f = __builtin_amdgcn_exp2f((thi[e] - hi) + (tlo[e] - lo)) * dt;
+              const float v = gs[e] * f, u = ms[e] * f;
+              m[4 * half + e] = ahead > 0 ? 0.f : ahead == 0 ? v + D : v;
+              s[4 * half + e] = ahead > 0 ? 0.f : u;
+              pair[e] = s[4 * half + e] * gs[e];
               diag += ahead == 0 ? ms[e] : 0.f;
             }
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pair[e] = s[4 * half + e] * gs[e];
           // from each i to the chunk's end, then over the j before i
           pair[2] += pair[3];
           pair[1] += pair[2];
           pair[0] += pair[1];
           const Pair rows = rows_of_half(pair[0]), both = halves(rows.first + rows.second);
           const float after = later + (q & 1 ? 0.f : rows.second) + (q < 2 ? both.second : 0.f);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) lower[e] = (pair[e] + after) * dt;
-          if (it == mine) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) lower[e] = r < 4 * q + e ? lower[e] : 0.f;
-          }
           f32x4 over;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) over[e] = lanes_sum<16>(lower[e]);
+          for (int e = 0; e < 4; ++e) {
+            const float v = pair[e] + after;
+            over[e] = lanes_sum<16>(it > mine || r < 4 * q + e ? v : 0.f);
+          }
           if (r == 0) {
             f32x4 *o = reinterpret_cast<f32x4 *>(sum.cross[mine] + 16 * it + 4 * q);
             *o = pt_now ? *o + over : over;
           }
           later += both.first + both.second;
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] *= dt;
         mf[ip] = O::split(m);
         sf[ip] = O::split(s);
       }
-      col += later;
+      col += dt > 0.f ? later / dt : 0.f;  // (a step of 0 has a slope of 0)
       const float into = left * dt;
       const Matrix<T, VEC> xm((const T *)a.dx + ((b * a.T + t0) * a.H + h_now) * a.P + p0, (int64_t)a.H * a.P, a.T - t0, a.P - p0);
 #pragma unroll
@@ -1202,15 +1218,20 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) voi
           f32x4 ms = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(xn + (16 * jt + r) * XY::kRow, 32 * k, q), yf[k]);
+          if (jt < mine) {
+            const float past = tm.past[jt][tw];
+            const f32x4 till = *reinterpret_cast<const f32x4 *>(tm.till + 16 * jt + 4 * q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * half + e] = ms[e] * (past * till[e]);
+            continue;
+          }
           const f32x4 thi = *reinterpret_cast<const f32x4 *>(tm.hi + 16 * jt + 4 * q);
           const f32x4 tlo = *reinterpret_cast<const f32x4 *>(tm.lo + 16 * jt + 4 * q);
           const f32x4 tdt = *reinterpret_cast<const f32x4 *>(tm.dt + 16 * jt + 4 * q);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s[4 * half + e] = ms[e] * (__builtin_amdgcn_exp2f((hi - thi[e]) + (lo - tlo[e])) * tdt[e]);
-          if (jt == mine) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * half + e] = 4 * q + e <= r ? s[4 * half + e] : 0.f;
+          for (int e = 0; e < 4; ++e) {
+            const float v = ms[e] * (__builtin_amdgcn_exp2f((hi - thi[e]) + (lo - tlo[e])) * tdt[e]);
+            s[4 * half + e] = 4 * q + e <= r ? v : 0.f;
           }
         }
         sf[jp] = O::split(s);
