@@ -73,7 +73,8 @@ struct ScanArgs {
 // One operand of a product over 32 values of the contracted index k, for lane (q = lane / 16,
 // r = lane % 16): row (or column) r and 8 values of k. Which 8 is free as long as both
 // operands agree: 8q..8q+7 ("near"), or 4q..4q+3 and 16+4q..16+4q+3 ("far"), which is how
-// two results of 16 rows each hold them.
+// two results of 16 rows each hold them. Features of floats are near in the far order, so
+// that a block with 16 or fewer of them is half the instructions.
 struct FragF {
   float v[8];
 };
@@ -132,6 +133,11 @@ struct Ops<bf16> {
     mma(acc, a.lo, b);
     mma(acc, a.hi, b);
   }
+  // a product over features of which `left` are left: nothing is saved within a block
+  template <class A, class B>
+  static __device__ __forceinline__ void mma_left(f32x4 &acc, const A &a, const B &b, int) {
+    mma(acc, a, b);
+  }
   static __device__ __forceinline__ void mma(f32x4 &acc, const Split3 &a, const Frag &b) {
     mma(acc, a.lo, b);
     mma(acc, a.mid, b);
@@ -146,8 +152,8 @@ struct Ops<float> {
   using Split3 = FragF;
   static __device__ __forceinline__ Frag near(const float *row, int k0, int q) {
     Frag f;
-    const f32x4 a = *reinterpret_cast<const f32x4 *>(row + k0 + 8 * q);
-    const f32x4 b = *reinterpret_cast<const f32x4 *>(row + k0 + 8 * q + 4);
+    const f32x4 a = *reinterpret_cast<const f32x4 *>(row + k0 + 4 * q);
+    const f32x4 b = *reinterpret_cast<const f32x4 *>(row + k0 + 16 + 4 * q);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f.v[i] = a[i];
@@ -170,12 +176,32 @@ struct Ops<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
   }
+  static __device__ __forceinline__ void mma_left(f32x4 &acc, const Frag &a, const Frag &b, int left) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
+    if (left <= 16) return;
+#pragma unroll
+    for (int i = 4; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
+  }
 };
 
 template <class T>
 struct V4 {
   typedef T type __attribute__((ext_vector_type(4)));
 };
+
+// Whether the 16 (or 32) rows, columns or contracted values from `at` on hold any of the `n`
+// that count, and how many are left of them. Looked at for floats with up to 32 states only,
+// where a state of 16 halves the products: in the larger tiles, and for bf16, the branches
+// cost more registers than the skipped instructions are worth.
+template <class T, int NT>
+__device__ __forceinline__ bool on(int at, int n) {
+  return !(sizeof(T) == 4 && NT == 32) || at < n;
+}
+template <class T, int NT>
+__device__ __forceinline__ int rest(int n) {
+  return sizeof(T) == 4 && NT == 32 ? n : 32;
+}
 
 // A tile of F features by Q positions in LDS, read along its features (`rows`: position
 // major) or along its positions. bf16 operands are read 16 bytes at a time, so each order
@@ -236,7 +262,7 @@ struct StateTile {
   __device__ __forceinline__ FragF across(int k, int r0, int q) const {
     FragF s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s.v[i] = p[(r0 + 8 * q + i) * kRow + k];
+    for (int i = 0; i < 8; ++i) s.v[i] = p[(r0 + 4 * q + (i & 3) + 16 * (i >> 2)) * kRow + k];
     return s;
   }
   __device__ __forceinline__ void put4(int r, int k, const float (&v)[4]) const {
@@ -251,12 +277,10 @@ struct StateTile {
   }
   // the 8 values from element i on, as floats
   __device__ __forceinline__ void get8(int r, int k, float (&v)[8]) const {
-    Ops<T>::expand(Ops<T>::near(p + r * kRow, k, 0), v);
-    if constexpr (kTwo) {
-      float lo[8];
-      Ops<T>::expand(Ops<T>::near(p + R * kRow + r * kRow, k, 0), lo);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += lo[i];
+    for (int i = 0; i < 8; ++i) {
+      v[i] = (float)p[r * kRow + k + i];
+      if constexpr (kTwo) v[i] += (float)p[R * kRow + r * kRow + k + i];
     }
   }
 };
@@ -380,10 +404,11 @@ struct Stage {
   }
 };
 
-// A row's 8 elements from f + 8 q on (an operand that is read from memory as it is).
+// A row's 8 elements of a near operand from feature f on, read from memory as they are.
 template <class T, bool VEC>
 __device__ __forceinline__ typename Ops<T>::Frag load_near(const Matrix<T, VEC> &m, int row, int f, int q) {
-  const typename V4<T>::type a = m.load(row, f + 8 * q), b = m.load(row, f + 8 * q + 4);
+  const bool far = sizeof(T) == 4;
+  const typename V4<T>::type a = m.load(row, f + (far ? 4 : 8) * q), b = m.load(row, f + (far ? 16 + 4 * q : 8 * q + 4));
   typename Ops<T>::Frag r;
   if constexpr (sizeof(T) == 2) {
     r = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -485,10 +510,11 @@ struct Mine {
   static __device__ __forceinline__ int p_of(int wave, int i, int r) { return ((wave + WAVES * i) / kN) * 16 + r; }
 };
 
-// S = total S + X^T (weight K): X over PT features, K over NT, weight a position's.
+// S = total S + X^T (weight K): X over PT features of which `np` count, K over NT of which
+// `nn` count, weight a position's.
 template <class T, int PT, int NT, int WAVES>
 __device__ __forceinline__ void update_state(f32x4 *S, float total, const float *weight, const Along<T, PT> &X,
-                                             const Along<T, NT> &K, int wave, int q, int r) {
+                                             const Along<T, NT> &K, int wave, int q, int r, int np, int nn) {
   using M = Mine<PT, NT, WAVES>;
 #pragma unroll
   for (int i = 0; i < M::kEach; ++i) S[i] *= total;
@@ -500,6 +526,7 @@ __device__ __forceinline__ void update_state(f32x4 *S, float total, const float 
     typename Ops<T>::Split3 kf;
 #pragma unroll
     for (int i = 0; i < M::kEach; ++i) {
+      if (!on<T, NT>(16 * M::nt_of(wave, i), nn) || !on<T, NT>(M::p_of(wave, i, 0), np)) continue;
       if (i == 0 || !M::kOneN) {
         float v[8];
         Ops<T>::expand(K.near(16 * M::nt_of(wave, i) + r, t0, q), v);
@@ -661,7 +688,8 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int n = 0; n < NT / 32; ++n)
-        Ops<T>::mma(v, Ops<T>::near(bn + (16 * jt + r) * Tile<T, NT>::kRow, 32 * n, q), cf[n]);
+        if (on<T, NT>(32 * n, a.N))
+          Ops<T>::mma_left(v, Ops<T>::near(bn + (16 * jt + r) * Tile<T, NT>::kRow, 32 * n, q), cf[n], rest<T, NT>(a.N - 32 * n));
       return v;
     };
     if constexpr (!ST) {
@@ -712,11 +740,13 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
     const float from = tm.from[ti];
 #pragma unroll
     for (int i = 0; i < PP / 16; ++i) {
+      if (!on<T, NT>(f0 + 16 * i, a.P - p0)) continue;
       f32x4 y = {0.f, 0.f, 0.f, 0.f};
       if constexpr (ST) {
         if (any) {
 #pragma unroll
-          for (int n = 0; n < NT / 32; ++n) Ops<T>::mma(y, hl.near(f0 + 16 * i + r, 32 * n, q), cf[n]);
+          for (int n = 0; n < NT / 32; ++n)
+            if (on<T, NT>(32 * n, a.N)) Ops<T>::mma_left(y, hl.near(f0 + 16 * i + r, 32 * n, q), cf[n], rest<T, NT>(a.N - 32 * n));
           y *= from;
         }
       }
@@ -727,7 +757,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
     }
     if (more && c1 - c0 > 1) load_c();  // this item's is done with
     if (cc + 1 < c1 || a.final_state) {
-      update_state<T, PT, NT, kWaves>(S, tm.total, tm.into, xa, ba, wave, q, r);
+      update_state<T, PT, NT, kWaves>(S, tm.total, tm.into, xa, ba, wave, q, r, a.P - p0, a.N);
       any = true;
       if (a.final_state && cc + 1 == a.chunks) store_state<PT, NT, kWaves, VEC>(S, a.final_state + bh * pn, a, p0, wave, q, r);
     }
@@ -814,7 +844,7 @@ __global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs a) {
     __syncthreads();
     if (n + 1 < n_chunks) load(n + 1);
     if (KEEP && a.chunks > 1) store_state<PT, NT, kWaves, VEC>(S, a.ds + (bh * a.chunks + chunk_of(n)) * pn, a, p0, wave, q, r);
-    update_state<T, PT, NT, kWaves>(S, tm.total, REV ? tm.from : tm.into, xa, ka, wave, q, r);
+    update_state<T, PT, NT, kWaves>(S, tm.total, REV ? tm.from : tm.into, xa, ka, wave, q, r, a.P - p0, a.N);
     if (wave == 0 && n + 1 < n_chunks) step(n + 1);
   }
   if (!KEEP) {
@@ -927,7 +957,7 @@ struct StageState {
 // sums give for dt by the wavefront of the last 16 j: those have the fewest pairs. ST:
 // whether there are states before or after the chunk.
 template <class T, int PT, int NT, bool ST, bool VEC>
-__global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) void scan_grad_kernel(ScanArgs a) {
+__global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) void scan_grad_kernel(ScanArgs a) {
   using L = GradLds<T, PT, NT, ST>;
   using O = Ops<T>;
   using BC = Tile<T, NT>;
@@ -1046,7 +1076,7 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) voi
 
   int h = h_lo, pt = 0;
   for (bool first = true;; first = false) {
-    const int p0 = pt * PT, h_now = h, pt_now = pt;
+    const int p0 = pt * PT, np = a.P - p0, h_now = h, pt_now = pt;
     const Times &tm = times[h & 1];
     HeadSums &sum = sums[h & 1];
     const bool dh = ST && dh_next, h0 = ST && h0_next;
@@ -1113,9 +1143,11 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) voi
           }
           f32x4 gs = {0.f, 0.f, 0.f, 0.f}, ms = gs;
 #pragma unroll
-          for (int k = 0; k < NT / 32; ++k) O::mma(gs, O::near(cn + (16 * it + r) * BC::kRow, 32 * k, q), bf[k]);
+          for (int k = 0; k < NT / 32; ++k)
+            if (on<T, NT>(32 * k, a.N)) O::mma_left(gs, O::near(cn + (16 * it + r) * BC::kRow, 32 * k, q), bf[k], rest<T, NT>(a.N - 32 * k));
 #pragma unroll
-          for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(yn + (16 * it + r) * XY::kRow, 32 * k, q), xf[k]);
+          for (int k = 0; k < PT / 32; ++k)
+            if (on<T, NT>(32 * k, np)) O::mma_left(ms, O::near(yn + (16 * it + r) * XY::kRow, 32 * k, q), xf[k], rest<T, NT>(np - 32 * k));
           float pair[4];  // with dt_j
           if (it > mine) {
             const f32x4 past = *reinterpret_cast<const f32x4 *>(tm.past[mine] + 16 * it + 4 * q);
@@ -1166,10 +1198,12 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) voi
       const Matrix<T, VEC> xm((const T *)a.dx + ((b * a.T + t0) * a.H + h_now) * a.P + p0, (int64_t)a.H * a.P, a.T - t0, a.P - p0);
 #pragma unroll
       for (int i = 0; i < PT / 16; ++i) {
+        if (!on<T, NT>(16 * i, np)) continue;
         f32x4 dx = {0.f, 0.f, 0.f, 0.f};
         if (dh) {
 #pragma unroll
-          for (int k = 0; k < NT / 32; ++k) O::mma(dx, dhl.near(16 * i + r, 32 * k, q), bf[k]);
+          for (int k = 0; k < NT / 32; ++k)
+            if (on<T, NT>(32 * k, a.N)) O::mma_left(dx, dhl.near(16 * i + r, 32 * k, q), bf[k], rest<T, NT>(a.N - 32 * k));
           dx *= into;
         }
         if (i & 1) __builtin_amdgcn_sched_barrier(0);  // (reads further ahead cost more registers than there are)
@@ -1180,14 +1214,16 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) voi
       }
 #pragma unroll
       for (int i = 0; i < NT / 16; ++i) {
+        if (!on<T, NT>(16 * i, a.N)) continue;
         if (dh) {
           f32x4 u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < PT / 32; ++k) {
+            if (!on<T, NT>(32 * k, np)) continue;
             if constexpr (L::two)
-              O::mma(u, dhtl.near(16 * i + r, 32 * k, q), xf[k]);
+              O::mma_left(u, dhtl.near(16 * i + r, 32 * k, q), xf[k], rest<T, NT>(np - 32 * k));
             else
-              O::mma(u, dhl.across(16 * i + r, 32 * k, q), xf[k]);
+              O::mma_left(u, dhl.across(16 * i + r, 32 * k, q), xf[k], rest<T, NT>(np - 32 * k));
           }
           const typename V4<T>::type bv = *reinterpret_cast<const typename V4<T>::type *>(bn + tw * BC::kRow + 16 * i + 4 * q);
 #pragma unroll
@@ -1217,7 +1253,8 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) voi
           }
           f32x4 ms = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < PT / 32; ++k) O::mma(ms, O::near(xn + (16 * jt + r) * XY::kRow, 32 * k, q), yf[k]);
+          for (int k = 0; k < PT / 32; ++k)
+            if (on<T, NT>(32 * k, np)) O::mma_left(ms, O::near(xn + (16 * jt + r) * XY::kRow, 32 * k, q), yf[k], rest<T, NT>(np - 32 * k));
           if (jt < mine) {
             const float past = tm.past[jt][tw];
             const f32x4 till = *reinterpret_cast<const f32x4 *>(tm.till + 16 * jt + 4 * q);
@@ -1239,14 +1276,16 @@ __global__ __launch_bounds__(512, ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) voi
       const float from = tm.from[tw];
 #pragma unroll
       for (int i = 0; i < NT / 16; ++i) {
+        if (!on<T, NT>(16 * i, a.N)) continue;
         if (h0) {
           f32x4 u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < PT / 32; ++k) {
+            if (!on<T, NT>(32 * k, np)) continue;
             if constexpr (L::two)
-              O::mma(u, h0l.near(16 * i + r, 32 * k, q), yf[k]);
+              O::mma_left(u, h0l.near(16 * i + r, 32 * k, q), yf[k], rest<T, NT>(np - 32 * k));
             else
-              O::mma(u, h0f.across(16 * i + r, 32 * k, q), yf[k]);
+              O::mma_left(u, h0f.across(16 * i + r, 32 * k, q), yf[k], rest<T, NT>(np - 32 * k));
           }
           u *= from;
           const typename V4<T>::type cv = *reinterpret_cast<const typename V4<T>::type *>(cn + tw * BC::kRow + 16 * i + 4 * q);
