@@ -68,6 +68,22 @@ struct ScanArgs {
   bool vec;  // 4 elements of every row can be accessed at once
 };
 
+// A kernel's arguments where they were passed, and the same for one more round of a loop:
+// what the loop takes from them is loaded again (from the scalar cache) instead of being
+// kept for all rounds, for which there are not enough scalar registers: they would be moved
+// to and from lanes of vector registers, one instruction a word.
+template <class A>
+__device__ __forceinline__ const A *arguments() {
+  return (const A *)__builtin_amdgcn_kernarg_segment_ptr();
+}
+template <class A>
+__device__ __forceinline__ const A *again(const A *p) {
+  typedef const __attribute__((address_space(4))) A *Constant;
+  Constant c = (Constant)p;
+  asm volatile("" : "+s"(c));
+  return (const A *)c;
+}
+
 // ---------------------------------------------------------------- operands of the products
 
 // One operand of a product over 32 values of the contracted index k, for lane (q = lane / 16,
@@ -581,7 +597,9 @@ struct ForwardLds {
 // of positions, works out its step sizes. Where the segment is a single chunk, B, C and their
 // scores are loaded and computed once for all heads. ST: whether there are states before a chunk.
 template <class T, int PT, int NT, int PW, bool ST, bool VEC>
-__global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 128) || (PT == 64 && NT == 64 && !ST) ? 3 : 4) void scan_forward_kernel(ScanArgs a) {
+__global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 128) || (PT == 64 && NT == 64 && !ST) ? 3 : 4) void scan_forward_kernel(ScanArgs args) {
+  (void)args;
+  const ScanArgs *ap = arguments<ScanArgs>();
   using L = ForwardLds<T, PT, NT, ST>;
   constexpr int kThreads = 256 * PW, kWaves = 4 * PW, PP = PT / PW;
   using M = Mine<PT, NT, kWaves>;
@@ -596,42 +614,42 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave & 3, f0 = (wave >> 2) * PP;
   const int ti = 16 * wi + r;  // this lane's position
   int64_t id = workgroup_id();
-  const int per = a.H / a.G, heads = per * a.ptiles;  // a group's heads and tiles of features
-  const int part = (int)(id % a.parts);
-  id /= a.parts;
-  const int g = (int)(id % a.G);
-  id /= a.G;
-  const int seg = (int)(id % a.segs);
-  const int64_t b = id / a.segs;
-  const int len = row_length(a.lengths, b, a.T);
-  const int c0 = seg * a.seg_chunks, c1 = min(c0 + a.seg_chunks, a.chunks);
-  const int last = (int)((int64_t)heads * (part + 1) / a.parts);
-  const int64_t pn = (int64_t)a.P * a.N;
-  const T *bg = (const T *)a.b + b * a.bsb + g * a.bsg;
-  const T *cg = (const T *)a.c + b * a.csb + g * a.csg;
+  const int per = ap->H / ap->G, heads = per * ap->ptiles;  // a group's heads and tiles of features
+  const int part = (int)(id % ap->parts);
+  id /= ap->parts;
+  const int g = (int)(id % ap->G);
+  id /= ap->G;
+  const int seg = (int)(id % ap->segs);
+  const int64_t b = id / ap->segs;
+  const int len = row_length(ap->lengths, b, ap->T);
+  const int c0 = seg * ap->seg_chunks, c1 = min(c0 + ap->seg_chunks, ap->chunks);
+  const int last = (int)((int64_t)heads * (part + 1) / ap->parts);
+  const int64_t pn = (int64_t)ap->P * ap->N;
+  const T *bg = (const T *)ap->b + b * ap->bsb + g * ap->bsg;
+  const T *cg = (const T *)ap->c + b * ap->csb + g * ap->csg;
 
   Stage<T, PT, kThreads, VEC> xs;
   Stage<T, NT, kThreads, VEC> bs;
   typename Ops<T>::Frag cf[NT / 32];  // this position's C, read as it is used
   T raw = (T)0.f;
   // the item that is loaded next: a head, its tile of features and a chunk
-  int hp = (int)((int64_t)heads * part / a.parts), c = c0;
-  int h = g * per + hp / a.ptiles, pt = hp % a.ptiles;
-  const T *xg = (const T *)a.x + b * a.xsb + (int64_t)c0 * Q * a.xst;
+  int hp = (int)((int64_t)heads * part / ap->parts), c = c0;
+  int h = g * per + hp / ap->ptiles, pt = hp % ap->ptiles;
+  const T *xg = (const T *)ap->x + b * ap->xsb + (int64_t)c0 * Q * ap->xst;
   auto load = [&](bool with_bc) __attribute__((always_inline)) {
     const int64_t t0 = (int64_t)c * Q;
-    xs.load(Matrix<T, VEC>(xg + (t0 - (int64_t)c0 * Q) * a.xst + h * a.xsh + pt * PT, a.xst, len - t0, a.P - pt * PT), tid);
-    if (with_bc) bs.load(Matrix<T, VEC>(bg + t0 * a.bst, a.bst, len - t0, a.N), tid);
-    if (wave == 0) raw = raw_step<T, VEC>(a, b, h, t0, len, lane);
+    xs.load(Matrix<T, VEC>(xg + (t0 - (int64_t)c0 * Q) * ap->xst + h * ap->xsh + pt * PT, ap->xst, len - t0, ap->P - pt * PT), tid);
+    if (with_bc) bs.load(Matrix<T, VEC>(bg + t0 * ap->bst, ap->bst, len - t0, ap->N), tid);
+    if (wave == 0) raw = raw_step<T, VEC>(*ap, b, h, t0, len, lane);
   };
   auto load_c = [&]() __attribute__((always_inline)) {
     const int64_t t0 = (int64_t)c * Q;
-    const Matrix<T, VEC> cm(cg + t0 * a.cst, a.cst, len - t0, a.N);
+    const Matrix<T, VEC> cm(cg + t0 * ap->cst, ap->cst, len - t0, ap->N);
 #pragma unroll
     for (int n = 0; n < NT / 32; ++n) cf[n] = load_near(cm, ti, 32 * n, q);
   };
   auto step = [&](int k) __attribute__((always_inline)) {
-    make_times(times[k & 1], (float)raw, a.bias ? a.bias[h] : 0.f, (int64_t)c * Q + lane < len, a.A[h], lane);
+    make_times(times[k & 1], (float)raw, ap->bias ? ap->bias[h] : 0.f, (int64_t)c * Q + lane < len, ap->A[h], lane);
   };
   if (hp >= last) return;
   load(true);
@@ -641,8 +659,9 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
   f32x4 S[M::kEach], sc[4];
   bool fresh = true, any = false;
   for (int k = 0;; ++k) {
+    ap = again(ap);
     const int p0 = pt * PT, cc = c, h_now = h;
-    const int64_t t0 = (int64_t)c * Q, bh = b * a.H + h;
+    const int64_t t0 = (int64_t)c * Q, bh = b * ap->H + h;
     const bool new_bc = fresh || c1 - c0 > 1;
     const Times &tm = times[k & 1];
     if (k) __syncthreads();  // nobody reads the last item's tiles any more
@@ -652,10 +671,10 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
       xs.put(xl, nullptr, tid);
     if (new_bc) bs.put(bn, bt, tid);
     if (c == c0) {
-      const float *start = !ST ? nullptr : a.segs > 1 ? a.seg + (bh * a.segs + seg) * pn : a.initial ? a.initial + bh * pn : nullptr;
+      const float *start = !ST ? nullptr : ap->segs > 1 ? ap->seg + (bh * ap->segs + seg) * pn : ap->initial ? ap->initial + bh * pn : nullptr;
       any = start != nullptr;
       if (any) {
-        load_state<PT, NT, kWaves, VEC>(S, start, a, p0, wave, q, r);
+        load_state<PT, NT, kWaves, VEC>(S, start, *ap, p0, wave, q, r);
       } else {
 #pragma unroll
         for (int i = 0; i < M::kEach; ++i) S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -669,13 +688,13 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
           hl.put4(M::p_of(wave, i, r), M::n_of(wave, i, q), v);
         }
       }
-      if (a.cs) store_state<PT, NT, kWaves, VEC>(S, a.cs + (bh * a.chunks + c) * pn, a, p0, wave, q, r);
+      if (ap->cs) store_state<PT, NT, kWaves, VEC>(S, ap->cs + (bh * ap->chunks + c) * pn, *ap, p0, wave, q, r);
     }
     __syncthreads();
     if (++c == c1) {
       c = c0;
       ++hp;
-      if (++pt == a.ptiles) {
+      if (++pt == ap->ptiles) {
         pt = 0;
         ++h;
       }
@@ -688,8 +707,8 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int n = 0; n < NT / 32; ++n)
-        if (on<T, NT>(32 * n, a.N))
-          Ops<T>::mma_left(v, Ops<T>::near(bn + (16 * jt + r) * Tile<T, NT>::kRow, 32 * n, q), cf[n], rest<T, NT>(a.N - 32 * n));
+        if (on<T, NT>(32 * n, ap->N))
+          Ops<T>::mma_left(v, Ops<T>::near(bn + (16 * jt + r) * Tile<T, NT>::kRow, 32 * n, q), cf[n], rest<T, NT>(ap->N - 32 * n));
       return v;
     };
     if constexpr (!ST) {
@@ -700,7 +719,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
       }
     }
     fresh = false;
-    const float hi = tm.hi[ti], lo = tm.lo[ti], D = a.D ? a.D[h_now] : 0.f;
+    const float hi = tm.hi[ti], lo = tm.lo[ti], D = ap->D ? ap->D[h_now] : 0.f;
     typename Ops<T>::Split mf[2];
 #pragma unroll
     for (int jp = 0; jp < 2; ++jp) {
@@ -736,17 +755,17 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
       mf[jp] = Ops<T>::split(m);
     }
     // then Y^T, 16 features at a time
-    const Matrix<T, VEC> ym((const T *)a.y + ((b * a.T + t0) * a.H + h_now) * a.P + p0, (int64_t)a.H * a.P, a.T - t0, a.P - p0);
+    const Matrix<T, VEC> ym((const T *)ap->y + ((b * ap->T + t0) * ap->H + h_now) * ap->P + p0, (int64_t)ap->H * ap->P, ap->T - t0, ap->P - p0);
     const float from = tm.from[ti];
 #pragma unroll
     for (int i = 0; i < PP / 16; ++i) {
-      if (!on<T, NT>(f0 + 16 * i, a.P - p0)) continue;
+      if (!on<T, NT>(f0 + 16 * i, ap->P - p0)) continue;
       f32x4 y = {0.f, 0.f, 0.f, 0.f};
       if constexpr (ST) {
         if (any) {
 #pragma unroll
           for (int n = 0; n < NT / 32; ++n)
-            if (on<T, NT>(32 * n, a.N)) Ops<T>::mma_left(y, hl.near(f0 + 16 * i + r, 32 * n, q), cf[n], rest<T, NT>(a.N - 32 * n));
+            if (on<T, NT>(32 * n, ap->N)) Ops<T>::mma_left(y, hl.near(f0 + 16 * i + r, 32 * n, q), cf[n], rest<T, NT>(ap->N - 32 * n));
           y *= from;
         }
       }
@@ -756,10 +775,10 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
       ym.store(ti, f0 + 16 * i + 4 * q, v);
     }
     if (more && c1 - c0 > 1) load_c();  // this item's is done with
-    if (cc + 1 < c1 || a.final_state) {
-      update_state<T, PT, NT, kWaves>(S, tm.total, tm.into, xa, ba, wave, q, r, a.P - p0, a.N);
+    if (cc + 1 < c1 || ap->final_state) {
+      update_state<T, PT, NT, kWaves>(S, tm.total, tm.into, xa, ba, wave, q, r, ap->P - p0, ap->N);
       any = true;
-      if (a.final_state && cc + 1 == a.chunks) store_state<PT, NT, kWaves, VEC>(S, a.final_state + bh * pn, a, p0, wave, q, r);
+      if (ap->final_state && cc + 1 == ap->chunks) store_state<PT, NT, kWaves, VEC>(S, ap->final_state + bh * pn, *ap, p0, wave, q, r);
     }
     if (!more) break;
     if (wave == 0) step(k + 1);
@@ -782,7 +801,9 @@ struct StatesLds {
 // what comes into each chunk (ds); otherwise from zero, writing what comes out and the
 // segment's decay. Pipelined like the forward kernel.
 template <class T, int PT, int NT, int PW, bool REV, bool KEEP, bool VEC>
-__global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs a) {
+__global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs args) {
+  (void)args;
+  const ScanArgs *ap = arguments<ScanArgs>();
   using L = StatesLds<T, PT, NT>;
   constexpr int kThreads = 256 * PW, kWaves = 4 * PW;
   using M = Mine<PT, NT, kWaves>;
@@ -794,25 +815,25 @@ __global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, r = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t id = workgroup_id();
-  const int pt = (int)(id % a.ptiles);
-  id /= a.ptiles;
-  const int h = (int)(id % a.H);
-  id /= a.H;
-  const int seg = (int)(id % a.segs);
-  const int64_t b = id / a.segs;
-  const int g = h / (a.H / a.G), p0 = pt * PT, len = row_length(a.lengths, b, a.T);
-  const int c0 = seg * a.seg_chunks, c1 = min(c0 + a.seg_chunks, a.chunks);
-  const float A = a.A[h], bias = a.bias ? a.bias[h] : 0.f;
-  const T *xg = REV ? (const T *)a.dy + (b * a.T * a.H + h) * a.P + p0 : (const T *)a.x + b * a.xsb + h * a.xsh + p0;
-  const int64_t xstride = REV ? (int64_t)a.H * a.P : a.xst;
-  const T *kg = REV ? (const T *)a.c + b * a.csb + g * a.csg : (const T *)a.b + b * a.bsb + g * a.bsg;
-  const int64_t kstride = REV ? a.cst : a.bst;
-  const int64_t bh = b * a.H + h, pn = (int64_t)a.P * a.N;
+  const int pt = (int)(id % ap->ptiles);
+  id /= ap->ptiles;
+  const int h = (int)(id % ap->H);
+  id /= ap->H;
+  const int seg = (int)(id % ap->segs);
+  const int64_t b = id / ap->segs;
+  const int g = h / (ap->H / ap->G), p0 = pt * PT, len = row_length(ap->lengths, b, ap->T);
+  const int c0 = seg * ap->seg_chunks, c1 = min(c0 + ap->seg_chunks, ap->chunks);
+  const float A = ap->A[h], bias = ap->bias ? ap->bias[h] : 0.f;
+  const T *xg = REV ? (const T *)ap->dy + (b * ap->T * ap->H + h) * ap->P + p0 : (const T *)ap->x + b * ap->xsb + h * ap->xsh + p0;
+  const int64_t xstride = REV ? (int64_t)ap->H * ap->P : ap->xst;
+  const T *kg = REV ? (const T *)ap->c + b * ap->csb + g * ap->csg : (const T *)ap->b + b * ap->bsb + g * ap->bsg;
+  const int64_t kstride = REV ? ap->cst : ap->bst;
+  const int64_t bh = b * ap->H + h, pn = (int64_t)ap->P * ap->N;
   // the last chunk that is walked: backwards, what comes out of the first one is not always wanted
-  const int n_chunks = c1 - c0 - (REV && KEEP && c0 == 0 && !a.dinitial ? 1 : 0);
+  const int n_chunks = c1 - c0 - (REV && KEEP && c0 == 0 && !ap->dinitial ? 1 : 0);
   f32x4 S[M::kEach];
-  const float *start = !KEEP ? nullptr : a.segs > 1 ? a.seg + (bh * a.segs + seg) * pn : a.dfinal ? a.dfinal + bh * pn : nullptr;
-  load_state<PT, NT, kWaves, VEC>(S, start, a, p0, wave, q, r);
+  const float *start = !KEEP ? nullptr : ap->segs > 1 ? ap->seg + (bh * ap->segs + seg) * pn : ap->dfinal ? ap->dfinal + bh * pn : nullptr;
+  load_state<PT, NT, kWaves, VEC>(S, start, *ap, p0, wave, q, r);
   double decay = 0.;
   T raw = (T)0.f;
   Stage<T, PT, kThreads, VEC> xs;
@@ -820,9 +841,9 @@ __global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs a) {
   auto chunk_of = [&](int n) __attribute__((always_inline)) { return REV ? c1 - 1 - n : c0 + n; };
   auto load = [&](int n) __attribute__((always_inline)) {
     const int64_t t0 = (int64_t)chunk_of(n) * Q;
-    xs.load(Matrix<T, VEC>(xg + t0 * xstride, xstride, len - t0, a.P - p0), tid);
-    ks.load(Matrix<T, VEC>(kg + t0 * kstride, kstride, len - t0, a.N), tid);
-    if (wave == 0) raw = raw_step<T, VEC>(a, b, h, t0, len, lane);
+    xs.load(Matrix<T, VEC>(xg + t0 * xstride, xstride, len - t0, ap->P - p0), tid);
+    ks.load(Matrix<T, VEC>(kg + t0 * kstride, kstride, len - t0, ap->N), tid);
+    if (wave == 0) raw = raw_step<T, VEC>(*ap, b, h, t0, len, lane);
   };
   auto step = [&](int n) __attribute__((always_inline)) {
     decay += make_times(times[n & 1], (float)raw, bias, (int64_t)chunk_of(n) * Q + lane < len, A, lane);
@@ -833,6 +854,7 @@ __global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs a) {
   }
   for (int n = 0; n < n_chunks; ++n) {
     const Times &tm = times[n & 1];
+    ap = again(ap);
     if (n) __syncthreads();
     if constexpr (sizeof(T) == 2) {
       xs.put(nullptr, xl, tid);
@@ -843,18 +865,18 @@ __global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs a) {
     }
     __syncthreads();
     if (n + 1 < n_chunks) load(n + 1);
-    if (KEEP && a.chunks > 1) store_state<PT, NT, kWaves, VEC>(S, a.ds + (bh * a.chunks + chunk_of(n)) * pn, a, p0, wave, q, r);
-    update_state<T, PT, NT, kWaves>(S, tm.total, REV ? tm.from : tm.into, xa, ka, wave, q, r, a.P - p0, a.N);
+    if (KEEP && ap->chunks > 1) store_state<PT, NT, kWaves, VEC>(S, ap->ds + (bh * ap->chunks + chunk_of(n)) * pn, *ap, p0, wave, q, r);
+    update_state<T, PT, NT, kWaves>(S, tm.total, REV ? tm.from : tm.into, xa, ka, wave, q, r, ap->P - p0, ap->N);
     if (wave == 0 && n + 1 < n_chunks) step(n + 1);
   }
   if (!KEEP) {
-    store_state<PT, NT, kWaves, VEC>(S, a.seg + (bh * a.segs + seg) * pn, a, p0, wave, q, r);
-    if (tid == 0 && pt == 0) a.seg_log2[bh * a.segs + seg] = (float)decay;
+    store_state<PT, NT, kWaves, VEC>(S, ap->seg + (bh * ap->segs + seg) * pn, *ap, p0, wave, q, r);
+    if (tid == 0 && pt == 0) ap->seg_log2[bh * ap->segs + seg] = (float)decay;
   } else if (c0 == 0) {
-    if (a.dinitial)
-      store_state<PT, NT, kWaves, VEC>(S, a.dinitial + bh * pn, a, p0, wave, q, r);
-    else if (a.chunks > 1)
-      store_state<PT, NT, kWaves, VEC>(S, a.ds + bh * a.chunks * pn, a, p0, wave, q, r);
+    if (ap->dinitial)
+      store_state<PT, NT, kWaves, VEC>(S, ap->dinitial + bh * pn, *ap, p0, wave, q, r);
+    else if (ap->chunks > 1)
+      store_state<PT, NT, kWaves, VEC>(S, ap->ds + bh * ap->chunks * pn, *ap, p0, wave, q, r);
   }
 }
 
@@ -957,7 +979,9 @@ struct StageState {
 // sums give for dt by the wavefront of the last 16 j: those have the fewest pairs. ST:
 // whether there are states before or after the chunk.
 template <class T, int PT, int NT, bool ST, bool VEC>
-__global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) void scan_grad_kernel(ScanArgs a) {
+__global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) void scan_grad_kernel(ScanArgs args) {
+  (void)args;
+  const ScanArgs *ap = arguments<ScanArgs>();
   using L = GradLds<T, PT, NT, ST>;
   using O = Ops<T>;
   using BC = Tile<T, NT>;
@@ -976,16 +1000,16 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, r = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t id = workgroup_id();
-  const int slice = (int)(id % a.slices);
-  id /= a.slices;
-  const int g = (int)(id % a.G);
-  id /= a.G;
-  const int c = (int)(id % a.chunks);
-  const int64_t b = id / a.chunks;
-  const int len = row_length(a.lengths, b, a.T), per = a.H / a.G;
-  const int64_t t0 = (int64_t)c * Q, pn = (int64_t)a.P * a.N;
-  const int h_lo = g * per + (int)((int64_t)per * slice / a.slices);
-  const int h_hi = g * per + (int)((int64_t)per * (slice + 1) / a.slices);
+  const int slice = (int)(id % ap->slices);
+  id /= ap->slices;
+  const int g = (int)(id % ap->G);
+  id /= ap->G;
+  const int c = (int)(id % ap->chunks);
+  const int64_t b = id / ap->chunks;
+  const int len = row_length(ap->lengths, b, ap->T), per = ap->H / ap->G;
+  const int64_t t0 = (int64_t)c * Q, pn = (int64_t)ap->P * ap->N;
+  const int h_lo = g * per + (int)((int64_t)per * slice / ap->slices);
+  const int h_hi = g * per + (int)((int64_t)per * (slice + 1) / ap->slices);
   const bool own_j = wave < 4;
   const int mine = wave & 3, tw = 16 * mine + r;  // this lane's position
   const bool live = t0 + lane < len;
@@ -999,19 +1023,19 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
   const float *dh_next = nullptr, *h0_next = nullptr;
   auto load = [&](int h, int pt) __attribute__((always_inline)) {
     const int p0 = pt * PT;
-    const int64_t bh = b * a.H + h;
-    const T *row = lower ? (const T *)a.x + b * a.xsb + t0 * a.xst + h * a.xsh + p0
-                         : (const T *)a.dy + ((b * a.T + t0) * a.H + h) * a.P + p0;
-    xy.load(Matrix<T, VEC>(row, lower ? a.xst : (int64_t)a.H * a.P, len - t0, a.P - p0), ht);
+    const int64_t bh = b * ap->H + h;
+    const T *row = lower ? (const T *)ap->x + b * ap->xsb + t0 * ap->xst + h * ap->xsh + p0
+                         : (const T *)ap->dy + ((b * ap->T + t0) * ap->H + h) * ap->P + p0;
+    xy.load(Matrix<T, VEC>(row, lower ? ap->xst : (int64_t)ap->H * ap->P, len - t0, ap->P - p0), ht);
     if constexpr (ST) {
-      h0_next = a.chunks > 1 ? a.cs + (bh * a.chunks + c) * pn : a.initial ? a.initial + bh * pn : nullptr;
-      dh_next = a.chunks > 1 ? a.ds + (bh * a.chunks + c) * pn : a.dfinal ? a.dfinal + bh * pn : nullptr;
-      hd.load(lower ? h0_next : dh_next, a, p0, ht);
+      h0_next = ap->chunks > 1 ? ap->cs + (bh * ap->chunks + c) * pn : ap->initial ? ap->initial + bh * pn : nullptr;
+      dh_next = ap->chunks > 1 ? ap->ds + (bh * ap->chunks + c) * pn : ap->dfinal ? ap->dfinal + bh * pn : nullptr;
+      hd.load(lower ? h0_next : dh_next, *ap, p0, ht);
     }
-    if (pt == 0 && wave == kTimesWave) raw = raw_step<T, VEC>(a, b, h, t0, len, lane);
+    if (pt == 0 && wave == kTimesWave) raw = raw_step<T, VEC>(*ap, b, h, t0, len, lane);
   };
   auto step = [&](int h) __attribute__((always_inline)) {
-    make_times(times[h & 1], (float)raw, a.bias ? a.bias[h] : 0.f, live, a.A[h], lane);
+    make_times(times[h & 1], (float)raw, ap->bias ? ap->bias[h] : 0.f, live, ap->A[h], lane);
   };
   // dt's gradient of head h from its sums, and the chunk's part of those of A, dt_bias and D
   auto finish = [&](int h) __attribute__((always_inline)) {
@@ -1049,11 +1073,11 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
       if (lane == 0) before = 0.f;
     }
     const float da = (before + after) + (cross + tm.total * dot);
-    const float ddt = (a.A[h] * da + bdv) * tm.slope[lane];
-    if (t0 + lane < a.T) ((T *)a.ddt)[(b * a.T + t0 + lane) * a.H + h] = (T)ddt;
+    const float ddt = (ap->A[h] * da + bdv) * tm.slope[lane];
+    if (t0 + lane < ap->T) ((T *)ap->ddt)[(b * ap->T + t0 + lane) * ap->H + h] = (T)ddt;
     const float dA = wave_sum(da * dt), dbias = wave_sum(ddt);
     if (lane == 0) {
-      float *o = a.part + ((b * a.chunks + c) * a.H + h) * 3;
+      float *o = ap->part + ((b * ap->chunks + c) * ap->H + h) * 3;
       o[0] = dA;
       o[1] = dbias;
       o[2] = diag;
@@ -1062,8 +1086,8 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
 
   {
     Stage<T, NT, 512, VEC> s, u;
-    s.load(Matrix<T, VEC>((const T *)a.b + b * a.bsb + t0 * a.bst + g * a.bsg, a.bst, len - t0, a.N), tid);
-    u.load(Matrix<T, VEC>((const T *)a.c + b * a.csb + t0 * a.cst + g * a.csg, a.cst, len - t0, a.N), tid);
+    s.load(Matrix<T, VEC>((const T *)ap->b + b * ap->bsb + t0 * ap->bst + g * ap->bsg, ap->bst, len - t0, ap->N), tid);
+    u.load(Matrix<T, VEC>((const T *)ap->c + b * ap->csb + t0 * ap->cst + g * ap->csg, ap->cst, len - t0, ap->N), tid);
     load(h_lo, 0);
     s.put(bn, bt, tid);
     u.put(cn, ct, tid);
@@ -1076,11 +1100,12 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
 
   int h = h_lo, pt = 0;
   for (bool first = true;; first = false) {
-    const int p0 = pt * PT, np = a.P - p0, h_now = h, pt_now = pt;
+    ap = again(ap);
+    const int p0 = pt * PT, np = ap->P - p0, h_now = h, pt_now = pt;
     const Times &tm = times[h & 1];
     HeadSums &sum = sums[h & 1];
     const bool dh = ST && dh_next, h0 = ST && h0_next;
-    const float D = a.D ? a.D[h] : 0.f;
+    const float D = ap->D ? ap->D[h] : 0.f;
     if (!first) __syncthreads();
     if (lower)
       xy.put(xn, nullptr, ht);
@@ -1095,7 +1120,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
         hd.put(&dhl, L::two ? &dhtl : (Cols) nullptr, ht);
     }
     __syncthreads();
-    if (++pt == a.ptiles) {
+    if (++pt == ap->ptiles) {
       pt = 0;
       ++h;
     }
@@ -1144,7 +1169,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
           f32x4 gs = {0.f, 0.f, 0.f, 0.f}, ms = gs;
 #pragma unroll
           for (int k = 0; k < NT / 32; ++k)
-            if (on<T, NT>(32 * k, a.N)) O::mma_left(gs, O::near(cn + (16 * it + r) * BC::kRow, 32 * k, q), bf[k], rest<T, NT>(a.N - 32 * k));
+            if (on<T, NT>(32 * k, ap->N)) O::mma_left(gs, O::near(cn + (16 * it + r) * BC::kRow, 32 * k, q), bf[k], rest<T, NT>(ap->N - 32 * k));
 #pragma unroll
           for (int k = 0; k < PT / 32; ++k)
             if (on<T, NT>(32 * k, np)) O::mma_left(ms, O::near(yn + (16 * it + r) * XY::kRow, 32 * k, q), xf[k], rest<T, NT>(np - 32 * k));
@@ -1195,7 +1220,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
       }
       col += dt > 0.f ? later / dt : 0.f;  // (a step of 0 has a slope of 0)
       const float into = left * dt;
-      const Matrix<T, VEC> xm((const T *)a.dx + ((b * a.T + t0) * a.H + h_now) * a.P + p0, (int64_t)a.H * a.P, a.T - t0, a.P - p0);
+      const Matrix<T, VEC> xm((const T *)ap->dx + ((b * ap->T + t0) * ap->H + h_now) * ap->P + p0, (int64_t)ap->H * ap->P, ap->T - t0, ap->P - p0);
 #pragma unroll
       for (int i = 0; i < PT / 16; ++i) {
         if (!on<T, NT>(16 * i, np)) continue;
@@ -1203,7 +1228,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
         if (dh) {
 #pragma unroll
           for (int k = 0; k < NT / 32; ++k)
-            if (on<T, NT>(32 * k, a.N)) O::mma_left(dx, dhl.near(16 * i + r, 32 * k, q), bf[k], rest<T, NT>(a.N - 32 * k));
+            if (on<T, NT>(32 * k, ap->N)) O::mma_left(dx, dhl.near(16 * i + r, 32 * k, q), bf[k], rest<T, NT>(ap->N - 32 * k));
           dx *= into;
         }
         if (i & 1) __builtin_amdgcn_sched_barrier(0);  // (reads further ahead cost more registers than there are)
@@ -1214,7 +1239,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
       }
 #pragma unroll
       for (int i = 0; i < NT / 16; ++i) {
-        if (!on<T, NT>(16 * i, a.N)) continue;
+        if (!on<T, NT>(16 * i, ap->N)) continue;
         if (dh) {
           f32x4 u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -1276,7 +1301,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
       const float from = tm.from[tw];
 #pragma unroll
       for (int i = 0; i < NT / 16; ++i) {
-        if (!on<T, NT>(16 * i, a.N)) continue;
+        if (!on<T, NT>(16 * i, ap->N)) continue;
         if (h0) {
           f32x4 u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -1298,7 +1323,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
         if (mine > 1) O::mma(acc[i], ba.far(16 * i + r, 32, q), sf[1]);
       }
     }
-    if (pt_now + 1 == a.ptiles) {
+    if (pt_now + 1 == ap->ptiles) {
       // a position's n are spread over the four lanes of one r
       if constexpr (ST) {
         inter = rows_sum(inter);
@@ -1317,17 +1342,17 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
   }
   __syncthreads();
   if (wave == kStepWave) finish(h_hi - 1);
-  const int64_t first_row = ((b * a.T + t0) * a.G + g) * a.N;
-  if (a.slices == 1) {
-    const Matrix<T, VEC> m((const T *)(own_j ? a.db : a.dc) + first_row, (int64_t)a.G * a.N, a.T - t0, a.N);
+  const int64_t first_row = ((b * ap->T + t0) * ap->G + g) * ap->N;
+  if (ap->slices == 1) {
+    const Matrix<T, VEC> m((const T *)(own_j ? ap->db : ap->dc) + first_row, (int64_t)ap->G * ap->N, ap->T - t0, ap->N);
 #pragma unroll
     for (int i = 0; i < NT / 16; ++i) {
       const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
       m.store(tw, 16 * i + 4 * q, v);
     }
   } else {
-    const Matrix<float, VEC> m(a.dbc + (int64_t)(slice * 2 + !own_j) * a.B * a.T * a.G * a.N + first_row, (int64_t)a.G * a.N,
-                               a.T - t0, a.N);
+    const Matrix<float, VEC> m(ap->dbc + (int64_t)(slice * 2 + !own_j) * ap->B * ap->T * ap->G * ap->N + first_row, (int64_t)ap->G * ap->N,
+                               ap->T - t0, ap->N);
 #pragma unroll
     for (int i = 0; i < NT / 16; ++i) {
       const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
