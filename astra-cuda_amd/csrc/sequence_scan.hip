@@ -933,8 +933,9 @@ struct GradLds {
   static constexpr size_t dht = dh + (ST ? StateTile<T, PT, NT, 1>::kBytes : 0);           // [n][p]
   static constexpr size_t h0 = dht + (ST && two ? StateTile<T, NT, PT, 2>::kBytes : 0);    // [n][p], floats [p][n]
   static constexpr size_t times = h0 + (!ST ? 0 : two ? StateTile<T, NT, PT, 2>::kBytes : StateTile<T, PT, NT, 1>::kBytes);
-  static constexpr size_t sums = times + 2 * sizeof(Times);
+  static constexpr size_t sums = times + 3 * sizeof(Times);
   static constexpr size_t bytes = sums + 2 * sizeof(HeadSums);
+  static_assert(bytes <= 160 * 1024, "more LDS than a CU has");
 };
 
 // 4 x 4 blocks of a state [P, N] on their way from memory to LDS.
@@ -991,6 +992,8 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
   T *xn = (T *)(lds + L::xn), *yn = (T *)(lds + L::yn), *yt = (T *)(lds + L::yt);
   const StateTile<T, PT, NT, 1> dhl{(T *)(lds + L::dh)}, h0f{(T *)(lds + L::h0)};
   const StateTile<T, NT, PT, 2> dhtl{(T *)(lds + L::dht)}, h0l{(T *)(lds + L::h0)};
+  // Times of three heads: the next one's are written while one wavefront may still read the last
+  // one's in finish(); HeadSums of two, whose writers are a barrier behind that.
   Times *times = (Times *)(lds + L::times);
   HeadSums *sums = (HeadSums *)(lds + L::sums);
   const Along<T, NT> ba{bn, bt}, ca{cn, ct};
@@ -1035,11 +1038,11 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
     if (pt == 0 && wave == kTimesWave) raw = raw_step<T, VEC>(*ap, b, h, t0, len, lane);
   };
   auto step = [&](int h) __attribute__((always_inline)) {
-    make_times(times[h & 1], (float)raw, ap->bias ? ap->bias[h] : 0.f, live, ap->A[h], lane);
+    make_times(times[(unsigned)h % 3], (float)raw, ap->bias ? ap->bias[h] : 0.f, live, ap->A[h], lane);
   };
   // dt's gradient of head h from its sums, and the chunk's part of those of A, dt_bias and D
   auto finish = [&](int h) __attribute__((always_inline)) {
-    const Times &tm = times[h & 1];
+    const Times &tm = times[(unsigned)h % 3];
     const HeadSums &s = sums[h & 1];
     float dot = 0.f, diag = 0.f, cross = 0.f;
     if constexpr (ST) {
@@ -1102,7 +1105,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
   for (bool first = true;; first = false) {
     ap = again(ap);
     const int p0 = pt * PT, np = ap->P - p0, h_now = h, pt_now = pt;
-    const Times &tm = times[h & 1];
+    const Times &tm = times[(unsigned)h % 3];
     HeadSums &sum = sums[h & 1];
     const bool dh = ST && dh_next, h0 = ST && h0_next;
     const float D = ap->D ? ap->D[h] : 0.f;
