@@ -50,7 +50,8 @@ __device__ __forceinline__ void load_input(const ConvArgs &a, int64_t b, int64_t
 
 // One thread: V channels, `run` positions, the last K-1 inputs in registers. U positions at
 // a time, so that their loads are in flight together; where all of them count, without a
-// check each.
+// check each. Bound by traffic: 65,537 positions of 1,280 float channels 138 us, 4.9 TB/s (a
+// large copy 4.7); 2,048 games of 40 positions and 640 bf16 channels 45 us.
 template <class T, int K, int V>
 __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a) {
   constexpr int U = 4;
@@ -118,7 +119,9 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a) {
 // positions, `gridDim.y` rows of workgroups apart, and keeps its part of dw and dbias in
 // registers. A run recomputes the K-1 values of g after its end. U positions at a time, so
 // that their loads are in flight together and the windows of x and g need few moves; inside
-// a run without a check each.
+// a run without a check each. 2,048 games of 40 positions and 640 bf16 channels: 105 us, 3.0
+// TB/s, where its bytes take 67; the sigmoid's exp and reciprocal and some 30 further vector
+// operations an element come to as long.
 constexpr int kConvCols = 16;
 template <class T, int K, int V>
 __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {

@@ -8,7 +8,9 @@
 //
 // Some 12 operations an element (45 in the gradient): bound by memory traffic, so a row is
 // read once into registers, both sums are taken there, and each thread keeps the weights
-// of its columns over all the rows that it works on.
+// of its columns over all the rows that it works on. Times: 81,920 rows of 256 in bf16
+// forwards 53 us (4.0 TB/s), backwards 86 (3.9); 16,384 rows of 4,096 with a residual in
+// 32 bits 170 (4.7, a large copy's rate) and 276 (4.4).
 #include "sequence.h"
 
 #define ASTRA_SRC_NAME "sequence_join.hip"
