@@ -26,11 +26,12 @@
 //
 // Types. x, B, C and dY enter the products as they are; sums and states are in 32 bits. For
 // bf16 inputs, what is computed in between enters a product as
-//   - one bf16 value: the states in y and dX, whose results are rounded to bf16;
 //   - the sum of two (2^-18): the scores M and Q (with one, results of bf16 type were up to
 //     1.1e-3 of their term further from 64 bits than their own rounding; the second part
-//     costs 2 to 13% of a pass), and the states in U = h0^T dY and V = dh1^T x, which end in
-//     the float gradient d(dt A);
+//     costs 2 to 13% of a pass), and the states, in y and dX as well as in U = h0^T dY and
+//     V = dh1^T x, which end in the float gradient d(dt A). With one, the error of y goes with
+//     |h| |C| and not with |h C|: a state whose values have a mean 16 times their spread, read
+//     out by a C of zero mean, left 2.8e-2 of y where bf16's rounding is 1.7e-3;
 //   - the sum of three (2^-26) in those that end in float states: w B and exp(s) C.
 // For float inputs the products use the float matrix instructions, at 1/16 of the bf16
 // ones' rate.
@@ -260,18 +261,25 @@ struct Along {  // operands contracted over positions
   }
 };
 
-// A state tile [R, K] (K contracted) in LDS: one bf16 part or two, or floats.
-template <class T, int R, int K, int PARTS>
+// A state tile [R, K] (K contracted) in LDS: two bf16 parts, or floats. Rows of 256 bytes,
+// which start on the same bank, are not padded: their 16-byte blocks change places by row
+// (so that two workgroups of the forward kernel with 64 x 128 states fit a CU's LDS).
+template <class T, int R, int K>
 struct StateTile {
-  static constexpr bool kTwo = sizeof(T) == 2 && PARTS == 2;
-  static constexpr int kRow = K + 16 / (int)sizeof(T);
+  static constexpr bool kTwo = sizeof(T) == 2, kSwapped = kTwo && K == 128;
+  static constexpr int kRow = kSwapped ? K : K + 16 / (int)sizeof(T);
   static constexpr size_t kBytes = (kTwo ? 2 : 1) * R * kRow * sizeof(T);
   T *p;
+  static __device__ __forceinline__ int at(int r, int k) {
+    if constexpr (kSwapped) return r * kRow + (k ^ (r & 15) << 3);
+    return r * kRow + k;
+  }
   __device__ __forceinline__ auto near(int r, int k0, int q) const {
     if constexpr (kTwo) {
+      const int i = at(r, k0 + 8 * q);
       typename Ops<T>::Split s;
-      s.hi = Ops<T>::near(p + r * kRow, k0, q);
-      s.lo = Ops<T>::near(p + R * kRow + r * kRow, k0, q);
+      s.hi = Ops<T>::near(p + i, 0, 0);
+      s.lo = Ops<T>::near(p + R * kRow + i, 0, 0);
       return s;
     } else {
       return Ops<T>::near(p + r * kRow, k0, q);
@@ -291,15 +299,17 @@ struct StateTile {
       hi[i] = (T)v[i];
       if constexpr (kTwo) lo[i] = (T)(v[i] - (float)hi[i]);
     }
-    *reinterpret_cast<typename V4<T>::type *>(p + r * kRow + k) = hi;
-    if constexpr (kTwo) *reinterpret_cast<typename V4<T>::type *>(p + R * kRow + r * kRow + k) = lo;
+    T *const o = p + at(r, k);
+    *reinterpret_cast<typename V4<T>::type *>(o) = hi;
+    if constexpr (kTwo) *reinterpret_cast<typename V4<T>::type *>(o + R * kRow) = lo;
   }
-  // the 8 values from element i on, as floats
+  // the 8 values from element k (a multiple of 8) on, as floats
   __device__ __forceinline__ void get8(int r, int k, float (&v)[8]) const {
+    const T *const o = p + at(r, k);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[i] = (float)p[r * kRow + k + i];
-      if constexpr (kTwo) v[i] += (float)p[R * kRow + r * kRow + k + i];
+      v[i] = (float)o[i];
+      if constexpr (kTwo) v[i] += (float)o[R * kRow + i];
     }
   }
 };
@@ -446,15 +456,21 @@ __device__ __forceinline__ typename Ops<T>::Frag load_near(const Matrix<T, VEC> 
 // What one wavefront, a lane a position, works out of a head's dt over a chunk.
 struct Times {
   float dt[Q], hi[Q], lo[Q];  // the step; log2 of the decay from the chunk's start, in two parts
-  float from[Q], left[Q];     // exp(s_t), exp(s_Q - s_t)
+  float from[Q];              // exp(s_t)
   float into[Q];              // dt exp(s_Q - s_t): what a position's input counts after the chunk
-  float slope[Q];             // the step's derivative by dt_raw, 0 where no position counts
   // Between tiles of 16 positions exp(s_i - s_j) is a product by way of the end e of j's
   // tile (both factors are at most 1 where A <= 0, and small only where the product is):
-  float past[3][Q];           // exp(s_i - s_e) for i after tile 0, 1, 2
+  float after[48 + 32 + 16];  // exp(s_i - s_e) for the i after tile 0, 1, 2
   float till[Q];              // exp(s_e - s_j) dt_j for j's own tile
   float total;                // exp(s_Q)
-  float pad[3];
+  float nowhere[3];
+  // `after` of a tile, such that position i's is at [i] (i >= 16 (tile + 1))
+  static __device__ __forceinline__ int past_at(int tile) { return tile == 0 ? -16 : tile == 1 ? 48 - 32 : 80 - 48; }
+  __device__ __forceinline__ float past(int tile, int i) const { return after[past_at(tile) + i]; }
+};
+struct GradTimes : Times {
+  float left[Q];   // exp(s_Q - s_t)
+  float slope[Q];  // the step's derivative by dt_raw, 0 where no position counts
 };
 
 __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
@@ -474,7 +490,8 @@ __device__ __forceinline__ double moved64(double v) {
 }
 
 // Fills `o` from this lane's dt and the head's bias and A; returns log2 of the chunk's decay.
-__device__ __forceinline__ double make_times(Times &o, float dt_raw, float bias, bool live, float A, int lane) {
+template <class O>
+__device__ __forceinline__ double make_times(O &o, float dt_raw, float bias, bool live, float A, int lane) {
   const float raw = dt_raw + bias, dt = live ? softplus(raw) : 0.f;
   double s = (double)dt * (double)A * 1.4426950408889634;
   s += moved64<kUp + 1>(s);
@@ -490,7 +507,8 @@ __device__ __forceinline__ double make_times(Times &o, float dt_raw, float bias,
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)at, 16 * i + 15);
     const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), 16 * i + 15);
     ends[i] = __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
-    if (i < 3) o.past[i][lane] = __builtin_amdgcn_exp2f((float)(s - ends[i]));
+    // (the other lanes' go nowhere: a place to put them costs less than a branch around them)
+    if (i < 3) *(lane >= 16 * (i + 1) ? o.after + Times::past_at(i) + lane : o.nowhere) = __builtin_amdgcn_exp2f((float)(s - ends[i]));
   }
   const double total = ends[3];
   const float left = __builtin_amdgcn_exp2f((float)(total - s));
@@ -500,9 +518,11 @@ __device__ __forceinline__ double make_times(Times &o, float dt_raw, float bias,
   o.hi[lane] = (float)s;
   o.lo[lane] = (float)(s - (double)(float)s);
   o.from[lane] = __builtin_amdgcn_exp2f((float)s);
-  o.left[lane] = left;
   o.into[lane] = dt * left;
-  o.slope[lane] = live ? sigmoid(raw) : 0.f;
+  if constexpr (sizeof(O) == sizeof(GradTimes)) {
+    o.left[lane] = left;
+    o.slope[lane] = live ? sigmoid(raw) : 0.f;
+  }
   if (lane == 0) o.total = __builtin_amdgcn_exp2f((float)total);
   return total;
 }
@@ -589,7 +609,7 @@ struct ForwardLds {
   static constexpr size_t bn = x + (sizeof(T) == 2 ? Tile<T, PT>::kColsBytes : Tile<T, PT>::kRowsBytes);
   static constexpr size_t bt = bn + Tile<T, NT>::kRowsBytes;
   static constexpr size_t h = bt + Tile<T, NT>::kColsBytes;
-  static constexpr size_t times = h + (ST ? StateTile<T, PT, NT, 1>::kBytes : 0);
+  static constexpr size_t times = h + (ST ? StateTile<T, PT, NT>::kBytes : 0);
   static constexpr size_t bytes = times + 2 * sizeof(Times);
 };
 
@@ -612,7 +632,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
   using M = Mine<PT, NT, kWaves>;
   extern __shared__ __align__(16) char lds[];
   T *xl = (T *)(lds + L::x), *bn = (T *)(lds + L::bn), *bt = (T *)(lds + L::bt);
-  const StateTile<T, PT, NT, 1> hl{(T *)(lds + L::h)};
+  const StateTile<T, PT, NT> hl{(T *)(lds + L::h)};
   Times *times = (Times *)(lds + L::times);
   const Along<T, PT> xa{xl, xl};
   const Along<T, NT> ba{bn, bt};
@@ -742,7 +762,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
         }
         const f32x4 g = ST ? scores(jt) : sc[jt];
         if (jt < wi) {
-          const float past = tm.past[jt][ti];
+          const float past = tm.past(jt, ti);
           const f32x4 till = *reinterpret_cast<const f32x4 *>(tm.till + 16 * jt + 4 * q);
 #pragma unroll
           for (int e = 0; e < 4; ++e) m[4 * half + e] = g[e] * (past * till[e]);
@@ -939,10 +959,10 @@ struct GradLds {
   static constexpr size_t yn = xn + Tile<T, PT>::kRowsBytes;
   static constexpr size_t yt = yn + Tile<T, PT>::kRowsBytes;
   static constexpr size_t dh = yt + Tile<T, PT>::kColsBytes;                               // [p][n]
-  static constexpr size_t dht = dh + (ST ? StateTile<T, PT, NT, 1>::kBytes : 0);           // [n][p]
-  static constexpr size_t h0 = dht + (ST && two ? StateTile<T, NT, PT, 2>::kBytes : 0);    // [n][p], floats [p][n]
-  static constexpr size_t times = h0 + (!ST ? 0 : two ? StateTile<T, NT, PT, 2>::kBytes : StateTile<T, PT, NT, 1>::kBytes);
-  static constexpr size_t sums = times + 3 * sizeof(Times);
+  static constexpr size_t dht = dh + (ST ? StateTile<T, PT, NT>::kBytes : 0);              // [n][p]
+  static constexpr size_t h0 = dht + (ST && two ? StateTile<T, NT, PT>::kBytes : 0);       // [n][p], floats [p][n]
+  static constexpr size_t times = h0 + (!ST ? 0 : two ? StateTile<T, NT, PT>::kBytes : StateTile<T, PT, NT>::kBytes);
+  static constexpr size_t sums = times + 3 * sizeof(GradTimes);
   static constexpr size_t bytes = sums + 2 * sizeof(HeadSums);
   static_assert(bytes <= 160 * 1024, "more LDS than a CU has");
 };
@@ -1002,11 +1022,11 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
   extern __shared__ __align__(16) char lds[];
   T *bn = (T *)(lds + L::bn), *bt = (T *)(lds + L::bt), *cn = (T *)(lds + L::cn), *ct = (T *)(lds + L::ct);
   T *xn = (T *)(lds + L::xn), *yn = (T *)(lds + L::yn), *yt = (T *)(lds + L::yt);
-  const StateTile<T, PT, NT, 1> dhl{(T *)(lds + L::dh)}, h0f{(T *)(lds + L::h0)};
-  const StateTile<T, NT, PT, 2> dhtl{(T *)(lds + L::dht)}, h0l{(T *)(lds + L::h0)};
+  const StateTile<T, PT, NT> dhl{(T *)(lds + L::dh)}, h0f{(T *)(lds + L::h0)};
+  const StateTile<T, NT, PT> dhtl{(T *)(lds + L::dht)}, h0l{(T *)(lds + L::h0)};
   // Times of three heads: the next one's are written while one wavefront may still read the last
   // one's in finish(); HeadSums of two, whose writers are a barrier behind that.
-  Times *times = (Times *)(lds + L::times);
+  GradTimes *times = (GradTimes *)(lds + L::times);
   HeadSums *sums = (HeadSums *)(lds + L::sums);
   const Along<T, NT> ba{bn, bt}, ca{cn, ct};
   const Along<T, PT> ya{yn, yt};
@@ -1054,7 +1074,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
   };
   // dt's gradient of head h from its sums, and the chunk's part of those of A, dt_bias and D
   auto finish = [&](int h) __attribute__((always_inline)) {
-    const Times &tm = times[(unsigned)h % 3];
+    const GradTimes &tm = times[(unsigned)h % 3];
     const HeadSums &s = sums[h & 1];
     float dot = 0.f, diag = 0.f, cross = 0.f;
     if constexpr (ST) {
@@ -1117,7 +1137,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
   for (bool first = true;; first = false) {
     ap = again(ap);
     const int p0 = pt * PT, np = ap->P - p0, h_now = h, pt_now = pt;
-    const Times &tm = times[(unsigned)h % 3];
+    const GradTimes &tm = times[(unsigned)h % 3];
     HeadSums &sum = sums[h & 1];
     const bool dh = ST && dh_next, h0 = ST && h0_next;
     const float D = ap->D ? ap->D[h] : 0.f;
@@ -1127,8 +1147,8 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
     else
       xy.put(yn, yt, ht);
     if constexpr (ST) {
-      using Rows = const StateTile<T, PT, NT, 1> *;
-      using Cols = const StateTile<T, NT, PT, 2> *;
+      using Rows = const StateTile<T, PT, NT> *;
+      using Cols = const StateTile<T, NT, PT> *;
       if (lower)
         hd.put(L::two ? (Rows) nullptr : &h0f, L::two ? &h0l : (Cols) nullptr, ht);
       else
@@ -1190,7 +1210,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
             if (on<T, NT>(32 * k, np)) O::mma_left(ms, O::near(yn + (16 * it + r) * XY::kRow, 32 * k, q), xf[k], rest<T, NT>(np - 32 * k));
           float pair[4];  // with dt_j
           if (it > mine) {
-            const f32x4 past = *reinterpret_cast<const f32x4 *>(tm.past[mine] + 16 * it + 4 * q);
+            const f32x4 past = *reinterpret_cast<const f32x4 *>(tm.after + Times::past_at(mine) + 16 * it + 4 * q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float f = past[e] * till;
@@ -1296,7 +1316,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
           for (int k = 0; k < PT / 32; ++k)
             if (on<T, NT>(32 * k, np)) O::mma_left(ms, O::near(xn + (16 * jt + r) * XY::kRow, 32 * k, q), yf[k], rest<T, NT>(np - 32 * k));
           if (jt < mine) {
-            const float past = tm.past[jt][tw];
+            const float past = tm.past(jt, tw);
             const f32x4 till = *reinterpret_cast<const f32x4 *>(tm.till + 16 * jt + 4 * q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[4 * half + e] = ms[e] * (past * till[e]);
