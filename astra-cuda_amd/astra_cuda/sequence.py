@@ -9,7 +9,9 @@ time in rollouts with a state of fixed size per env (include/sequence/astra_sequ
                      read-out and step size given per position
 ``join_norm``        what stands between two blocks: the norm after one, its gate and
                      residual scale, the residual sum, the norm before the next
-``short_conv_step``, ``state_scan_step``   one position, the state moved on in place
+``short_conv_step``, ``state_scan_step``   one position, the state moved on in place (and its
+version raised: a backward pass that had saved it refuses to run, as after torch's own
+operations in place)
 
 The first three are differentiable in every tensor they take (once). Tensors are float32
 or bfloat16 on one HIP device; sums, states and norms are float32 throughout, and each

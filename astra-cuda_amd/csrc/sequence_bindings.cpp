@@ -214,6 +214,12 @@ py::object short_conv(const Tensor &x_, const Tensor &weight_, const Optional &b
         "whole-sequence operator");
 }
 
+// A state was written through its pointer: what saved it for a backward pass has to notice, as
+// after torch's own operations in place. (Inference tensors have no version.)
+void moved_on(const Tensor &state) {
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor short_conv_step(const Tensor &x_, const Tensor &state, const Tensor &weight_, const Optional &bias_,
                        const std::optional<std::string> &activation) {
   check_data("x", x_);
@@ -240,6 +246,7 @@ Tensor short_conv_step(const Tensor &x_, const Tensor &state, const Tensor &weig
   o.type = type_of(x);
   o.activation = (int32_t)activation_of(activation);
   check(astra_short_conv_step(&o, stream_of(x.get_device())));
+  moved_on(state);
   return y;
 }
 
@@ -425,6 +432,7 @@ Tensor state_scan_step(const Tensor &x_, const Tensor &dt, const Tensor &A_, con
   o.state = (int32_t)N;
   o.type = type_of(x);
   check(astra_state_scan_step(&o, stream_of(x.get_device())));
+  moved_on(state);
   return y;
 }
 

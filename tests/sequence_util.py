@@ -53,3 +53,17 @@ def run_scan(seq, own, lengths=None):
 
 def ref_scan(ref, lengths=None):
     return oracle.scan(ref["x"], ref["dt"], ref["A"], ref["B"], ref["C"], ref["D"], ref["dt_bias"], ref["h"], lengths)
+
+
+def small_conv(dtype=F32):
+    """x, weight, bias, window."""
+    g = gen(31)
+    return (normal(g, 2, 6, 8, dtype=dtype), normal(g, 8, 4), normal(g, 8), normal(g, 2, 3, 8, dtype=dtype))
+
+
+def small_scan(dtype=F32):
+    """(state_scan's arguments, a state)."""
+    g = gen(32)
+    return dict(x=normal(g, 2, 6, 2, 8, dtype=dtype), dt=normal(g, 2, 6, 2, dtype=dtype),
+                A=-torch.ones(2, device=DEV), B=normal(g, 2, 6, 1, 4, dtype=dtype), C=normal(g, 2, 6, 1, 4, dtype=dtype),
+                D=normal(g, 2), dt_bias=normal(g, 2)), normal(g, 2, 2, 8, 4)
