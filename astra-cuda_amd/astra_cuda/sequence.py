@@ -13,7 +13,8 @@ time in rollouts with a state of fixed size per env (include/sequence/astra_sequ
 version raised: a backward pass that had saved it refuses to run, as after torch's own
 operations in place)
 
-The first three are differentiable in every tensor they take (once). Tensors are float32
+The first three are differentiable in every tensor they take (once, backwards: tensors with
+a forward-mode tangent are refused). Tensors are float32
 or bfloat16 on one HIP device; sums, states and norms are float32 throughout, and each
 result is rounded to its type once. Calls run on the caller's current stream and do not
 synchronise. Tensors may be strided as long as their last dimension is contiguous (others
