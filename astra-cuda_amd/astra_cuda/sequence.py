@@ -14,7 +14,7 @@ version raised: a backward pass that had saved it refuses to run, as after torch
 operations in place)
 
 The first three are differentiable in every tensor they take (once, backwards: tensors with
-a forward-mode tangent are refused). Tensors are float32
+a forward-mode tangent are refused, and so is being part of a torch.jit trace). Tensors are float32
 or bfloat16 on one HIP device; sums, states and norms are float32 throughout, and each
 result is rounded to its type once. Calls run on the caller's current stream and do not
 synchronise. Tensors may be strided as long as their last dimension is contiguous (others

@@ -6,6 +6,7 @@
 
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <optional>
 
@@ -83,12 +84,14 @@ bool with_grad(std::initializer_list<const Tensor *> ts) {
   return false;
 }
 
-// Forward-mode derivatives stop here: what is refused would otherwise come back without its
-// tangent, since the kernels write plain memory.
+// Forward-mode derivatives and traces stop here: a result would come back without its tangent,
+// and a trace would hold its allocation without what fills it, since the kernels write plain
+// memory.
 bool has_tangent(const Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
 bool has_tangent(const Optional &t) { return t && has_tangent(*t); }
 template <class... Ts>
-void backward_mode_only(const char *name, const Ts &...ts) {
+void calls_only(const char *name, const Ts &...ts) {
+  if (torch::jit::tracer::isTracing()) fatal(std::string("sequence: ") + name + " cannot be part of a trace");
   if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && (has_tangent(ts) || ...))
     fatal(std::string("sequence: ") + name + " has no forward-mode derivative");
 }
@@ -200,7 +203,7 @@ void check_weight(const Tensor &weight) {
 py::object short_conv(const Tensor &x_, const Tensor &weight_, const Optional &bias_,
                       const std::optional<std::string> &activation, const Optional &initial, const Optional &lengths_,
                       bool return_state) {
-  backward_mode_only("short_conv", x_, weight_, bias_, initial);
+  calls_only("short_conv", x_, weight_, bias_, initial);
   check_data("x", x_);
   need(x_.dim() == 3 && x_.size(2) >= 1, "x", "must have shape [batch, length, width], got " + shape_text(x_.sizes()));
   check_weight(weight_);
@@ -234,7 +237,7 @@ void moved_on(const Tensor &state) {
 
 Tensor short_conv_step(const Tensor &x_, const Tensor &state, const Tensor &weight_, const Optional &bias_,
                        const std::optional<std::string> &activation) {
-  backward_mode_only("short_conv_step", x_, state, weight_, bias_);
+  calls_only("short_conv_step", x_, state, weight_, bias_);
   check_data("x", x_);
   need(x_.dim() == 2 && x_.size(1) >= 1, "x", "must have shape [batch, width], got " + shape_text(x_.sizes()));
   check_weight(weight_);
@@ -393,7 +396,7 @@ void check_scan(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor
 py::object state_scan(const Tensor &x_, const Tensor &dt, const Tensor &A_, const Tensor &b_, const Tensor &c_,
                       const Optional &D_, const Optional &dt_bias_, const Optional &initial_, const Optional &lengths_,
                       bool return_state) {
-  backward_mode_only("state_scan", x_, dt, A_, b_, c_, D_, dt_bias_, initial_);
+  calls_only("state_scan", x_, dt, A_, b_, c_, D_, dt_bias_, initial_);
   check_scan(x_, dt, A_, b_, c_, 2);
   const int64_t B = x_.size(0), H = x_.size(2);
   const Tensor A = param("A", A_, x_, {H}), D = param("D", D_, x_, {H}), dt_bias = param("dt_bias", dt_bias_, x_, {H});
@@ -409,7 +412,7 @@ py::object state_scan(const Tensor &x_, const Tensor &dt, const Tensor &A_, cons
 
 Tensor state_scan_step(const Tensor &x_, const Tensor &dt, const Tensor &A_, const Tensor &b_, const Tensor &c_,
                        const Tensor &state, const Optional &D_, const Optional &dt_bias_) {
-  backward_mode_only("state_scan_step", x_, dt, A_, b_, c_, state, D_, dt_bias_);
+  calls_only("state_scan_step", x_, dt, A_, b_, c_, state, D_, dt_bias_);
   check_scan(x_, dt, A_, b_, c_, 1);
   const int64_t B = x_.size(0), H = x_.size(1), P = x_.size(2), N = b_.size(2);
   const Tensor A = param("A", A_, x_, {H}), D = param("D", D_, x_, {H}), dt_bias = param("dt_bias", dt_bias_, x_, {H});
@@ -559,7 +562,7 @@ void check_width(int64_t D) {
 
 py::object join_norm(const Tensor &residual, const Tensor &block, const Tensor &post_, const Optional &next_,
                      const Optional &gate_, const Optional &scale_, double eps) {
-  backward_mode_only("join_norm", residual, block, post_, next_, gate_, scale_);
+  calls_only("join_norm", residual, block, post_, next_, gate_, scale_);
   check_data("block", block);
   check_data("residual", residual);
   need(residual.scalar_type() == block.scalar_type() || residual.scalar_type() == torch::kFloat32, "residual",
@@ -589,7 +592,7 @@ py::object join_norm(const Tensor &residual, const Tensor &block, const Tensor &
 }
 
 Tensor rms_norm(const Tensor &x, const Tensor &weight_, double eps) {
-  backward_mode_only("rms_norm", x, weight_);
+  calls_only("rms_norm", x, weight_);
   check_data("x", x);
   need(x.dim() >= 1, "x", "must have at least one dimension");
   const int64_t D = x.size(-1);

@@ -1,4 +1,4 @@
-"""Derivatives that the sequence operators cannot give are refused instead of lost."""
+"""Derivatives and traces that the sequence operators cannot give are refused instead of lost."""
 import pytest
 import torch
 
@@ -50,3 +50,13 @@ def test_forward_mode_derivatives_are_refused(name):
             duals[0] = fwd.make_dual(args[0].clone().requires_grad_(), torch.ones_like(args[0]))
             with pytest.raises(RuntimeError, match="Astra Fatal Error.*forward-mode"):
                 fn(*duals)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_traces_are_refused(name):
+    """A trace would hold the allocation of the result and not what fills it."""
+    from astra_cuda import sequence as seq
+    fn, args = calls(seq)[name]
+    with pytest.raises(RuntimeError, match="Astra Fatal Error.*trace"):
+        torch.jit.trace(fn, args, check_trace=False)
+    fn(*args)
