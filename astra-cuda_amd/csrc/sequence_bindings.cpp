@@ -8,6 +8,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <limits>
 #include <optional>
 
 #include "sequence/astra_sequence.h"
@@ -64,7 +65,9 @@ Tensor lengths_of(const Optional &t, const Tensor &x, int64_t batch) {
        std::string("must be int32 or int64, got ") + c10::toString(t->scalar_type()));
   need(t->dim() == 1 && t->size(0) == batch, "lengths",
        "must have shape [" + std::to_string(batch) + "], got " + shape_text(t->sizes()));
-  return t->to(torch::kInt32).contiguous();
+  // (64-bit lengths beyond what 32 bits hold are clamped like all others, not cut off)
+  const Tensor wide = t->scalar_type() == torch::kInt64 ? t->clamp(0, std::numeric_limits<int32_t>::max()) : *t;
+  return wide.to(torch::kInt32).contiguous();
 }
 
 // t with a contiguous last dimension (a dimension of size 1 has no stride to speak of).
