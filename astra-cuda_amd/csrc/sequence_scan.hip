@@ -493,7 +493,10 @@ __device__ __forceinline__ double moved64(double v) {
 template <class O>
 __device__ __forceinline__ double make_times(O &o, float dt_raw, float bias, bool live, float A, int lane) {
   const float raw = dt_raw + bias, dt = live ? softplus(raw) : 0.f;
-  double s = (double)dt * (double)A * 1.4426950408889634;
+  // No position lets less through than nothing: 2^-2000 is 0 in 32 bits, and a bound keeps sums
+  // and differences of these finite where A is not (a head without memory).
+  double s = dt > 0.f ? (double)dt * (double)A * 1.4426950408889634 : 0.;
+  s = s < -2000. ? -2000. : s;
   s += moved64<kUp + 1>(s);
   s += moved64<kUp + 2>(s);
   s += moved64<kUp + 4>(s);

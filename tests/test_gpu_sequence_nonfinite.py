@@ -1,0 +1,36 @@
+"""Infinities and NaN at positions that count: they reach what the definitions say they
+reach. Outputs of earlier positions stay what they are without them, outputs and gradients
+after a row's end stay zero, and a head that forgets at once (A = -inf) is an ordinary head."""
+import math
+
+import pytest
+import torch
+
+import sequence_oracle as oracle
+from sequence_util import BF16, DEV, F32, close, gen, normal, ref_scan, run_scan, scan_inputs, wide
+
+pytestmark = pytest.mark.gpu
+TYPES = [F32, BF16]
+SHAPES = [(1, 64, 1, 128), (2, 64, 1, 64), (3, 32, 1, 16), (2, 33, 2, 17)]  # heads, dim, groups, state
+
+
+def same(a, b):
+    return torch.equal(a.nan_to_num(nan=12345.0), b.nan_to_num(nan=12345.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_head_without_memory(dtype):
+    """A = -inf: every position forgets what was before it. The same as a decay that
+    underflows, and as the definition."""
+    from astra_cuda import sequence as seq
+    g = gen(43)
+    for T in (1, 40, 200):
+        own = {k: v.detach() for k, v in scan_inputs(g, 2, T, 2, 32, 1, 16, dtype, True).items()}
+        own["A"] = torch.tensor([-math.inf, -1.0], device=DEV)
+        got = run_scan(seq, own)
+        want = ref_scan({k: wide(v) for k, v in own.items()})
+        for i, what in enumerate(("y", "state")):
+            close(got[i], want[i], (what, T), 2.0 ** -8 if got[i].dtype == BF16 else 1e-5)
+        own["A"] = torch.tensor([-1e30, -1.0], device=DEV)
+        again = run_scan(seq, own)
+        assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
