@@ -146,6 +146,11 @@ struct Ops<bf16> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)f[i];
   }
+  // zeros in the place of what is not finite
+  static __device__ __forceinline__ void finite(Frag &f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)f[i] - (float)f[i] == 0.f ? f[i] : (bf16)0.f;
+  }
   static __device__ __forceinline__ void mma(f32x4 &acc, const Frag &a, const Frag &b) {
     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
   }
@@ -188,6 +193,10 @@ struct Ops<float> {
     return s;
   }
   static __device__ __forceinline__ Split3 split3(const float (&v)[8]) { return split(v); }
+  static __device__ __forceinline__ void finite(Frag &f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.v[i] = f.v[i] - f.v[i] == 0.f ? f.v[i] : 0.f;
+  }
   static __device__ __forceinline__ void expand(const Frag &f, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = f.v[i];
@@ -238,6 +247,10 @@ struct Tile {
 template <class T, int F>
 struct Along {  // operands contracted over positions
   const T *rows, *cols;
+  __device__ __forceinline__ float one(int f, int t) const {
+    if constexpr (sizeof(T) == 2) return (float)cols[f * Tile<T, F>::kCol + t];
+    return (float)rows[t * Tile<T, F>::kRow + f];
+  }
   __device__ __forceinline__ typename Ops<T>::Frag near(int f, int t0, int q) const {
     if constexpr (sizeof(T) == 2) {
       return Ops<T>::near(cols + f * Tile<T, F>::kCol, t0, q);
@@ -784,12 +797,12 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
       }
       mf[jp] = Ops<T>::split(m);
     }
-    // then Y^T, 16 features at a time
+    // then Y^T, 16 features at a time. A product over positions has a factor of 0 for those that
+    // come later, which 0 * inf makes a NaN of: where a result is not finite, the tiles are done
+    // once more with what is not finite in X left out where it does not count.
     const Matrix<T, VEC> ym((const T *)ap->y + ((b * ap->T + t0) * ap->H + h_now) * ap->P + p0, (int64_t)ap->H * ap->P, ap->T - t0, ap->P - p0);
     const float from = tm.from[ti];
-#pragma unroll
-    for (int i = 0; i < PP / 16; ++i) {
-      if (!on<T, NT>(f0 + 16 * i, ap->P - p0)) continue;
+    auto before = [&](int i) __attribute__((always_inline)) {  // what the state before the chunk gives
       f32x4 y = {0.f, 0.f, 0.f, 0.f};
       if constexpr (ST) {
         if (any) {
@@ -799,10 +812,43 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
           y *= from;
         }
       }
+      return y;
+    };
+    float odd = 0.f;  // 0, or NaN where a result is not finite
+#pragma unroll
+    for (int i = 0; i < PP / 16; ++i) {
+      if (!on<T, NT>(f0 + 16 * i, ap->P - p0)) continue;
+      f32x4 y = before(i);
       Ops<T>::mma(y, xa.far(f0 + 16 * i + r, 0, q), mf[0]);
       if (wi > 1) Ops<T>::mma(y, xa.far(f0 + 16 * i + r, 32, q), mf[1]);
       const float v[4] = {y[0], y[1], y[2], y[3]};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd += v[e] - v[e];
       ym.store(ti, f0 + 16 * i + 4 * q, v);
+    }
+    if (__builtin_expect(__any(!(odd == 0.f)), 0)) {
+#pragma unroll 1
+      for (int i = 0; i < PP / 16; ++i) {
+        if (!on<T, NT>(f0 + 16 * i, ap->P - p0)) continue;
+        f32x4 all = before(i), kept = all;
+#pragma unroll
+        for (int jp = 0; jp < 2; ++jp) {
+          if (2 * jp > wi) break;
+          typename Ops<T>::Frag x = xa.far(f0 + 16 * i + r, 32 * jp, q);
+          Ops<T>::mma(all, x, mf[jp]);
+          Ops<T>::finite(x);
+          Ops<T>::mma(kept, x, mf[jp]);
+        }
+        float v[4] = {kept[0], kept[1], kept[2], kept[3]};
+#pragma unroll 1
+        for (int j = 0; j <= ti; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = xa.one(f0 + 16 * i + 4 * q + e, j);
+            if (!(x - x == 0.f)) v[e] = all[e];
+          }
+        ym.store(ti, f0 + 16 * i + 4 * q, v);
+      }
     }
     if (more && c1 - c0 > 1) load_c();  // this item's is done with
     if (cc + 1 < c1 || ap->final_state) {

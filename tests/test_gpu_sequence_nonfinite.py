@@ -19,6 +19,35 @@ def same(a, b):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_no_output_depends_on_later_positions(shape, dtype):
+    from astra_cuda import sequence as seq
+    H, P, G, N = shape
+    print("causal", shape, dtype, flush=True)
+    g = gen(41)
+    for T, carried in ((40, False), (150, True)):
+        own = {k: None if v is None else v.detach() for k, v in scan_inputs(g, 1, T, H, P, G, N, dtype, carried).items()}
+        y = run_scan(seq, own)[0]
+        assert bool(torch.isfinite(y).all())
+        for at in (0, 1, 17, 31, 38):
+            for name in ("x", "dt", "B", "C"):
+                for bad in (math.inf, -math.inf, math.nan):
+                    if name == "dt" and bad == -math.inf:
+                        continue  # a step of zero
+                    spoilt = own[name].clone()
+                    spoilt[0, at].view(-1)[0] = bad
+                    got = run_scan(seq, {**own, name: spoilt})[0]
+                    assert torch.equal(got[:, :at], y[:, :at]), (name, bad, at, T)
+                    if name == "x":  # only the first feature of the first head took it in
+                        assert not bool(torch.isfinite(got[:, at:, 0, 0]).any()), (bad, at, T)
+                        rest = torch.ones(H, P, dtype=torch.bool, device=DEV)
+                        rest[0, 0] = False
+                        assert torch.equal(got[:, :, rest], y[:, :, rest]), (bad, at, T)
+                    if name == "C":  # only this position reads with it
+                        assert torch.equal(got[:, at + 1:], y[:, at + 1:]), (bad, at, T)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_a_head_without_memory(dtype):
     """A = -inf: every position forgets what was before it. The same as a decay that
     underflows, and as the definition."""
