@@ -25,6 +25,9 @@ accessed widest.
 is not read (it may hold anything), its outputs and gradients are zero, and states are
 those after position ``lengths[b]``; a row of length 0 keeps its initial state.
 
+Values that are not finite reach the outputs that the definitions say and no others. The
+gradients of up to 64 positions before and after them may be NaN as well.
+
 Errors follow ``astra_cuda.order_matching``: ``RuntimeError("Astra Fatal Error: ...")``.
 The checks, the calls and their autograd nodes are compiled (``astra_cuda._C.sequence``,
 csrc/sequence_bindings.cpp): a call of one position takes less time on the GPU than a

@@ -799,7 +799,8 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
     }
     // then Y^T, 16 features at a time. A product over positions has a factor of 0 for those that
     // come later, which 0 * inf makes a NaN of: where a result is not finite, the tiles are done
-    // once more with what is not finite in X left out where it does not count.
+    // once more with what is not finite in X left out where it does not count, and zeros after
+    // the row's end (where C is 0, but the state may not be finite).
     const Matrix<T, VEC> ym((const T *)ap->y + ((b * ap->T + t0) * ap->H + h_now) * ap->P + p0, (int64_t)ap->H * ap->P, ap->T - t0, ap->P - p0);
     const float from = tm.from[ti];
     auto before = [&](int i) __attribute__((always_inline)) {  // what the state before the chunk gives
@@ -847,6 +848,7 @@ __global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 1
             const float x = xa.one(f0 + 16 * i + 4 * q + e, j);
             if (!(x - x == 0.f)) v[e] = all[e];
           }
+        if (t0 + ti >= len) v[0] = v[1] = v[2] = v[3] = 0.f;
         ym.store(ti, f0 + 16 * i + 4 * q, v);
       }
     }
@@ -1096,7 +1098,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
   const int h_hi = g * per + (int)((int64_t)per * (slice + 1) / ap->slices);
   const bool own_j = wave < 4;
   const int mine = wave & 3, tw = 16 * mine + r;  // this lane's position
-  const bool live = t0 + lane < len;
+  const bool live = t0 + lane < len, own_live = t0 + tw < len;
 
   // one half of the workgroup brings x and the state, the other dY and the state's gradient
   const bool lower = wave < 4;
@@ -1157,7 +1159,7 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
       if (lane == 0) before = 0.f;
     }
     const float da = (before + after) + (cross + tm.total * dot);
-    const float ddt = (ap->A[h] * da + bdv) * tm.slope[lane];
+    const float ddt = live ? (ap->A[h] * da + bdv) * tm.slope[lane] : 0.f;
     if (t0 + lane < ap->T) ((T *)ap->ddt)[(b * ap->T + t0 + lane) * ap->H + h] = (T)ddt;
     const float dA = wave_sum(da * dt), dbias = wave_sum(ddt);
     if (lane == 0) {
@@ -1318,7 +1320,9 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
         if (i & 1) __builtin_amdgcn_sched_barrier(0);  // (reads further ahead cost more registers than there are)
         if (mine < 2) O::mma(dx, ya.far(16 * i + r, 0, q), mf[0]);
         O::mma(dx, ya.far(16 * i + r, 32, q), mf[1]);
-        const float v[4] = {dx[0], dx[1], dx[2], dx[3]};
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = own_live ? dx[e] : 0.f;
         xm.store(tw, 16 * i + 4 * q, v);
       }
 #pragma unroll
@@ -1426,6 +1430,10 @@ __global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || 
   }
   __syncthreads();
   if (wave == kStepWave) finish(h_hi - 1);
+  // after a row's end the factors are 0, but a state's gradient, say, may not be finite
+  if (!own_live)
+#pragma unroll
+    for (int i = 0; i < NT / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int64_t first_row = ((b * ap->T + t0) * ap->G + g) * ap->N;
   if (ap->slices == 1) {
     const Matrix<T, VEC> m((const T *)(own_j ? ap->db : ap->dc) + first_row, (int64_t)ap->G * ap->N, ap->T - t0, ap->N);

@@ -48,6 +48,45 @@ def test_no_output_depends_on_later_positions(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_rows_end_in_zeros_whatever_they_held(shape, dtype):
+    """A state, an input or a gradient that is not finite while a row lasts: outputs and
+    gradients of the positions after it are zero, and other rows do not notice."""
+    from astra_cuda import sequence as seq
+    H, P, G, N = shape
+    print("zeros", shape, dtype, flush=True)
+    g = gen(42)
+    T = 140
+    lengths = torch.tensor([10, 70, 0, 140], device=DEV, dtype=torch.int32)
+    live = torch.arange(T, device=DEV)[None] < lengths[:, None]
+    own = scan_inputs(g, 4, T, H, P, G, N, dtype, True)
+    dy, dh = normal(g, 4, T, H, P, dtype=dtype), normal(g, 4, H, P, N)
+
+    def both(p, dy, dh):
+        out = run_scan(seq, p, lengths)
+        return out, torch.autograd.grad(out, [p[k] for k in ("x", "dt", "B", "C", "h")], [dy, dh])
+
+    (y, h), grads = both(own, dy, dh)
+    for name in ("x", "dt", "B", "C", "h", "dy", "dh"):
+        for bad in (math.inf, math.nan):
+            spoilt = {"dy": dy, "dh": dh, **own}[name].detach().clone()
+            spoilt[:3].view(3, -1)[:, 0] = bad  # position 0, or the state's first value
+            p = dict(own)
+            if name in p:
+                p[name] = spoilt.requires_grad_()
+            (y2, h2), grads2 = both(p, spoilt if name == "dy" else dy, spoilt if name == "dh" else dh)
+            assert not bool(y2[~live].any()), (name, bad)
+            for n, v in zip(("dx", "ddt", "dB", "dC"), grads2):
+                assert not bool(v[~live].any()), (name, bad, n)
+            assert torch.equal(y2[3], y[3]) and torch.equal(h2[3], h[3]), (name, bad)
+            assert all(torch.equal(a[3], b[3]) for a, b in zip(grads2, grads)), (name, bad)
+            if name not in ("h", "dh"):  # a row without positions keeps its state
+                assert torch.equal(h2[2], own["h"][2]) and torch.equal(grads2[4][2], dh[2]), (name, bad)
+            elif name == "h":
+                assert same(h2[2], p["h"][2])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_a_head_without_memory(dtype):
     """A = -inf: every position forgets what was before it. The same as a decay that
     underflows, and as the definition."""
@@ -63,3 +102,25 @@ def test_a_head_without_memory(dtype):
         own["A"] = torch.tensor([-1e30, -1.0], device=DEV)
         again = run_scan(seq, own)
         assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+def test_conv_rows_end_in_zeros_whatever_they_held():
+    from astra_cuda import sequence as seq
+    g = gen(44)
+    B, T, D, K = 3, 70, 16, 4
+    lengths = torch.tensor([5, 66, 0], device=DEV, dtype=torch.int32)
+    live = torch.arange(T, device=DEV)[None] < lengths[:, None]
+    for dtype in TYPES:
+        x = normal(g, B, T, D, dtype=dtype)
+        w, window = normal(g, D, K), normal(g, B, K - 1, D, dtype=dtype)
+        x[0, 4, 0] = math.inf
+        x[1, 65, 1] = math.nan
+        window[2] = math.inf
+        x.requires_grad_()
+        y, last = seq.short_conv(x, w, initial_state=window, lengths=lengths, return_state=True)
+        assert not bool(y[~live].any())
+        assert torch.equal(last[2], window[2])
+        want = oracle.conv(x.detach().double(), w.double(), None, window.double(), lengths)[0]
+        assert torch.equal(torch.isfinite(y), torch.isfinite(want))
+        dx, = torch.autograd.grad(y, [x], torch.ones_like(y))
+        assert not bool(dx[~live].any())
