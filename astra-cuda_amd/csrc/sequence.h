@@ -110,9 +110,19 @@ __device__ __forceinline__ float row_sum(float v, float *lds) {
   return v;
 }
 
-// 1 / (1 + exp(-v)): the hardware's exp2 and reciprocal are each good to 1 ulp.
+// 1 / (1 + exp(-v)) for results of type T. The hardware's exp2 and reciprocal are each good to
+// 1 ulp, but its argument -log2(e) v is rounded, which is up to |v| 2^-24 of the result: 3.6e-6
+// at v = -60. That is nothing beside a bf16's 2^-9; for floats, exp2 is multiplied by
+// exp(-v - t ln 2) for the rounded argument t, as 1 plus a first-order term.
+template <class T>
 __device__ __forceinline__ float sigmoid(float v) {
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
+  const float t = -kLog2e * v;
+  float e = __builtin_amdgcn_exp2f(t);
+  if constexpr (sizeof(T) == 4) {
+    const float rest = fmaf(-t, -1.9046543e-9f, fmaf(-t, 0.693147182f, -v));
+    e = fabsf(t) < 126.f ? fmaf(e, rest, e) : e;  // (beyond that the result is 0 or 1, and e may be infinite)
+  }
+  return __builtin_amdgcn_rcpf(1.f + e);
 }
 
 __device__ __forceinline__ int row_length(const int32_t *lengths, int64_t b, int64_t T) {

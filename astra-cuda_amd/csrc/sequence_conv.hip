@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a) {
         float p = bias[i];
 #pragma unroll
         for (int k = 0; k < K; ++k) p += w[k][i] * in[u + k][i];
-        out[i] = a.silu ? p * sigmoid(p) : p;
+        out[i] = a.silu ? p * sigmoid<T>(p) : p;
         if (!all) out[i] = t + u < len ? out[i] : 0.f;
       }
       Vec<T, V>::store(y + u * yst, out);
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {
             float p = bias[i];
 #pragma unroll
             for (int k = 0; k < K; ++k) p += w[k][i] * in[u + k][i];
-            const float s = sigmoid(p);
+            const float s = sigmoid<T>(p);
             v *= s + p * (s - s * s);
           }
           if (!all) v = t + u < len ? v : 0.f;
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a) {
     float p = bias[i];
 #pragma unroll
     for (int k = 0; k < K; ++k) p += w[k][i] * in[k][i];
-    out[i] = a.silu ? p * sigmoid(p) : p;
+    out[i] = a.silu ? p * sigmoid<T>(p) : p;
   }
   Vec<T, V>::store((T *)a.y + b * a.D + d, out);
 #pragma unroll

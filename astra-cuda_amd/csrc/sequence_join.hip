@@ -98,7 +98,7 @@ __global__ __launch_bounds__(block_of<TPR>) void join_forward_kernel(JoinArgs a)
 #pragma unroll
           for (int i = 0; i < V; ++i) r[j][i] += cw[j][i] * (u[j][i] * i1);
       } else if (a.gate_row) {
-        const float sg = sigmoid((float)((const T *)a.gate)[row * a.gs]);
+        const float sg = sigmoid<TR>((float)((const T *)a.gate)[row * a.gs]);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(block_of<TPR>) void join_forward_kernel(JoinArgs a)
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int i = 0; i < V; ++i) r[j][i] += sigmoid(g[j][i]) * cw[j][i] * (u[j][i] * i1);
+          for (int i = 0; i < V; ++i) r[j][i] += sigmoid<TR>(g[j][i]) * cw[j][i] * (u[j][i] * i1);
       }
       store_row<TR, V, NV, TPR>((TR *)a.r1 + row * a.D, t, a.D, r);
     }
@@ -162,9 +162,9 @@ __global__ __launch_bounds__(block_of<TPR>) void join_backward_kernel(JoinArgs a
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[j][i] = sigmoid(g[j][i]);
+        for (int i = 0; i < V; ++i) g[j][i] = sigmoid<TR>(g[j][i]);
     } else {
-      const float sg = a.gate ? sigmoid((float)((const T *)a.gate)[row * a.gs]) : 1.f;
+      const float sg = a.gate ? sigmoid<TR>((float)((const T *)a.gate)[row * a.gs]) : 1.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll

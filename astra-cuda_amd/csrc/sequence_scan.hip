@@ -537,7 +537,7 @@ __device__ __forceinline__ double make_times(O &o, float dt_raw, float bias, boo
   o.into[lane] = dt * left;
   if constexpr (sizeof(O) == sizeof(GradTimes)) {
     o.left[lane] = left;
-    o.slope[lane] = live ? sigmoid(raw) : 0.f;
+    o.slope[lane] = live ? sigmoid<float>(raw) : 0.f;
   }
   if (lane == 0) o.total = __builtin_amdgcn_exp2f((float)total);
   return total;
