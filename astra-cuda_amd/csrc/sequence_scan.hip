@@ -45,6 +45,8 @@
 // transposed, so that they enter the next product from registers.
 #include "sequence.h"
 
+#include <atomic>
+
 #define ASTRA_SRC_NAME "sequence_scan.hip"
 
 namespace astra_seq {
@@ -1656,20 +1658,27 @@ size_t slice_floats(const ScanArgs &a) {
 // parts of a workspace start on 16 bytes
 size_t round4(size_t floats) { return (floats + 3) / 4 * 4; }
 
-// More than 64 KB of LDS has to be asked for, once per kernel and device.
-template <class K>
-int allow_lds(K *kernel, size_t bytes) {
-  if (bytes > 64 * 1024)
-    ASTRA_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
-                    "hipFuncSetAttribute");
+// More than 64 KB of LDS has to be asked for, once per kernel and device (a kernel is always
+// launched with the same number of bytes).
+template <auto kernel>
+int allow_lds(size_t bytes) {
+  if (bytes <= 64 * 1024) return ASTRA_OK;
+  static std::atomic<uint64_t> asked{0};  // a bit a device; devices from 64 on ask every time
+  int device = 0;
+  ASTRA_HIP_CHECK(hipGetDevice(&device), "hipGetDevice");
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (asked.load(std::memory_order_relaxed) & bit) return ASTRA_OK;
+  ASTRA_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
+                  "hipFuncSetAttribute");
+  asked.fetch_or(bit, std::memory_order_relaxed);
   return ASTRA_OK;
 }
 
 #define SCAN_LAUNCH(kernel, blocks, threads, bytes)                                                    \
   do {                                                                                                 \
     ASTRA_ABI_CHECK(blocks, <, 2147483648ll);                                                          \
-    if (int rc = allow_lds(&kernel, bytes)) return rc;                                                 \
+    if (int rc = allow_lds<&kernel>(bytes)) return rc;                                                 \
     hipLaunchKernelGGL((kernel), dim3((unsigned)(blocks)), dim3(threads), bytes, st, a);               \
     ASTRA_HIP_CHECK(rt_last_error(), #kernel " launch");                                               \
   } while (false)
