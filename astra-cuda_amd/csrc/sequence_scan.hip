@@ -631,6 +631,20 @@ struct ForwardLds {
   static constexpr size_t bytes = times + 2 * sizeof(Times);
 };
 
+// Wavefronts a SIMD that the kernel's registers leave room for. Measured both ways for every
+// tile, with four heads and 40 positions (no states) or 200 (states):
+//   floats  4 with up to 32 states (64 x 32: 55 us against 62 with 2; rows that allow single
+//           elements only: 133 against 181), else 2 (64 x 64 with states 65 against 90 with 4)
+//   bf16    4 (64 x 128 with states 66 us against 73 with 3), but 3 where 4 would spill within
+//           an item: 32 x 128 (44 against 73), and 64 x 64 without states, whose scores stay in
+//           registers over a workgroup's heads (eight heads: 146 against 152; a workgroup with
+//           one head is better with 4, 22 against 27)
+template <class T, int PT, int NT, bool ST>
+constexpr int forward_waves() {
+  if (sizeof(T) == 4) return NT == 32 ? 4 : 2;
+  return (PT == 32 && NT == 128) || (PT == 64 && NT == 64 && !ST) ? 3 : 4;
+}
+
 // A workgroup of 4 PW wavefronts: a segment of chunks of one row, for some of a group's heads
 // (and tiles of PT features) in turn. Wavefront w has positions 16 (w % 4) + 0..15 and the
 // (w / 4)th part of the features. While an item (a head's chunk) is computed, the next one's
@@ -642,7 +656,7 @@ struct ForwardLds {
 // take 97 at a large copy's 4.7 TB/s; a record of 65,536 (16 heads of 64, 128 states) 271 after
 // 119 for the segments' states, where its bytes take 64 (traced; both together 340 untraced).
 template <class T, int PT, int NT, int PW, bool ST, bool VEC>
-__global__ __launch_bounds__(256 * PW, sizeof(T) == 4 ? 2 : (PT == 32 && NT == 128) || (PT == 64 && NT == 64 && !ST) ? 3 : 4) void scan_forward_kernel(ScanArgs args) {
+__global__ __launch_bounds__(256 * PW, (forward_waves<T, PT, NT, ST>())) void scan_forward_kernel(ScanArgs args) {
   (void)args;
   const ScanArgs *ap = arguments<ScanArgs>();
   using L = ForwardLds<T, PT, NT, ST>;
@@ -1054,6 +1068,18 @@ struct StageState {
   }
 };
 
+// Wavefronts a SIMD that the kernel's registers leave room for: with 4, two workgroups share a
+// CU. Measured both ways for every tile like the forward kernel's: 4 for 32 x 32 tiles (with
+// states 192 us against 241, although 43 to 56 vector registers spill) and without states (64 x 32
+// 90 against 139 in bf16, 233 against 258 in floats), but for 128 states (32 x 128: 88 with 2, 141
+// with 4) and floats of 64 x 64 (150, 157); with states otherwise 2 (64 x 32: 144 against 205).
+template <class T, int PT, int NT, bool ST>
+constexpr int grad_waves() {
+  if (PT * NT == 1024) return 4;
+  if (ST || NT == 128) return 2;
+  return sizeof(T) == 4 && NT == 64 && PT == 64 ? 2 : 4;
+}
+
 // One workgroup of eight wavefronts: a chunk of one row and one group's B and C, its heads
 // (and their tiles of PT features) one after the other, so that dB and dC are sums in
 // registers. The first four wavefronts own 16 positions j each (dX, dB), the other four 16
@@ -1065,7 +1091,7 @@ struct StageState {
 // item: 2,048 games of 40 positions 200 us; two records of 8,192 with 128 states, one
 // workgroup a CU for its 145 KB of LDS, 231 us; 300 float games of up to 100 positions 114 us.
 template <class T, int PT, int NT, bool ST, bool VEC>
-__global__ __launch_bounds__(512, PT * NT == 1024 ? 4 : ST || sizeof(T) == 4 || NT == 128 ? 2 : 4) void scan_grad_kernel(ScanArgs args) {
+__global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_kernel(ScanArgs args) {
   (void)args;
   const ScanArgs *ap = arguments<ScanArgs>();
   using L = GradLds<T, PT, NT, ST>;
