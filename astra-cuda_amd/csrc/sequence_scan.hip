@@ -28,16 +28,16 @@
 // bf16 inputs, what is computed in between enters a product as
 //   - the sum of two (2^-18): the scores M and Q (with one, results of bf16 type were up to
 //     1.1e-3 of their term further from 64 bits than their own rounding; the second part
-//     costs 2 to 13% of a pass), and the states, in y and dX as well as in U = h0^T dY and
-//     V = dh1^T x, which end in the float gradient d(dt A). With one, the error of y goes with
+//     costs 2 to 13% of a pass), and the states in y and dX. With one, the error of y goes with
 //     |h| |C| and not with |h C|: a state whose values have a mean 16 times their spread, read
 //     out by a C of zero mean, left 2.8e-2 of y where bf16's rounding is 1.7e-3;
-//   - the sum of three (2^-26) in those that end in float states: w B and exp(s) C.
+//   - the sum of three (2^-26) in those that end in float results: w B and exp(s) C in states,
+//     and the states in U = h0^T dY and V = dh1^T x, which are part of d(dt A).
 // For float inputs the products use the float matrix instructions, at 1/16 of the bf16
 // ones' rate.
 // Against 64 bits, two records of 8,192: bf16 results 1.7e-3 (their own rounding), states'
-// gradients 1e-7, dA 1.0e-6 to 1.3e-6, ddt_bias 1.5e-6 to 2.1e-6 (all in 32 bits: 0.4e-6 to
-// 0.8e-6 and 1.0e-6 to 1.3e-6; a third part of both states does not fit 160 KB of LDS).
+// gradients 1e-7, dA 4e-7 to 7e-7, ddt_bias 2e-7 (the same in 32-bit torch operations: 2e-7,
+// 4e-7 to 8e-7, 1.0e-6 to 1.3e-6).
 //
 // A chunk is handled by wavefronts that each own 16 of its positions. A product's result
 // has its column in lane % 16 and four consecutive rows in its registers, which is the
@@ -165,9 +165,13 @@ struct Ops<bf16> {
   static __device__ __forceinline__ void mma_left(f32x4 &acc, const A &a, const B &b, int) {
     mma(acc, a, b);
   }
-  static __device__ __forceinline__ void mma(f32x4 &acc, const Split3 &a, const Frag &b) {
-    mma(acc, a.lo, b);
-    mma(acc, a.mid, b);
+  // The small parts are added up by themselves, and to the result by the caller: a sum that is
+  // much smaller or larger than the products that it is added to is rounded down, by 0.13 or
+  // 0.04 2^-24 of the result on average (measured; 0.01 where they are alike), and sums over
+  // many positions drift.
+  static __device__ __forceinline__ void mma_apart(f32x4 &acc, f32x4 &small, const Split3 &a, const Frag &b) {
+    mma(small, a.lo, b);
+    mma(small, a.mid, b);
     mma(acc, a.hi, b);
   }
 };
@@ -207,6 +211,7 @@ struct Ops<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
   }
+  static __device__ __forceinline__ void mma_apart(f32x4 &acc, f32x4 &, const Frag &a, const Frag &b) { mma(acc, a, b); }
   static __device__ __forceinline__ void mma_left(f32x4 &acc, const Frag &a, const Frag &b, int left) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
@@ -276,28 +281,33 @@ struct Along {  // operands contracted over positions
   }
 };
 
-// A state tile [R, K] (K contracted) in LDS: two bf16 parts, or floats. Rows of 256 bytes,
-// which start on the same bank, are not padded: their 16-byte blocks change places by row
-// (so that two workgroups of the forward kernel with 64 x 128 states fit a CU's LDS).
-template <class T, int R, int K>
+// A state tile [R, K] (K contracted) in LDS: the bf16 parts whose sum it is, or floats. bf16 rows
+// of 64 and of 256 bytes, of which every fourth or each starts on the same bank, are not padded:
+// their 16-byte blocks change places by row (so that two workgroups of the forward kernel, and
+// one of the gradient's, with 128 states fit a CU's LDS).
+template <class T, int R, int K, int PARTS>
 struct StateTile {
-  static constexpr bool kTwo = sizeof(T) == 2, kSwapped = kTwo && K == 128;
+  static constexpr int kParts = sizeof(T) == 2 ? PARTS : 1;
+  static constexpr int kSwapped = sizeof(T) == 2 && (K == 128 || K == 32) ? K : 0;
   static constexpr int kRow = kSwapped ? K : K + 16 / (int)sizeof(T);
-  static constexpr size_t kBytes = (kTwo ? 2 : 1) * R * kRow * sizeof(T);
+  static constexpr int kPart = R * kRow;
+  static constexpr size_t kBytes = kParts * kPart * sizeof(T);
   T *p;
   static __device__ __forceinline__ int at(int r, int k) {
-    if constexpr (kSwapped) return r * kRow + (k ^ (r & 15) << 3);
+    if constexpr (kSwapped == 128) return r * kRow + (k ^ (r & 15) << 3);
+    if constexpr (kSwapped == 32) return r * kRow + (k ^ (r >> 2 & 3) << 3);
     return r * kRow + k;
   }
   __device__ __forceinline__ auto near(int r, int k0, int q) const {
-    if constexpr (kTwo) {
-      const int i = at(r, k0 + 8 * q);
-      typename Ops<T>::Split s;
-      s.hi = Ops<T>::near(p + i, 0, 0);
-      s.lo = Ops<T>::near(p + R * kRow + i, 0, 0);
-      return s;
-    } else {
+    if constexpr (kParts == 1) {
       return Ops<T>::near(p + r * kRow, k0, q);
+    } else {
+      const T *const o = p + at(r, k0 + 8 * q);
+      if constexpr (kParts == 2) {
+        return typename Ops<T>::Split{Ops<T>::near(o, 0, 0), Ops<T>::near(o + kPart, 0, 0)};
+      } else {
+        return typename Ops<T>::Split3{Ops<T>::near(o, 0, 0), Ops<T>::near(o + kPart, 0, 0), Ops<T>::near(o + 2 * kPart, 0, 0)};
+      }
     }
   }
   // contracted over the rows instead (floats only)
@@ -308,23 +318,30 @@ struct StateTile {
     return s;
   }
   __device__ __forceinline__ void put4(int r, int k, const float (&v)[4]) const {
-    typename V4<T>::type hi, lo;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      hi[i] = (T)v[i];
-      if constexpr (kTwo) lo[i] = (T)(v[i] - (float)hi[i]);
-    }
     T *const o = p + at(r, k);
-    *reinterpret_cast<typename V4<T>::type *>(o) = hi;
-    if constexpr (kTwo) *reinterpret_cast<typename V4<T>::type *>(o + R * kRow) = lo;
+    float left[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int j = 0; j < kParts; ++j) {
+      typename V4<T>::type part;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        part[i] = (T)left[i];
+        left[i] -= (float)part[i];
+      }
+      *reinterpret_cast<typename V4<T>::type *>(o + j * kPart) = part;
+    }
   }
-  // the 8 values from element k (a multiple of 8) on, as floats
-  __device__ __forceinline__ void get8(int r, int k, float (&v)[8]) const {
+  // the first N parts of 4 values, as floats
+  template <int N>
+  __device__ __forceinline__ void get4(int r, int k, float (&v)[4]) const {
     const T *const o = p + at(r, k);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = (float)o[i];
-      if constexpr (kTwo) v[i] += (float)o[R * kRow + i];
+    for (int i = 0; i < 4; ++i) v[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < (N < kParts ? N : kParts); ++j) {
+      const typename V4<T>::type part = *reinterpret_cast<const typename V4<T>::type *>(o + j * kPart);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += (float)part[i];
     }
   }
 };
@@ -504,6 +521,14 @@ __device__ __forceinline__ double moved64(double v) {
   return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
+// v of one lane, in all of them.
+__device__ __forceinline__ double lane64(double v, int lane) {
+  const int64_t i = __builtin_bit_cast(int64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)i, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(i >> 32), lane);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
 // Fills `o` from this lane's dt and the head's bias and A; returns log2 of the chunk's decay.
 template <class O>
 __device__ __forceinline__ double make_times(O &o, float dt_raw, float bias, bool live, float A, int lane) {
@@ -521,10 +546,7 @@ __device__ __forceinline__ double make_times(O &o, float dt_raw, float bias, boo
   double ends[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t at = __builtin_bit_cast(int64_t, s);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)at, 16 * i + 15);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), 16 * i + 15);
-    ends[i] = __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+    ends[i] = lane64(s, 16 * i + 15);
     // (the other lanes' go nowhere: a place to put them costs less than a branch around them)
     if (i < 3) *(lane >= 16 * (i + 1) ? o.after + Times::past_at(i) + lane : o.nowhere) = __builtin_amdgcn_exp2f((float)(s - ends[i]));
   }
@@ -568,13 +590,19 @@ struct Mine {
 };
 
 // S = total S + X^T (weight K): X over PT features of which `np` count, K over NT of which
-// `nn` count, weight a position's.
-template <class T, int PT, int NT, int WAVES>
+// `nn` count, weight a position's. What the small parts of K give is added to S at the end, or
+// (TWICE) after each half of the positions, for kernels that have no registers to keep it in.
+template <class T, int PT, int NT, int WAVES, bool TWICE>
 __device__ __forceinline__ void update_state(f32x4 *S, float total, const float *weight, const Along<T, PT> &X,
                                              const Along<T, NT> &K, int wave, int q, int r, int np, int nn) {
   using M = Mine<PT, NT, WAVES>;
+  constexpr bool kSmall = sizeof(T) == 2;
+  f32x4 small[M::kEach];
 #pragma unroll
-  for (int i = 0; i < M::kEach; ++i) S[i] *= total;
+  for (int i = 0; i < M::kEach; ++i) {
+    S[i] *= total;
+    small[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 #pragma unroll
   for (int t0 = 0; t0 < Q; t0 += 32) {
     float w[8];
@@ -591,8 +619,14 @@ __device__ __forceinline__ void update_state(f32x4 *S, float total, const float 
         for (int e = 0; e < 8; ++e) v[e] *= w[e];
         kf = Ops<T>::split3(v);
       }
-      Ops<T>::mma(S[i], kf, X.near(M::p_of(wave, i, r), t0, q));
+      if (TWICE) small[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      Ops<T>::mma_apart(S[i], small[i], kf, X.near(M::p_of(wave, i, r), t0, q));
+      if (kSmall && TWICE) S[i] += small[i];
     }
+  }
+  if (kSmall && !TWICE) {
+#pragma unroll
+    for (int i = 0; i < M::kEach; ++i) S[i] += small[i];
   }
 }
 
@@ -627,7 +661,7 @@ struct ForwardLds {
   static constexpr size_t bn = x + (sizeof(T) == 2 ? Tile<T, PT>::kColsBytes : Tile<T, PT>::kRowsBytes);
   static constexpr size_t bt = bn + Tile<T, NT>::kRowsBytes;
   static constexpr size_t h = bt + Tile<T, NT>::kColsBytes;
-  static constexpr size_t times = h + (ST ? StateTile<T, PT, NT>::kBytes : 0);
+  static constexpr size_t times = h + (ST ? StateTile<T, PT, NT, 2>::kBytes : 0);
   static constexpr size_t bytes = times + 2 * sizeof(Times);
 };
 
@@ -664,7 +698,7 @@ __global__ __launch_bounds__(256 * PW, (forward_waves<T, PT, NT, ST>())) void sc
   using M = Mine<PT, NT, kWaves>;
   extern __shared__ __align__(16) char lds[];
   T *xl = (T *)(lds + L::x), *bn = (T *)(lds + L::bn), *bt = (T *)(lds + L::bt);
-  const StateTile<T, PT, NT> hl{(T *)(lds + L::h)};
+  const StateTile<T, PT, NT, 2> hl{(T *)(lds + L::h)};
   Times *times = (Times *)(lds + L::times);
   const Along<T, PT> xa{xl, xl};
   const Along<T, NT> ba{bn, bt};
@@ -870,7 +904,7 @@ __global__ __launch_bounds__(256 * PW, (forward_waves<T, PT, NT, ST>())) void sc
     }
     if (more && c1 - c0 > 1) load_c();  // this item's is done with
     if (cc + 1 < c1 || ap->final_state) {
-      update_state<T, PT, NT, kWaves>(S, tm.total, tm.into, xa, ba, wave, q, r, ap->P - p0, ap->N);
+      update_state<T, PT, NT, kWaves, true>(S, tm.total, tm.into, xa, ba, wave, q, r, ap->P - p0, ap->N);
       any = true;
       if (ap->final_state && cc + 1 == ap->chunks) store_state<PT, NT, kWaves, VEC>(S, ap->final_state + bh * pn, *ap, p0, wave, q, r);
     }
@@ -962,7 +996,7 @@ __global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs args)
     __syncthreads();
     if (n + 1 < n_chunks) load(n + 1);
     if (KEEP && ap->chunks > 1) store_state<PT, NT, kWaves, VEC>(S, ap->ds + (bh * ap->chunks + chunk_of(n)) * pn, *ap, p0, wave, q, r);
-    update_state<T, PT, NT, kWaves>(S, tm.total, REV ? tm.from : tm.into, xa, ka, wave, q, r, ap->P - p0, ap->N);
+    update_state<T, PT, NT, kWaves, false>(S, tm.total, REV ? tm.from : tm.into, xa, ka, wave, q, r, ap->P - p0, ap->N);
     if (wave == 0 && n + 1 < n_chunks) step(n + 1);
   }
   if (!KEEP) {
@@ -1011,8 +1045,8 @@ struct HeadSums {
   float vb[Q];        // exp(s_Q - s_j) B_j . (dh1^T x_j)
   float col[Q];       // sum over i >= j of the pairs (i, j), without dt_j
   float cross[4][Q];  // sum of the pairs (i, j) with j < t <= i, over the j of each wavefront
-  float dot[8], diag[4];  // parts of <dh1, h0>, and of the sum of dY x
-  float pad[4];
+  float dot[32];      // parts of <dh1, h0>, of the rows of 16 lanes
+  float diag[4];      // parts of the sum of dY x
 };
 
 template <class T, int PT, int NT, bool ST>
@@ -1026,15 +1060,15 @@ struct GradLds {
   static constexpr size_t yn = xn + Tile<T, PT>::kRowsBytes;
   static constexpr size_t yt = yn + Tile<T, PT>::kRowsBytes;
   static constexpr size_t dh = yt + Tile<T, PT>::kColsBytes;                               // [p][n]
-  static constexpr size_t dht = dh + (ST ? StateTile<T, PT, NT>::kBytes : 0);              // [n][p]
-  static constexpr size_t h0 = dht + (ST && two ? StateTile<T, NT, PT>::kBytes : 0);       // [n][p], floats [p][n]
-  static constexpr size_t times = h0 + (!ST ? 0 : two ? StateTile<T, NT, PT>::kBytes : StateTile<T, PT, NT>::kBytes);
+  static constexpr size_t dht = dh + (ST ? StateTile<T, PT, NT, 2>::kBytes : 0);           // [n][p]
+  static constexpr size_t h0 = dht + (ST && two ? StateTile<T, NT, PT, 3>::kBytes : 0);    // [n][p], floats [p][n]
+  static constexpr size_t times = h0 + (!ST ? 0 : two ? StateTile<T, NT, PT, 3>::kBytes : StateTile<T, PT, NT, 2>::kBytes);
   static constexpr size_t sums = times + 3 * sizeof(GradTimes);
   static constexpr size_t bytes = sums + 2 * sizeof(HeadSums);
   static_assert(bytes <= 160 * 1024, "more LDS than a CU has");
 };
 
-// 4 x 4 blocks of a state [P, N] on their way from memory to LDS.
+// 4 x 4 blocks of a state [P, N] on their way from memory to LDS, of THREADS threads.
 template <int PT, int NT, int THREADS, bool VEC>
 struct StageState {
   static constexpr int kBlocks = (PT / 4) * (NT / 4), kEach = (kBlocks + THREADS - 1) / THREADS;
@@ -1063,6 +1097,33 @@ struct StageState {
         const float across[4] = {v[e][0][k], v[e][1][k], v[e][2][k], v[e][3][k]};
         if (rows) rows->put4(p + k, n, along);
         if (cols) cols->put4(n + k, p, across);
+      }
+    }
+  }
+  // Adds to `sum` this thread's part of the product with the other state in LDS: of h0, all of it
+  // with the other's two parts; of the other, what its two parts leave with h0's first.
+  template <bool TWO, class Rows, class Cols>
+  __device__ __forceinline__ void dot(bool all, const Rows &rows, const Cols &cols, float &sum, int tid) const {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int blk = tid + e * THREADS, n = (blk % (NT / 4)) * 4, p = (blk / (NT / 4)) * 4;
+      if (kBlocks % THREADS && blk >= kBlocks) continue;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float o[4], four = 0.f;
+        if (all) {
+          rows.template get4<2>(p + k, n, o);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) four += v[e][k][i] * o[i];
+        } else if constexpr (TWO) {
+          cols.template get4<1>(n + k, p, o);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = v[e][i][k], rest = x - (float)(bf16)x;
+            four += (rest - (float)(bf16)rest) * o[i];
+          }
+        }
+        sum += four;
       }
     }
   }
@@ -1101,8 +1162,8 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
   extern __shared__ __align__(16) char lds[];
   T *bn = (T *)(lds + L::bn), *bt = (T *)(lds + L::bt), *cn = (T *)(lds + L::cn), *ct = (T *)(lds + L::ct);
   T *xn = (T *)(lds + L::xn), *yn = (T *)(lds + L::yn), *yt = (T *)(lds + L::yt);
-  const StateTile<T, PT, NT> dhl{(T *)(lds + L::dh)}, h0f{(T *)(lds + L::h0)};
-  const StateTile<T, NT, PT> dhtl{(T *)(lds + L::dht)}, h0l{(T *)(lds + L::h0)};
+  const StateTile<T, PT, NT, 2> dhl{(T *)(lds + L::dh)}, h0f{(T *)(lds + L::h0)};
+  const StateTile<T, NT, PT, 3> dhtl{(T *)(lds + L::dht)}, h0l{(T *)(lds + L::h0)};
   // Times of three heads: the next one's are written while one wavefront may still read the last
   // one's in finish(); HeadSums of two, whose writers are a barrier behind that.
   GradTimes *times = (GradTimes *)(lds + L::times);
@@ -1137,16 +1198,18 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
   const float *dh_next = nullptr, *h0_next = nullptr;
   auto load = [&](int h, int pt) __attribute__((always_inline)) {
     const int p0 = pt * PT;
-    const int64_t bh = b * ap->H + h;
     const T *row = lower ? (const T *)ap->x + b * ap->xsb + t0 * ap->xst + h * ap->xsh + p0
                          : (const T *)ap->dy + ((b * ap->T + t0) * ap->H + h) * ap->P + p0;
     xy.load(Matrix<T, VEC>(row, lower ? ap->xst : (int64_t)ap->H * ap->P, len - t0, ap->P - p0), ht);
+    if (pt == 0 && wave == kTimesWave) raw = raw_step<T, VEC>(*ap, b, h, t0, len, lane);
+  };
+  auto load_states = [&](int h, int pt) __attribute__((always_inline)) {
     if constexpr (ST) {
+      const int64_t bh = b * ap->H + h;
       h0_next = ap->chunks > 1 ? ap->cs + (bh * ap->chunks + c) * pn : ap->initial ? ap->initial + bh * pn : nullptr;
       dh_next = ap->chunks > 1 ? ap->ds + (bh * ap->chunks + c) * pn : ap->dfinal ? ap->dfinal + bh * pn : nullptr;
-      hd.load(lower ? h0_next : dh_next, *ap, p0, ht);
+      hd.load(lower ? h0_next : dh_next, *ap, pt * PT, ht);
     }
-    if (pt == 0 && wave == kTimesWave) raw = raw_step<T, VEC>(*ap, b, h, t0, len, lane);
   };
   auto step = [&](int h) __attribute__((always_inline)) {
     make_times(times[(unsigned)h % 3], (float)raw, ap->bias ? ap->bias[h] : 0.f, live, ap->A[h], lane);
@@ -1155,10 +1218,15 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
   auto finish = [&](int h) __attribute__((always_inline)) {
     const GradTimes &tm = times[(unsigned)h % 3];
     const HeadSums &s = sums[h & 1];
-    float dot = 0.f, diag = 0.f, cross = 0.f;
+    double dot = 0.;
+    float diag = 0.f, cross = 0.f;
     if constexpr (ST) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dot += s.dot[i];
+      dot = s.dot[lane & 31];
+      dot += moved64<kUp + 1>(dot);
+      dot += moved64<kUp + 2>(dot);
+      dot += moved64<kUp + 4>(dot);
+      dot += moved64<kUp + 8>(dot);
+      dot = lane64(dot, 15) + lane64(dot, 31);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1186,7 +1254,7 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
       before = __shfl_up(before, 1, kWave);
       if (lane == 0) before = 0.f;
     }
-    const float da = (before + after) + (cross + tm.total * dot);
+    const float da = (before + after) + (cross + (float)(tm.total * dot));
     const float ddt = live ? (ap->A[h] * da + bdv) * tm.slope[lane] : 0.f;
     if (t0 + lane < ap->T) ((T *)ap->ddt)[(b * ap->T + t0 + lane) * ap->H + h] = (T)ddt;
     const float dA = wave_sum(da * dt), dbias = wave_sum(ddt);
@@ -1203,6 +1271,7 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
     s.load(Matrix<T, VEC>((const T *)ap->b + b * ap->bsb + t0 * ap->bst + g * ap->bsg, ap->bst, len - t0, ap->N), tid);
     u.load(Matrix<T, VEC>((const T *)ap->c + b * ap->csb + t0 * ap->cst + g * ap->csg, ap->cst, len - t0, ap->N), tid);
     load(h_lo, 0);
+    load_states(h_lo, 0);
     s.put(bn, bt, tid);
     u.put(cn, ct, tid);
   }
@@ -1226,8 +1295,8 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
     else
       xy.put(yn, yt, ht);
     if constexpr (ST) {
-      using Rows = const StateTile<T, PT, NT> *;
-      using Cols = const StateTile<T, NT, PT> *;
+      using Rows = const StateTile<T, PT, NT, 2> *;
+      using Cols = const StateTile<T, NT, PT, 3> *;
       if (lower)
         hd.put(L::two ? (Rows) nullptr : &h0f, L::two ? &h0l : (Cols) nullptr, ht);
       else
@@ -1242,20 +1311,12 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
     if (more) load(h, pt);
     if (wave == kStepWave && pt_now == 0 && !first) finish(h_now - 1);
     if (pt_now == 0) diag = inter = col = dot = 0.f;
-    if (dh && h0) {
-      for (int i = tid; i < PT * NT / 8; i += 512) {
-        float u[8], v[8];
-        if constexpr (L::two) {
-          h0l.get8(i / (PT / 8), i % (PT / 8) * 8, u);
-          dhtl.get8(i / (PT / 8), i % (PT / 8) * 8, v);
-        } else {
-          h0f.get8(i / (NT / 8), i % (NT / 8) * 8, u);
-          dhl.get8(i / (NT / 8), i % (NT / 8) * 8, v);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dot += u[e] * v[e];
-      }
-    }
+    // <dh1, h0> = <h0, dh1 in two parts> + <what those leave of dh1, h0's first part>, from the
+    // float32 values that each half of the workgroup still holds (products of parts on both
+    // sides were 2e-6 of dA off); the sums of 16 threads are added up in 64 bits: thousands of
+    // terms that may cancel
+    if (dh && h0) hd.template dot<L::two>(lower, dhl, h0l, dot, ht);
+    if (more) load_states(h, pt);
 
     const float hi = tm.hi[tw], lo = tm.lo[tw];
     if (own_j) {
@@ -1357,18 +1418,21 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
       for (int i = 0; i < NT / 16; ++i) {
         if (!on<T, NT>(16 * i, ap->N)) continue;
         if (dh) {
-          f32x4 u = {0.f, 0.f, 0.f, 0.f};
+          f32x4 u = {0.f, 0.f, 0.f, 0.f}, small = u;
 #pragma unroll
           for (int k = 0; k < PT / 32; ++k) {
             if (!on<T, NT>(32 * k, np)) continue;
             if constexpr (L::two)
-              O::mma_left(u, dhtl.near(16 * i + r, 32 * k, q), xf[k], rest<T, NT>(np - 32 * k));
+              O::mma_apart(u, small, dhtl.near(16 * i + r, 32 * k, q), xf[k]);
             else
               O::mma_left(u, dhl.across(16 * i + r, 32 * k, q), xf[k], rest<T, NT>(np - 32 * k));
           }
+          if constexpr (L::two) u += small;
+          float four = 0.f;
           const typename V4<T>::type bv = *reinterpret_cast<const typename V4<T>::type *>(bn + tw * BC::kRow + 16 * i + 4 * q);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) inter += left * u[e] * (float)bv[e];
+          for (int e = 0; e < 4; ++e) four += u[e] * (float)bv[e];
+          inter += left * four;
           acc[i] += u * into;
         }
         if (i & 1) __builtin_amdgcn_sched_barrier(0);
@@ -1419,19 +1483,22 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
       for (int i = 0; i < NT / 16; ++i) {
         if (!on<T, NT>(16 * i, ap->N)) continue;
         if (h0) {
-          f32x4 u = {0.f, 0.f, 0.f, 0.f};
+          f32x4 u = {0.f, 0.f, 0.f, 0.f}, small = u;
 #pragma unroll
           for (int k = 0; k < PT / 32; ++k) {
             if (!on<T, NT>(32 * k, np)) continue;
             if constexpr (L::two)
-              O::mma_left(u, h0l.near(16 * i + r, 32 * k, q), yf[k], rest<T, NT>(np - 32 * k));
+              O::mma_apart(u, small, h0l.near(16 * i + r, 32 * k, q), yf[k]);
             else
               O::mma_left(u, h0f.across(16 * i + r, 32 * k, q), yf[k], rest<T, NT>(np - 32 * k));
           }
+          if constexpr (L::two) u += small;
           u *= from;
+          float four = 0.f;
           const typename V4<T>::type cv = *reinterpret_cast<const typename V4<T>::type *>(cn + tw * BC::kRow + 16 * i + 4 * q);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) inter += u[e] * (float)cv[e];
+          for (int e = 0; e < 4; ++e) four += u[e] * (float)cv[e];
+          inter += four;
           acc[i] += u;
         }
         if (i & 1) __builtin_amdgcn_sched_barrier(0);
@@ -1444,8 +1511,8 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
       if constexpr (ST) {
         inter = rows_sum(inter);
         if (q == 0) (own_j ? sum.vb : sum.uc)[tw] = inter;
-        const float v = wave_sum(dot);
-        if (lane == 0) sum.dot[wave] = v;
+        const float row = lanes_sum<16>(dot);
+        if (r == 0) sum.dot[4 * wave + q] = row;
       }
       if (own_j) {
         diag = wave_sum(diag);
