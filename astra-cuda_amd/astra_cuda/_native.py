@@ -89,6 +89,8 @@ class HLObservation(ctypes.Structure):
         (n, ctypes.c_float) for n in ("player_sin", "player_cos", "round_fraction")]
 
 
+# The arguments of the entry points of include/sequence/astra_sequence.h, for callers of the C ABI
+# from Python (the package itself calls it through astra_cuda._C).
 def _fields(pointers: str, sizes: str, ints: str) -> list:
     return [(n, _vp) for n in pointers.split()] + [(n, ctypes.c_int64) for n in sizes.split()] + [
         (n, _c_i32) for n in ints.split()]

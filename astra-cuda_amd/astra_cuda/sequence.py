@@ -9,19 +9,22 @@ time in rollouts with a state of fixed size per env (include/sequence/astra_sequ
                      read-out and step size given per position
 ``join_norm``        what stands between two blocks: the norm after one, its gate and
                      residual scale, the residual sum, the norm before the next
-``short_conv_step``, ``state_scan_step``   one position, the state moved on in place (and its
-version raised: a backward pass that had saved it refuses to run, as after torch's own
-operations in place)
+``short_conv_step``, ``state_scan_step``   one position, the state moved on in place
 
-The first three are differentiable in every tensor they take (once, backwards: tensors with
-a forward-mode tangent are refused, and so is being part of a torch.jit trace). Tensors are float32
-or bfloat16 on one HIP device; sums, states and norms are float32 throughout, and each
-result is rounded to its type once. Calls run on the caller's current stream and do not
+The first three are differentiable in every tensor they take, backwards and once: tensors with
+a forward-mode tangent are refused, and so is being part of a torch.jit trace. A step raises its
+state's version: a backward pass that had saved the state refuses to run, as after torch's own
+operations in place.
+
+Tensors are float32 or bfloat16 on one HIP device. Sums, states and norms are float32
+throughout, and each result is rounded to its type once; what is computed in between enters
+the matrix products of a bfloat16 scan as the sum of two bfloat16 values (2^-18), or of three
+where it ends in a float32 result. Calls run on the caller's current stream and do not
 synchronise. Tensors may be strided as long as their last dimension is contiguous (others
 are copied); rows of 16-byte aligned, multiple-of-8 (bf16) or 4 (float32) elements are
 accessed widest.
 
-``lengths`` (int32 ``[B]``) says how many positions of each row count: what comes after
+``lengths`` (int32 or int64 ``[B]``) says how many positions of each row count: what comes after
 is not read (it may hold anything), its outputs and gradients are zero, and states are
 those after position ``lengths[b]``; a row of length 0 keeps its initial state.
 

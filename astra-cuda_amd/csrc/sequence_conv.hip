@@ -119,9 +119,10 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a) {
 // positions, `gridDim.y` rows of workgroups apart, and keeps its part of dw and dbias in
 // registers. A run recomputes the K-1 values of g after its end. U positions at a time, so
 // that their loads are in flight together and the windows of x and g need few moves; inside
-// a run without a check each. 2,048 games of 40 positions and 640 bf16 channels: 105 us, 3.0
-// TB/s, where its bytes take 67; the sigmoid's exp and reciprocal and some 30 further vector
-// operations an element come to as long.
+// a run without a check each. 2,048 games of 40 positions and 640 bf16 channels: 104 us, 3.0
+// TB/s, where its bytes take 67; in floats 150 us, 4.2 TB/s. Neither traffic nor vector work
+// (43% busy) is the limit, but what is in flight: 188 registers leave room for two wavefronts
+// a SIMD, and 1.5 are there on average. Channel by channel (odd widths) 220 and 258 us.
 constexpr int kConvCols = 16;
 template <class T, int K, int V>
 __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a) {

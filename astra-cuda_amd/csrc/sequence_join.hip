@@ -9,8 +9,12 @@
 // Some 12 operations an element (45 in the gradient): bound by memory traffic, so a row is
 // read once into registers, both sums are taken there, and each thread keeps the weights
 // of its columns over all the rows that it works on. Times: 81,920 rows of 256 in bf16
-// forwards 53 us (4.0 TB/s), backwards 86 (3.9); 16,384 rows of 4,096 with a residual in
-// 32 bits 170 (4.7, a large copy's rate) and 276 (4.4).
+// forwards 52 us (4.1 TB/s), backwards 86 (3.9); 16,384 rows of 4,096 with a residual in
+// 32 bits 172 (4.7, a large copy's rate) and 277 (4.4).
+// That holds up to two vectors a thread. With four of 8 bf16 columns (widths 1,025 to 2,048 and
+// 4,097 to 8,192) a thread needs 207 registers forwards and 256 with 70 to 120 more in the
+// accumulation file backwards, one or two wavefronts a SIMD: 2.5 and 1.8 to 2.0 TB/s with a gate
+// of full width; backwards beyond 8,192 columns 118 to 170 registers spill: 1.8 (bf16) to 3.3.
 #include "sequence.h"
 
 #define ASTRA_SRC_NAME "sequence_join.hip"

@@ -671,8 +671,9 @@ struct ForwardLds {
 //           elements only: 133 against 181), else 2 (64 x 64 with states 65 against 90 with 4)
 //   bf16    4 (64 x 128 with states 66 us against 73 with 3), but 3 where 4 would spill within
 //           an item: 32 x 128 (44 against 73), and 64 x 64 without states, whose scores stay in
-//           registers over a workgroup's heads (eight heads: 146 against 152; a workgroup with
-//           one head is better with 4, 22 against 27)
+//           registers over a workgroup's heads (2,048 games with eight heads, forward and
+//           gradient: 336 us against 338; a workgroup with one head is better with 4, 22
+//           against 28)
 template <class T, int PT, int NT, bool ST>
 constexpr int forward_waves() {
   if (sizeof(T) == 4) return NT == 32 ? 4 : 2;
@@ -685,10 +686,14 @@ constexpr int forward_waves() {
 // inputs are on their way to registers, and the first wavefront, which has the fewest pairs
 // of positions, works out its step sizes. Where the segment is a single chunk, B, C and their
 // scores are loaded and computed once for all heads. ST: whether there are states before a chunk.
+// Positions that do not exist are worked on like others, up to the chunk's 64. A segment of
+// several chunks is one head's, which stages B and C and computes the scores for itself.
 // Bound by latency and issue between the two barriers of an item, not by traffic: 2,048 games
-// of 40 positions (8 heads of 64, 64 states) 146 us where their bytes, final states among them,
-// take 97 at a large copy's 4.7 TB/s; a record of 65,536 (16 heads of 64, 128 states) 271 after
-// 119 for the segments' states, where its bytes take 64 (traced; both together 340 untraced).
+// of 40 positions (8 heads of 64, 64 states) 154 us where their bytes, final states among them,
+// take 97 at a large copy's 4.7 TB/s; a record of 65,536 (16 heads of 64, 128 states) 300 after
+// 119 for the segments' states, where its bytes take 64 and the products of both, some 160
+// GFLOP, 133. Counters of the two: vector units busy 39 and 45% of the time, matrix units 10 and
+// 17, LDS 22 and 38 (nearly half of it conflicts), 2.3 and 3.4 wavefronts a SIMD.
 template <class T, int PT, int NT, int PW, bool ST, bool VEC>
 __global__ __launch_bounds__(256 * PW, (forward_waves<T, PT, NT, ST>())) void scan_forward_kernel(ScanArgs args) {
   (void)args;
@@ -929,7 +934,7 @@ struct StatesLds {
 // what comes into each chunk (ds); otherwise from zero, writing what comes out and the
 // segment's decay. Pipelined like the forward kernel. Taken where rows are few, because the
 // chunks of a row are a chain: the inputs are read twice for it. Bound like the forward kernel:
-// two records of 8,192 35 us without the states between and 45 with them.
+// two records of 8,192 34 to 35 us without the states between and 46 with them.
 template <class T, int PT, int NT, int PW, bool REV, bool KEEP, bool VEC>
 __global__ __launch_bounds__(256 * PW, 4) void scan_states_kernel(ScanArgs args) {
   (void)args;
@@ -1131,9 +1136,10 @@ struct StageState {
 
 // Wavefronts a SIMD that the kernel's registers leave room for: with 4, two workgroups share a
 // CU. Measured both ways for every tile like the forward kernel's: 4 for 32 x 32 tiles (with
-// states 192 us against 241, although 43 to 56 vector registers spill) and without states (64 x 32
-// 90 against 139 in bf16, 233 against 258 in floats), but for 128 states (32 x 128: 88 with 2, 141
-// with 4) and floats of 64 x 64 (150, 157); with states otherwise 2 (64 x 32: 144 against 205).
+// states 227 us against 259 in bf16, 308 against 381 in floats, although 43 and 54 vector registers
+// spill) and without states (64 x 32: 90 against 139 in bf16, 235 against 258 in floats), but for
+// 128 states (32 x 128: 89 with 2, 141 with 4) and floats of 64 x 64 (151, 158); with states
+// otherwise 2 (64 x 32: 157 against 209).
 template <class T, int PT, int NT, bool ST>
 constexpr int grad_waves() {
   if (PT * NT == 1024) return 4;
@@ -1149,8 +1155,11 @@ constexpr int grad_waves() {
 // sums give for dt by the wavefront of the last 16 j: those have the fewest pairs. ST:
 // whether there are states before or after the chunk.
 // Bound by the vector operations on pairs and the LDS reads of operands, with two barriers an
-// item: 2,048 games of 40 positions 200 us; two records of 8,192 with 128 states, one
-// workgroup a CU for its 145 KB of LDS, 231 us; 300 float games of up to 100 positions 114 us.
+// item: 2,048 games of 40 positions 203 us (vector units 49% busy, LDS 37, matrix units 11, 3.5
+// wavefronts a SIMD); two records of 8,192 with 128 states 239 us (41, 39, 12; one workgroup a CU
+// for its 160 KB of LDS as for its 236 registers, and C B^T again for every head); 300 float
+// games of up to 100 positions 117 us (26, 13, 26; of 204 MB written, 39 are results, the rest
+// spilled registers).
 template <class T, int PT, int NT, bool ST, bool VEC>
 __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_kernel(ScanArgs args) {
   (void)args;
