@@ -212,6 +212,15 @@ struct Ops<float> {
     for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
   }
   static __device__ __forceinline__ void mma_apart(f32x4 &acc, f32x4 &, const Frag &a, const Frag &b) { mma(acc, a, b); }
+  // a product over two tiles of positions with the own one last: the second, before which the
+  // first one is zero, or the first
+  static __device__ __forceinline__ void mma_own(f32x4 &acc, const Frag &a, const Frag &b, int second) {
+#pragma unroll
+    for (int i = 4; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
+    if (second) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
+  }
   static __device__ __forceinline__ void mma_left(f32x4 &acc, const Frag &a, const Frag &b, int left) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
@@ -1136,10 +1145,10 @@ struct StageState {
 
 // Wavefronts a SIMD that the kernel's registers leave room for: with 4, two workgroups share a
 // CU. Measured both ways for every tile like the forward kernel's: 4 for 32 x 32 tiles (with
-// states 227 us against 259 in bf16, 308 against 381 in floats, although 43 and 54 vector registers
-// spill) and without states (64 x 32: 90 against 139 in bf16, 235 against 258 in floats), but for
-// 128 states (32 x 128: 89 with 2, 141 with 4) and floats of 64 x 64 (151, 158); with states
-// otherwise 2 (64 x 32: 157 against 209).
+// states 225 us against 258 in bf16, 325 against 382 in floats, although 43 and 58 vector registers
+// spill) and without states (64 x 32: 90 against 137 in bf16, 248 against 255 in floats), but for
+// 128 states (32 x 128: 88 with 2, 142 with 4) and floats of 64 x 64 (152, 158); with states
+// otherwise 2 (64 x 32: 156 against 211).
 template <class T, int PT, int NT, bool ST>
 constexpr int grad_waves() {
   if (PT * NT == 1024) return 4;
@@ -1158,7 +1167,7 @@ constexpr int grad_waves() {
 // item: 2,048 games of 40 positions 203 us (vector units 49% busy, LDS 37, matrix units 11, 3.5
 // wavefronts a SIMD); two records of 8,192 with 128 states 239 us (41, 39, 12; one workgroup a CU
 // for its 160 KB of LDS as for its 236 registers, and C B^T again for every head); 300 float
-// games of up to 100 positions 117 us (26, 13, 26; of 204 MB written, 39 are results, the rest
+// games of up to 100 positions 120 us (26, 12, 24; of 217 MB written, 39 are results, the rest
 // spilled registers).
 template <class T, int PT, int NT, bool ST, bool VEC>
 __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_kernel(ScanArgs args) {
@@ -1416,8 +1425,19 @@ __global__ __launch_bounds__(512, (grad_waves<T, PT, NT, ST>())) void scan_grad_
           dx *= into;
         }
         if (i & 1) __builtin_amdgcn_sched_barrier(0);  // (reads further ahead cost more registers than there are)
-        if (mine < 2) O::mma(dx, ya.far(16 * i + r, 0, q), mf[0]);
-        O::mma(dx, ya.far(16 * i + r, 32, q), mf[1]);
+        if constexpr (L::two) {
+          if (mine < 2) O::mma(dx, ya.far(16 * i + r, 0, q), mf[0]);
+          O::mma(dx, ya.far(16 * i + r, 32, q), mf[1]);
+        } else {
+          // the own tile last: what D dY is rounded to is not rounded again with every later term
+          // (dX 7e-8 off instead of 1.2e-7)
+          if (mine < 2) O::mma(dx, ya.far(16 * i + r, 32, q), mf[1]);
+          const typename O::Frag y = ya.far(16 * i + r, mine < 2 ? 0 : 32, q);
+          if (mine < 2)
+            O::mma_own(dx, y, mf[0], mine & 1);
+          else
+            O::mma_own(dx, y, mf[1], mine & 1);
+        }
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = own_live ? dx[e] : 0.f;
