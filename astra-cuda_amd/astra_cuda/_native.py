@@ -63,6 +63,11 @@ SEQUENCE_PROTOTYPES = {
     "astra_join_norm_forward": (_c_int, [_vp, _vp]),
     "astra_join_norm_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
     "astra_join_norm_backward": (_c_int, [_vp, _vp]),
+    "astra_gated_linear_projections": (_c_int, [_vp, ctypes.POINTER(_sz)]),
+    "astra_gated_linear_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
+    "astra_gated_linear_forward": (_c_int, [_vp, _vp]),
+    "astra_gated_linear_grad_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
+    "astra_gated_linear_backward": (_c_int, [_vp, _vp]),
 }
 
 
@@ -145,6 +150,17 @@ class JoinNormGrad(ctypes.Structure):
     """astra_join_norm_grad (include/sequence/astra_sequence.h)."""
     _fields_ = [("f", JoinNorm)] + _fields("djoined dnormed dresidual dblock dgate dpost dnext dscale workspace",
                                            "", "") + [("workspace_bytes", _sz)]
+
+
+class GatedLinear(ctypes.Structure):
+    """astra_gated_linear (include/sequence/astra_sequence.h)."""
+    _fields_ = _fields("x gate up h projections", "rows x_stride gate_stride up_stride",
+                       "width hidden type activation") + [("workspace", _vp), ("workspace_bytes", _sz)]
+
+
+class GatedLinearGrad(ctypes.Structure):
+    """astra_gated_linear_grad (include/sequence/astra_sequence.h)."""
+    _fields_ = [("f", GatedLinear)] + _fields("dh dx dgate dup workspace", "", "") + [("workspace_bytes", _sz)]
 
 
 _lib = None

@@ -23,8 +23,8 @@ CSRC = os.path.join(os.path.dirname(PKG_DIR), "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB_NAME = "libastra_market.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = [os.path.join(CSRC, f) for f in ("market.hip", "high_low.hip", "sequence_conv.hip", "sequence_join.hip",
-                                           "sequence_scan.hip")]
+SOURCES = [os.path.join(CSRC, f) for f in ("market.hip", "high_low.hip", "sequence_conv.hip", "sequence_gated.hip",
+                                           "sequence_join.hip", "sequence_scan.hip")]
 
 ARCH = os.environ.get("ASTRA_OFFLOAD_ARCH", "gfx950")
 

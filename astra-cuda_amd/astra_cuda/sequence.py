@@ -43,6 +43,7 @@ import torch  # noqa: F401  (before the compiled binding)
 MAX_TAPS = 4        # ASTRA_SEQ_MAX_TAPS
 MAX_STATE = 128     # ASTRA_SEQ_MAX_STATE
 MAX_NORM_WIDTH = 16384  # ASTRA_SEQ_MAX_NORM_WIDTH
+MAX_LINEAR_WIDTH = 1048576  # ASTRA_SEQ_MAX_LINEAR_WIDTH
 
 _ops = None
 
@@ -114,3 +115,14 @@ def rms_norm(x, weight, *, eps=1e-6):
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension: the norm before the
     first block, where there is nothing to join yet."""
     return (_ops or _compiled()).rms_norm(x, weight, eps)
+
+
+def gated_linear(x, gate_weight, up_weight, *, activation="silu"):
+    """The gated feed-forward block before its way back: ``act(x gate_weight^T) * (x up_weight^T)``.
+
+    ``x`` ``[..., D]``, the weights ``[F, D]`` of x's type, as those of two ``nn.Linear``; returns
+    ``[..., F]``. ``activation``: ``"silu"``, or ``"gelu"`` (v times the normal distribution function
+    at v, by erf). Bfloat16 products are summed in float32 and the result is rounded once; the
+    gradients of the two projections are rounded to x's type before their own products.
+    """
+    return (_ops or _compiled()).gated_linear(x, gate_weight, up_weight, activation)

@@ -163,7 +163,7 @@ __device__ __forceinline__ bool sum_rows(const float *part, int64_t rows, int64_
 
 inline bool aligned(const void *p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+constexpr int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 inline size_t elem_size(int32_t type) { return type == ASTRA_SEQ_BF16 ? 2 : 4; }
 

@@ -603,6 +603,98 @@ Tensor rms_norm(const Tensor &x, const Tensor &weight_, double eps) {
   return join(flat(x), {}, {}, param("weight", weight_, x, {D}), {}, {}, eps)[0].view(x.sizes());
 }
 
+// ---------------------------------------------------------------------- gated_linear
+
+// Every tensor is 2-D here, with contiguous rows.
+astra_gated_linear gated_struct(const Tensor &x, const Tensor &gate, const Tensor &up, const Tensor &projections,
+                                int64_t activation) {
+  astra_gated_linear f{};
+  f.x = ptr(x);
+  f.gate = ptr(gate);
+  f.up = ptr(up);
+  f.projections = ptr<float>(projections);
+  f.rows = x.size(0);
+  f.x_stride = x.stride(0);
+  f.gate_stride = gate.stride(0);
+  f.up_stride = up.stride(0);
+  f.width = (int32_t)x.size(1);
+  f.hidden = (int32_t)gate.size(0);
+  f.type = type_of(x);
+  f.activation = (int32_t)activation;
+  return f;
+}
+
+// h, and with `keep` the projections that the backward call is faster with
+Tensor gated_forward(const Tensor &x, const Tensor &gate, const Tensor &up, int64_t activation, Tensor *keep) {
+  const c10::DeviceGuard guard(x.device());
+  const Tensor h = empty(x, {x.size(0), gate.size(0)}, x.scalar_type());
+  astra_gated_linear f = gated_struct(x, gate, up, Tensor(), activation);
+  f.h = ptr(h);
+  if (keep) {
+    size_t n = 0;
+    check(astra_gated_linear_projections(&f, &n));
+    if (n) *keep = empty(x, {(int64_t)n}, torch::kFloat32);
+    f.projections = ptr<float>(*keep);
+  }
+  check(astra_gated_linear_workspace_size(&f, &f.workspace_bytes));
+  const Tensor ws = workspace(x, f.workspace_bytes);
+  f.workspace = ptr(ws);
+  check(astra_gated_linear_forward(&f, stream_of(x.get_device())));
+  return h;
+}
+
+struct GatedLinear : torch::autograd::Function<GatedLinear> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &gate, const Tensor &up, int64_t activation) {
+    Tensor projections;
+    const Tensor h = gated_forward(x, gate, up, activation, &projections);
+    ctx->save_for_backward({x, gate, up, projections});
+    ctx->saved_data["activation"] = activation;
+    return h;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    check_once();
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &gate = s[1], &up = s[2];
+    variable_list out(4);
+    const Tensor dh = undefined_or_contiguous(grads[0]);
+    if (!dh.defined()) return out;
+    const c10::DeviceGuard guard(x.device());
+    for (int i = 0; i < 3; ++i)
+      if (s[i].requires_grad()) out[i] = empty(s[i], s[i].sizes(), s[i].scalar_type());
+    astra_gated_linear_grad g{};
+    g.f = gated_struct(x, gate, up, s[3], ctx->saved_data["activation"].toInt());
+    g.dh = ptr(dh);
+    g.dx = ptr(out[0]);
+    g.dgate = ptr(out[1]);
+    g.dup = ptr(out[2]);
+    check(astra_gated_linear_grad_workspace_size(&g.f, &g.workspace_bytes));
+    const Tensor ws = workspace(x, g.workspace_bytes);
+    g.workspace = ptr(ws);
+    check(astra_gated_linear_backward(&g, stream_of(x.get_device())));
+    return out;
+  }
+};
+
+Tensor gated_linear(const Tensor &x_, const Tensor &gate_, const Tensor &up_, const std::string &activation) {
+  calls_only("gated_linear", x_, gate_, up_);
+  check_data("x", x_);
+  need(x_.dim() >= 1 && x_.size(-1) >= 1, "x", "must have shape [..., width], got " + shape_text(x_.sizes()));
+  need(gate_.dim() == 2 && gate_.size(0) >= 1, "gate_weight", "must have shape [hidden, width], got " + shape_text(gate_.sizes()));
+  const int64_t D = x_.size(-1), F = gate_.size(0);
+  for (int64_t n : {D, F})
+    need(n <= ASTRA_SEQ_MAX_LINEAR_WIDTH, "width", "must be 1 to " + std::to_string(ASTRA_SEQ_MAX_LINEAR_WIDTH) + ", got " + std::to_string(n));
+  check_like("gate_weight", gate_, x_, {F, D});
+  check_like("up_weight", up_, x_, {F, D});
+  need(activation == "silu" || activation == "gelu", "activation", "must be 'silu' or 'gelu', got '" + activation + "'");
+  const int64_t act = activation == "silu" ? ASTRA_SEQ_SILU : ASTRA_SEQ_GELU;
+  const Tensor x = flat(x_), gate = rows(gate_), up = rows(up_);
+  const Tensor h = with_grad({&x, &gate, &up}) ? GatedLinear::apply(x, gate, up, act) : gated_forward(x, gate, up, act, nullptr);
+  if (x_.dim() == 2) return h;
+  std::vector<int64_t> shape(x_.sizes().begin(), x_.sizes().end());
+  shape.back() = F;
+  return h.view(shape);
+}
+
 }  // namespace
 
 void bind_sequence(py::module_ &m) {
@@ -618,6 +710,7 @@ void bind_sequence(py::module_ &m) {
   s.def("join_norm", &join_norm, py::arg("residual"), py::arg("block"), py::arg("post_weight"), py::arg("next_weight"),
         py::arg("gate"), py::arg("scale"), py::arg("eps"));
   s.def("rms_norm", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("eps"));
+  s.def("gated_linear", &gated_linear, py::arg("x"), py::arg("gate_weight"), py::arg("up_weight"), py::arg("activation"));
   s.attr("MAX_TAPS") = ASTRA_SEQ_MAX_TAPS;
   s.attr("MAX_STATE") = ASTRA_SEQ_MAX_STATE;
   s.attr("MAX_NORM_WIDTH") = ASTRA_SEQ_MAX_NORM_WIDTH;

@@ -1,0 +1,889 @@
+// sequence_gated.hip -- the gated feed-forward block before its way back:
+//
+//   a = x Wg^T,  b = x Wu^T,  h = act(a) * b          x [M,D]; Wg, Wu [F,D]; h [M,F]
+//   da = dh b act'(a),  db = dh act(a)
+//   dx = da Wg + db Wu,  dWg = da^T x,  dWu = db^T x
+//
+// All are matrix products out[r, l] = sum_k left[l, k] right[r, k] on the matrix cores, with
+// what surrounds them done on the accumulators.
+#include "sequence.h"
+
+#define ASTRA_SRC_NAME "sequence_gated.hip"
+
+namespace astra_seq {
+namespace {
+
+// ------------------------------------------------------------------ tiles of a product
+//
+// A workgroup of WL x WR wavefronts has a tile of BL x BR results, a wavefront NL x NR of 16 x 16.
+// 128 bytes of the contraction at a time (64 bf16 or 32 floats) are brought straight into LDS, one
+// such step ahead of the products, which read them as fragments: lane i has 16 bytes of line
+// i % 16, the (i / 16)-th of its four.
+//
+// An operand lies along the contraction (a line of the tile is 128 contiguous bytes) or across it
+// (TR: the tile is 64 or 32 rows of memory, a line is a column). Its memory starts on 16 bytes, as
+// does every row of it, and what lies outside of it is never read: accesses are checked against the
+// buffer's size, and bring zeros from outside.
+//
+// The 16-byte pieces of a row in LDS are permuted (by an exclusive or with a number of the row) so
+// that the lanes of a fragment fall on all banks.
+typedef uint32_t Piece __attribute__((ext_vector_type(4)));
+constexpr int kStep = 128;           // bytes of the contraction in a step
+constexpr uint32_t kOutside = 0x7ffffff0u;
+
+template <class T>
+constexpr int kStepOf = kStep / (int)sizeof(T);
+
+template <class T>
+struct Fragment;
+template <>
+struct Fragment<bf16> {
+  typedef bf16x8 type;
+};
+template <>
+struct Fragment<float> {
+  typedef f32x4 type;
+};
+template <class T>
+using Frag = typename Fragment<T>::type;
+
+__device__ __forceinline__ void multiply(f32x4 &acc, const bf16x8 &l, const bf16x8 &r) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(l, r, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void multiply(f32x4 &acc, const f32x4 &l, const f32x4 &r) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(l[i], r[i], acc, 0, 0, 0);
+}
+
+// An operand: `lines` lines of `len` elements of the contraction, rows `ld` elements apart.
+struct Operand {
+  const void *p;
+  int64_t ld, lines, len;
+};
+
+// The part of an operand that one wavefront of NW brings into LDS: B lines from `line0` on.
+template <class T, bool TR, int B, int NW, bool PAIRED>
+struct Loader {
+  static constexpr int N = B * kStep / 1024 / NW;               // loads of 1024 bytes
+  static constexpr int kRow = TR ? B * (int)sizeof(T) : kStep;  // bytes of a row in LDS
+  static constexpr int kPieces = kRow / 16, kRows = 64 / kPieces;  // (rows of one load)
+  static_assert(!TR || kRow >= 256, "rows of a tile across the contraction cover all banks");
+  static_assert(TR || NW % 2 == 0, "along the contraction a lane has the same piece of all its rows");
+  const char *base;
+  int32_t ld, lines;  // bytes from row to row; lines of the tile inside the operand (TR: their bytes)
+  int64_t left;       // bytes (TR: rows) of the contraction from base on
+  uint32_t off[N];
+  int32_t piece;
+
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (!TR) return PAIRED ? 2 * ((row >> 3) & 3) + ((row >> 1) & 1) : (row >> 1) & 7;
+    if constexpr (sizeof(T) == 2) return 2 * ((row & 3) + 4 * ((row >> 3) & 1));
+    return 4 * ((row >> 2) & 3);
+  }
+
+  __device__ __forceinline__ void init(const Operand &o, int64_t line0, int wave, int lane) {
+    ld = (int32_t)(o.ld * (int64_t)sizeof(T));
+    lines = (int32_t)max((int64_t)0, min((int64_t)B, o.lines - line0)) * (TR ? (int)sizeof(T) : 1);
+    base = (const char *)o.p + line0 * (TR ? (int64_t)sizeof(T) : (int64_t)ld);
+    left = o.len * (TR ? 1 : (int64_t)sizeof(T));
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int row = (wave + NW * j) * kRows + lane / kPieces;
+      piece = ((lane % kPieces) ^ swizzle(row)) * 16;
+      off[j] = (TR ? piece : row) < lines ? (uint32_t)(row * ld + piece) : kOutside;
+    }
+  }
+
+  // Brings the next step into `lds` and moves on; zeros after the last.
+  __device__ __forceinline__ void load(char *lds, int wave) {
+    constexpr int kMost = TR ? kStepOf<T> : kStep;
+    const int most = (int)min(left, (int64_t)kMost);
+    int bytes = TR ? (most - 1) * ld + lines : (lines - 1) * ld + most;
+    bytes = ((most > 0) & (lines > 0)) ? bytes : 0;
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, bytes, 0x00020000);
+    const bool out = !TR && piece >= most;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (__attribute__((address_space(3))) void *)(lds + (wave + NW * j) * 1024), 16,
+          out ? kOutside : off[j], 0, 0, 0);
+    base += TR ? (int64_t)kMost * ld : kMost;
+    left -= kMost;
+  }
+};
+
+// A lane's fragments of an operand's tile in LDS, from its tile `first` of 16 lines on: tile `t` of a
+// wavefront, half `s` of the step. With PAIRED, lines 4 q .. 4 q + 3 of two neighbouring tiles are 8
+// neighbouring lines of the operand, so that a lane has 8 neighbouring results.
+template <class T, bool TR, int B, bool PAIRED>
+struct Reader {
+  static constexpr int kRow = TR ? B * (int)sizeof(T) : kStep;
+  uint32_t at;
+
+  __device__ __forceinline__ void init(int first, int lane) {
+    const int i = lane % 16, g = lane / 16;
+    if constexpr (!TR) {
+      const int row = PAIRED ? 8 * (i / 4) + i % 4 : i, swz = PAIRED ? 2 * (i / 4) + (i % 4) / 2 : i / 2;
+      at = (16 * first + row) * kStep + ((g ^ swz) * 16);
+    } else if constexpr (sizeof(T) == 2) {
+      const int x = 2 * ((i / 4) + 4 * (g & 1));
+      at = (8 * g + i / 4) * kRow + (((2 * first + (i % 4) / 2) ^ x) * 16) + (i % 2) * 8;
+    } else {
+      at = 4 * g * kRow + (((4 * first + i / 4) ^ (4 * g)) * 16) + (i % 4) * 4;
+    }
+  }
+  // Takes the addresses of the tiles anew from here on: an operation each, where the compiler would
+  // keep them all in registers that are not there.
+  __device__ __forceinline__ void again() { asm volatile("" : "+v"(at)); }
+
+  __device__ __forceinline__ Frag<T> read(const char *lds, int t, int s) const {
+    if constexpr (!TR) {
+      const int row = PAIRED ? 32 * (t / 2) + 4 * (t % 2) : 16 * t;
+      return *reinterpret_cast<const Frag<T> *>(lds + (at ^ (64 * s)) + row * kStep);
+    } else if constexpr (sizeof(T) == 2) {
+      // rows 32 s + 8 g + 0..3 and + 4..7: 4 lanes bring 16 lines of a row, each lane gets a line
+      const char *p = lds + (at ^ (32 * t)) + 32 * s * kRow;
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4 *Lds;
+      const bf16x4 a = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)p));
+      const bf16x4 b = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p + 4 * kRow)));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      Frag<T> f;
+      const char *p = lds + (at ^ (64 * t)) + 16 * s * kRow;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) f[n] = *reinterpret_cast<const float *>(p + n * kRow);
+      return f;
+    }
+  }
+};
+
+// HALVES: the left tile is two operands of BL / 2 lines each, of which a wavefront has the same
+// lines, PAIRED as above.
+template <class T, bool LTR, bool RTR, int NL_, int NR_, int WL_, int WR_, bool HALVES_>
+struct Product {
+  static constexpr int NL = NL_, NR = NR_, WL = WL_, WR = WR_;
+  static constexpr bool HALVES = HALVES_;
+  static constexpr int NW = WL * WR, BL = 16 * NL * WL, BR = 16 * NR * WR;
+  static constexpr int kBytes = (BL + BR) * kStep, kThreads = 64 * NW;
+  static constexpr int BLL = HALVES ? BL / 2 : BL;  // lines of a left operand
+  static constexpr int NLL = HALVES ? NL / 2 : NL;  // tiles of it to a wavefront
+  typedef T type;
+  typedef Loader<T, LTR, BLL, NW, HALVES> Left;
+  typedef Loader<T, RTR, BR, NW, false> Right;
+
+  typedef Reader<T, LTR, BLL, HALVES> LeftReader;
+  typedef Reader<T, RTR, BR, false> RightReader;
+
+  // One step's products while the next is on its way: two tiles that do not overlap.
+  template <class Load>
+  static __device__ __forceinline__ void step(f32x4 (&acc)[NL][NR], char *__restrict next, const char *__restrict now,
+                                              const Load &load, LeftReader &left, RightReader &right) {
+    load(next);
+    __builtin_amdgcn_sched_barrier(0);  // (on its way before the products, not after them)
+    if (LTR) left.again();
+    if (RTR) right.again();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      Frag<T> a[NL], b[NR];
+#pragma unroll
+      for (int l = 0; l < NL; ++l) a[l] = left.read(now + (l / NLL) * BLL * kStep, l % NLL, s);
+#pragma unroll
+      for (int r = 0; r < NR; ++r) b[r] = right.read(now + BL * kStep, r, s);
+#pragma unroll
+      for (int l = 0; l < NL; ++l)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) multiply(acc[l][r], a[l], b[r]);
+    }
+  }
+
+  // (A barrier does not wait for what is on its way to LDS.)
+  static __device__ __forceinline__ void arrived() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+
+  // acc[l][r] += the products of `steps` steps, each brought into a tile by load(lds).
+  template <class Load>
+  static __device__ __forceinline__ void run(f32x4 (&acc)[NL][NR], int64_t steps, const Load &load, int wave, int lane) {
+    __shared__ __attribute__((aligned(1024))) char first[kBytes], second[kBytes];
+    LeftReader left;
+    RightReader right;
+    left.init(wave % WL * NLL, lane);
+    right.init(wave / WL * NR, lane);
+    load(first);
+    for (int64_t k = 0; k < steps; k += 2) {
+      arrived();
+      step(acc, second, first, load, left, right);
+      arrived();
+      step(acc, first, second, load, left, right);
+    }
+    arrived();  // (nothing is on its way, and nobody reads, when the tiles are used again)
+  }
+};
+
+// Tile `n` of nl x nr, spread so that an XCD (workgroups are given to the eight in turn) works on
+// neighbouring tiles, kBand right tiles by all left ones: what they share stays in its L2.
+constexpr int kXcds = 8, kBand = 8;
+__device__ __forceinline__ void tile_of(int64_t n, int64_t nl, int64_t nr, int64_t *l, int64_t *r) {
+  const int64_t total = nl * nr, each = total / kXcds, rest = total % kXcds;
+  const int64_t xcd = n % kXcds, at = n / kXcds;
+  n = xcd * each + min(xcd, rest) + at;
+  const int64_t band = n / (kBand * nl), in = n % (kBand * nl);
+  const int64_t high = min((int64_t)kBand, nr - band * kBand);
+  *l = in / high;
+  *r = band * kBand + in % high;
+}
+
+// ------------------------------------------------------------------------ activations
+
+// act(a) and its derivative
+template <class T>
+__device__ __forceinline__ float act(float a, int kind) {
+  if (kind == ASTRA_SEQ_SILU) return a * sigmoid<T>(a);
+  return a * 0.5f * erfcf(a * -0.70710678f);
+}
+template <class T>
+__device__ __forceinline__ void act_slope(float a, int kind, float *value, float *slope) {
+  if (kind == ASTRA_SEQ_SILU) {
+    const float s = sigmoid<T>(a);
+    *value = a * s;
+    *slope = s * (1.f + a * (1.f - s));
+  } else {
+    const float phi = 0.5f * erfcf(a * -0.70710678f);
+    *value = a * phi;
+    *slope = phi + a * (0.39894228f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * a * a));
+  }
+}
+
+// ---------------------------------------------------------------- results and their rows
+
+// n of four neighbouring elements, in one access where `wide` says that it may be
+template <class T>
+__device__ __forceinline__ f32x4 load4(const T *p, int n, bool wide) {
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (wide && n >= 4) {
+    Vec<T, 4>::load(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) v[i] = (float)p[i];
+  }
+  return f32x4{v[0], v[1], v[2], v[3]};
+}
+template <class T>
+__device__ __forceinline__ void store4(T *p, const f32x4 &x, int n, bool wide) {
+  if (wide && n >= 4) {
+    const float v[4] = {x[0], x[1], x[2], x[3]};
+    Vec<T, 4>::store(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = (T)x[i];
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void load8(const T *p, float (&v)[8], int n, bool wide) {
+  if (wide && n >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      Vec<T, 8>::load(p, v);
+    } else {
+      float u[4], w[4];
+      Vec<T, 4>::load(p, u);
+      Vec<T, 4>::load(p + 4, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = u[i], v[4 + i] = w[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8(T *p, const float (&v)[8], int n, bool wide) {
+  if (wide && n >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      Vec<T, 8>::store(p, v);
+    } else {
+      const float u[4] = {v[0], v[1], v[2], v[3]}, w[4] = {v[4], v[5], v[6], v[7]};
+      Vec<T, 4>::store(p, u);
+      Vec<T, 4>::store(p + 4, w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = (T)v[i];
+  }
+}
+
+struct GatedArgs {
+  Operand x, gate, up;       // as left or right operands of the first products
+  const void *dh;            // [M, F]
+  void *h;                   // [M, F]
+  float *ab;                 // [2, M, F] (may be NULL): a and b, for the gradients
+  void *dab;                 // [M, 2 Fp]: da, db, zero from F to Fp
+  int64_t M, F, Fp;
+  int32_t kind, wide;
+};
+
+template <class P>
+struct LoadHalves {
+  typename P::Left &first, &second;
+  typename P::Right &right;
+  int wave;
+  __device__ __forceinline__ void operator()(char *lds) const {
+    first.load(lds, wave);
+    second.load(lds + P::BLL * kStep, wave);
+    right.load(lds + P::BL * kStep, wave);
+  }
+};
+
+// h (and a, b), or with GRAD da and db from dh: the left tile is half gate, half up, so that a lane
+// has a and b of the same elements.
+template <class P, bool GRAD>
+__global__ __launch_bounds__(P::kThreads) void gated_kernel(GatedArgs g) {
+  typedef typename P::type T;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int64_t F = GRAD ? g.Fp : g.F;
+  int64_t tl, tr;
+  tile_of(blockIdx.x, cdiv(F, P::BLL), cdiv(g.M, P::BR), &tl, &tr);
+  typename P::Left gate, up;
+  typename P::Right x;
+  gate.init(g.gate, tl * P::BLL, wave, lane);
+  up.init(g.up, tl * P::BLL, wave, lane);
+  x.init(g.x, tr * P::BR, wave, lane);
+  f32x4 acc[P::NL][P::NR] = {};
+  P::run(acc, cdiv(g.x.len, kStepOf<T>), LoadHalves<P>{gate, up, x, wave}, wave, lane);
+  const int wl = wave % P::WL, wr = wave / P::WL;
+#pragma unroll
+  for (int r = 0; r < P::NR; ++r) {
+    const int64_t m = tr * P::BR + (wr * P::NR + r) * 16 + lane % 16;
+    if (m >= g.M) continue;
+#pragma unroll
+    for (int l = 0; l < P::NLL; l += 2) {
+      const int64_t f = tl * P::BLL + (wl * P::NLL + l) * 16 + 8 * (lane / 16);
+      const int n = (int)min((int64_t)8, g.F - f);
+      float a[8], b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[i] = acc[l + i / 4][r][i % 4];
+        b[i] = acc[P::NLL + l + i / 4][r][i % 4];
+      }
+      if constexpr (GRAD) {
+        if (f >= g.Fp) continue;
+        float dh[8], da[8], db[8];
+        load8((const T *)g.dh + m * g.F + f, dh, n, g.wide);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float v, s;
+          act_slope<T>(a[i], g.kind, &v, &s);
+          da[i] = i < n ? dh[i] * b[i] * s : 0.f;
+          db[i] = i < n ? dh[i] * v : 0.f;
+        }
+        T *p = (T *)g.dab + m * 2 * g.Fp + f;
+        const int np = (int)min((int64_t)8, g.Fp - f);
+        store8(p, da, np, true);
+        store8(p + g.Fp, db, np, true);
+      } else {
+        if (n <= 0) continue;
+        float h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = act<T>(a[i], g.kind) * b[i];
+        store8((T *)g.h + m * g.F + f, h, n, g.wide);
+        if (g.ab) {
+          store8(g.ab + m * g.F + f, a, n, g.wide);
+          store8(g.ab + (g.M + m) * g.F + f, b, n, g.wide);
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------- gradients' products
+
+struct ProductArgs {
+  Operand left[2], right[2];  // summed over both pairs where there are two
+  int32_t pairs;
+  // results [r, l]: rows from `split` on are the second output's
+  void *out[2];
+  int64_t out_ld, nl, nr, split, rows;  // rows: of each output
+  float *part;                          // [slices, nr, nl] or NULL: partial sums instead of results
+  int32_t slices, wide;
+  int64_t steps;  // of a slice
+};
+
+template <class P>
+struct LoadBoth {
+  typename P::Left &left;
+  typename P::Right &right;
+  int wave;
+  __device__ __forceinline__ void operator()(char *lds) const {
+    left.load(lds, wave);
+    right.load(lds + P::BL * kStep, wave);
+  }
+};
+
+template <class P>
+__global__ __launch_bounds__(P::kThreads) void product_kernel(ProductArgs g) {
+  typedef typename P::type T;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int64_t tiles = cdiv(g.nl, P::BL) * cdiv(g.nr, P::BR);
+  const int64_t slice = blockIdx.x / tiles;
+  int64_t tl, tr;
+  tile_of(blockIdx.x % tiles, cdiv(g.nl, P::BL), cdiv(g.nr, P::BR), &tl, &tr);
+  f32x4 acc[P::NL][P::NR] = {};
+  for (int pair = 0; pair < g.pairs; ++pair) {
+    Operand lo = g.left[pair], ro = g.right[pair];
+    int64_t steps = cdiv(lo.len, kStepOf<T>);
+    if (g.slices > 1) {
+      const int64_t k0 = slice * g.steps * kStepOf<T>;
+      // (only operands across the contraction are cut)
+      lo.p = (const T *)lo.p + k0 * lo.ld;
+      ro.p = (const T *)ro.p + k0 * ro.ld;
+      lo.len = ro.len = max((int64_t)0, min(g.steps * kStepOf<T>, lo.len - k0));
+      steps = cdiv(lo.len, kStepOf<T>);
+    }
+    typename P::Left left;
+    typename P::Right right;
+    left.init(lo, tl * P::BL, wave, lane);
+    right.init(ro, tr * P::BR, wave, lane);
+    P::run(acc, steps, LoadBoth<P>{left, right, wave}, wave, lane);
+  }
+  const int wl = wave % P::WL, wr = wave / P::WL;
+#pragma unroll
+  for (int r = 0; r < P::NR; ++r) {
+    const int64_t row = tr * P::BR + (wr * P::NR + r) * 16 + lane % 16;
+    if (row >= g.nr) continue;
+    const bool second = row >= g.split;
+    const int64_t at = second ? row - g.split : row;
+    if (!g.part && at >= g.rows) continue;
+#pragma unroll
+    for (int l = 0; l < P::NL; ++l) {
+      const int64_t col = tl * P::BL + (wl * P::NL + l) * 16 + 4 * (lane / 16);
+      const int n = (int)min((int64_t)4, g.nl - col);
+      if (n <= 0) continue;
+      if (g.part)
+        store4(g.part + (slice * g.nr + row) * g.nl + col, acc[l][r], n, g.nl % 4 == 0);
+      else
+        store4((T *)g.out[second] + at * g.out_ld + col, acc[l][r], n, g.wide);
+    }
+  }
+}
+
+// The results from the slices' partial sums, in order.
+template <class T>
+__global__ __launch_bounds__(256) void join_slices_kernel(ProductArgs g) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, total = g.nr * g.nl;
+  if (i >= total) return;
+  const int n = (int)min((int64_t)4, total - i);
+  const bool wide = total % 4 == 0;
+  f32x4 s = {};
+  for (int k = 0; k < g.slices; ++k) s += load4(g.part + k * total + i, n, wide);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j >= n) break;
+    const int64_t row = (i + j) / g.nl, col = (i + j) % g.nl;
+    const bool second = row >= g.split;
+    const int64_t at = second ? row - g.split : row;
+    if (at < g.rows) ((T *)g.out[second])[at * g.out_ld + col] = (T)s[j];
+  }
+}
+
+// ---------------------------------------------------------------------- aligned copies
+
+// [rows, width] with rows of `ld` elements, any alignment, as rows of `wide` elements (a multiple of
+// 16 bytes) filled up with zeros.
+template <class T>
+__global__ __launch_bounds__(256) void align_kernel(const T *in, T *out, int64_t rows, int64_t width, int64_t ld, int64_t wide) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = wide / V;
+  if (i >= rows * per) return;
+  const int64_t row = i / per, c = (i - row * per) * V;
+  float v[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = c + j < width ? (float)in[row * ld + c + j] : 0.f;
+  Vec<T, V>::store(out + row * wide + c, v);
+}
+
+// da and db from a and b that the forward call kept.
+template <class T>
+__global__ __launch_bounds__(256) void gated_slopes_kernel(GatedArgs g) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = g.Fp / 4;
+  if (i >= g.M * per) return;
+  const int64_t m = i / per, f = (i - m * per) * 4;
+  const int n = (int)min((int64_t)4, g.F - f);
+  const f32x4 a = load4(g.ab + m * g.F + f, n, g.wide), b = load4(g.ab + (g.M + m) * g.F + f, n, g.wide);
+  const f32x4 dh = load4((const T *)g.dh + m * g.F + f, n, g.wide);
+  f32x4 da, db;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float v, s;
+    act_slope<T>(a[j], g.kind, &v, &s);
+    da[j] = j < n ? dh[j] * b[j] * s : 0.f;
+    db[j] = j < n ? dh[j] * v : 0.f;
+  }
+  T *p = (T *)g.dab + m * 2 * g.Fp + f;
+  store4(p, da, 4, true);
+  store4(p + g.Fp, db, 4, true);
+}
+
+// --------------------------------------------------------------------------- few rows
+
+// One fragment straight from memory: 16 bytes from byte `k` of the contraction on (zeros beyond).
+template <class T, bool ALIGNED>
+__device__ __forceinline__ Frag<T> fragment(const T *row, int64_t k, int64_t len) {
+  constexpr int V = 16 / sizeof(T);
+  Frag<T> f = {};
+  if constexpr (ALIGNED) {
+    if (k < len) f = *reinterpret_cast<const Frag<T> *>(row + k);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (k + i < len) f[i] = row[k + i];
+  }
+  return f;
+}
+
+// Up to 16 MT rows of x: the weights are read once, each by the lanes that multiply with it, and
+// nothing is staged. A workgroup has 16 columns of the result; its wavefronts share the contraction.
+template <class T, int MT, bool ALIGNED>
+__global__ __launch_bounds__(256) void gated_few_kernel(GatedArgs g) {
+  constexpr int V = 16 / sizeof(T), kStepE = kStepOf<T>;
+  __shared__ f32x4 sums[4][2 * MT][64];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int i = lane % 16, q = lane / 16;
+  const int64_t f0 = (int64_t)blockIdx.x * 16, line = min(f0 + i, g.F - 1), K = g.x.len;
+  const T *gate = (const T *)g.gate.p + line * g.gate.ld, *up = (const T *)g.up.p + line * g.up.ld;
+  const T *x[MT];
+#pragma unroll
+  for (int r = 0; r < MT; ++r) x[r] = (const T *)g.x.p + min((int64_t)(16 * r + i), g.M - 1) * g.x.ld;
+  f32x4 a[MT] = {}, b[MT] = {};
+  for (int64_t k = wave * kStepE + q * V; k - q * V < K; k += 4 * kStepE) {
+    Frag<T> ga[2], ub[2], xr[2][MT];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int64_t at = k + s * (kStepE / 2);
+      ga[s] = fragment<T, ALIGNED>(gate, at, K);
+      ub[s] = fragment<T, ALIGNED>(up, at, K);
+#pragma unroll
+      for (int r = 0; r < MT; ++r) xr[s][r] = fragment<T, ALIGNED>(x[r], at, K);
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int r = 0; r < MT; ++r) {
+        multiply(a[r], ga[s], xr[s][r]);
+        multiply(b[r], ub[s], xr[s][r]);
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < MT; ++r) {
+    sums[wave][r][lane] = a[r];
+    sums[wave][MT + r][lane] = b[r];
+  }
+  __syncthreads();
+  const int64_t f = f0 + 4 * q;
+  const int n = (int)min((int64_t)4, g.F - f);
+  for (int r = wave; r < MT; r += 4) {
+    const int64_t m = 16 * r + i;
+    if (m >= g.M || n <= 0) continue;
+    f32x4 sa = sums[0][r][lane], sb = sums[0][MT + r][lane], h;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      sa += sums[w][r][lane];
+      sb += sums[w][MT + r][lane];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = act<T>(sa[j], g.kind) * sb[j];
+    store4((T *)g.h + m * g.F + f, h, n, g.wide);
+    if (g.ab) {
+      store4(g.ab + m * g.F + f, sa, n, g.wide);
+      store4(g.ab + (g.M + m) * g.F + f, sb, n, g.wide);
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------- launches
+
+int check(const astra_gated_linear *f) {
+  ASTRA_SEQ_POINTER(f);
+  ASTRA_SEQ_TYPE_CHECK(f->type);
+  ASTRA_ABI_CHECK(f->rows, >=, 0);
+  ASTRA_ABI_CHECK(f->width, >=, 1);
+  ASTRA_ABI_CHECK(f->width, <=, ASTRA_SEQ_MAX_LINEAR_WIDTH);
+  ASTRA_ABI_CHECK(f->hidden, >=, 1);
+  ASTRA_ABI_CHECK(f->hidden, <=, ASTRA_SEQ_MAX_LINEAR_WIDTH);
+  ASTRA_ABI_CHECK(f->x_stride, >=, 0);
+  ASTRA_ABI_CHECK(f->gate_stride, >=, 0);
+  ASTRA_ABI_CHECK(f->up_stride, >=, 0);
+  if (f->activation != ASTRA_SEQ_SILU && f->activation != ASTRA_SEQ_GELU)
+    return fail(ASTRA_ERR_INVALID_ARGUMENT, "astra_gated_linear: the activation is ASTRA_SEQ_SILU or ASTRA_SEQ_GELU");
+  return ASTRA_OK;
+}
+
+int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
+int64_t per16(int32_t type) { return 16 / (int64_t)elem_size(type); }
+// rows of the hidden width in a workspace
+int64_t padded_hidden(const astra_gated_linear &f) { return round_up(f.hidden, per16(f.type)); }
+
+bool few(const astra_gated_linear &f) { return f.rows <= 64; }
+
+// Whether an operand is read as it lies, or copied to a workspace first. (256 rows of a tile have to
+// be within the 2 GB that one access can reach.)
+bool direct(const astra_gated_linear &f, const void *p, int64_t stride) {
+  const int64_t v = per16(f.type);
+  return aligned(p, 16) && stride % v == 0 && f.width % v == 0 && stride < (int64_t(1) << 20);
+}
+size_t copy_bytes(const astra_gated_linear &f, const void *p, int64_t stride, int64_t rows) {
+  return direct(f, p, stride) ? 0 : (size_t)(rows * round_up(f.width, per16(f.type))) * elem_size(f.type);
+}
+
+struct Operands {
+  Operand x, gate, up;
+};
+size_t copies_bytes(const astra_gated_linear &f) {
+  return copy_bytes(f, f.x, f.x_stride, f.rows) + copy_bytes(f, f.gate, f.gate_stride, f.hidden) +
+         copy_bytes(f, f.up, f.up_stride, f.hidden);
+}
+
+template <class T>
+Operand operand(const astra_gated_linear &f, const void *p, int64_t stride, int64_t rows, char **ws, hipStream_t st) {
+  if (direct(f, p, stride)) return {p, stride, rows, f.width};
+  const int64_t wide = round_up(f.width, per16(f.type)), pieces = rows * (wide / per16(f.type));
+  T *out = (T *)*ws;
+  *ws += (size_t)(rows * wide) * sizeof(T);
+  if (pieces)
+    hipLaunchKernelGGL(align_kernel<T>, dim3((unsigned)cdiv(pieces, 256)), dim3(256), 0, st, (const T *)p, out, rows,
+                       (int64_t)f.width, stride, wide);
+  return {out, wide, rows, wide};
+}
+
+template <class T>
+Operands operands(const astra_gated_linear &f, char **ws, hipStream_t st) {
+  return {operand<T>(f, f.x, f.x_stride, f.rows, ws, st), operand<T>(f, f.gate, f.gate_stride, f.hidden, ws, st),
+          operand<T>(f, f.up, f.up_stride, f.hidden, ws, st)};
+}
+
+GatedArgs args_of(const astra_gated_linear &f) {
+  GatedArgs g{};
+  g.h = f.h;
+  g.ab = f.projections;
+  g.M = f.rows;
+  g.F = f.hidden;
+  g.Fp = padded_hidden(f);
+  g.kind = f.activation;
+  return g;
+}
+
+// The two sizes of tiles: 256 x 256 results by 2 x 2 wavefronts, or 128 x 128.
+template <class T, bool LTR, bool RTR, bool HALVES>
+using Large = Product<T, LTR, RTR, 8, 4, 2, 4, HALVES>;
+template <class T, bool LTR, bool RTR, bool HALVES>
+using Small = Product<T, LTR, RTR, 4, 4, 2, 2, HALVES>;
+
+// Large tiles where there are enough of them for all CUs.
+template <class P>
+int64_t tiles(int64_t nl, int64_t nr) {
+  return cdiv(nl, P::BLL) * cdiv(nr, P::BR);
+}
+constexpr int64_t kCus = 256;
+
+#define GATED_LAUNCH(kernel, blocks, threads, ...)                                                   \
+  do {                                                                                               \
+    const int64_t blocks_ = (blocks);                                                                \
+    ASTRA_ABI_CHECK(blocks_, <, 2147483648ll);                                                       \
+    hipLaunchKernelGGL((kernel), dim3((unsigned)blocks_), dim3(threads), 0, st, __VA_ARGS__);        \
+    ASTRA_HIP_CHECK(rt_last_error(), #kernel " launch");                                             \
+  } while (false)
+
+template <class T, bool GRAD>
+int launch_gated(const GatedArgs &g, hipStream_t st) {
+  typedef Large<T, false, false, true> L;
+  typedef Small<T, false, false, true> S;
+  const int64_t F = GRAD ? g.Fp : g.F;
+  if (tiles<L>(F, g.M) >= kCus)
+    GATED_LAUNCH((gated_kernel<L, GRAD>), tiles<L>(F, g.M), L::kThreads, g);
+  else
+    GATED_LAUNCH((gated_kernel<S, GRAD>), tiles<S>(F, g.M), S::kThreads, g);
+  return ASTRA_OK;
+}
+
+template <class T, bool ALIGNED>
+int launch_few(const GatedArgs &g, hipStream_t st) {
+  if (g.M <= 16)
+    GATED_LAUNCH((gated_few_kernel<T, 1, ALIGNED>), cdiv(g.F, 16), 256, g);
+  else if (g.M <= 32)
+    GATED_LAUNCH((gated_few_kernel<T, 2, ALIGNED>), cdiv(g.F, 16), 256, g);
+  else
+    GATED_LAUNCH((gated_few_kernel<T, 4, ALIGNED>), cdiv(g.F, 16), 256, g);
+  return ASTRA_OK;
+}
+
+template <class T>
+int forward(const astra_gated_linear &f, hipStream_t st) {
+  GatedArgs g = args_of(f);
+  g.wide = f.hidden % per16(f.type) == 0 && aligned(f.h, 16) && aligned(f.projections, 16);
+  if (few(f)) {
+    g.x = {f.x, f.x_stride, f.rows, f.width};
+    g.gate = {f.gate, f.gate_stride, f.hidden, f.width};
+    g.up = {f.up, f.up_stride, f.hidden, f.width};
+    const bool all = direct(f, f.x, f.x_stride) && direct(f, f.gate, f.gate_stride) && direct(f, f.up, f.up_stride);
+    return all ? launch_few<T, true>(g, st) : launch_few<T, false>(g, st);
+  }
+  const size_t need = copies_bytes(f);
+  if (need) ASTRA_SEQ_POINTER(f.workspace);
+  ASTRA_ABI_CHECK(f.workspace_bytes, >=, need);
+  char *ws = (char *)f.workspace;
+  const Operands o = operands<T>(f, &ws, st);
+  ASTRA_HIP_CHECK(rt_last_error(), "align_kernel launch");
+  g.x = o.x;
+  g.gate = o.gate;
+  g.up = o.up;
+  return launch_gated<T, false>(g, st);
+}
+
+// dx = da Wg + db Wu, [M, D]
+template <class P>
+int launch_dx(ProductArgs &g, hipStream_t st) {
+  GATED_LAUNCH(product_kernel<P>, tiles<P>(g.nl, g.nr), P::kThreads, g);
+  return ASTRA_OK;
+}
+
+// The slices of the rows that the weights' gradients are summed over: enough workgroups for all
+// CUs, and 8 steps at least to a slice.
+template <class T>
+int64_t slices_of(const astra_gated_linear &f) {
+  typedef Large<T, true, true, false> P;
+  const int64_t n = tiles<P>(f.width, 2 * padded_hidden(f)), steps = cdiv(f.rows, kStepOf<T>);
+  const int64_t want = cdiv(kCus, n), most = steps / 8;
+  return want < most ? want : most > 1 ? most : 1;
+}
+template <class T>
+size_t part_bytes(const astra_gated_linear &f) {
+  const int64_t s = slices_of<T>(f);
+  return s > 1 ? (size_t)(s * 2 * padded_hidden(f) * f.width) * sizeof(float) : 0;
+}
+
+template <class T>
+size_t grad_bytes(const astra_gated_linear &f) {
+  return (size_t)(f.rows * 2 * padded_hidden(f)) * sizeof(T) + copies_bytes(f) + part_bytes<T>(f);
+}
+
+template <class T>
+int backward(const astra_gated_linear_grad &b, hipStream_t st) {
+  const astra_gated_linear &f = b.f;
+  GatedArgs g = args_of(f);
+  const size_t need = grad_bytes<T>(f);
+  if (need) ASTRA_SEQ_POINTER(b.workspace);
+  ASTRA_ABI_CHECK(b.workspace_bytes, >=, need);
+  if (need && !aligned(b.workspace, 16)) return fail(ASTRA_ERR_INVALID_ARGUMENT, "astra_gated_linear_backward: the workspace starts on 16 bytes");
+  char *ws = (char *)b.workspace;
+  const int64_t Fp = g.Fp, v = per16(f.type);
+  g.dab = ws;
+  g.dh = b.dh;
+  ws += (size_t)(f.rows * 2 * Fp) * sizeof(T);
+  const Operands o = operands<T>(f, &ws, st);
+  ASTRA_HIP_CHECK(rt_last_error(), "align_kernel launch");
+  g.x = o.x;
+  g.gate = o.gate;
+  g.up = o.up;
+  g.wide = f.hidden % per16(f.type) == 0 && aligned(b.dh, 16) && aligned(f.projections, 16);
+  if (f.rows) {
+    if (f.projections) {
+      GATED_LAUNCH(gated_slopes_kernel<T>, cdiv(f.rows * (Fp / 4), 256), 256, g);
+    } else if (int rc = launch_gated<T, true>(g, st)) {
+      return rc;
+    }
+  }
+  if (b.dx && f.rows) {
+    ProductArgs p{};
+    p.pairs = 2;
+    for (int i = 0; i < 2; ++i) {
+      const Operand &w = i ? o.up : o.gate;
+      p.left[i] = {w.p, w.ld, round_up(f.width, v), f.hidden};       // lines: columns of the weight
+      p.right[i] = {(const T *)g.dab + i * Fp, 2 * Fp, f.rows, Fp};
+    }
+    p.out[0] = b.dx;
+    p.out_ld = p.nl = f.width;
+    p.nr = p.split = p.rows = f.rows;
+    p.slices = 1;
+    p.wide = f.width % 4 == 0 && aligned(b.dx, 4 * sizeof(T));
+    typedef Large<T, true, false, false> L;
+    typedef Small<T, true, false, false> S;
+    if (int rc = tiles<L>(p.nl, p.nr) >= kCus ? launch_dx<L>(p, st) : launch_dx<S>(p, st)) return rc;
+  }
+  if (b.dgate || b.dup) {
+    typedef Large<T, true, true, false> P;
+    ProductArgs p{};
+    p.pairs = 1;
+    p.left[0] = {o.x.p, o.x.ld, round_up(f.width, v), f.rows};
+    // (one weight's gradient alone is the product with its half of the columns)
+    p.nr = b.dgate && b.dup ? 2 * Fp : Fp;
+    p.right[0] = {(const T *)g.dab + (b.dgate ? 0 : Fp), 2 * Fp, p.nr, f.rows};
+    p.out[0] = b.dgate ? b.dgate : b.dup;
+    p.out[1] = b.dup;
+    p.out_ld = p.nl = f.width;
+    p.split = Fp;
+    p.rows = f.hidden;
+    p.slices = (int32_t)slices_of<T>(f);
+    p.part = p.slices > 1 ? (float *)ws : nullptr;
+    p.steps = cdiv(cdiv(f.rows, kStepOf<T>), p.slices);
+    p.wide = f.width % 4 == 0 && aligned(b.dgate, 4 * sizeof(T)) && aligned(b.dup, 4 * sizeof(T));
+    GATED_LAUNCH(product_kernel<P>, tiles<P>(p.nl, p.nr) * p.slices, P::kThreads, p);
+    if (p.part) GATED_LAUNCH(join_slices_kernel<T>, cdiv(cdiv(p.nr * p.nl, 4), 256), 256, p);
+  }
+  return ASTRA_OK;
+}
+
+}  // namespace
+}  // namespace astra_seq
+
+using namespace astra_seq;
+
+extern "C" {
+
+int astra_gated_linear_workspace_size(const astra_gated_linear *f, size_t *bytes) {
+  if (int rc = check(f)) return rc;
+  ASTRA_SEQ_POINTER(bytes);
+  *bytes = few(*f) ? 0 : copies_bytes(*f);
+  return ASTRA_OK;
+}
+
+int astra_gated_linear_projections(const astra_gated_linear *f, size_t *floats) {
+  if (int rc = check(f)) return rc;
+  ASTRA_SEQ_POINTER(floats);
+  *floats = 0;
+  return ASTRA_OK;
+}
+
+int astra_gated_linear_forward(const astra_gated_linear *f, void *stream) {
+  if (int rc = check(f)) return rc;
+  if (f->rows == 0) return ASTRA_OK;
+  ASTRA_SEQ_POINTER(f->x);
+  ASTRA_SEQ_POINTER(f->gate);
+  ASTRA_SEQ_POINTER(f->up);
+  ASTRA_SEQ_POINTER(f->h);
+  return f->type == ASTRA_SEQ_F32 ? forward<float>(*f, as_stream(stream)) : forward<bf16>(*f, as_stream(stream));
+}
+
+int astra_gated_linear_grad_workspace_size(const astra_gated_linear *f, size_t *bytes) {
+  if (int rc = check(f)) return rc;
+  ASTRA_SEQ_POINTER(bytes);
+  *bytes = f->type == ASTRA_SEQ_F32 ? grad_bytes<float>(*f) : grad_bytes<bf16>(*f);
+  return ASTRA_OK;
+}
+
+int astra_gated_linear_backward(const astra_gated_linear_grad *g, void *stream) {
+  ASTRA_SEQ_POINTER(g);
+  if (int rc = check(&g->f)) return rc;
+  if (g->f.rows) {
+    ASTRA_SEQ_POINTER(g->f.x);
+    ASTRA_SEQ_POINTER(g->dh);
+  }
+  ASTRA_SEQ_POINTER(g->f.gate);
+  ASTRA_SEQ_POINTER(g->f.up);
+  return g->f.type == ASTRA_SEQ_F32 ? backward<float>(*g, as_stream(stream)) : backward<bf16>(*g, as_stream(stream));
+}
+
+}  // extern "C"

@@ -7,6 +7,9 @@
  *   state_scan   dt = softplus(dt_raw + dt_bias);  h_t = exp(dt_t A) h_{t-1} + dt_t x_t (x) B_t
  *                y_t = h_t C_t + D x_t               (per head; x_t [P], B_t and C_t [N], h [P,N])
  *   join_norm    r' = r + scale * gate * rms(block) * post;  n = rms(r') * next
+ *   gated_linear h = act(x Wg^T) * (x Wu^T)
+ *   log_probs    per row and part of a move, over the allowed entries: log probability of the
+ *                choice, entropy, the likeliest entries
  *
  * All pointers are device pointers; work is queued on `stream` and nothing synchronises or
  * allocates. "Type" arguments are ASTRA_SEQ_F32 or ASTRA_SEQ_BF16. Strides count elements;
@@ -32,10 +35,14 @@ extern "C" {
 
 #define ASTRA_SEQ_LINEAR 0 /* short_conv's activation: none */
 #define ASTRA_SEQ_SILU 1
+#define ASTRA_SEQ_GELU 2 /* gated_linear: v times the normal distribution function at v */
 
 #define ASTRA_SEQ_MAX_TAPS 4
 #define ASTRA_SEQ_MAX_STATE 128
 #define ASTRA_SEQ_MAX_NORM_WIDTH 16384
+#define ASTRA_SEQ_MAX_LINEAR_WIDTH 1048576
+#define ASTRA_SEQ_MAX_PARTS 16
+#define ASTRA_SEQ_MAX_TOP 64
 
 /* ---- short_conv ------------------------------------------------------------------- */
 
@@ -168,6 +175,39 @@ typedef struct astra_join_norm_grad {
 } astra_join_norm_grad;
 int astra_join_norm_workspace_size(const astra_join_norm *f, size_t *bytes);
 int astra_join_norm_backward(const astra_join_norm_grad *a, void *stream);
+
+/* ---- gated_linear ----------------------------------------------------------------- */
+
+/* Forward. x [M,D], gate and up [F,D] of `type` with row strides; h [M,F] contiguous.
+ * activation: ASTRA_SEQ_SILU or ASTRA_SEQ_GELU. projections (may be NULL) keeps x gate^T and
+ * x up^T for the backward call, astra_gated_linear_projections() floats: zero where the
+ * backward call is faster without. The workspace holds aligned copies of operands whose rows
+ * do not start on 16 bytes. */
+typedef struct astra_gated_linear {
+  const void *x, *gate, *up;
+  void *h;
+  float *projections;
+  int64_t rows, x_stride, gate_stride, up_stride;
+  int32_t width, hidden, type, activation;
+  void *workspace;
+  size_t workspace_bytes;
+} astra_gated_linear;
+int astra_gated_linear_projections(const astra_gated_linear *f, size_t *floats);
+int astra_gated_linear_workspace_size(const astra_gated_linear *f, size_t *bytes);
+int astra_gated_linear_forward(const astra_gated_linear *f, void *stream);
+
+/* Backward: `f` as in the forward call, with the projections that it wrote or without (h and
+ * f's workspace are not used). dh [M,F] contiguous; dx [M,D], dgate and dup [F,D], contiguous,
+ * of `type`: each may be NULL if not wanted. The workspace starts on 16 bytes. */
+typedef struct astra_gated_linear_grad {
+  astra_gated_linear f;
+  const void *dh;
+  void *dx, *dgate, *dup;
+  void *workspace;
+  size_t workspace_bytes;
+} astra_gated_linear_grad;
+int astra_gated_linear_grad_workspace_size(const astra_gated_linear *f, size_t *bytes);
+int astra_gated_linear_backward(const astra_gated_linear_grad *a, void *stream);
 
 #ifdef __cplusplus
 }
