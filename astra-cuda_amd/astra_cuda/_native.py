@@ -68,6 +68,8 @@ SEQUENCE_PROTOTYPES = {
     "astra_gated_linear_forward": (_c_int, [_vp, _vp]),
     "astra_gated_linear_grad_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
     "astra_gated_linear_backward": (_c_int, [_vp, _vp]),
+    "astra_log_probs_forward": (_c_int, [_vp, _vp]),
+    "astra_log_probs_backward": (_c_int, [_vp, _vp]),
 }
 
 
@@ -161,6 +163,17 @@ class GatedLinear(ctypes.Structure):
 class GatedLinearGrad(ctypes.Structure):
     """astra_gated_linear_grad (include/sequence/astra_sequence.h)."""
     _fields_ = [("f", GatedLinear)] + _fields("dh dx dgate dup workspace", "", "") + [("workspace_bytes", _sz)]
+
+
+class LogProbs(ctypes.Structure):
+    """astra_log_probs (include/sequence/astra_sequence.h)."""
+    _fields_ = _fields("logits mask choice log_prob entropy stats top_log_prob top_index", "rows stride mask_stride",
+                       "parts top choice_bytes type") + [("sizes", _c_i32 * 16)]
+
+
+class LogProbsGrad(ctypes.Structure):
+    """astra_log_probs_grad (include/sequence/astra_sequence.h)."""
+    _fields_ = [("f", LogProbs)] + _fields("dlog_prob dentropy dlogits", "", "")
 
 
 _lib = None

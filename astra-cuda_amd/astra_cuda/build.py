@@ -24,7 +24,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB_NAME = "libastra_market.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = [os.path.join(CSRC, f) for f in ("market.hip", "high_low.hip", "sequence_conv.hip", "sequence_gated.hip",
-                                           "sequence_join.hip", "sequence_scan.hip")]
+                                           "sequence_join.hip", "sequence_probs.hip", "sequence_scan.hip")]
 
 ARCH = os.environ.get("ASTRA_OFFLOAD_ARCH", "gfx950")
 

@@ -9,9 +9,12 @@ time in rollouts with a state of fixed size per env (include/sequence/astra_sequ
                      read-out and step size given per position
 ``join_norm``        what stands between two blocks: the norm after one, its gate and
                      residual scale, the residual sum, the norm before the next
+``gated_linear``     the gated feed-forward block before its way back: both projections, the
+                     activation and the product
+``log_probs``        log probability of a move, entropy and likeliest alternatives from logits
 ``short_conv_step``, ``state_scan_step``   one position, the state moved on in place
 
-The first three are differentiable in every tensor they take, backwards and once: tensors with
+All but the steps are differentiable in every floating point tensor they take, backwards and once: tensors with
 a forward-mode tangent are refused, and so is being part of a torch.jit trace. A step raises its
 state's version: a backward pass that had saved the state refuses to run, as after torch's own
 operations in place.
@@ -44,6 +47,9 @@ MAX_TAPS = 4        # ASTRA_SEQ_MAX_TAPS
 MAX_STATE = 128     # ASTRA_SEQ_MAX_STATE
 MAX_NORM_WIDTH = 16384  # ASTRA_SEQ_MAX_NORM_WIDTH
 MAX_LINEAR_WIDTH = 1048576  # ASTRA_SEQ_MAX_LINEAR_WIDTH
+MAX_PARTS = 16      # ASTRA_SEQ_MAX_PARTS
+MAX_TOP = 64        # ASTRA_SEQ_MAX_TOP
+MAX_ENTRIES = 1 << 30  # ASTRA_SEQ_MAX_ENTRIES
 
 _ops = None
 
@@ -126,3 +132,23 @@ def gated_linear(x, gate_weight, up_weight, *, activation="silu"):
     gradients of the two projections are rounded to x's type before their own products.
     """
     return (_ops or _compiled()).gated_linear(x, gate_weight, up_weight, activation)
+
+
+def log_probs(logits, choice=None, *, sizes=None, mask=None, top=0):
+    """What a head's ``logits`` ``[..., W]`` say: returns ``(log_prob, entropy)``, and with ``top`` k
+    ``(log_prob, entropy, top_log_prob, top_index)``.
+
+    ``sizes`` cuts a row into the parts of a move, each a distribution of its own (default: one
+    part of W entries); outputs are ``[..., parts]``, without ``sizes`` ``[...]``. ``choice`` of that
+    shape (int32 or int64) is the entry of each part whose log probability is wanted (None: no
+    log_prob). ``mask`` (bool, broadcast along the leading dimensions) says which entries are
+    allowed; logits of -inf are not, either. ``top_log_prob`` and ``top_index`` ``[..., k]`` are the
+    likeliest allowed entries, ties to the lower index, -inf and -1 where there are fewer.
+
+    A choice of -1 says that a part does not count (a game that is over): its logits are not read,
+    its log_prob, entropy and gradient are 0. The log probability of an entry that is left out is
+    -inf and has no gradient, that of a choice outside of its part is NaN. Where nothing is allowed
+    the entropy is 0. An allowed NaN or infinity makes its part's log probabilities, entropy and
+    gradient NaN. log_prob and entropy are float32 and differentiable in logits; the top ones are not.
+    """
+    return (_ops or _compiled()).log_probs(logits, choice, sizes, mask, top)

@@ -695,6 +695,132 @@ Tensor gated_linear(const Tensor &x_, const Tensor &gate_, const Tensor &up_, co
   return h.view(shape);
 }
 
+// ------------------------------------------------------------------------- log_probs
+
+// logits [R, W] and mask [R, W] with contiguous rows, choice [R, parts] contiguous.
+astra_log_probs probs_struct(const Tensor &logits, const Tensor &choice, const Tensor &mask, c10::IntArrayRef sizes,
+                             const Tensor &stats) {
+  astra_log_probs f{};
+  f.logits = ptr(logits);
+  f.mask = mask.defined() ? static_cast<const uint8_t *>(mask.data_ptr()) : nullptr;
+  f.choice = ptr(choice);
+  f.stats = ptr<float>(stats);
+  f.rows = logits.size(0);
+  f.stride = logits.stride(0);
+  f.mask_stride = mask.defined() ? mask.stride(0) : 0;
+  f.parts = (int32_t)sizes.size();
+  f.choice_bytes = choice.defined() && choice.scalar_type() == torch::kInt32 ? 4 : 8;
+  f.type = type_of(logits);
+  for (size_t i = 0; i < sizes.size(); ++i) f.sizes[i] = (int32_t)sizes[i];
+  return f;
+}
+
+// the log probability where there is a choice, the entropy, the top ones and their indices
+variable_list probs_forward(const Tensor &logits, const Tensor &choice, const Tensor &mask, c10::IntArrayRef sizes,
+                            int64_t top, Tensor *stats) {
+  const c10::DeviceGuard guard(logits.device());
+  const int64_t R = logits.size(0), P = (int64_t)sizes.size();
+  if (stats) *stats = empty(logits, {R, P, 3}, torch::kFloat32);
+  astra_log_probs f = probs_struct(logits, choice, mask, sizes, stats ? *stats : Tensor());
+  variable_list out;
+  if (choice.defined()) {
+    out.push_back(empty(logits, {R, P}, torch::kFloat32));
+    f.log_prob = ptr<float>(out.back());
+  }
+  out.push_back(empty(logits, {R, P}, torch::kFloat32));
+  f.entropy = ptr<float>(out.back());
+  f.top = (int32_t)top;
+  if (top) {
+    out.push_back(empty(logits, {R, P, top}, torch::kFloat32));
+    f.top_log_prob = ptr<float>(out.back());
+    out.push_back(empty(logits, {R, P, top}, torch::kInt64));
+    f.top_index = ptr<int64_t>(out.back());
+  }
+  check(astra_log_probs_forward(&f, stream_of(logits.get_device())));
+  return out;
+}
+
+struct LogProbs : torch::autograd::Function<LogProbs> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Optional &choice, const Optional &mask,
+                               std::vector<int64_t> sizes, int64_t top) {
+    Tensor stats;
+    variable_list out = probs_forward(logits, value(choice), value(mask), sizes, top, &stats);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, value(choice), value(mask), stats});
+    ctx->saved_data["sizes"] = sizes;
+    if (top) ctx->mark_non_differentiable({out[out.size() - 2], out.back()});
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    check_once();
+    const auto s = ctx->get_saved_variables();
+    const Tensor &logits = s[0], &choice = s[1];
+    variable_list out(5);
+    size_t at = 0;
+    const Tensor dlog_prob = choice.defined() ? undefined_or_contiguous(grads[at++]) : Tensor();
+    const Tensor dentropy = undefined_or_contiguous(grads[at]);
+    if (!dlog_prob.defined() && !dentropy.defined()) return out;
+    const c10::DeviceGuard guard(logits.device());
+    out[0] = empty(logits, logits.sizes(), logits.scalar_type());
+    astra_log_probs_grad g{};
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    g.f = probs_struct(logits, choice, s[2], sizes, s[3]);
+    g.dlog_prob = ptr<float>(dlog_prob);
+    g.dentropy = ptr<float>(dentropy);
+    g.dlogits = ptr(out[0]);
+    check(astra_log_probs_backward(&g, stream_of(logits.get_device())));
+    return out;
+  }
+};
+
+py::object log_probs(const Tensor &logits_, const Optional &choice_, const std::optional<std::vector<int64_t>> &sizes_,
+                     const Optional &mask_, int64_t top) {
+  calls_only("log_probs", logits_);
+  check_data("logits", logits_);
+  need(logits_.dim() >= 1 && logits_.size(-1) >= 1, "logits", "must have shape [..., entries], got " + shape_text(logits_.sizes()));
+  const int64_t W = logits_.size(-1);
+  need(W <= ASTRA_SEQ_MAX_ENTRIES, "logits", "must have at most " + std::to_string(ASTRA_SEQ_MAX_ENTRIES) + " entries, got " + std::to_string(W));
+  const std::vector<int64_t> sizes = sizes_ ? *sizes_ : std::vector<int64_t>{W};
+  need(!sizes.empty() && sizes.size() <= ASTRA_SEQ_MAX_PARTS, "sizes",
+       "must be 1 to " + std::to_string(ASTRA_SEQ_MAX_PARTS) + " parts, got " + std::to_string(sizes.size()));
+  int64_t all = 0;
+  for (int64_t n : sizes) {
+    need(n >= 1 && n <= W, "sizes", "must be at least 1 each and add up to " + std::to_string(W) + ", got " + shape_text(sizes));
+    need(top >= 0 && top <= ASTRA_SEQ_MAX_TOP && top <= n, "top",
+         "must be 0 to " + std::to_string(ASTRA_SEQ_MAX_TOP) + " and at most every part's size, got " + std::to_string(top));
+    all += n;
+  }
+  need(all == W, "sizes", "must add up to " + std::to_string(W) + ", got " + shape_text(sizes));
+  // the outputs' shape: logits' leading dimensions, and the parts where sizes are given
+  std::vector<int64_t> shape(logits_.sizes().begin(), logits_.sizes().end() - 1);
+  if (sizes_) shape.push_back((int64_t)sizes.size());
+  Tensor choice, mask;
+  if (choice_) {
+    need(choice_->device() == logits_.device(), "choice", "must be on " + logits_.device().str() + ", got " + choice_->device().str());
+    need(choice_->scalar_type() == torch::kInt32 || choice_->scalar_type() == torch::kInt64, "choice",
+         std::string("must be int32 or int64, got ") + c10::toString(choice_->scalar_type()));
+    need(choice_->sizes() == c10::IntArrayRef(shape), "choice", "must have shape " + shape_text(shape) + ", got " + shape_text(choice_->sizes()));
+    choice = choice_->contiguous();
+  }
+  if (mask_) {
+    need(mask_->device() == logits_.device(), "mask", "must be on " + logits_.device().str() + ", got " + mask_->device().str());
+    need(mask_->scalar_type() == torch::kBool, "mask", std::string("must be bool, got ") + c10::toString(mask_->scalar_type()));
+    bool fits = mask_->dim() >= 1 && mask_->dim() <= logits_.dim() && mask_->size(-1) == W;
+    for (int64_t i = 2; fits && i <= mask_->dim(); ++i) fits = mask_->size(-i) == 1 || mask_->size(-i) == logits_.size(-i);
+    need(fits, "mask", "must have logits' shape " + shape_text(logits_.sizes()) + " or broadcast to it along leading dimensions, got " + shape_text(mask_->sizes()));
+    mask = flat(mask_->expand(logits_.sizes()));
+  }
+  const Tensor logits = flat(logits_);
+  const variable_list out = with_grad({&logits}) ? LogProbs::apply(logits, maybe(choice), maybe(mask), sizes, top)
+                                                 : probs_forward(logits, choice, mask, sizes, top, nullptr);
+  size_t at = 0;
+  const py::object log_prob = choice.defined() ? py::cast(out[at++].view(shape)) : py::none();
+  const Tensor entropy = out[at++].view(shape);
+  if (!top) return py::make_tuple(log_prob, entropy);
+  shape.push_back(top);
+  return py::make_tuple(log_prob, entropy, out[at].view(shape), out[at + 1].view(shape));
+}
+
 }  // namespace
 
 void bind_sequence(py::module_ &m) {
@@ -711,6 +837,7 @@ void bind_sequence(py::module_ &m) {
         py::arg("gate"), py::arg("scale"), py::arg("eps"));
   s.def("rms_norm", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("eps"));
   s.def("gated_linear", &gated_linear, py::arg("x"), py::arg("gate_weight"), py::arg("up_weight"), py::arg("activation"));
+  s.def("log_probs", &log_probs, py::arg("logits"), py::arg("choice"), py::arg("sizes"), py::arg("mask"), py::arg("top"));
   s.attr("MAX_TAPS") = ASTRA_SEQ_MAX_TAPS;
   s.attr("MAX_STATE") = ASTRA_SEQ_MAX_STATE;
   s.attr("MAX_NORM_WIDTH") = ASTRA_SEQ_MAX_NORM_WIDTH;

@@ -43,6 +43,7 @@ extern "C" {
 #define ASTRA_SEQ_MAX_LINEAR_WIDTH 1048576
 #define ASTRA_SEQ_MAX_PARTS 16
 #define ASTRA_SEQ_MAX_TOP 64
+#define ASTRA_SEQ_MAX_ENTRIES 1073741824
 
 /* ---- short_conv ------------------------------------------------------------------- */
 
@@ -208,6 +209,42 @@ typedef struct astra_gated_linear_grad {
 } astra_gated_linear_grad;
 int astra_gated_linear_grad_workspace_size(const astra_gated_linear *f, size_t *bytes);
 int astra_gated_linear_backward(const astra_gated_linear_grad *a, void *stream);
+
+/* ---- log_probs -------------------------------------------------------------------- */
+
+/* Forward. logits [R,W] of `type` with a row stride: the entries of `parts` parts of a move,
+ * sizes[i] each, one behind the other (W is their sum). mask [R,W] (may be NULL) with a row
+ * stride (0: one row for all): entries whose byte is 0 are left out, and so are entries of -inf.
+ * choice [R,parts], contiguous, of choice_bytes 4 or 8 (may be NULL): the entry of each part, -1
+ * where the part does not count. entropy and log_prob (NULL without a choice) float [R,parts];
+ * top_log_prob float and top_index int64 [R,parts,top] (top up to every part's size): the
+ * likeliest entries, ties to the lower index, -inf and -1 where there are fewer. stats float
+ * [R,parts,3] (may be NULL) is kept for the backward call.
+ * A part that does not count is not read: its log_prob and entropy are 0, and there are no
+ * likeliest entries. The log probability of an entry that is left out is -inf, that of a choice
+ * in no entry NaN; where nothing is allowed the entropy is 0. */
+typedef struct astra_log_probs {
+  const void *logits;
+  const uint8_t *mask;
+  const void *choice;
+  float *log_prob, *entropy, *stats, *top_log_prob;
+  int64_t *top_index;
+  int64_t rows, stride, mask_stride;
+  int32_t parts, top, choice_bytes, type;
+  int32_t sizes[ASTRA_SEQ_MAX_PARTS];
+} astra_log_probs;
+int astra_log_probs_forward(const astra_log_probs *f, void *stream);
+
+/* Backward: `f` as in the forward call with the stats that it wrote (its outputs are not
+ * used). dlog_prob and dentropy float [R,parts] (each may be NULL: zeros); dlogits [R,W] of
+ * `type`, contiguous, zero for entries that are left out and parts that do not count. The log
+ * probability of an entry that is left out has no gradient. */
+typedef struct astra_log_probs_grad {
+  astra_log_probs f;
+  const float *dlog_prob, *dentropy;
+  void *dlogits;
+} astra_log_probs_grad;
+int astra_log_probs_backward(const astra_log_probs_grad *a, void *stream);
 
 #ifdef __cplusplus
 }
