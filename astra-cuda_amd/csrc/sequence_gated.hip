@@ -55,6 +55,9 @@ __device__ __forceinline__ void multiply(f32x4 &acc, const f32x4 &l, const f32x4
   for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(l[i], r[i], acc, 0, 0, 0);
 }
 
+template <class T>
+constexpr int kProducts = sizeof(T) == 2 ? 1 : 4;  // instructions
+
 // An operand: `lines` lines of `len` elements of the contraction, rows `ld` elements apart.
 struct Operand {
   const void *p;
@@ -67,6 +70,7 @@ struct Loader {
   static constexpr int N = B * kStep / 1024 / NW;               // loads of 1024 bytes
   static constexpr int kRow = TR ? B * (int)sizeof(T) : kStep;  // bytes of a row in LDS
   static constexpr int kPieces = kRow / 16, kRows = 64 / kPieces;  // (rows of one load)
+  static constexpr int kReads = !TR ? 1 : sizeof(T) == 2 ? 2 : 4;  // LDS accesses of a fragment
   static_assert(!TR || kRow >= 256, "rows of a tile across the contraction cover all banks");
   static_assert(TR || NW % 2 == 0, "along the contraction a lane has the same piece of all its rows");
   const char *base;
@@ -158,81 +162,131 @@ struct Reader {
   }
 };
 
-// HALVES: the left tile is two operands of BL / 2 lines each, of which a wavefront has the same
-// lines, PAIRED as above.
-template <class T, bool LTR, bool RTR, int NL_, int NR_, int WL_, int WR_, bool HALVES_>
+// A workgroup's tile: WL x WR wavefronts of NL x NR times 16 x 16 results. HALVES: the left tile is
+// two operands of BL / 2 lines each, of which a wavefront has the same lines, PAIRED as above. GROUPS
+// workgroups share a CU.
+template <class T, bool LTR, bool RTR, int NL_, int NR_, bool HALVES_, int GROUPS_, int WL_ = 2, int WR_ = 2>
 struct Product {
-  static constexpr int NL = NL_, NR = NR_, WL = WL_, WR = WR_;
+  static constexpr int NL = NL_, NR = NR_, WL = WL_, WR = WR_, GROUPS = GROUPS_;
   static constexpr bool HALVES = HALVES_;
   static constexpr int NW = WL * WR, BL = 16 * NL * WL, BR = 16 * NR * WR;
   static constexpr int kBytes = (BL + BR) * kStep, kThreads = 64 * NW;
   static constexpr int BLL = HALVES ? BL / 2 : BL;  // lines of a left operand
   static constexpr int NLL = HALVES ? NL / 2 : NL;  // tiles of it to a wavefront
+  static_assert(kBytes * (GROUPS == 1 ? 2 : GROUPS) <= 160 * 1024, "the LDS of a CU");
   typedef T type;
   typedef Loader<T, LTR, BLL, NW, HALVES> Left;
   typedef Loader<T, RTR, BR, NW, false> Right;
-
   typedef Reader<T, LTR, BLL, HALVES> LeftReader;
   typedef Reader<T, RTR, BR, false> RightReader;
 
-  // One step's products while the next is on its way: two tiles that do not overlap.
+  // The fragments of half a step.
+  struct Half {
+    Frag<T> l[NL], r[NR];
+  };
+  static __device__ __forceinline__ void read(Half &h, const char *lds, int s, const LeftReader &left, const RightReader &right) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) h.r[r] = right.read(lds + BL * kStep, r, s);
+#pragma unroll
+    for (int l = 0; l < NL; ++l) h.l[l] = left.read(lds + (l / NLL) * BLL * kStep, l % NLL, s);
+  }
+  static __device__ __forceinline__ void products(f32x4 (&acc)[NL][NR], const Half &h) {
+#pragma unroll
+    for (int l = 0; l < NL; ++l)
+#pragma unroll
+      for (int r = 0; r < NR; ++r) multiply(acc[l][r], h.l[l], h.r[r]);
+  }
+
+  // What this wavefront has asked for of LDS, or sent to it, has come, and all others are as far. (The
+  // compiler's own barrier may not wait for loads to LDS.)
+  static __device__ __forceinline__ void everybody_has_read() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  static __device__ __forceinline__ void everything_has_come() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // One step of a workgroup that has its CU to itself: the step after comes into a tile of its own
+  // meanwhile (they do not overlap). Its loads go out between products: one after the other, they
+  // would keep every wavefront from multiplying until the last is taken.
   template <class Load>
   static __device__ __forceinline__ void step(f32x4 (&acc)[NL][NR], char *__restrict next, const char *__restrict now,
                                               const Load &load, LeftReader &left, RightReader &right) {
-    load(next);
-    __builtin_amdgcn_sched_barrier(0);  // (on its way before the products, not after them)
+    constexpr int kReads = NL * Left::kReads + NR * Right::kReads, kLoads = (HALVES ? 2 : 1) * Left::N + Right::N;
+    constexpr int kHalf = NL * NR * kProducts<T>;
     if (LTR) left.again();
     if (RTR) right.again();
+    Half h;
+    read(h, now, 0, left, right);
+    load(next);
+    products(acc, h);
+    read(h, now, 1, left, right);
+    products(acc, h);
+    __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      Frag<T> a[NL], b[NR];
-#pragma unroll
-      for (int l = 0; l < NL; ++l) a[l] = left.read(now + (l / NLL) * BLL * kStep, l % NLL, s);
-#pragma unroll
-      for (int r = 0; r < NR; ++r) b[r] = right.read(now + BL * kStep, r, s);
-#pragma unroll
-      for (int l = 0; l < NL; ++l)
-#pragma unroll
-        for (int r = 0; r < NR; ++r) multiply(acc[l][r], a[l], b[r]);
+    for (int i = 0; i < kLoads; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, kHalf / kLoads, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, kHalf, 0);
+    everything_has_come();
   }
 
-  // (A barrier does not wait for what is on its way to LDS.)
-  static __device__ __forceinline__ void arrived() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  }
-
-  // acc[l][r] += the products of `steps` steps, each brought into a tile by load(lds).
+  // acc[l][r] += the products of `steps` steps, each brought into a tile by load(lds). Where several
+  // workgroups share a CU the others multiply while one waits, and one tile is enough: the step
+  // after is sent for as soon as everybody has read it.
   template <class Load>
-  static __device__ __forceinline__ void run(f32x4 (&acc)[NL][NR], int64_t steps, const Load &load, int wave, int lane) {
-    __shared__ __attribute__((aligned(1024))) char first[kBytes], second[kBytes];
+  static __device__ __forceinline__ void run(f32x4 (&acc)[NL][NR], int steps, const Load &load, int wave, int lane) {
     LeftReader left;
     RightReader right;
     left.init(wave % WL * NLL, lane);
     right.init(wave / WL * NR, lane);
-    load(first);
-    for (int64_t k = 0; k < steps; k += 2) {
-      arrived();
-      step(acc, second, first, load, left, right);
-      arrived();
-      step(acc, first, second, load, left, right);
+    if constexpr (GROUPS == 1) {
+      __shared__ __attribute__((aligned(1024))) char one[kBytes], two[kBytes];
+      load(one);
+      everything_has_come();
+      for (int k = 0; k < steps; k += 2) {
+        step(acc, two, one, load, left, right);
+        if (k + 1 >= steps) break;
+        step(acc, one, two, load, left, right);
+      }
+    } else {
+      __shared__ __attribute__((aligned(1024))) char lds[kBytes];
+      load(lds);
+      for (int k = 0; k < steps; ++k) {
+        everything_has_come();
+        if (LTR) left.again();
+        if (RTR) right.again();
+        Half h;
+        read(h, lds, 0, left, right);
+        products(acc, h);
+        read(h, lds, 1, left, right);
+        everybody_has_read();
+        load(lds);
+        __builtin_amdgcn_sched_barrier(0);
+        products(acc, h);
+      }
+      everything_has_come();  // (the tile may be used again)
     }
-    arrived();  // (nothing is on its way, and nobody reads, when the tiles are used again)
   }
 };
 
 // Tile `n` of nl x nr, spread so that an XCD (workgroups are given to the eight in turn) works on
 // neighbouring tiles, kBand right tiles by all left ones: what they share stays in its L2.
 constexpr int kXcds = 8, kBand = 8;
-__device__ __forceinline__ void tile_of(int64_t n, int64_t nl, int64_t nr, int64_t *l, int64_t *r) {
-  const int64_t total = nl * nr, each = total / kXcds, rest = total % kXcds;
-  const int64_t xcd = n % kXcds, at = n / kXcds;
-  n = xcd * each + min(xcd, rest) + at;
-  const int64_t band = n / (kBand * nl), in = n % (kBand * nl);
-  const int64_t high = min((int64_t)kBand, nr - band * kBand);
-  *l = in / high;
-  *r = band * kBand + in % high;
+__device__ __forceinline__ void tile_of(uint32_t n, uint32_t nl, uint32_t nr, int *l, int *r) {
+  const uint32_t total = nl * nr, each = total / kXcds, rest = total % kXcds;
+  const uint32_t xcd = n % kXcds;
+  n = xcd * each + min(xcd, rest) + n / kXcds;
+  const uint32_t band = n / (kBand * nl), in = n - band * (kBand * nl);
+  const uint32_t high = min((uint32_t)kBand, nr - band * kBand);
+  *l = (int)(in / high);
+  *r = (int)(band * kBand + in % high);
 }
 
 // ------------------------------------------------------------------------ activations
@@ -258,64 +312,33 @@ __device__ __forceinline__ void act_slope(float a, int kind, float *value, float
 
 // ---------------------------------------------------------------- results and their rows
 
-// n of four neighbouring elements, in one access where `wide` says that it may be
-template <class T>
-__device__ __forceinline__ f32x4 load4(const T *p, int n, bool wide) {
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-  if (wide && n >= 4) {
-    Vec<T, 4>::load(p, v);
-  } else {
+// N neighbouring elements from any address, n of them inside.
+template <class T, int N>
+struct Loose {
+  typedef T Raw __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  static __device__ __forceinline__ void load(const T *p, float (&v)[N], int n) {
+    if (n >= N) {
+      const Raw r = *reinterpret_cast<const Raw *>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) v[i] = (float)p[i];
-  }
-  return f32x4{v[0], v[1], v[2], v[3]};
-}
-template <class T>
-__device__ __forceinline__ void store4(T *p, const f32x4 &x, int n, bool wide) {
-  if (wide && n >= 4) {
-    const float v[4] = {x[0], x[1], x[2], x[3]};
-    Vec<T, 4>::store(p, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) p[i] = (T)x[i];
-  }
-}
-
-template <class T>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8], int n, bool wide) {
-  if (wide && n >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      Vec<T, 8>::load(p, v);
+      for (int i = 0; i < N; ++i) v[i] = (float)r[i];
     } else {
-      float u[4], w[4];
-      Vec<T, 4>::load(p, u);
-      Vec<T, 4>::load(p + 4, w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = u[i], v[4 + i] = w[i];
+      for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.f;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
   }
-}
-template <class T>
-__device__ __forceinline__ void store8(T *p, const float (&v)[8], int n, bool wide) {
-  if (wide && n >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      Vec<T, 8>::store(p, v);
+  static __device__ __forceinline__ void store(T *p, const float (&v)[N], int n) {
+    if (n >= N) {
+      Raw r;
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = (T)v[i];
+      *reinterpret_cast<Raw *>(p) = r;
     } else {
-      const float u[4] = {v[0], v[1], v[2], v[3]}, w[4] = {v[4], v[5], v[6], v[7]};
-      Vec<T, 4>::store(p, u);
-      Vec<T, 4>::store(p + 4, w);
-    }
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = (T)v[i];
+      for (int i = 0; i < N; ++i)
+        if (i < n) p[i] = (T)v[i];
+    }
   }
-}
+};
 
 struct GatedArgs {
   Operand x, gate, up;       // as left or right operands of the first products
@@ -324,8 +347,22 @@ struct GatedArgs {
   float *ab;                 // [2, M, F] (may be NULL): a and b, for the gradients
   void *dab;                 // [M, 2 Fp]: da, db, zero from F to Fp
   int64_t M, F, Fp;
-  int32_t kind, wide;
+  int32_t kind;
+  int32_t tiles_l, tiles_r, steps;
 };
+
+// da and db of 8 elements, n of them inside (zero beyond).
+template <class T>
+__device__ __forceinline__ void slopes(const GatedArgs &g, const float (&a)[8], const float (&b)[8], const float (&dh)[8],
+                                       float (&da)[8], float (&db)[8], int n) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float v, s;
+    act_slope<T>(a[i], g.kind, &v, &s);
+    da[i] = i < n ? dh[i] * b[i] * s : 0.f;
+    db[i] = i < n ? dh[i] * v : 0.f;
+  }
+}
 
 template <class P>
 struct LoadHalves {
@@ -342,61 +379,77 @@ struct LoadHalves {
 // h (and a, b), or with GRAD da and db from dh: the left tile is half gate, half up, so that a lane
 // has a and b of the same elements.
 template <class P, bool GRAD>
-__global__ __launch_bounds__(P::kThreads) void gated_kernel(GatedArgs g) {
+__global__ __launch_bounds__(P::kThreads, P::GROUPS * P::NW / 4) void gated_kernel(GatedArgs g) {
   typedef typename P::type T;
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int64_t F = GRAD ? g.Fp : g.F;
-  int64_t tl, tr;
-  tile_of(blockIdx.x, cdiv(F, P::BLL), cdiv(g.M, P::BR), &tl, &tr);
+  int tl, tr;
+  tile_of(blockIdx.x, g.tiles_l, g.tiles_r, &tl, &tr);
+  const int64_t m0 = (int64_t)tr * P::BR, f0 = (int64_t)tl * P::BLL;
   typename P::Left gate, up;
   typename P::Right x;
-  gate.init(g.gate, tl * P::BLL, wave, lane);
-  up.init(g.up, tl * P::BLL, wave, lane);
-  x.init(g.x, tr * P::BR, wave, lane);
+  gate.init(g.gate, f0, wave, lane);
+  up.init(g.up, f0, wave, lane);
+  x.init(g.x, m0, wave, lane);
   f32x4 acc[P::NL][P::NR] = {};
-  P::run(acc, cdiv(g.x.len, kStepOf<T>), LoadHalves<P>{gate, up, x, wave}, wave, lane);
-  const int wl = wave % P::WL, wr = wave / P::WL;
+  P::run(acc, g.steps, LoadHalves<P>{gate, up, x, wave}, wave, lane);
+  // results from here on are rows and columns of the tile (less than 2^31 bytes of memory)
+  const int rows = (int)min((int64_t)P::BR, g.M - m0), cols = (int)min((int64_t)P::BLL, g.F - f0);
+  const int wl = wave % P::WL, wr = wave / P::WL, F = (int)g.F, Fp = (int)g.Fp, zeros = (int)min((int64_t)P::BLL, g.Fp - f0);
+  const int64_t start = m0 * g.F + f0;
 #pragma unroll
   for (int r = 0; r < P::NR; ++r) {
-    const int64_t m = tr * P::BR + (wr * P::NR + r) * 16 + lane % 16;
-    if (m >= g.M) continue;
+    const int m = (wr * P::NR + r) * 16 + lane % 16;
+    if (m >= rows) continue;
 #pragma unroll
     for (int l = 0; l < P::NLL; l += 2) {
-      const int64_t f = tl * P::BLL + (wl * P::NLL + l) * 16 + 8 * (lane / 16);
-      const int n = (int)min((int64_t)8, g.F - f);
+      const int f = (wl * P::NLL + l) * 16 + 8 * (lane / 16), n = cols - f;
       float a[8], b[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         a[i] = acc[l + i / 4][r][i % 4];
         b[i] = acc[P::NLL + l + i / 4][r][i % 4];
       }
+      const int at = m * F + f;
       if constexpr (GRAD) {
-        if (f >= g.Fp) continue;
+        if (f >= zeros) continue;
         float dh[8], da[8], db[8];
-        load8((const T *)g.dh + m * g.F + f, dh, n, g.wide);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float v, s;
-          act_slope<T>(a[i], g.kind, &v, &s);
-          da[i] = i < n ? dh[i] * b[i] * s : 0.f;
-          db[i] = i < n ? dh[i] * v : 0.f;
-        }
-        T *p = (T *)g.dab + m * 2 * g.Fp + f;
-        const int np = (int)min((int64_t)8, g.Fp - f);
-        store8(p, da, np, true);
-        store8(p + g.Fp, db, np, true);
+        Loose<T, 8>::load((const T *)g.dh + start + at, dh, n);
+        slopes<T>(g, a, b, dh, da, db, n);
+        T *p = (T *)g.dab + m0 * 2 * g.Fp + f0 + (m * 2 * Fp + f);
+        Loose<T, 8>::store(p, da, zeros - f);
+        Loose<T, 8>::store(p + Fp, db, zeros - f);
       } else {
         if (n <= 0) continue;
         float h[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[i] = act<T>(a[i], g.kind) * b[i];
-        store8((T *)g.h + m * g.F + f, h, n, g.wide);
+        Loose<T, 8>::store((T *)g.h + start + at, h, n);
         if (g.ab) {
-          store8(g.ab + m * g.F + f, a, n, g.wide);
-          store8(g.ab + (g.M + m) * g.F + f, b, n, g.wide);
+          Loose<float, 8>::store(g.ab + start + at, a, n);
+          Loose<float, 8>::store(g.ab + g.M * g.F + start + at, b, n);
         }
       }
     }
+  }
+}
+
+// da and db from a and b that the forward call kept: 2^shift threads a row.
+template <class T>
+__global__ __launch_bounds__(256) void gated_slopes_kernel(GatedArgs g, int shift) {
+  const int64_t m = (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
+  if (m >= g.M) return;
+  const float *a_row = g.ab + m * g.F, *b_row = a_row + g.M * g.F;
+  const T *dh_row = (const T *)g.dh + m * g.F;
+  T *out = (T *)g.dab + m * 2 * g.Fp;
+  const int F = (int)g.F, Fp = (int)g.Fp;
+  for (int f = (threadIdx.x & ((1 << shift) - 1)) * 8; f < Fp; f += 8 << shift) {
+    float a[8], b[8], dh[8], da[8], db[8];
+    Loose<float, 8>::load(a_row + f, a, F - f);
+    Loose<float, 8>::load(b_row + f, b, F - f);
+    Loose<T, 8>::load(dh_row + f, dh, F - f);
+    slopes<T>(g, a, b, dh, da, db, F - f);
+    Loose<T, 8>::store(out + f, da, Fp - f);
+    Loose<T, 8>::store(out + Fp + f, db, Fp - f);
   }
 }
 
@@ -409,8 +462,8 @@ struct ProductArgs {
   void *out[2];
   int64_t out_ld, nl, nr, split, rows;  // rows: of each output
   float *part;                          // [slices, nr, nl] or NULL: partial sums instead of results
-  int32_t slices, wide;
-  int64_t steps;  // of a slice
+  int32_t slices;
+  int32_t tiles_l, tiles_r, steps;  // steps: of a slice
 };
 
 template <class P>
@@ -425,48 +478,47 @@ struct LoadBoth {
 };
 
 template <class P>
-__global__ __launch_bounds__(P::kThreads) void product_kernel(ProductArgs g) {
+__global__ __launch_bounds__(P::kThreads, P::GROUPS * P::NW / 4) void product_kernel(ProductArgs g) {
   typedef typename P::type T;
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int64_t tiles = cdiv(g.nl, P::BL) * cdiv(g.nr, P::BR);
-  const int64_t slice = blockIdx.x / tiles;
-  int64_t tl, tr;
-  tile_of(blockIdx.x % tiles, cdiv(g.nl, P::BL), cdiv(g.nr, P::BR), &tl, &tr);
+  const uint32_t tiles = (uint32_t)g.tiles_l * g.tiles_r, slice = blockIdx.x / tiles;
+  int tl, tr;
+  tile_of(blockIdx.x - slice * tiles, g.tiles_l, g.tiles_r, &tl, &tr);
   f32x4 acc[P::NL][P::NR] = {};
   for (int pair = 0; pair < g.pairs; ++pair) {
     Operand lo = g.left[pair], ro = g.right[pair];
-    int64_t steps = cdiv(lo.len, kStepOf<T>);
     if (g.slices > 1) {
-      const int64_t k0 = slice * g.steps * kStepOf<T>;
+      const int64_t k0 = (int64_t)slice * g.steps * kStepOf<T>;
       // (only operands across the contraction are cut)
       lo.p = (const T *)lo.p + k0 * lo.ld;
       ro.p = (const T *)ro.p + k0 * ro.ld;
-      lo.len = ro.len = max((int64_t)0, min(g.steps * kStepOf<T>, lo.len - k0));
-      steps = cdiv(lo.len, kStepOf<T>);
+      lo.len = ro.len = max((int64_t)0, min((int64_t)g.steps * kStepOf<T>, lo.len - k0));
     }
+    const int steps = (int)((lo.len + kStepOf<T> - 1) / kStepOf<T>);
     typename P::Left left;
     typename P::Right right;
-    left.init(lo, tl * P::BL, wave, lane);
-    right.init(ro, tr * P::BR, wave, lane);
+    left.init(lo, (int64_t)tl * P::BL, wave, lane);
+    right.init(ro, (int64_t)tr * P::BR, wave, lane);
     P::run(acc, steps, LoadBoth<P>{left, right, wave}, wave, lane);
   }
   const int wl = wave % P::WL, wr = wave / P::WL;
 #pragma unroll
   for (int r = 0; r < P::NR; ++r) {
-    const int64_t row = tr * P::BR + (wr * P::NR + r) * 16 + lane % 16;
+    const int64_t row = (int64_t)tr * P::BR + (wr * P::NR + r) * 16 + lane % 16;
     if (row >= g.nr) continue;
     const bool second = row >= g.split;
     const int64_t at = second ? row - g.split : row;
     if (!g.part && at >= g.rows) continue;
 #pragma unroll
     for (int l = 0; l < P::NL; ++l) {
-      const int64_t col = tl * P::BL + (wl * P::NL + l) * 16 + 4 * (lane / 16);
+      const int64_t col = (int64_t)tl * P::BL + (wl * P::NL + l) * 16 + 4 * (lane / 16);
       const int n = (int)min((int64_t)4, g.nl - col);
       if (n <= 0) continue;
+      const float v[4] = {acc[l][r][0], acc[l][r][1], acc[l][r][2], acc[l][r][3]};
       if (g.part)
-        store4(g.part + (slice * g.nr + row) * g.nl + col, acc[l][r], n, g.nl % 4 == 0);
+        Loose<float, 4>::store(g.part + ((int64_t)slice * g.nr + row) * g.nl + col, v, n);
       else
-        store4((T *)g.out[second] + at * g.out_ld + col, acc[l][r], n, g.wide);
+        Loose<T, 4>::store((T *)g.out[second] + at * g.out_ld + col, v, n);
     }
   }
 }
@@ -474,20 +526,21 @@ __global__ __launch_bounds__(P::kThreads) void product_kernel(ProductArgs g) {
 // The results from the slices' partial sums, in order.
 template <class T>
 __global__ __launch_bounds__(256) void join_slices_kernel(ProductArgs g) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, total = g.nr * g.nl;
-  if (i >= total) return;
-  const int n = (int)min((int64_t)4, total - i);
-  const bool wide = total % 4 == 0;
-  f32x4 s = {};
-  for (int k = 0; k < g.slices; ++k) s += load4(g.part + k * total + i, n, wide);
+  const int64_t per = cdiv(g.nl, 4), i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per;
+  if (row >= g.nr) return;
+  const int64_t col = (i - row * per) * 4, total = g.nr * g.nl;
+  const bool second = row >= g.split;
+  const int64_t at = second ? row - g.split : row;
+  if (at >= g.rows) return;
+  const int n = (int)min((int64_t)4, g.nl - col);
+  float s[4] = {};
+  for (int k = 0; k < g.slices; ++k) {
+    float v[4];
+    Loose<float, 4>::load(g.part + k * total + row * g.nl + col, v, n);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j >= n) break;
-    const int64_t row = (i + j) / g.nl, col = (i + j) % g.nl;
-    const bool second = row >= g.split;
-    const int64_t at = second ? row - g.split : row;
-    if (at < g.rows) ((T *)g.out[second])[at * g.out_ld + col] = (T)s[j];
+    for (int j = 0; j < 4; ++j) s[j] += v[j];
   }
+  Loose<T, 4>::store((T *)g.out[second] + at * g.out_ld + col, s, n);
 }
 
 // ---------------------------------------------------------------------- aligned copies
@@ -506,26 +559,31 @@ __global__ __launch_bounds__(256) void align_kernel(const T *in, T *out, int64_t
   Vec<T, V>::store(out + row * wide + c, v);
 }
 
-// da and db from a and b that the forward call kept.
+// [D, 2 Fp] from the weights [F, D]: row d is column d of gate, zeros up to Fp, and column d of up.
+constexpr int kTurn = 64;
 template <class T>
-__global__ __launch_bounds__(256) void gated_slopes_kernel(GatedArgs g) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = g.Fp / 4;
-  if (i >= g.M * per) return;
-  const int64_t m = i / per, f = (i - m * per) * 4;
-  const int n = (int)min((int64_t)4, g.F - f);
-  const f32x4 a = load4(g.ab + m * g.F + f, n, g.wide), b = load4(g.ab + (g.M + m) * g.F + f, n, g.wide);
-  const f32x4 dh = load4((const T *)g.dh + m * g.F + f, n, g.wide);
-  f32x4 da, db;
+__global__ __launch_bounds__(256) void turn_kernel(Operand gate, Operand up, T *out, int64_t D, int64_t F, int64_t Fp) {
+  __shared__ T tile[kTurn][kTurn + 4];
+  const Operand &w = blockIdx.z ? up : gate;
+  const int64_t f0 = (int64_t)blockIdx.x * kTurn, d0 = (int64_t)blockIdx.y * kTurn;
+  const int i = threadIdx.x / 16, j = threadIdx.x % 16 * 4;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float v, s;
-    act_slope<T>(a[j], g.kind, &v, &s);
-    da[j] = j < n ? dh[j] * b[j] * s : 0.f;
-    db[j] = j < n ? dh[j] * v : 0.f;
+  for (int n = 0; n < kTurn; n += 16) {
+    float v[4];
+    const int64_t f = f0 + i + n;
+    Loose<T, 4>::load((const T *)w.p + f * w.ld + d0 + j, v, f < F ? (int)min((int64_t)4, D - d0 - j) : 0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) tile[i + n][j + k] = (T)v[k];
   }
-  T *p = (T *)g.dab + m * 2 * g.Fp + f;
-  store4(p, da, 4, true);
-  store4(p + g.Fp, db, 4, true);
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < kTurn; n += 16) {
+    const int64_t d = d0 + i + n;
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (float)tile[j + k][i + n];
+    if (d < D) Loose<T, 4>::store(out + d * 2 * Fp + blockIdx.z * Fp + f0 + j, v, (int)min((int64_t)4, Fp - f0 - j));
+  }
 }
 
 // --------------------------------------------------------------------------- few rows
@@ -543,6 +601,12 @@ __device__ __forceinline__ Frag<T> fragment(const T *row, int64_t k, int64_t len
       if (k + i < len) f[i] = row[k + i];
   }
   return f;
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T *p, const f32x4 &x, int n) {
+  const float v[4] = {x[0], x[1], x[2], x[3]};
+  Loose<T, 4>::store(p, v, n);
 }
 
 // Up to 16 MT rows of x: the weights are read once, each by the lanes that multiply with it, and
@@ -596,10 +660,10 @@ __global__ __launch_bounds__(256) void gated_few_kernel(GatedArgs g) {
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) h[j] = act<T>(sa[j], g.kind) * sb[j];
-    store4((T *)g.h + m * g.F + f, h, n, g.wide);
+    store4((T *)g.h + m * g.F + f, h, n);
     if (g.ab) {
-      store4(g.ab + m * g.F + f, sa, n, g.wide);
-      store4(g.ab + (g.M + m) * g.F + f, sb, n, g.wide);
+      store4(g.ab + m * g.F + f, sa, n);
+      store4(g.ab + (g.M + m) * g.F + f, sb, n);
     }
   }
 }
@@ -626,6 +690,10 @@ int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 int64_t per16(int32_t type) { return 16 / (int64_t)elem_size(type); }
 // rows of the hidden width in a workspace
 int64_t padded_hidden(const astra_gated_linear &f) { return round_up(f.hidden, per16(f.type)); }
+
+// Whether the backward call gets a and b, 16 bytes an element written and read, or computes them
+// again, 4 D operations.
+bool keeps(const astra_gated_linear &f) { return f.width >= (f.type == ASTRA_SEQ_BF16 ? 1024 : 128); }
 
 bool few(const astra_gated_linear &f) { return f.rows <= 64; }
 
@@ -676,18 +744,31 @@ GatedArgs args_of(const astra_gated_linear &f) {
   return g;
 }
 
-// The two sizes of tiles: 256 x 256 results by 2 x 2 wavefronts, or 128 x 128.
+// Tiles of 128 x 192 results, three workgroups to a CU, or 128 x 128, four; or 256 x 256 with a CU to
+// themselves.
 template <class T, bool LTR, bool RTR, bool HALVES>
-using Large = Product<T, LTR, RTR, 8, 4, 2, 4, HALVES>;
+using Large = Product<T, LTR, RTR, 4, 6, HALVES, 3>;
 template <class T, bool LTR, bool RTR, bool HALVES>
-using Small = Product<T, LTR, RTR, 4, 4, 2, 2, HALVES>;
+using Small = Product<T, LTR, RTR, 4, 4, HALVES, 4>;
+using Alone = Product<bf16, true, true, 8, 4, false, 1, 2, 4>;
 
-// Large tiles where there are enough of them for all CUs.
+constexpr int64_t kCus = 256;
 template <class P>
 int64_t tiles(int64_t nl, int64_t nr) {
   return cdiv(nl, P::BLL) * cdiv(nr, P::BR);
 }
-constexpr int64_t kCus = 256;
+// The results that the CUs have room for until the last tile is done: in the first rounds they all
+// wait for it, later their ends have spread.
+template <class P>
+int64_t room(int64_t nl, int64_t nr) {
+  const int64_t n = tiles<P>(nl, nr), each = kCus * P::GROUPS;
+  return (n < 3 * each ? round_up(n, each) : n) * P::BL * P::BR;
+}
+// Large tiles read less for each product, small ones overlap more of what is not products.
+template <class L, class S>
+bool larger(int64_t nl, int64_t nr, int64_t len) {
+  return len >= 1024 && 9 * room<L>(nl, nr) <= 10 * room<S>(nl, nr);
+}
 
 #define GATED_LAUNCH(kernel, blocks, threads, ...)                                                   \
   do {                                                                                               \
@@ -697,16 +778,22 @@ constexpr int64_t kCus = 256;
     ASTRA_HIP_CHECK(rt_last_error(), #kernel " launch");                                             \
   } while (false)
 
+template <class P, bool GRAD>
+int launch_gated_tiles(GatedArgs g, hipStream_t st) {
+  const int64_t F = GRAD ? g.Fp : g.F;
+  const int64_t n = tiles<P>(F, g.M);
+  ASTRA_ABI_CHECK(n, <, 2147483648ll);
+  g.tiles_l = (int32_t)cdiv(F, P::BLL);
+  g.tiles_r = (int32_t)cdiv(g.M, P::BR);
+  g.steps = (int32_t)cdiv(g.x.len, kStepOf<typename P::type>);
+  GATED_LAUNCH((gated_kernel<P, GRAD>), n, P::kThreads, g);
+  return ASTRA_OK;
+}
 template <class T, bool GRAD>
 int launch_gated(const GatedArgs &g, hipStream_t st) {
   typedef Large<T, false, false, true> L;
   typedef Small<T, false, false, true> S;
-  const int64_t F = GRAD ? g.Fp : g.F;
-  if (tiles<L>(F, g.M) >= kCus)
-    GATED_LAUNCH((gated_kernel<L, GRAD>), tiles<L>(F, g.M), L::kThreads, g);
-  else
-    GATED_LAUNCH((gated_kernel<S, GRAD>), tiles<S>(F, g.M), S::kThreads, g);
-  return ASTRA_OK;
+  return larger<L, S>(GRAD ? g.Fp : g.F, g.M, g.x.len) ? launch_gated_tiles<L, GRAD>(g, st) : launch_gated_tiles<S, GRAD>(g, st);
 }
 
 template <class T, bool ALIGNED>
@@ -723,7 +810,6 @@ int launch_few(const GatedArgs &g, hipStream_t st) {
 template <class T>
 int forward(const astra_gated_linear &f, hipStream_t st) {
   GatedArgs g = args_of(f);
-  g.wide = f.hidden % per16(f.type) == 0 && aligned(f.h, 16) && aligned(f.projections, 16);
   if (few(f)) {
     g.x = {f.x, f.x_stride, f.rows, f.width};
     g.gate = {f.gate, f.gate_stride, f.hidden, f.width};
@@ -743,31 +829,49 @@ int forward(const astra_gated_linear &f, hipStream_t st) {
   return launch_gated<T, false>(g, st);
 }
 
-// dx = da Wg + db Wu, [M, D]
 template <class P>
-int launch_dx(ProductArgs &g, hipStream_t st) {
-  GATED_LAUNCH(product_kernel<P>, tiles<P>(g.nl, g.nr), P::kThreads, g);
+int launch_product(ProductArgs &g, hipStream_t st) {
+  const int64_t n = tiles<P>(g.nl, g.nr) * g.slices;
+  ASTRA_ABI_CHECK(n, <, 2147483648ll);
+  g.tiles_l = (int32_t)cdiv(g.nl, P::BL);
+  g.tiles_r = (int32_t)cdiv(g.nr, P::BR);
+  GATED_LAUNCH(product_kernel<P>, n, P::kThreads, g);
   return ASTRA_OK;
 }
 
-// The slices of the rows that the weights' gradients are summed over: enough workgroups for all
+// The weights' gradients are sums over the rows, which are cut into slices: enough workgroups for all
 // CUs, and 8 steps at least to a slice.
+struct Slices {
+  bool alone;
+  int64_t n;
+};
 template <class T>
-int64_t slices_of(const astra_gated_linear &f) {
-  typedef Large<T, true, true, false> P;
-  const int64_t n = tiles<P>(f.width, 2 * padded_hidden(f)), steps = cdiv(f.rows, kStepOf<T>);
-  const int64_t want = cdiv(kCus, n), most = steps / 8;
-  return want < most ? want : most > 1 ? most : 1;
+Slices slices_of(const astra_gated_linear &f) {
+  const int64_t D = f.width, F2 = 2 * padded_hidden(f);
+  typedef Small<T, true, true, false> S;
+  // float products take their time whatever the tiles are; of bf16 ones, small tiles ask for 1.4 times as much
+  const bool alone = f.type == ASTRA_SEQ_BF16 && 10 * tiles<Alone>(D, F2) * Alone::BL * Alone::BR <= 14 * tiles<S>(D, F2) * S::BL * S::BR;
+  const int64_t want = alone ? cdiv(kCus, tiles<Alone>(D, F2)) : cdiv(kCus * S::GROUPS, tiles<S>(D, F2));
+  const int64_t most = cdiv(f.rows, kStepOf<T>) / 8;
+  return {alone, want < most ? want : most > 1 ? most : 1};
 }
 template <class T>
 size_t part_bytes(const astra_gated_linear &f) {
-  const int64_t s = slices_of<T>(f);
+  const int64_t s = slices_of<T>(f).n;
   return s > 1 ? (size_t)(s * 2 * padded_hidden(f) * f.width) * sizeof(float) : 0;
+}
+
+// With many rows the weights are turned for the inputs' gradient: products along the contraction are
+// a fifth faster, which 4,096 rows make more than the turning takes.
+bool turned(const astra_gated_linear &f) { return f.rows >= 4096; }
+template <class T>
+size_t turned_bytes(const astra_gated_linear &f) {
+  return turned(f) ? (size_t)round_up(f.width * 2 * padded_hidden(f), 16) * sizeof(T) : 0;
 }
 
 template <class T>
 size_t grad_bytes(const astra_gated_linear &f) {
-  return (size_t)(f.rows * 2 * padded_hidden(f)) * sizeof(T) + copies_bytes(f) + part_bytes<T>(f);
+  return (size_t)(f.rows * 2 * padded_hidden(f)) * sizeof(T) + copies_bytes(f) + turned_bytes<T>(f) + part_bytes<T>(f);
 }
 
 template <class T>
@@ -779,7 +883,7 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
   ASTRA_ABI_CHECK(b.workspace_bytes, >=, need);
   if (need && !aligned(b.workspace, 16)) return fail(ASTRA_ERR_INVALID_ARGUMENT, "astra_gated_linear_backward: the workspace starts on 16 bytes");
   char *ws = (char *)b.workspace;
-  const int64_t Fp = g.Fp, v = per16(f.type);
+  const int64_t Fp = g.Fp, Dp = round_up(f.width, per16(f.type));
   g.dab = ws;
   g.dh = b.dh;
   ws += (size_t)(f.rows * 2 * Fp) * sizeof(T);
@@ -788,50 +892,64 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
   g.x = o.x;
   g.gate = o.gate;
   g.up = o.up;
-  g.wide = f.hidden % per16(f.type) == 0 && aligned(b.dh, 16) && aligned(f.projections, 16);
-  if (f.rows) {
-    if (f.projections) {
-      GATED_LAUNCH(gated_slopes_kernel<T>, cdiv(f.rows * (Fp / 4), 256), 256, g);
-    } else if (int rc = launch_gated<T, true>(g, st)) {
-      return rc;
-    }
+  if (f.rows && f.projections) {
+    int shift = 4;
+    while (shift < 8 && (int64_t(8) << shift) < Fp) ++shift;
+    GATED_LAUNCH(gated_slopes_kernel<T>, cdiv(f.rows, 256 >> shift), 256, g, shift);
+  } else if (f.rows) {
+    if (int rc = launch_gated<T, true>(g, st)) return rc;
   }
-  if (b.dx && f.rows) {
+  if (b.dx && f.rows) {  // da Wg + db Wu
     ProductArgs p{};
-    p.pairs = 2;
-    for (int i = 0; i < 2; ++i) {
-      const Operand &w = i ? o.up : o.gate;
-      p.left[i] = {w.p, w.ld, round_up(f.width, v), f.hidden};       // lines: columns of the weight
-      p.right[i] = {(const T *)g.dab + i * Fp, 2 * Fp, f.rows, Fp};
-    }
     p.out[0] = b.dx;
     p.out_ld = p.nl = f.width;
     p.nr = p.split = p.rows = f.rows;
     p.slices = 1;
-    p.wide = f.width % 4 == 0 && aligned(b.dx, 4 * sizeof(T));
-    typedef Large<T, true, false, false> L;
-    typedef Small<T, true, false, false> S;
-    if (int rc = tiles<L>(p.nl, p.nr) >= kCus ? launch_dx<L>(p, st) : launch_dx<S>(p, st)) return rc;
+    if (turned(f)) {
+      const dim3 grid((unsigned)cdiv(Fp, kTurn), (unsigned)cdiv(f.width, kTurn), 2);
+      hipLaunchKernelGGL(turn_kernel<T>, grid, dim3(256), 0, st, o.gate, o.up, (T *)ws, (int64_t)f.width, (int64_t)f.hidden, Fp);
+      ASTRA_HIP_CHECK(rt_last_error(), "turn_kernel launch");
+      p.pairs = 1;
+      p.left[0] = {ws, 2 * Fp, f.width, 2 * Fp};
+      p.right[0] = {g.dab, 2 * Fp, f.rows, 2 * Fp};
+      typedef Large<T, false, false, false> L;
+      typedef Small<T, false, false, false> S;
+      if (int rc = larger<L, S>(p.nl, p.nr, 2 * Fp) ? launch_product<L>(p, st) : launch_product<S>(p, st)) return rc;
+    } else {
+      p.pairs = 2;
+      for (int i = 0; i < 2; ++i) {
+        const Operand &w = i ? o.up : o.gate;
+        p.left[i] = {w.p, w.ld, Dp, f.hidden};  // lines: columns of the weight
+        p.right[i] = {(const T *)g.dab + i * Fp, 2 * Fp, f.rows, Fp};
+      }
+      if (int rc = launch_product<Small<T, true, false, false>>(p, st)) return rc;
+    }
   }
+  ws += turned_bytes<T>(f);
   if (b.dgate || b.dup) {
-    typedef Large<T, true, true, false> P;
+    const Slices s = slices_of<T>(f);
     ProductArgs p{};
     p.pairs = 1;
-    p.left[0] = {o.x.p, o.x.ld, round_up(f.width, v), f.rows};
     // (one weight's gradient alone is the product with its half of the columns)
     p.nr = b.dgate && b.dup ? 2 * Fp : Fp;
+    p.left[0] = {o.x.p, o.x.ld, Dp, f.rows};
     p.right[0] = {(const T *)g.dab + (b.dgate ? 0 : Fp), 2 * Fp, p.nr, f.rows};
     p.out[0] = b.dgate ? b.dgate : b.dup;
     p.out[1] = b.dup;
     p.out_ld = p.nl = f.width;
     p.split = Fp;
     p.rows = f.hidden;
-    p.slices = (int32_t)slices_of<T>(f);
-    p.part = p.slices > 1 ? (float *)ws : nullptr;
-    p.steps = cdiv(cdiv(f.rows, kStepOf<T>), p.slices);
-    p.wide = f.width % 4 == 0 && aligned(b.dgate, 4 * sizeof(T)) && aligned(b.dup, 4 * sizeof(T));
-    GATED_LAUNCH(product_kernel<P>, tiles<P>(p.nl, p.nr) * p.slices, P::kThreads, p);
-    if (p.part) GATED_LAUNCH(join_slices_kernel<T>, cdiv(cdiv(p.nr * p.nl, 4), 256), 256, p);
+    p.slices = (int32_t)s.n;
+    p.part = s.n > 1 ? (float *)ws : nullptr;
+    p.steps = (int32_t)cdiv(cdiv(f.rows, kStepOf<T>), s.n);
+    int rc = ASTRA_OK;
+    if constexpr (sizeof(T) == 2) {
+      rc = s.alone ? launch_product<Alone>(p, st) : launch_product<Small<T, true, true, false>>(p, st);
+    } else {
+      rc = launch_product<Small<T, true, true, false>>(p, st);
+    }
+    if (rc) return rc;
+    if (p.part) GATED_LAUNCH(join_slices_kernel<T>, cdiv(p.nr * cdiv(p.nl, 4), 256), 256, p);
   }
   return ASTRA_OK;
 }
@@ -853,7 +971,7 @@ int astra_gated_linear_workspace_size(const astra_gated_linear *f, size_t *bytes
 int astra_gated_linear_projections(const astra_gated_linear *f, size_t *floats) {
   if (int rc = check(f)) return rc;
   ASTRA_SEQ_POINTER(floats);
-  *floats = 0;
+  *floats = keeps(*f) ? (size_t)2 * f->rows * f->hidden : 0;
   return ASTRA_OK;
 }
 
