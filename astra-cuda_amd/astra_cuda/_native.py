@@ -68,6 +68,7 @@ SEQUENCE_PROTOTYPES = {
     "astra_gated_linear_forward": (_c_int, [_vp, _vp]),
     "astra_gated_linear_grad_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
     "astra_gated_linear_backward": (_c_int, [_vp, _vp]),
+    "astra_log_probs_workspace_size": (_c_int, [_vp, ctypes.POINTER(_sz)]),
     "astra_log_probs_forward": (_c_int, [_vp, _vp]),
     "astra_log_probs_backward": (_c_int, [_vp, _vp]),
 }
@@ -168,7 +169,7 @@ class GatedLinearGrad(ctypes.Structure):
 class LogProbs(ctypes.Structure):
     """astra_log_probs (include/sequence/astra_sequence.h)."""
     _fields_ = _fields("logits mask choice log_prob entropy stats top_log_prob top_index", "rows stride mask_stride",
-                       "parts top choice_bytes type") + [("sizes", _c_i32 * 16)]
+                       "parts top choice_bytes type") + [("sizes", _c_i32 * 16), ("workspace", _vp), ("workspace_bytes", _sz)]
 
 
 class LogProbsGrad(ctypes.Structure):

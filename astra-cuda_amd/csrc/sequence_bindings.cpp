@@ -736,6 +736,9 @@ variable_list probs_forward(const Tensor &logits, const Tensor &choice, const Te
     out.push_back(empty(logits, {R, P, top}, torch::kInt64));
     f.top_index = ptr<int64_t>(out.back());
   }
+  check(astra_log_probs_workspace_size(&f, &f.workspace_bytes));
+  const Tensor ws = workspace(logits, f.workspace_bytes);
+  f.workspace = ptr(ws);
   check(astra_log_probs_forward(&f, stream_of(logits.get_device())));
   return out;
 }

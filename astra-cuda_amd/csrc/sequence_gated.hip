@@ -588,18 +588,16 @@ __global__ __launch_bounds__(256) void turn_kernel(Operand gate, Operand up, T *
 
 // --------------------------------------------------------------------------- few rows
 
-// One fragment straight from memory: 16 bytes from byte `k` of the contraction on (zeros beyond).
-template <class T, bool ALIGNED>
-__device__ __forceinline__ Frag<T> fragment(const T *row, int64_t k, int64_t len) {
+// One fragment straight from memory, from any address: 16 bytes from element `k` of the contraction on
+// (zeros beyond).
+template <class T>
+__device__ __forceinline__ Frag<T> fragment(const T *row, int k, int len) {
   constexpr int V = 16 / sizeof(T);
+  if (k + V <= len) return *reinterpret_cast<const typename Loose<T, V>::Raw *>(row + k);
   Frag<T> f = {};
-  if constexpr (ALIGNED) {
-    if (k < len) f = *reinterpret_cast<const Frag<T> *>(row + k);
-  } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (k + i < len) f[i] = row[k + i];
-  }
+  for (int i = 0; i < V; ++i)
+    if (k + i < len) f[i] = row[k + i];
   return f;
 }
 
@@ -610,60 +608,78 @@ __device__ __forceinline__ void store4(T *p, const f32x4 &x, int n) {
 }
 
 // Up to 16 MT rows of x: the weights are read once, each by the lanes that multiply with it, and
-// nothing is staged. A workgroup has 16 columns of the result; its wavefronts share the contraction.
-template <class T, int MT, bool ALIGNED>
-__global__ __launch_bounds__(256) void gated_few_kernel(GatedArgs g) {
+// nothing is staged. A workgroup has NT tiles of 16 columns of the result, its NW wavefronts share the
+// contraction; what the next step needs is on its way while the last is multiplied.
+template <class T, int MT, int NT, int NW>
+__global__ __launch_bounds__(64 * NW) void gated_few_kernel(GatedArgs g) {
   constexpr int V = 16 / sizeof(T), kStepE = kStepOf<T>;
-  __shared__ f32x4 sums[4][2 * MT][64];
+  __shared__ f32x4 sums[NW][NT * 2 * MT][64];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int i = lane % 16, q = lane / 16;
-  const int64_t f0 = (int64_t)blockIdx.x * 16, line = min(f0 + i, g.F - 1), K = g.x.len;
-  const T *gate = (const T *)g.gate.p + line * g.gate.ld, *up = (const T *)g.up.p + line * g.up.ld;
-  const T *x[MT];
+  const int i = lane % 16, q = lane / 16, K = (int)g.x.len;
+  const int64_t f0 = (int64_t)blockIdx.x * 16 * NT;
+  const T *w[2 * NT], *x[MT];  // gate and up of each tile; rows
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t line = min(f0 + 16 * t + i, g.F - 1);
+    w[2 * t] = (const T *)g.gate.p + line * g.gate.ld;
+    w[2 * t + 1] = (const T *)g.up.p + line * g.up.ld;
+  }
 #pragma unroll
   for (int r = 0; r < MT; ++r) x[r] = (const T *)g.x.p + min((int64_t)(16 * r + i), g.M - 1) * g.x.ld;
-  f32x4 a[MT] = {}, b[MT] = {};
-  for (int64_t k = wave * kStepE + q * V; k - q * V < K; k += 4 * kStepE) {
-    Frag<T> ga[2], ub[2], xr[2][MT];
+  struct Step {
+    Frag<T> w[2][2 * NT], x[2][MT];
+  };
+  const auto load = [&](Step &s, int k) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int64_t at = k + s * (kStepE / 2);
-      ga[s] = fragment<T, ALIGNED>(gate, at, K);
-      ub[s] = fragment<T, ALIGNED>(up, at, K);
+    for (int h = 0; h < 2; ++h) {
+      const int at = k + h * (kStepE / 2);
 #pragma unroll
-      for (int r = 0; r < MT; ++r) xr[s][r] = fragment<T, ALIGNED>(x[r], at, K);
+      for (int t = 0; t < 2 * NT; ++t) s.w[h][t] = fragment<T>(w[t], at, K);
+#pragma unroll
+      for (int r = 0; r < MT; ++r) s.x[h][r] = fragment<T>(x[r], at, K);
     }
+  };
+  f32x4 acc[2 * NT][MT] = {};
+  const auto multiply_all = [&](const Step &s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int r = 0; r < MT; ++r) {
-        multiply(a[r], ga[s], xr[s][r]);
-        multiply(b[r], ub[s], xr[s][r]);
-      }
+      for (int t = 0; t < 2 * NT; ++t)
+#pragma unroll
+        for (int r = 0; r < MT; ++r) multiply(acc[t][r], s.w[h][t], s.x[h][r]);
+  };
+  Step one, two;
+  int k = wave * kStepE + q * V;  // (beyond K there are zeros)
+  load(one, k);
+  for (int n = (K + NW * kStepE - 1) / (NW * kStepE); n > 0; n -= 2) {
+    load(two, k + NW * kStepE);
+    multiply_all(one);
+    load(one, k + 2 * NW * kStepE);
+    multiply_all(two);
+    k += 2 * NW * kStepE;
   }
 #pragma unroll
-  for (int r = 0; r < MT; ++r) {
-    sums[wave][r][lane] = a[r];
-    sums[wave][MT + r][lane] = b[r];
-  }
+  for (int t = 0; t < 2 * NT; ++t)
+#pragma unroll
+    for (int r = 0; r < MT; ++r) sums[wave][t * MT + r][lane] = acc[t][r];
   __syncthreads();
-  const int64_t f = f0 + 4 * q;
-  const int n = (int)min((int64_t)4, g.F - f);
-  for (int r = wave; r < MT; r += 4) {
-    const int64_t m = 16 * r + i;
-    if (m >= g.M || n <= 0) continue;
-    f32x4 sa = sums[0][r][lane], sb = sums[0][MT + r][lane], h;
+  for (int n = wave; n < NT * MT; n += NW) {
+    const int t = n / MT, r = n % MT;
+    const int64_t m = 16 * r + i, f = f0 + 16 * t + 4 * q;
+    const int left = (int)min((int64_t)4, g.F - f);
+    if (m >= g.M || left <= 0) continue;
+    f32x4 a = sums[0][2 * t * MT + r][lane], b = sums[0][(2 * t + 1) * MT + r][lane], h;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      sa += sums[w][r][lane];
-      sb += sums[w][MT + r][lane];
+    for (int v = 1; v < NW; ++v) {
+      a += sums[v][2 * t * MT + r][lane];
+      b += sums[v][(2 * t + 1) * MT + r][lane];
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = act<T>(sa[j], g.kind) * sb[j];
-    store4((T *)g.h + m * g.F + f, h, n);
+    for (int j = 0; j < 4; ++j) h[j] = act<T>(a[j], g.kind) * b[j];
+    store4((T *)g.h + m * g.F + f, h, left);
     if (g.ab) {
-      store4(g.ab + m * g.F + f, sa, n);
-      store4(g.ab + (g.M + m) * g.F + f, sb, n);
+      store4(g.ab + m * g.F + f, a, left);
+      store4(g.ab + (g.M + m) * g.F + f, b, left);
     }
   }
 }
@@ -796,15 +812,21 @@ int launch_gated(const GatedArgs &g, hipStream_t st) {
   return larger<L, S>(GRAD ? g.Fp : g.F, g.M, g.x.len) ? launch_gated_tiles<L, GRAD>(g, st) : launch_gated_tiles<S, GRAD>(g, st);
 }
 
-template <class T, bool ALIGNED>
-int launch_few(const GatedArgs &g, hipStream_t st) {
-  if (g.M <= 16)
-    GATED_LAUNCH((gated_few_kernel<T, 1, ALIGNED>), cdiv(g.F, 16), 256, g);
-  else if (g.M <= 32)
-    GATED_LAUNCH((gated_few_kernel<T, 2, ALIGNED>), cdiv(g.F, 16), 256, g);
+// Two tiles a workgroup, which read x half as often, and eight wavefronts, where the weights are
+// large enough to keep all CUs busy with them.
+template <class T, int MT>
+int launch_few_rows(const GatedArgs &g, hipStream_t st) {
+  if (g.F >= 32 * kCus && g.x.len >= 2048)
+    GATED_LAUNCH((gated_few_kernel<T, MT, 2, 8>), cdiv(g.F, 32), 512, g);
   else
-    GATED_LAUNCH((gated_few_kernel<T, 4, ALIGNED>), cdiv(g.F, 16), 256, g);
+    GATED_LAUNCH((gated_few_kernel<T, MT, 1, 4>), cdiv(g.F, 16), 256, g);
   return ASTRA_OK;
+}
+template <class T>
+int launch_few(const GatedArgs &g, hipStream_t st) {
+  if (g.M <= 16) return launch_few_rows<T, 1>(g, st);
+  if (g.M <= 32) return launch_few_rows<T, 2>(g, st);
+  return launch_few_rows<T, 4>(g, st);
 }
 
 template <class T>
@@ -814,8 +836,7 @@ int forward(const astra_gated_linear &f, hipStream_t st) {
     g.x = {f.x, f.x_stride, f.rows, f.width};
     g.gate = {f.gate, f.gate_stride, f.hidden, f.width};
     g.up = {f.up, f.up_stride, f.hidden, f.width};
-    const bool all = direct(f, f.x, f.x_stride) && direct(f, f.gate, f.gate_stride) && direct(f, f.up, f.up_stride);
-    return all ? launch_few<T, true>(g, st) : launch_few<T, false>(g, st);
+    return launch_few<T>(g, st);
   }
   const size_t need = copies_bytes(f);
   if (need) ASTRA_SEQ_POINTER(f.workspace);

@@ -10,6 +10,8 @@
 // traffic where there are many, by latency where there are few. One pass: a thread keeps the
 // maximum, Z and the entropy's sum of what it has seen, and scales both when the maximum moves.
 // Sums are float32; m and log Z are kept apart, so that l is as exact as x is.
+#include <type_traits>
+
 #include "sequence.h"
 
 #define ASTRA_SRC_NAME "sequence_probs.hip"
@@ -17,9 +19,10 @@
 namespace astra_seq {
 namespace {
 
-constexpr int kParts = ASTRA_SEQ_MAX_PARTS, kTop = ASTRA_SEQ_MAX_TOP;
+constexpr int kParts = ASTRA_SEQ_MAX_PARTS;
+static_assert(ASTRA_SEQ_MAX_TOP <= kWave, "a lane for each of the largest");
 constexpr int V = 8;             // entries a lane takes at a time
-constexpr int kNarrow = 1024;    // parts up to here are a group of lanes' work, larger ones a workgroup's
+constexpr int kNarrow = 1024;    // parts up to here are a group of lanes' work, larger ones workgroups'
 constexpr int kStats = 3;        // m, log Z, H of a row and part
 
 struct ProbArgs {
@@ -30,8 +33,11 @@ struct ProbArgs {
   int64_t *top_index;
   const float *dlog_prob, *dentropy;
   void *dlogits;
+  float *pieces;       // what each piece of a larger part saw,
+  uint64_t *lists;     // and its largest entries
   int64_t R, stride, mask_stride;
   int32_t W, parts, top, wide_choice;
+  int32_t block_rows;          // rows of a workgroup that has all their parts
   int32_t begin[kParts + 1];   // of each part in a row
   int64_t block[kParts + 1];   // the first workgroup of each part in this launch
 };
@@ -58,22 +64,30 @@ struct Loose {
 };
 typedef uint8_t LooseMask __attribute__((ext_vector_type(V), aligned(1)));
 
-// Entries i .. i + V - 1 of a part, -inf for those beyond it or left out.
+// V entries of a part in v, -inf for those that are not i .. i + V - 1, beyond it or left out; the first is
+// entry *at. `room` is what there is to read from the part's begin on, to the end of the row: the
+// last lanes of a row start a little before their entries rather than take them one by one.
 template <class T>
-__device__ __forceinline__ void entries(const T *x, const uint8_t *mask, int i, int size, float (&v)[V]) {
-  if (i + V <= size) {
-    const auto r = *reinterpret_cast<const typename Loose<T>::Raw *>(x + i);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = (float)r[j];
-    if (mask) {
-      const LooseMask u = *reinterpret_cast<const LooseMask *>(mask + i);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = u[j] ? v[j] : -INFINITY;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = i + j < size && (!mask || mask[i + j]) ? (float)x[i + j] : -INFINITY;
+__device__ __forceinline__ void entries(const T *x, const uint8_t *mask, int i, int size, int room, float (&v)[V], int *at) {
+  const int from = min(i, room - V);
+  *at = from;
+  typename Loose<T>::Raw r;
+  LooseMask u;
+  if (i < size) {
+    r = *reinterpret_cast<const typename Loose<T>::Raw *>(x + from);
+    if (mask) u = *reinterpret_cast<const LooseMask *>(mask + from);
   }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const bool in = from + j >= i && from + j < size && (!mask || u[j]);
+    v[j] = in ? (float)r[j] : -INFINITY;
+  }
+}
+// The same in rows of less than V entries.
+template <class T>
+__device__ __forceinline__ void short_entries(const T *x, const uint8_t *mask, int size, float (&v)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = j < size && (!mask || mask[j]) ? (float)x[j] : -INFINITY;
 }
 template <class T>
 __device__ __forceinline__ float entry(const T *x, const uint8_t *mask, int i) {
@@ -174,25 +188,83 @@ __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// A wavefront's list of the largest keys, one a lane, falling; `last` is the top-th.
-struct Largest {
-  uint64_t key = 0, last = 0;
+// v of lane ^ X, by data-parallel moves and row swaps.
+template <int X>
+__device__ __forceinline__ uint32_t across(uint32_t v, int lane) {
+  constexpr int kReverse4 = 0x1B, kTurn8 = 0x128;  // quad_perm 3,2,1,0; row_ror:8
+  const auto dpp = [](uint32_t u, auto ctrl) __attribute__((always_inline)) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, decltype(ctrl)::value, 0xf, 0xf, false);
+  };
+  if constexpr ((X & 3) == 3) v = dpp(v, std::integral_constant<int, kReverse4>());
+  if constexpr ((X & 3) == 1) v = dpp(v, std::integral_constant<int, kSwap1>());
+  if constexpr ((X & 3) == 2) v = dpp(v, std::integral_constant<int, kSwap2>());
+  if constexpr (X & 4) v = dpp(dpp(v, std::integral_constant<int, kMirror8>()), std::integral_constant<int, kReverse4>());
+  if constexpr (X & 8) v = dpp(v, std::integral_constant<int, kTurn8>());
+  if constexpr (X & 16) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t even = p[0], odd = p[1];
+    v = lane & 16 ? even : odd;
+  }
+  if constexpr (X & 32) {
+    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t low = p[0], high = p[1];
+    v = lane & 32 ? low : high;
+  }
+  return v;
+}
+template <int X>
+__device__ __forceinline__ uint64_t across(uint64_t v, int lane) {
+  return (uint64_t)across<X>((uint32_t)(v >> 32), lane) << 32 | across<X>((uint32_t)v, lane);
+}
 
-  __device__ __forceinline__ void put(uint64_t k, int lane, int top) {
-    const int at = __popcll(__ballot(key > k));
-    const uint32_t lo = __shfl_up((uint32_t)key, 1), hi = __shfl_up((uint32_t)(key >> 32), 1);
-    key = lane < at ? key : lane == at ? k : (uint64_t)hi << 32 | lo;
-    last = lane_of(key, top - 1);
-  }
-  // a key of each lane (called by the whole wavefront)
-  __device__ __forceinline__ void see(uint64_t k, int lane, int top) {
-    for (uint64_t more = __ballot(k > last); more; more = __ballot(k > last)) {
-      const int from = __builtin_ctzll(more);
-      put(lane_of(k, from), lane, top);
-      if (lane == from) k = 0;
-    }
-  }
-};
+// One round of a sorting network: lanes i and i ^ X, of which the lower one gets the larger value.
+// The partners differ in X's highest bit.
+template <int X, class K>
+__device__ __forceinline__ void exchange(K &v, int lane) {
+  constexpr int kHigh = X >= 32 ? 32 : X >= 16 ? 16 : X >= 8 ? 8 : X >= 4 ? 4 : X >= 2 ? 2 : 1;
+  const K o = across<X>(v, lane);
+  const bool larger = v > o, lower = !(lane & kHigh);
+  v = larger == lower ? v : o;
+}
+// Rounds that sort (falling) what rises and falls once within S lanes: halves, quarters, ...
+template <int S, class K>
+__device__ __forceinline__ void settle(K &v, int lane) {
+  if constexpr (S >= 64) exchange<32>(v, lane);
+  if constexpr (S >= 32) exchange<16>(v, lane);
+  if constexpr (S >= 16) exchange<8>(v, lane);
+  if constexpr (S >= 8) exchange<4>(v, lane);
+  if constexpr (S >= 4) exchange<2>(v, lane);
+  exchange<1>(v, lane);
+}
+// A bitonic sort of the wavefront's values (Batcher's), falling: sorted groups of lanes are joined
+// by comparing one with the other's mirror image.
+template <class K>
+__device__ __forceinline__ void sort(K &v, int lane) {
+  exchange<1>(v, lane);
+  exchange<3>(v, lane);
+  settle<2>(v, lane);
+  exchange<7>(v, lane);
+  settle<4>(v, lane);
+  exchange<15>(v, lane);
+  settle<8>(v, lane);
+  exchange<31>(v, lane);
+  settle<16>(v, lane);
+  exchange<63>(v, lane);
+  settle<32>(v, lane);
+}
+// The 64 largest of two sorted lists, sorted.
+__device__ __forceinline__ uint64_t joined(uint64_t v, uint64_t w, int lane) {
+  w = across<63>(w, lane);
+  v = v > w ? v : w;
+  settle<64>(v, lane);
+  return v;
+}
+
+// LDS that only this wavefront uses: what was written before is there to be read.
+__device__ __forceinline__ void in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
 __device__ __forceinline__ void store_top(const ProbArgs &a, int64_t at, uint64_t key, const Result &r) {
   a.top_log_prob[at] = key ? value_of(key) - r.most - r.log_z : -INFINITY;
@@ -200,15 +272,8 @@ __device__ __forceinline__ void store_top(const ProbArgs &a, int64_t at, uint64_
 }
 
 template <class T>
-__device__ __forceinline__ void store_result(const ProbArgs &a, int64_t unit, int c, const T *x, const uint8_t *mask, const Result &r) {
-  a.entropy[unit] = c == -1 ? 0.f : r.entropy;
-  if (a.log_prob)
-    a.log_prob[unit] = c == -1 ? 0.f : c == INT32_MAX ? NAN : entry(x, mask, c) - r.most - r.log_z;
-  if (a.stats) {
-    a.stats[unit * kStats] = r.most;
-    a.stats[unit * kStats + 1] = r.log_z;
-    a.stats[unit * kStats + 2] = r.entropy;
-  }
+__device__ __forceinline__ float chosen(int c, const T *x, const uint8_t *mask, const Result &r) {
+  return c == -1 ? 0.f : c == INT32_MAX ? NAN : entry(x, mask, c) - r.most - r.log_z;
 }
 
 // ------------------------------------------------------------- parts of up to 1,024 entries
@@ -220,25 +285,30 @@ __host__ __device__ inline int lanes_of(int size) {
   return G;
 }
 
-// A group of lanes has one part of one row in registers.
+// A group of lanes has one part of one row in registers; results go to LDS, from where whole rows
+// of them are written.
+constexpr int kUnits = 1024;  // rows by parts of a workgroup
+struct Out {
+  float log_prob[kUnits], entropy[kUnits], stats[kUnits * kStats];
+};
 template <class T, int C, bool TOP>
-__device__ __forceinline__ void narrow_forward(const ProbArgs &a, int part, int64_t n) {
+__device__ __forceinline__ void narrow_forward(const ProbArgs &a, Out &out, int part, int local, int64_t row, bool in) {
   const int begin = a.begin[part], size = a.begin[part + 1] - begin, G = lanes_of(size);
   const int j = threadIdx.x & (G - 1);
-  const int64_t row = n * (256 / G) + threadIdx.x / G, unit = row * a.parts + part;
-  const bool in = row < a.R;
-  const T *x = (const T *)a.logits + (in ? row : 0) * a.stride + begin;
-  const uint8_t *mask = a.mask ? a.mask + (in ? row : 0) * a.mask_stride + begin : nullptr;
+  const int64_t unit = row * a.parts + part;
+  const T *x = (const T *)a.logits + row * a.stride + begin;
+  const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride + begin : nullptr;
   const int c = in ? choice_of(a, unit, size) : -1;
   float v[C][V];
+  int at[C];
   Seen s{-INFINITY, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < C; ++k) {
-    if (c != -1)
-      entries(x, mask, (k * G + j) * V, size, v[k]);
+    at[k] = 0;
+    if (a.W < V)
+      short_entries(x, mask, c != -1 ? size : 0, v[k]);
     else
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[k][i] = -INFINITY;
+      entries(x, mask, (k * G + j) * V, c != -1 ? size : 0, a.W - begin, v[k], &at[k]);
     see(s, v[k]);
   }
   const float most = group_max(s.most, G);
@@ -246,9 +316,16 @@ __device__ __forceinline__ void narrow_forward(const ProbArgs &a, int part, int6
   s.z = group_sum(s.z, G);
   s.s = group_sum(s.s, G);
   const Result r = result_of(s);
-  if (in && j == 0) store_result(a, unit, c, x, mask, r);
-  // the largest one after the other
+  if (in && j == 0) {
+    const int n = local * a.parts + part;
+    if (a.log_prob) out.log_prob[n] = chosen(c, x, mask, r);
+    out.entropy[n] = c == -1 ? 0.f : r.entropy;
+    out.stats[n * kStats] = r.most;
+    out.stats[n * kStats + 1] = r.log_z;
+    out.stats[n * kStats + 2] = r.entropy;
+  }
   if constexpr (!TOP) return;
+  // the largest one after the other
   uint32_t gone = 0;
   for (int t = 0; t < a.top; ++t) {
     uint64_t best = 0;
@@ -257,7 +334,7 @@ __device__ __forceinline__ void narrow_forward(const ProbArgs &a, int part, int6
     for (int k = 0; k < C; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const uint64_t key = gone >> (k * V + i) & 1 ? 0 : key_of(v[k][i], (k * G + j) * V + i);
+        const uint64_t key = gone >> (k * V + i) & 1 ? 0 : key_of(v[k][i], at[k] + i);
         which = key > best ? k * V + i : which;
         best = key > best ? key : best;
       }
@@ -271,14 +348,44 @@ __device__ __forceinline__ void narrow_forward(const ProbArgs &a, int part, int6
   }
 }
 
+// A workgroup has block_rows rows; its wavefronts take one part of some of them at a time.
 template <class T, bool TOP>
 __global__ __launch_bounds__(256) void narrow_forward_kernel(ProbArgs a) {
-  int64_t n;
-  const int part = part_of(a, &n);
-  if (a.begin[part + 1] - a.begin[part] <= 64 * V)
-    narrow_forward<T, 1, TOP>(a, part, n);
-  else
-    narrow_forward<T, 2, TOP>(a, part, n);
+  __shared__ Out out;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int64_t first = (int64_t)blockIdx.x * a.block_rows;
+  const int rows = (int)min((int64_t)a.block_rows, a.R - first);
+  int part = 0, done = 0;  // wavefronts' turns until here
+  for (int turn = wave;; turn += 4) {
+    int each = 0, turns = 0;
+    for (; part < a.parts; ++part) {
+      const int size = a.begin[part + 1] - a.begin[part];
+      each = kWave / lanes_of(size);
+      turns = size <= kNarrow ? (rows + each - 1) / each : 0;
+      if (turn < done + turns) break;
+      done += turns;
+    }
+    if (part == a.parts) break;
+    const int size = a.begin[part + 1] - a.begin[part];
+    const int local = (turn - done) * each + lane / lanes_of(size);
+    const bool in = local < rows;
+    const int64_t row = first + (in ? local : 0);
+    if (size <= 64 * V)
+      narrow_forward<T, 1, TOP>(a, out, part, local, row, in);
+    else
+      narrow_forward<T, 2, TOP>(a, out, part, local, row, in);
+  }
+  __syncthreads();
+  const int64_t at = first * a.parts;
+  for (int n = threadIdx.x; n < rows * a.parts * kStats; n += 256) {
+    const int unit = n / kStats, part_n = unit % a.parts;
+    if (a.begin[part_n + 1] - a.begin[part_n] > kNarrow) continue;
+    if (a.stats) a.stats[at * kStats + n] = out.stats[n];
+    if (n == unit * kStats) {
+      a.entropy[at + unit] = out.entropy[unit];
+      if (a.log_prob) a.log_prob[at + unit] = out.log_prob[unit];
+    }
+  }
 }
 
 // What the gradient of a row and part needs besides its entries.
@@ -305,10 +412,26 @@ __device__ __forceinline__ Slopes slopes_of(const ProbArgs &a, int64_t unit, int
 __device__ __forceinline__ float slope(const Slopes &s, float x, int i) {
   const float l = x - s.most - s.log_z, p = exp_of(l);
   const float d = s.dl * ((i == s.c ? 1.f : 0.f) - p) - s.dh * (p > 0.f ? p * (l + s.entropy) : 0.f);
-  return x == -INFINITY ? 0.f : d;
+  return x == -INFINITY || s.c == -1 ? 0.f : d;
 }
 
-// V entries of a gradient.
+// Entries i .. i + V - 1 of `size`, -inf for those left out.
+template <class T>
+__device__ __forceinline__ void load_entries(const T *x, const uint8_t *mask, int i, int size, float (&v)[V]) {
+  if (i + V <= size) {
+    const auto r = *reinterpret_cast<const typename Loose<T>::Raw *>(x + i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = (float)r[j];
+    if (mask) {
+      const LooseMask u = *reinterpret_cast<const LooseMask *>(mask + i);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = u[j] ? v[j] : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = i + j < size && (!mask || mask[i + j]) ? (float)x[i + j] : -INFINITY;
+  }
+}
 template <class T>
 __device__ __forceinline__ void store_entries(T *d, int i, int size, const float (&g)[V]) {
   if (i + V <= size) {
@@ -323,102 +446,271 @@ __device__ __forceinline__ void store_entries(T *d, int i, int size, const float
   }
 }
 
-template <class T>
-__device__ __forceinline__ void entries_backward(const Slopes &s, const T *x, const uint8_t *mask, T *d, int i, int size) {
-  float v[V];
-  if (s.c != -1) {
-    entries(x, mask, i, size, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = slope(s, v[j], i + j);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = 0.f;
-  }
-  store_entries(d, i, size, v);
-}
-
+// Whole rows, whatever parts they have (a lane's entries may be of several): a workgroup has
+// block_rows rows, and what their parts' gradients need in LDS.
 template <class T>
 __global__ __launch_bounds__(256) void narrow_backward_kernel(ProbArgs a) {
-  int64_t n;
-  const int part = part_of(a, &n);
-  const int begin = a.begin[part], size = a.begin[part + 1] - begin, G = lanes_of(size);
-  const int64_t row = n * (256 / G) + threadIdx.x / G;
-  if (row >= a.R) return;
-  const T *x = (const T *)a.logits + row * a.stride + begin;
-  const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride + begin : nullptr;
-  T *d = (T *)a.dlogits + row * a.W + begin;
-  const Slopes s = slopes_of(a, row * a.parts + part, size, x, mask);
-  for (int i = (threadIdx.x & (G - 1)) * V; i < size; i += G * V) entries_backward(s, x, mask, d, i, size);
+  __shared__ Slopes of_unit[kUnits];
+  const int64_t first = (int64_t)blockIdx.x * a.block_rows;
+  const int rows = (int)min((int64_t)a.block_rows, a.R - first);
+  for (int n = threadIdx.x; n < rows * a.parts; n += 256) {
+    const int local = n / a.parts, part = n - local * a.parts;
+    const int begin = a.begin[part], size = a.begin[part + 1] - begin;
+    const int64_t row = first + local;
+    of_unit[n] = slopes_of(a, row * a.parts + part, size, (const T *)a.logits + row * a.stride + begin,
+                           a.mask ? a.mask + row * a.mask_stride + begin : nullptr);
+  }
+  __syncthreads();
+  const int per = (a.W + V - 1) / V;
+  for (int n = threadIdx.x; n < rows * per; n += 256) {
+    const int local = n / per, i = (n - local * per) * V;
+    const int64_t row = first + local;
+    float v[V];
+    load_entries((const T *)a.logits + row * a.stride, a.mask ? a.mask + row * a.mask_stride : nullptr, i, a.W, v);
+    int part = 0, begin = 0, end = a.begin[1];
+    for (int p = 1; p < a.parts; ++p)
+      if (i >= a.begin[p]) part = p, begin = a.begin[p], end = a.begin[p + 1];
+    Slopes s = of_unit[local * a.parts + part];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (i + j == end && part + 1 < a.parts) {
+        ++part;
+        begin = end;
+        for (int p = 1; p < a.parts; ++p)
+          if (part == p) end = a.begin[p + 1];
+        s = of_unit[local * a.parts + part];
+      }
+      v[j] = slope(s, v[j], i + j - begin);
+    }
+    store_entries((T *)a.dlogits + row * a.W, i, a.W, v);
+  }
 }
 
 // ------------------------------------------------------------------------- larger parts
 
-// A workgroup has one part of one row.
-template <class T, int N, bool TOP>
-__global__ __launch_bounds__(N) void wide_forward_kernel(ProbArgs a) {
-  constexpr int kWaves = N / kWave;
-  __shared__ float lds[3][kWaves];
-  __shared__ uint64_t lists[TOP ? kWaves : 1][kTop];
+// The sum or maximum over a workgroup of WAVES wavefronts.
+template <int WAVES>
+__device__ __forceinline__ float block_sum(float v, float *lds) {
+  v = group_sum(v, 64);
+  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  v = lds[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) v += lds[w];
+  return v;
+}
+template <int WAVES>
+__device__ __forceinline__ float block_max(float v, float *lds) {
+  v = group_max(v, 64);
+  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  v = lds[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) v = fmaxf(v, lds[w]);
+  return v;
+}
+
+template <class T>
+__device__ __forceinline__ void store_result(const ProbArgs &a, int64_t unit, int c, const T *x, const uint8_t *mask, const Result &r) {
+  a.entropy[unit] = c == -1 ? 0.f : r.entropy;
+  if (a.log_prob) a.log_prob[unit] = chosen(c, x, mask, r);
+  if (a.stats) {
+    a.stats[unit * kStats] = r.most;
+    a.stats[unit * kStats + 1] = r.log_z;
+    a.stats[unit * kStats + 2] = r.entropy;
+  }
+}
+
+// Many rows: a workgroup goes through one part of one row.
+template <class T>
+__global__ __launch_bounds__(256) void wide_forward_kernel(ProbArgs a) {
+  __shared__ float lds[3][4];
   int64_t row;
   const int part = part_of(a, &row);
   const int begin = a.begin[part], size = a.begin[part + 1] - begin;
   const int64_t unit = row * a.parts + part;
   const T *x = (const T *)a.logits + row * a.stride + begin;
   const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride + begin : nullptr;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int c = choice_of(a, unit, size);
   Seen s{-INFINITY, 0.f, 0.f};
-  Largest best;
   if (c != -1) {
-    for (int i = threadIdx.x * V; i - lane * V < size; i += N * V) {
+    for (int i = threadIdx.x * V; i < size; i += 256 * V) {
       float v[V];
-      entries(x, mask, i, size, v);
+      load_entries(x, mask, i, size, v);
       see(s, v);
-      if constexpr (TOP) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) best.see(key_of(v[j], i + j), lane, a.top);
-      }
     }
   }
-  const auto over_all = [&](float v, float *p, bool sum) __attribute__((always_inline)) {
-    v = sum ? group_sum(v, 64) : group_max(v, 64);
-    if (lane == 0) p[wave] = v;
-    __syncthreads();
-    v = p[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) v = sum ? v + p[w] : fmaxf(v, p[w]);
-    return v;
+  s = moved_to(s, block_max<4>(s.most, lds[0]));
+  s.z = block_sum<4>(s.z, lds[1]);
+  s.s = block_sum<4>(s.s, lds[2]);
+  if (threadIdx.x == 0) store_result(a, unit, c, x, mask, result_of(s));
+}
+
+// Few rows, or the largest entries wanted: a workgroup has kPiece entries in registers.
+constexpr int kVectors = 4, kPiece = 256 * V * kVectors;
+__host__ __device__ inline int pieces_of(int size) { return (size + kPiece - 1) / kPiece; }
+
+// A wavefront's largest entries, sorted, of those in its lanes' registers. The top-th largest of
+// the lanes' maxima is a bound below them all: what reaches it (some 25 of 2,048 entries for the top
+// 20, if they are in no order) is gathered in LDS and sorted 64 at a time.
+__device__ __forceinline__ uint64_t largest_of(const float (&v)[kVectors][V], int first, float lane_max, int top, uint64_t *gather, int lane) {
+  uint32_t bound = (uint32_t)(key_of(lane_max, 0) >> 32);
+  sort(bound, lane);
+  bound = __builtin_amdgcn_readlane(bound, top - 1);
+  uint64_t best = 0, last = 0;
+  int have = 0;
+  const auto take = [&](int n) __attribute__((always_inline)) {
+    in_order();
+    uint64_t k = lane < n ? gather[lane] : 0;
+    const uint64_t rest = gather[64 + lane];
+    in_order();
+    gather[lane] = rest;
+    if (!__ballot(k > last)) return;
+    sort(k, lane);
+    best = joined(best, k, lane);
+    last = lane_of(best, top - 1);
   };
-  s = moved_to(s, over_all(s.most, lds[0], false));
-  s.z = over_all(s.z, lds[1], true);
-  s.s = over_all(s.s, lds[2], true);
-  const Result r = result_of(s);
-  if (threadIdx.x == 0) store_result(a, unit, c, x, mask, r);
-  if constexpr (TOP) {
-    lists[wave][lane] = best.key;
+#pragma unroll
+  for (int c = 0; c < kVectors; ++c)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const uint64_t key = key_of(v[c][j], first + (c * 256 + (int)threadIdx.x) * V + j);
+      const bool in = key > last && (uint32_t)(key >> 32) >= bound;
+      const uint64_t who = __ballot(in);
+      if (!who) continue;
+      if (in) gather[have + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
+      have += __popcll(who);
+      if (have >= 64) {
+        take(64);
+        have -= 64;
+      }
+    }
+  if (have) take(have);
+  return best;
+}
+
+// The lists of WAVES wavefronts, joined in pairs; the first wavefront has the result.
+template <int WAVES>
+__device__ __forceinline__ uint64_t join_lists(uint64_t best, uint64_t (*lists)[64], int wave, int lane) {
+  lists[wave][lane] = best;
+  for (int step = 1; step < WAVES; step *= 2) {
     __syncthreads();
-    if (wave == 0) {
-      for (int w = 1; w < kWaves; ++w) best.see(lane < a.top ? lists[w][lane] : 0, lane, a.top);
-      if (lane < a.top) store_top(a, unit * a.top + lane, best.key, r);
+    if (wave % (2 * step) == 0) {
+      best = joined(best, lists[wave + step][lane], lane);
+      lists[wave][lane] = best;
+    }
+  }
+  return best;
+}
+
+template <class T, bool TOP>
+__global__ __launch_bounds__(256) void piece_kernel(ProbArgs a) {
+  __shared__ float lds[3][4];
+  __shared__ uint64_t gather[TOP ? 4 : 1][128], lists[TOP ? 4 : 1][64];
+  int64_t n;
+  const int part = part_of(a, &n);
+  const int begin = a.begin[part], size = a.begin[part + 1] - begin, pieces = pieces_of(size);
+  const int64_t row = n / pieces, unit = row * a.parts + part;
+  const int first = (int)(n - row * pieces) * kPiece;
+  const T *x = (const T *)a.logits + row * a.stride + begin;
+  const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride + begin : nullptr;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int c = choice_of(a, unit, size);
+  float v[kVectors][V];
+#pragma unroll
+  for (int k = 0; k < kVectors; ++k) load_entries(x, mask, first + (k * 256 + (int)threadIdx.x) * V, c == -1 ? 0 : size, v[k]);
+  float lane_max = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kVectors; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) lane_max = fmaxf(lane_max, v[k][j]);
+  Seen s{block_max<4>(lane_max, lds[0]), 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < kVectors; ++k) see(s, v[k]);  // (the maximum is there already)
+  s.z = block_sum<4>(s.z, lds[1]);
+  s.s = block_sum<4>(s.s, lds[2]);
+  const Result r = result_of(s);
+  if (pieces == 1) {
+    if (threadIdx.x == 0) store_result(a, unit, c, x, mask, r);
+  } else if (threadIdx.x == 0) {
+    float *out = a.pieces + (int64_t)blockIdx.x * 3;
+    out[0] = s.most;
+    out[1] = s.z;
+    out[2] = s.s;
+  }
+  if constexpr (TOP) {
+    uint64_t best = largest_of(v, first, lane_max, a.top, gather[wave], lane);
+    best = join_lists<4>(best, lists, wave, lane);
+    if (wave == 0 && lane < a.top) {
+      if (pieces == 1)
+        store_top(a, unit * a.top + lane, best, r);
+      else
+        a.lists[(int64_t)blockIdx.x * a.top + lane] = best;
     }
   }
 }
 
-// Every workgroup has kPiece entries of a part of a row.
-constexpr int kPiece = 256 * V * 2;
+// The pieces of a part of a row, one workgroup each.
+constexpr int kJoinWaves = 16;
+template <class T, bool TOP>
+__global__ __launch_bounds__(64 * kJoinWaves) void join_pieces_kernel(ProbArgs a) {
+  __shared__ float lds[3][kJoinWaves];
+  __shared__ uint64_t lists[TOP ? kJoinWaves : 1][64];
+  const int part = blockIdx.y;
+  const int begin = a.begin[part], size = a.begin[part + 1] - begin, pieces = pieces_of(size);
+  if (size <= kNarrow || pieces == 1) return;
+  const int64_t row = blockIdx.x, unit = row * a.parts + part, at = a.block[part] + row * pieces;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  Seen s{-INFINITY, 0.f, 0.f};
+  for (int i = threadIdx.x; i < pieces; i += 64 * kJoinWaves) {
+    const float *p = a.pieces + (at + i) * 3;
+    const Seen o{p[0], p[1], p[2]};
+    const float most = fmaxf(s.most, o.most);
+    const Seen x = moved_to(s, most), y = moved_to(o, most);
+    s = {most, x.z + y.z, x.s + y.s};
+  }
+  s = moved_to(s, block_max<kJoinWaves>(s.most, lds[0]));
+  s.z = block_sum<kJoinWaves>(s.z, lds[1]);
+  s.s = block_sum<kJoinWaves>(s.s, lds[2]);
+  const Result r = result_of(s);
+  if (threadIdx.x == 0)
+    store_result(a, unit, choice_of(a, unit, size), (const T *)a.logits + row * a.stride + begin,
+                 a.mask ? a.mask + row * a.mask_stride + begin : nullptr, r);
+  if constexpr (TOP) {
+    uint64_t best = 0;
+    for (int i = wave; i < pieces; i += kJoinWaves) {
+      const uint64_t k = lane < a.top ? a.lists[(at + i) * a.top + lane] : 0;
+      if (__ballot(k > lane_of(best, a.top - 1))) best = joined(best, k, lane);
+    }
+    best = join_lists<kJoinWaves>(best, lists, wave, lane);
+    if (wave == 0 && lane < a.top) store_top(a, unit * a.top + lane, best, r);
+  }
+}
+
+// Every workgroup has kSpan entries of a part of a row, from the last to the first: what the forward
+// call read last is still in the caches.
+constexpr int kSpan = 256 * V * 2;
 template <class T>
 __global__ __launch_bounds__(256) void wide_backward_kernel(ProbArgs a) {
   int64_t n;
   const int part = part_of(a, &n);
   const int begin = a.begin[part], size = a.begin[part + 1] - begin;
-  const int64_t pieces = cdiv(size, kPiece), row = n / pieces;
-  const int first = (int)(n - row * pieces) * kPiece;
+  const int64_t spans = cdiv(size, kSpan);
+  n = a.R * spans - 1 - n;
+  const int64_t row = n / spans;
+  const int first = (int)(n - row * spans) * kSpan;
   const T *x = (const T *)a.logits + row * a.stride + begin;
   const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride + begin : nullptr;
   T *d = (T *)a.dlogits + row * a.W + begin;
   const Slopes s = slopes_of(a, row * a.parts + part, size, x, mask);
-  const int last = min(first + kPiece, size);
-  for (int i = first + threadIdx.x * V; i < last; i += 256 * V) entries_backward(s, x, mask, d, i, size);
+  const int last = min(first + kSpan, size);
+  for (int i = first + threadIdx.x * V; i < last; i += 256 * V) {
+    float v[V];
+    load_entries(x, mask, i, s.c == -1 ? 0 : size, v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = slope(s, v[j], i + j);
+    store_entries(d, i, size, v);
+  }
 }
 
 // ----------------------------------------------------------------------------- launches
@@ -465,53 +757,103 @@ ProbArgs args_of(const astra_log_probs &f) {
   return a;
 }
 
-// Gives the workgroups of a launch to the parts of one kind; how many there are.
-template <class Blocks>
-int64_t share(ProbArgs &a, bool narrow, Blocks &&blocks) {
+bool narrow(int size) { return size <= kNarrow; }
+
+// Gives the workgroups of a launch to the larger parts, `each(size)` for one; how many there are.
+template <class Each>
+int64_t share(ProbArgs &a, Each &&each) {
   int64_t n = 0;
   for (int i = 0; i < a.parts; ++i) {
     const int size = a.begin[i + 1] - a.begin[i];
     a.block[i] = n;
-    if ((size <= kNarrow) == narrow) n += blocks(size);
+    if (!narrow(size)) n += each(size);
   }
   for (int i = a.parts; i <= kParts; ++i) a.block[i] = n;
   return n;
 }
 
+// Rows of a workgroup that has all their smaller parts: few where there are few, so that all CUs
+// have some, and as many as LDS has room for.
+int rows_together(const ProbArgs &a) {
+  int n = 1;
+  while (2 * n * a.parts <= kUnits && 2 * n <= 64 && a.R >= 1024 * n) n *= 2;
+  return n;
+}
+bool some_narrow(const ProbArgs &a) {
+  for (int i = 0; i < a.parts; ++i)
+    if (narrow(a.begin[i + 1] - a.begin[i])) return true;
+  return false;
+}
+bool some_wide(const ProbArgs &a) {
+  for (int i = 0; i < a.parts; ++i)
+    if (!narrow(a.begin[i + 1] - a.begin[i])) return true;
+  return false;
+}
+
+// Larger parts are cut into pieces where there are few rows or the largest entries are wanted.
+bool in_pieces(const ProbArgs &a) { return a.top > 0 || a.R * a.parts < 512; }
+int64_t all_pieces(ProbArgs &a) {
+  return share(a, [&](int size) { return a.R * pieces_of(size); });
+}
+bool joins(const ProbArgs &a) {
+  for (int i = 0; i < a.parts; ++i)
+    if (pieces_of(a.begin[i + 1] - a.begin[i]) > 1) return true;
+  return false;
+}
+// the lists first, which are of 8 bytes
+size_t piece_bytes(ProbArgs a) {
+  return in_pieces(a) && joins(a) ? (size_t)all_pieces(a) * (3 * sizeof(float) + a.top * sizeof(uint64_t)) : 0;
+}
+
 #define PROBS_LAUNCH(kernel, blocks, threads)                                                          \
   do {                                                                                                 \
     const int64_t blocks_ = (blocks);                                                                  \
-    if (blocks_ == 0) break;                                                                           \
     ASTRA_ABI_CHECK(blocks_, <, 2147483648ll);                                                         \
     hipLaunchKernelGGL((kernel), dim3((unsigned)blocks_), dim3(threads), 0, st, a);                    \
     ASTRA_HIP_CHECK(rt_last_error(), #kernel " launch");                                               \
   } while (false)
 
-template <class T>
-int forward(ProbArgs a, hipStream_t st) {
-  const int64_t narrow = share(a, true, [&](int size) { return cdiv(a.R, 256 / lanes_of(size)); });
-  if (a.top) {
-    PROBS_LAUNCH((narrow_forward_kernel<T, true>), narrow, 256);
-  } else {
-    PROBS_LAUNCH((narrow_forward_kernel<T, false>), narrow, 256);
-  }
-  const int64_t wide = share(a, false, [&](int) { return a.R; });
-  if (wide >= 512 && a.top) {
-    PROBS_LAUNCH((wide_forward_kernel<T, 256, true>), wide, 256);
-  } else if (wide >= 512) {
-    PROBS_LAUNCH((wide_forward_kernel<T, 256, false>), wide, 256);
-  } else if (a.top) {
-    PROBS_LAUNCH((wide_forward_kernel<T, 1024, true>), wide, 1024);
-  } else {
-    PROBS_LAUNCH((wide_forward_kernel<T, 1024, false>), wide, 1024);
-  }
+template <class T, bool TOP>
+int forward_in_pieces(ProbArgs &a, hipStream_t st) {
+  PROBS_LAUNCH((piece_kernel<T, TOP>), all_pieces(a), 256);
+  if (!joins(a)) return ASTRA_OK;
+  ASTRA_ABI_CHECK(a.R, <, 2147483648ll);
+  hipLaunchKernelGGL((join_pieces_kernel<T, TOP>), dim3((unsigned)a.R, (unsigned)a.parts), dim3(64 * kJoinWaves), 0, st, a);
+  ASTRA_HIP_CHECK(rt_last_error(), "join_pieces_kernel launch");
   return ASTRA_OK;
 }
 
 template <class T>
+int forward(ProbArgs a, hipStream_t st) {
+  if (some_narrow(a)) {
+    a.block_rows = rows_together(a);
+    if (a.top) {
+      PROBS_LAUNCH((narrow_forward_kernel<T, true>), cdiv(a.R, a.block_rows), 256);
+    } else {
+      PROBS_LAUNCH((narrow_forward_kernel<T, false>), cdiv(a.R, a.block_rows), 256);
+    }
+  }
+  if (!some_wide(a)) return ASTRA_OK;
+  if (in_pieces(a)) return a.top ? forward_in_pieces<T, true>(a, st) : forward_in_pieces<T, false>(a, st);
+  PROBS_LAUNCH(wide_forward_kernel<T>, share(a, [&](int) { return a.R; }), 256);
+  return ASTRA_OK;
+}
+
+// Rows of which every part is small go through as a whole, others part by part.
+template <class T>
 int backward(ProbArgs a, hipStream_t st) {
-  PROBS_LAUNCH(narrow_backward_kernel<T>, share(a, true, [&](int size) { return cdiv(a.R, 256 / lanes_of(size)); }), 256);
-  PROBS_LAUNCH(wide_backward_kernel<T>, share(a, false, [&](int size) { return a.R * cdiv(size, kPiece); }), 256);
+  if (!some_wide(a)) {
+    a.block_rows = rows_together(a);
+    PROBS_LAUNCH(narrow_backward_kernel<T>, cdiv(a.R, a.block_rows), 256);
+    return ASTRA_OK;
+  }
+  int64_t n = 0;
+  for (int i = 0; i < a.parts; ++i) {
+    a.block[i] = n;
+    n += a.R * cdiv(a.begin[i + 1] - a.begin[i], kSpan);
+  }
+  for (int i = a.parts; i <= kParts; ++i) a.block[i] = n;
+  PROBS_LAUNCH(wide_backward_kernel<T>, n, 256);
   return ASTRA_OK;
 }
 
@@ -522,18 +864,33 @@ using namespace astra_seq;
 
 extern "C" {
 
+int astra_log_probs_workspace_size(const astra_log_probs *f, size_t *bytes) {
+  if (int rc = check(f)) return rc;
+  ASTRA_SEQ_POINTER(bytes);
+  *bytes = f->rows ? piece_bytes(args_of(*f)) : 0;
+  return ASTRA_OK;
+}
+
 int astra_log_probs_forward(const astra_log_probs *f, void *stream) {
   if (int rc = check(f)) return rc;
   if (f->rows == 0) return ASTRA_OK;
   ASTRA_SEQ_POINTER(f->logits);
   ASTRA_SEQ_POINTER(f->entropy);
+  ProbArgs a = args_of(*f);
+  if (const size_t need = piece_bytes(a)) {
+    ASTRA_SEQ_POINTER(f->workspace);
+    ASTRA_ABI_CHECK(f->workspace_bytes, >=, need);
+    if (!aligned(f->workspace, 8)) return fail(ASTRA_ERR_INVALID_ARGUMENT, "astra_log_probs_forward: the workspace starts on 8 bytes");
+    a.lists = (uint64_t *)f->workspace;
+    a.pieces = (float *)(a.lists + all_pieces(a) * a.top);
+  }
   if (f->choice) ASTRA_SEQ_POINTER(f->log_prob);
   if (f->log_prob) ASTRA_SEQ_POINTER(f->choice);
   if (f->top) {
     ASTRA_SEQ_POINTER(f->top_log_prob);
     ASTRA_SEQ_POINTER(f->top_index);
   }
-  return f->type == ASTRA_SEQ_F32 ? forward<float>(args_of(*f), as_stream(stream)) : forward<bf16>(args_of(*f), as_stream(stream));
+  return f->type == ASTRA_SEQ_F32 ? forward<float>(a, as_stream(stream)) : forward<bf16>(a, as_stream(stream));
 }
 
 int astra_log_probs_backward(const astra_log_probs_grad *g, void *stream) {

@@ -222,7 +222,7 @@ int astra_gated_linear_backward(const astra_gated_linear_grad *a, void *stream);
  * [R,parts,3] (may be NULL) is kept for the backward call.
  * A part that does not count is not read: its log_prob and entropy are 0, and there are no
  * likeliest entries. The log probability of an entry that is left out is -inf, that of a choice
- * in no entry NaN; where nothing is allowed the entropy is 0. */
+ * in no entry NaN; where nothing is allowed the entropy is 0. The workspace starts on 8 bytes. */
 typedef struct astra_log_probs {
   const void *logits;
   const uint8_t *mask;
@@ -232,7 +232,10 @@ typedef struct astra_log_probs {
   int64_t rows, stride, mask_stride;
   int32_t parts, top, choice_bytes, type;
   int32_t sizes[ASTRA_SEQ_MAX_PARTS];
+  void *workspace;
+  size_t workspace_bytes;
 } astra_log_probs;
+int astra_log_probs_workspace_size(const astra_log_probs *f, size_t *bytes);
 int astra_log_probs_forward(const astra_log_probs *f, void *stream);
 
 /* Backward: `f` as in the forward call with the stats that it wrote (its outputs are not
