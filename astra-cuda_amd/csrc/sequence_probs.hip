@@ -109,11 +109,8 @@ __device__ __forceinline__ Seen moved_to(const Seen &a, float most) {
   return {most, none ? a.z : a.z * f, none ? a.s : (a.s + a.z * d) * f};
 }
 
-__device__ __forceinline__ void see(Seen &a, const float (&x)[V]) {
-  float most = x[0];
-#pragma unroll
-  for (int j = 1; j < V; ++j) most = fmaxf(most, x[j]);
-  if (most > a.most) a = moved_to(a, most);
+// Entries of which none is larger than the maximum seen.
+__device__ __forceinline__ void add(Seen &a, const float (&x)[V]) {
   const float base = a.most == -INFINITY ? 0.f : a.most;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
@@ -121,6 +118,14 @@ __device__ __forceinline__ void see(Seen &a, const float (&x)[V]) {
     a.z += t;
     a.s = fmaf(t, fmaxf(d, -1000.f), a.s);  // (t is zero far before that; -inf times it would be NaN)
   }
+}
+
+__device__ __forceinline__ void see(Seen &a, const float (&x)[V]) {
+  float most = x[0];
+#pragma unroll
+  for (int j = 1; j < V; ++j) most = fmaxf(most, x[j]);
+  if (most > a.most) a = moved_to(a, most);
+  add(a, x);
 }
 
 struct Result {
@@ -132,38 +137,24 @@ __device__ __forceinline__ Result result_of(const Seen &a) {
   return {a.most == -INFINITY ? 0.f : a.most, log_z, log_z - a.s / a.z};
 }
 
-// Sum and maximum over `G` neighbouring lanes (a power of two, the same in the whole wavefront).
+// The maximum over N neighbouring lanes, in each of them (as lanes_sum).
 template <int CTRL>
 __device__ __forceinline__ float swapped(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
 }
-__device__ __forceinline__ float group_max(float v, int G) {
-  if (G >= 2) v = fmaxf(v, swapped<kSwap1>(v));
-  if (G >= 4) v = fmaxf(v, swapped<kSwap2>(v));
-  if (G >= 8) v = fmaxf(v, swapped<kMirror8>(v));
-  if (G >= 16) v = fmaxf(v, swapped<kMirror16>(v));
-  if (G >= 32) {
+template <int N>
+__device__ __forceinline__ float lanes_max(float v) {
+  if constexpr (N >= 2) v = fmaxf(v, swapped<kSwap1>(v));
+  if constexpr (N >= 4) v = fmaxf(v, swapped<kSwap2>(v));
+  if constexpr (N >= 8) v = fmaxf(v, swapped<kMirror8>(v));
+  if constexpr (N >= 16) v = fmaxf(v, swapped<kMirror16>(v));
+  if constexpr (N >= 32) {
     const Pair p = rows_of_half(v);
     v = fmaxf(p.first, p.second);
   }
-  if (G >= 64) {
+  if constexpr (N >= 64) {
     const Pair p = halves(v);
     v = fmaxf(p.first, p.second);
-  }
-  return v;
-}
-__device__ __forceinline__ float group_sum(float v, int G) {
-  if (G >= 2) v += swapped<kSwap1>(v);
-  if (G >= 4) v += swapped<kSwap2>(v);
-  if (G >= 8) v += swapped<kMirror8>(v);
-  if (G >= 16) v += swapped<kMirror16>(v);
-  if (G >= 32) {
-    const Pair p = rows_of_half(v);
-    v = p.first + p.second;
-  }
-  if (G >= 64) {
-    const Pair p = halves(v);
-    v = p.first + p.second;
   }
   return v;
 }
@@ -217,14 +208,16 @@ __device__ __forceinline__ uint64_t across(uint64_t v, int lane) {
   return (uint64_t)across<X>((uint32_t)(v >> 32), lane) << 32 | across<X>((uint32_t)v, lane);
 }
 
+__device__ __forceinline__ uint64_t larger(uint64_t v, uint64_t w) { return v > w ? v : w; }
+
 // One round of a sorting network: lanes i and i ^ X, of which the lower one gets the larger value.
 // The partners differ in X's highest bit.
 template <int X, class K>
 __device__ __forceinline__ void exchange(K &v, int lane) {
   constexpr int kHigh = X >= 32 ? 32 : X >= 16 ? 16 : X >= 8 ? 8 : X >= 4 ? 4 : X >= 2 ? 2 : 1;
   const K o = across<X>(v, lane);
-  const bool larger = v > o, lower = !(lane & kHigh);
-  v = larger == lower ? v : o;
+  const bool more = v > o, lower = !(lane & kHigh);
+  v = more == lower ? v : o;
 }
 // Rounds that sort (falling) what rises and falls once within S lanes: halves, quarters, ...
 template <int S, class K>
@@ -255,7 +248,7 @@ __device__ __forceinline__ void sort(K &v, int lane) {
 // The 64 largest of two sorted lists, sorted.
 __device__ __forceinline__ uint64_t joined(uint64_t v, uint64_t w, int lane) {
   w = across<63>(w, lane);
-  v = v > w ? v : w;
+  v = larger(v, w);
   settle<64>(v, lane);
   return v;
 }
@@ -271,19 +264,12 @@ __device__ __forceinline__ void store_top(const ProbArgs &a, int64_t at, uint64_
   a.top_index[at] = key ? index_of(key) : -1;
 }
 
-template <class T>
-__device__ __forceinline__ float chosen(int c, const T *x, const uint8_t *mask, const Result &r) {
-  return c == -1 ? 0.f : c == INT32_MAX ? NAN : entry(x, mask, c) - r.most - r.log_z;
+// The log probability of choice c, entry x.
+__device__ __forceinline__ float log_prob_of(int c, float x, const Result &r) {
+  return c == -1 ? 0.f : c == INT32_MAX ? NAN : x - r.most - r.log_z;
 }
 
 // ------------------------------------------------------------- parts of up to 1,024 entries
-
-// Lanes of a part: V entries each, or 2 V of the largest parts.
-__host__ __device__ inline int lanes_of(int size) {
-  int G = 1;
-  while (G < 64 && G * V < size) G *= 2;
-  return G;
-}
 
 // A group of lanes has one part of one row in registers; results go to LDS, from where whole rows
 // of them are written.
@@ -291,89 +277,107 @@ constexpr int kUnits = 1024;  // rows by parts of a workgroup
 struct Out {
   float log_prob[kUnits], entropy[kUnits], stats[kUnits * kStats];
 };
-template <class T, int C, bool TOP>
-__device__ __forceinline__ void narrow_forward(const ProbArgs &a, Out &out, int part, int local, int64_t row, bool in) {
-  const int begin = a.begin[part], size = a.begin[part + 1] - begin, G = lanes_of(size);
-  const int j = threadIdx.x & (G - 1);
-  const int64_t unit = row * a.parts + part;
-  const T *x = (const T *)a.logits + row * a.stride + begin;
-  const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride + begin : nullptr;
-  const int c = in ? choice_of(a, unit, size) : -1;
-  float v[C][V];
-  int at[C];
-  Seen s{-INFINITY, 0.f, 0.f};
+// One part of the workgroup's rows: G lanes a row, V entries each, C times.
+template <class T, int G, int C, bool TOP>
+__device__ void narrow_part(const ProbArgs &a, Out &out, int part, int64_t first, int rows, int turn) {
+  constexpr int kEach = kWave / G;
+  const int begin = a.begin[part], size = a.begin[part + 1] - begin, lane = threadIdx.x % kWave, j = lane % G;
+  const T *logits = (const T *)a.logits + first * a.stride + begin;
+  const uint8_t *masks = a.mask ? a.mask + first * a.mask_stride + begin : nullptr;
+  for (int task = turn; task * kEach < rows; task += 4) {
+    const int local = task * kEach + lane / G;
+    const bool in = local < rows;
+    const int64_t unit = (first + local) * a.parts + part;
+    const T *x = logits + (in ? local : 0) * a.stride;
+    const uint8_t *mask = masks ? masks + (in ? local : 0) * a.mask_stride : nullptr;
+    float v[C][V];
+    int at[C];
 #pragma unroll
-  for (int k = 0; k < C; ++k) {
-    at[k] = 0;
-    if (a.W < V)
-      short_entries(x, mask, c != -1 ? size : 0, v[k]);
-    else
-      entries(x, mask, (k * G + j) * V, c != -1 ? size : 0, a.W - begin, v[k], &at[k]);
-    see(s, v[k]);
-  }
-  const float most = group_max(s.most, G);
-  s = moved_to(s, most);
-  s.z = group_sum(s.z, G);
-  s.s = group_sum(s.s, G);
-  const Result r = result_of(s);
-  if (in && j == 0) {
-    const int n = local * a.parts + part;
-    if (a.log_prob) out.log_prob[n] = chosen(c, x, mask, r);
-    out.entropy[n] = c == -1 ? 0.f : r.entropy;
-    out.stats[n * kStats] = r.most;
-    out.stats[n * kStats + 1] = r.log_z;
-    out.stats[n * kStats + 2] = r.entropy;
-  }
-  if constexpr (!TOP) return;
-  // the largest one after the other
-  uint32_t gone = 0;
-  for (int t = 0; t < a.top; ++t) {
-    uint64_t best = 0;
-    int which = 0;
+    for (int k = 0; k < C; ++k) {
+      at[k] = 0;
+      if (G == 1 && a.W < V)
+        short_entries(x, mask, in ? size : 0, v[k]);
+      else
+        entries(x, mask, (k * G + j) * V, in ? size : 0, a.W - begin, v[k], &at[k]);
+    }
+    // (all on their way before the first is waited for)
+    const int c = in ? choice_of(a, unit, size) : -1;
+    const float x_c = c >= 0 && c < size ? entry(x, mask, c) : -INFINITY;
+    float most = -INFINITY;
 #pragma unroll
     for (int k = 0; k < C; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const uint64_t key = gone >> (k * V + i) & 1 ? 0 : key_of(v[k][i], at[k] + i);
-        which = key > best ? k * V + i : which;
-        best = key > best ? key : best;
+        v[k][i] = c == -1 ? -INFINITY : v[k][i];
+        most = fmaxf(most, v[k][i]);
       }
-    uint64_t all = best;
-    for (int d = 1; d < G; d *= 2) {
-      const uint64_t o = (uint64_t)__shfl_xor((uint32_t)(all >> 32), d) << 32 | (uint32_t)__shfl_xor((uint32_t)all, d);
-      all = o > all ? o : all;
+    Seen s{lanes_max<G>(most), 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < C; ++k) add(s, v[k]);
+    s.z = lanes_sum<G>(s.z);
+    s.s = lanes_sum<G>(s.s);
+    const Result r = result_of(s);
+    if (in && j == 0) {
+      const int n = local * a.parts + part;
+      out.log_prob[n] = log_prob_of(c, x_c, r);
+      out.entropy[n] = c == -1 ? 0.f : r.entropy;
+      out.stats[n * kStats] = r.most;
+      out.stats[n * kStats + 1] = r.log_z;
+      out.stats[n * kStats + 2] = r.entropy;
     }
-    if (best == all) gone |= 1u << which;
-    if (in && j == 0) store_top(a, unit * a.top + t, all, r);
+    if constexpr (TOP) {  // the largest one after the other
+      uint32_t gone = 0;
+      for (int t = 0; t < a.top; ++t) {
+        uint64_t best = 0;
+        int which = 0;
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const uint64_t key = gone >> (k * V + i) & 1 ? 0 : key_of(v[k][i], at[k] + i);
+            which = key > best ? k * V + i : which;
+            best = key > best ? key : best;
+          }
+        uint64_t all = best;
+        if constexpr (G >= 2) all = larger(all, across<1>(all, lane));
+        if constexpr (G >= 4) all = larger(all, across<2>(all, lane));
+        if constexpr (G >= 8) all = larger(all, across<4>(all, lane));
+        if constexpr (G >= 16) all = larger(all, across<8>(all, lane));
+        if constexpr (G >= 32) all = larger(all, across<16>(all, lane));
+        if constexpr (G >= 64) all = larger(all, across<32>(all, lane));
+        if (best == all) gone |= 1u << which;
+        if (in && j == 0) store_top(a, unit * a.top + t, all, r);
+      }
+    }
   }
 }
 
-// A workgroup has block_rows rows; its wavefronts take one part of some of them at a time.
+// A workgroup has block_rows rows, its wavefronts take turns with them.
 template <class T, bool TOP>
 __global__ __launch_bounds__(256) void narrow_forward_kernel(ProbArgs a) {
   __shared__ Out out;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t first = (int64_t)blockIdx.x * a.block_rows;
   const int rows = (int)min((int64_t)a.block_rows, a.R - first);
-  int part = 0, done = 0;  // wavefronts' turns until here
-  for (int turn = wave;; turn += 4) {
-    int each = 0, turns = 0;
-    for (; part < a.parts; ++part) {
-      const int size = a.begin[part + 1] - a.begin[part];
-      each = kWave / lanes_of(size);
-      turns = size <= kNarrow ? (rows + each - 1) / each : 0;
-      if (turn < done + turns) break;
-      done += turns;
-    }
-    if (part == a.parts) break;
-    const int size = a.begin[part + 1] - a.begin[part];
-    const int local = (turn - done) * each + lane / lanes_of(size);
-    const bool in = local < rows;
-    const int64_t row = first + (in ? local : 0);
-    if (size <= 64 * V)
-      narrow_forward<T, 1, TOP>(a, out, part, local, row, in);
+  for (int part = 0; part < a.parts; ++part) {
+    const int size = a.begin[part + 1] - a.begin[part], turn = (wave + part) & 3;
+    if (size > kNarrow) continue;
+    if (size <= V)
+      narrow_part<T, 1, 1, TOP>(a, out, part, first, rows, turn);
+    else if (size <= 2 * V)
+      narrow_part<T, 2, 1, TOP>(a, out, part, first, rows, turn);
+    else if (size <= 4 * V)
+      narrow_part<T, 4, 1, TOP>(a, out, part, first, rows, turn);
+    else if (size <= 8 * V)
+      narrow_part<T, 8, 1, TOP>(a, out, part, first, rows, turn);
+    else if (size <= 16 * V)
+      narrow_part<T, 16, 1, TOP>(a, out, part, first, rows, turn);
+    else if (size <= 32 * V)
+      narrow_part<T, 32, 1, TOP>(a, out, part, first, rows, turn);
+    else if (size <= 64 * V)
+      narrow_part<T, 64, 1, TOP>(a, out, part, first, rows, turn);
     else
-      narrow_forward<T, 2, TOP>(a, out, part, local, row, in);
+      narrow_part<T, 64, 2, TOP>(a, out, part, first, rows, turn);
   }
   __syncthreads();
   const int64_t at = first * a.parts;
@@ -446,43 +450,56 @@ __device__ __forceinline__ void store_entries(T *d, int i, int size, const float
   }
 }
 
-// Whole rows, whatever parts they have (a lane's entries may be of several): a workgroup has
-// block_rows rows, and what their parts' gradients need in LDS.
+// A workgroup has block_rows rows, and what their parts' gradients need in LDS: first V entries of a part
+// to a lane, then the last size % V entries of the parts, one to a lane: neighbours in memory are
+// neighbours among the lanes.
 template <class T>
 __global__ __launch_bounds__(256) void narrow_backward_kernel(ProbArgs a) {
   __shared__ Slopes of_unit[kUnits];
   const int64_t first = (int64_t)blockIdx.x * a.block_rows;
   const int rows = (int)min((int64_t)a.block_rows, a.R - first);
+  const T *logits = (const T *)a.logits + first * a.stride;
+  const uint8_t *masks = a.mask ? a.mask + first * a.mask_stride : nullptr;
+  T *out = (T *)a.dlogits + first * a.W;
+  int full = 0, rest = 0;  // of a row
+  for (int p = 0; p < a.parts; ++p) {
+    full += (a.begin[p + 1] - a.begin[p]) / V;
+    rest += (a.begin[p + 1] - a.begin[p]) % V;
+  }
   for (int n = threadIdx.x; n < rows * a.parts; n += 256) {
-    const int local = n / a.parts, part = n - local * a.parts;
-    const int begin = a.begin[part], size = a.begin[part + 1] - begin;
-    const int64_t row = first + local;
-    of_unit[n] = slopes_of(a, row * a.parts + part, size, (const T *)a.logits + row * a.stride + begin,
-                           a.mask ? a.mask + row * a.mask_stride + begin : nullptr);
+    const int local = n / a.parts, part = n - local * a.parts, begin = a.begin[part];
+    of_unit[n] = slopes_of(a, first * a.parts + n, a.begin[part + 1] - begin, logits + local * a.stride + begin,
+                           masks ? masks + local * a.mask_stride + begin : nullptr);
   }
   __syncthreads();
-  const int per = (a.W + V - 1) / V;
-  for (int n = threadIdx.x; n < rows * per; n += 256) {
-    const int local = n / per, i = (n - local * per) * V;
-    const int64_t row = first + local;
-    float v[V];
-    load_entries((const T *)a.logits + row * a.stride, a.mask ? a.mask + row * a.mask_stride : nullptr, i, a.W, v);
-    int part = 0, begin = 0, end = a.begin[1];
-    for (int p = 1; p < a.parts; ++p)
-      if (i >= a.begin[p]) part = p, begin = a.begin[p], end = a.begin[p + 1];
-    Slopes s = of_unit[local * a.parts + part];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (i + j == end && part + 1 < a.parts) {
-        ++part;
-        begin = end;
-        for (int p = 1; p < a.parts; ++p)
-          if (part == p) end = a.begin[p + 1];
-        s = of_unit[local * a.parts + part];
-      }
-      v[j] = slope(s, v[j], i + j - begin);
+  for (int n = threadIdx.x; n < rows * full; n += 256) {
+    const int local = n / full;
+    const int v = n - local * full;
+    int part = 0, begin = 0, i = 0;  // entry i of the part is entry `begin` of the row
+    for (int p = 0, seen = 0; p < a.parts; ++p) {  // the part that has vector v of the row
+      const int here = (a.begin[p + 1] - a.begin[p]) / V;
+      if (v >= seen && here) part = p, i = (v - seen) * V, begin = a.begin[p] + i;
+      seen += here;
     }
-    store_entries((T *)a.dlogits + row * a.W, i, a.W, v);
+    const Slopes s = of_unit[local * a.parts + part];
+    float x[V];
+    load_entries(logits + local * a.stride + begin, masks ? masks + local * a.mask_stride + begin : nullptr, 0, V, x);
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = slope(s, x[j], i + j);
+    store_entries(out + (int64_t)local * a.W + begin, 0, V, x);
+  }
+  for (int n = threadIdx.x; n < rows * rest; n += 256) {
+    const int local = n / rest;
+    const int v = n - local * rest;
+    int part = 0, at = 0, i = 0;
+    for (int p = 0, seen = 0; p < a.parts; ++p) {
+      const int size = a.begin[p + 1] - a.begin[p], here = size % V;
+      if (v >= seen && here) part = p, i = size - here + v - seen, at = a.begin[p] + i;
+      seen += here;
+    }
+    const Slopes s = of_unit[local * a.parts + part];
+    const float x = entry(logits + local * a.stride, masks ? masks + local * a.mask_stride : nullptr, at);
+    out[(int64_t)local * a.W + at] = (T)slope(s, x, i);
   }
 }
 
@@ -491,7 +508,7 @@ __global__ __launch_bounds__(256) void narrow_backward_kernel(ProbArgs a) {
 // The sum or maximum over a workgroup of WAVES wavefronts.
 template <int WAVES>
 __device__ __forceinline__ float block_sum(float v, float *lds) {
-  v = group_sum(v, 64);
+  v = wave_sum(v);
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
   __syncthreads();
   v = lds[0];
@@ -501,7 +518,7 @@ __device__ __forceinline__ float block_sum(float v, float *lds) {
 }
 template <int WAVES>
 __device__ __forceinline__ float block_max(float v, float *lds) {
-  v = group_max(v, 64);
+  v = lanes_max<kWave>(v);
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
   __syncthreads();
   v = lds[0];
@@ -513,7 +530,7 @@ __device__ __forceinline__ float block_max(float v, float *lds) {
 template <class T>
 __device__ __forceinline__ void store_result(const ProbArgs &a, int64_t unit, int c, const T *x, const uint8_t *mask, const Result &r) {
   a.entropy[unit] = c == -1 ? 0.f : r.entropy;
-  if (a.log_prob) a.log_prob[unit] = chosen(c, x, mask, r);
+  if (a.log_prob) a.log_prob[unit] = log_prob_of(c, c >= 0 && c < INT32_MAX ? entry(x, mask, c) : 0.f, r);
   if (a.stats) {
     a.stats[unit * kStats] = r.most;
     a.stats[unit * kStats + 1] = r.log_z;
@@ -626,7 +643,7 @@ __global__ __launch_bounds__(256) void piece_kernel(ProbArgs a) {
     for (int j = 0; j < V; ++j) lane_max = fmaxf(lane_max, v[k][j]);
   Seen s{block_max<4>(lane_max, lds[0]), 0.f, 0.f};
 #pragma unroll
-  for (int k = 0; k < kVectors; ++k) see(s, v[k]);  // (the maximum is there already)
+  for (int k = 0; k < kVectors; ++k) add(s, v[k]);
   s.z = block_sum<4>(s.z, lds[1]);
   s.s = block_sum<4>(s.s, lds[2]);
   const Result r = result_of(s);
@@ -776,7 +793,7 @@ int64_t share(ProbArgs &a, Each &&each) {
 // have some, and as many as LDS has room for.
 int rows_together(const ProbArgs &a) {
   int n = 1;
-  while (2 * n * a.parts <= kUnits && 2 * n <= 64 && a.R >= 1024 * n) n *= 2;
+  while (2 * n * a.parts <= kUnits && 2 * n <= 64 && a.R >= 4096 * n) n *= 2;
   return n;
 }
 bool some_narrow(const ProbArgs &a) {
