@@ -64,25 +64,30 @@ struct Loose {
 };
 typedef uint8_t LooseMask __attribute__((ext_vector_type(V), aligned(1)));
 
-// V entries of a part in v, -inf for those that are not i .. i + V - 1, beyond it or left out; the first is
-// entry *at. `room` is what there is to read from the part's begin on, to the end of the row: the
-// last lanes of a row start a little before their entries rather than take them one by one.
+// Entries i .. i + V - 1 of a part as they lie in memory, the first of them entry `from` of the part, and a
+// byte for each that is not 0 for those of them that are in the part and allowed. `room` is what there
+// is to read from the part's begin on, to the end of the row: the last lanes of a row start a little
+// before their entries rather than take them one by one.
 template <class T>
-__device__ __forceinline__ void entries(const T *x, const uint8_t *mask, int i, int size, int room, float (&v)[V], int *at) {
-  const int from = min(i, room - V);
-  *at = from;
-  typename Loose<T>::Raw r;
-  LooseMask u;
-  if (i < size) {
-    r = *reinterpret_cast<const typename Loose<T>::Raw *>(x + from);
-    if (mask) u = *reinterpret_cast<const LooseMask *>(mask + from);
+struct Entries {
+  typename Loose<T>::Raw raw;
+  uint64_t allowed;
+  int from;
+  __device__ __forceinline__ void load(const T *x, const uint8_t *mask, int i, int size, int room) {
+    from = min(i, room - V);
+    allowed = 0;
+    if (i < size) {
+      raw = *reinterpret_cast<const typename Loose<T>::Raw *>(x + from);
+      allowed = ~0ull << 8 * (i - from) & ~0ull >> 8 * (V - min(V, size - from));
+      if (mask) allowed &= __builtin_bit_cast(uint64_t, *reinterpret_cast<const LooseMask *>(mask + from));
+    }
   }
+  // -inf for those that are not allowed
+  __device__ __forceinline__ void values(float (&v)[V]) const {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const bool in = from + j >= i && from + j < size && (!mask || u[j]);
-    v[j] = in ? (float)r[j] : -INFINITY;
+    for (int j = 0; j < V; ++j) v[j] = (uint8_t)(allowed >> 8 * j) ? (float)raw[j] : -INFINITY;
   }
-}
+};
 // The same in rows of less than V entries.
 template <class T>
 __device__ __forceinline__ void short_entries(const T *x, const uint8_t *mask, int size, float (&v)[V]) {
@@ -290,27 +295,28 @@ __device__ void narrow_part(const ProbArgs &a, Out &out, int part, int64_t first
     const int64_t unit = (first + local) * a.parts + part;
     const T *x = logits + (in ? local : 0) * a.stride;
     const uint8_t *mask = masks ? masks + (in ? local : 0) * a.mask_stride : nullptr;
-    float v[C][V];
-    int at[C];
+    Entries<T> e[C];
+    const bool tiny = G == 1 && a.W < V;
+    if (!tiny) {
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      at[k] = 0;
-      if (G == 1 && a.W < V)
-        short_entries(x, mask, in ? size : 0, v[k]);
-      else
-        entries(x, mask, (k * G + j) * V, in ? size : 0, a.W - begin, v[k], &at[k]);
+      for (int k = 0; k < C; ++k) e[k].load(x, mask, (k * G + j) * V, in ? size : 0, a.W - begin);
     }
     // (all on their way before the first is waited for)
     const int c = in ? choice_of(a, unit, size) : -1;
     const float x_c = c >= 0 && c < size ? entry(x, mask, c) : -INFINITY;
-    float most = -INFINITY;
+    float v[C][V], most = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < C; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        v[k][i] = c == -1 ? -INFINITY : v[k][i];
-        most = fmaxf(most, v[k][i]);
+    for (int k = 0; k < C; ++k) {
+      if (tiny) {
+        short_entries(x, mask, c == -1 ? 0 : size, v[k]);
+        e[k].from = 0;
+      } else {
+        if (c == -1) e[k].allowed = 0;
+        e[k].values(v[k]);
       }
+#pragma unroll
+      for (int i = 0; i < V; ++i) most = fmaxf(most, v[k][i]);
+    }
     Seen s{lanes_max<G>(most), 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < C; ++k) add(s, v[k]);
@@ -334,7 +340,7 @@ __device__ void narrow_part(const ProbArgs &a, Out &out, int part, int64_t first
         for (int k = 0; k < C; ++k)
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const uint64_t key = gone >> (k * V + i) & 1 ? 0 : key_of(v[k][i], at[k] + i);
+            const uint64_t key = gone >> (k * V + i) & 1 ? 0 : key_of(v[k][i], e[k].from + i);
             which = key > best ? k * V + i : which;
             best = key > best ? key : best;
           }
@@ -413,10 +419,11 @@ __device__ __forceinline__ Slopes slopes_of(const ProbArgs &a, int64_t unit, int
   if (!a.choice) s.c = INT32_MAX;
   return s;
 }
+// dl (1[c = i] - p) - dh p (l + H); an entry that is left out has p = 0, and l = -inf or worse
 __device__ __forceinline__ float slope(const Slopes &s, float x, int i) {
   const float l = x - s.most - s.log_z, p = exp_of(l);
-  const float d = s.dl * ((i == s.c ? 1.f : 0.f) - p) - s.dh * (p > 0.f ? p * (l + s.entropy) : 0.f);
-  return x == -INFINITY || s.c == -1 ? 0.f : d;
+  const float d = (i == s.c ? s.dl : 0.f) - p * fmaf(s.dh, l + s.entropy, s.dl);
+  return x == -INFINITY || s.c == -1 ? 0.f : p == 0.f ? (i == s.c ? s.dl : 0.f) : d;
 }
 
 // Entries i .. i + V - 1 of `size`, -inf for those left out.
