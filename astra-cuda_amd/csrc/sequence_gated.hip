@@ -98,6 +98,12 @@ struct Loader {
     }
   }
 
+  // The operand's contraction from k0 on, `len` at most.
+  static __device__ __forceinline__ void cut(Operand &o, int64_t k0, int64_t len) {
+    o.p = (const T *)o.p + (TR ? k0 * o.ld : k0);
+    o.len = max((int64_t)0, min(len, o.len - k0));
+  }
+
   // Brings the next step into `lds` and moves on; zeros after the last.
   __device__ __forceinline__ void load(char *lds, int wave) {
     constexpr int kMost = TR ? kStepOf<T> : kStep;
@@ -348,7 +354,8 @@ struct GatedArgs {
   void *dab;                 // [M, 2 Fp]: da, db, zero from F to Fp
   int64_t M, F, Fp;
   int32_t kind;
-  int32_t tiles_l, tiles_r, steps;
+  float *part;  // [slices, 2, M, F] or NULL: partial sums of a and b instead of results
+  int32_t slices, tiles_l, tiles_r, steps;  // steps: of a slice
 };
 
 // da and db of 8 elements, n of them inside (zero beyond).
@@ -382,16 +389,23 @@ template <class P, bool GRAD>
 __global__ __launch_bounds__(P::kThreads, P::GROUPS * P::NW / 4) void gated_kernel(GatedArgs g) {
   typedef typename P::type T;
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t tiles = (uint32_t)g.tiles_l * g.tiles_r, slice = blockIdx.x / tiles;
   int tl, tr;
-  tile_of(blockIdx.x, g.tiles_l, g.tiles_r, &tl, &tr);
+  tile_of(blockIdx.x - slice * tiles, g.tiles_l, g.tiles_r, &tl, &tr);
   const int64_t m0 = (int64_t)tr * P::BR, f0 = (int64_t)tl * P::BLL;
+  if (g.slices > 1) {
+    const int64_t len = (int64_t)g.steps * kStepOf<T>, k0 = slice * len;
+    P::Left::cut(g.gate, k0, len);
+    P::Left::cut(g.up, k0, len);
+    P::Right::cut(g.x, k0, len);
+  }
   typename P::Left gate, up;
   typename P::Right x;
   gate.init(g.gate, f0, wave, lane);
   up.init(g.up, f0, wave, lane);
   x.init(g.x, m0, wave, lane);
   f32x4 acc[P::NL][P::NR] = {};
-  P::run(acc, g.steps, LoadHalves<P>{gate, up, x, wave}, wave, lane);
+  P::run(acc, (int)((g.x.len + kStepOf<T> - 1) / kStepOf<T>), LoadHalves<P>{gate, up, x, wave}, wave, lane);
   // results from here on are rows and columns of the tile (less than 2^31 bytes of memory)
   const int rows = (int)min((int64_t)P::BR, g.M - m0), cols = (int)min((int64_t)P::BLL, g.F - f0);
   const int wl = wave % P::WL, wr = wave / P::WL, F = (int)g.F, Fp = (int)g.Fp, zeros = (int)min((int64_t)P::BLL, g.Fp - f0);
@@ -410,6 +424,13 @@ __global__ __launch_bounds__(P::kThreads, P::GROUPS * P::NW / 4) void gated_kern
         b[i] = acc[P::NLL + l + i / 4][r][i % 4];
       }
       const int at = m * F + f;
+      if (g.part) {
+        if (n <= 0) continue;
+        float *part = g.part + (int64_t)slice * 2 * g.M * g.F + start + at;
+        Loose<float, 8>::store(part, a, n);
+        Loose<float, 8>::store(part + g.M * g.F, b, n);
+        continue;
+      }
       if constexpr (GRAD) {
         if (f >= zeros) continue;
         float dh[8], da[8], db[8];
@@ -433,23 +454,42 @@ __global__ __launch_bounds__(P::kThreads, P::GROUPS * P::NW / 4) void gated_kern
   }
 }
 
-// da and db from a and b that the forward call kept: 2^shift threads a row.
-template <class T>
-__global__ __launch_bounds__(256) void gated_slopes_kernel(GatedArgs g, int shift) {
+// The results from a and b that are in memory: sums of slices, or what the forward call kept for the
+// gradient (one slice). 2^shift threads a row.
+template <class T, bool GRAD>
+__global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs g, const float *ab, int shift) {
   const int64_t m = (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
   if (m >= g.M) return;
-  const float *a_row = g.ab + m * g.F, *b_row = a_row + g.M * g.F;
-  const T *dh_row = (const T *)g.dh + m * g.F;
-  T *out = (T *)g.dab + m * 2 * g.Fp;
+  const int64_t size = g.M * g.F, row = m * g.F;
   const int F = (int)g.F, Fp = (int)g.Fp;
-  for (int f = (threadIdx.x & ((1 << shift) - 1)) * 8; f < Fp; f += 8 << shift) {
-    float a[8], b[8], dh[8], da[8], db[8];
-    Loose<float, 8>::load(a_row + f, a, F - f);
-    Loose<float, 8>::load(b_row + f, b, F - f);
-    Loose<T, 8>::load(dh_row + f, dh, F - f);
-    slopes<T>(g, a, b, dh, da, db, F - f);
-    Loose<T, 8>::store(out + f, da, Fp - f);
-    Loose<T, 8>::store(out + Fp + f, db, Fp - f);
+  for (int f = (threadIdx.x & ((1 << shift) - 1)) * 8; f < (GRAD ? Fp : F); f += 8 << shift) {
+    float a[8], b[8];
+    Loose<float, 8>::load(ab + row + f, a, F - f);
+    Loose<float, 8>::load(ab + size + row + f, b, F - f);
+    for (int k = 1; k < g.slices; ++k) {
+      float x[8], y[8];
+      Loose<float, 8>::load(ab + 2 * k * size + row + f, x, F - f);
+      Loose<float, 8>::load(ab + (2 * k + 1) * size + row + f, y, F - f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] += x[i], b[i] += y[i];
+    }
+    if constexpr (GRAD) {
+      float dh[8], da[8], db[8];
+      Loose<T, 8>::load((const T *)g.dh + row + f, dh, F - f);
+      slopes<T>(g, a, b, dh, da, db, F - f);
+      T *out = (T *)g.dab + m * 2 * g.Fp + f;
+      Loose<T, 8>::store(out, da, Fp - f);
+      Loose<T, 8>::store(out + Fp, db, Fp - f);
+    } else {
+      float h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = act<T>(a[i], g.kind) * b[i];
+      Loose<T, 8>::store((T *)g.h + row + f, h, F - f);
+      if (g.ab) {
+        Loose<float, 8>::store(g.ab + row + f, a, F - f);
+        Loose<float, 8>::store(g.ab + size + row + f, b, F - f);
+      }
+    }
   }
 }
 
@@ -488,11 +528,8 @@ __global__ __launch_bounds__(P::kThreads, P::GROUPS * P::NW / 4) void product_ke
   for (int pair = 0; pair < g.pairs; ++pair) {
     Operand lo = g.left[pair], ro = g.right[pair];
     if (g.slices > 1) {
-      const int64_t k0 = (int64_t)slice * g.steps * kStepOf<T>;
-      // (only operands across the contraction are cut)
-      lo.p = (const T *)lo.p + k0 * lo.ld;
-      ro.p = (const T *)ro.p + k0 * ro.ld;
-      lo.len = ro.len = max((int64_t)0, min((int64_t)g.steps * kStepOf<T>, lo.len - k0));
+      P::Left::cut(lo, (int64_t)slice * g.steps * kStepOf<T>, (int64_t)g.steps * kStepOf<T>);
+      P::Right::cut(ro, (int64_t)slice * g.steps * kStepOf<T>, (int64_t)g.steps * kStepOf<T>);
     }
     const int steps = (int)((lo.len + kStepOf<T> - 1) / kStepOf<T>);
     typename P::Left left;
@@ -794,22 +831,53 @@ bool larger(int64_t nl, int64_t nr, int64_t len) {
     ASTRA_HIP_CHECK(rt_last_error(), #kernel " launch");                                             \
   } while (false)
 
+// Slices of a contraction of `steps` steps for `n` tiles of which the CUs hold `room` at a time: more of
+// them where there are less tiles than CUs, with 8 steps at least.
+int64_t slices_for(int64_t n, int64_t room, int64_t steps) {
+  if (n < 1 || n >= kCus) return 1;
+  const int64_t want = cdiv(room, n), most = steps / 8;
+  return want < most ? want : most > 1 ? most : 1;
+}
+
+template <class T, bool GRAD>
+int launch_join(GatedArgs g, const float *ab, hipStream_t st) {
+  int shift = 4;
+  while (shift < 8 && (int64_t(8) << shift) < g.F) ++shift;
+  GATED_LAUNCH((gated_join_kernel<T, GRAD>), cdiv(g.M, 256 >> shift), 256, g, ab, shift);
+  return ASTRA_OK;
+}
+
 template <class P, bool GRAD>
 int launch_gated_tiles(GatedArgs g, hipStream_t st) {
   const int64_t F = GRAD ? g.Fp : g.F;
-  const int64_t n = tiles<P>(F, g.M);
+  const int64_t n = tiles<P>(F, g.M) * g.slices;
   ASTRA_ABI_CHECK(n, <, 2147483648ll);
   g.tiles_l = (int32_t)cdiv(F, P::BLL);
   g.tiles_r = (int32_t)cdiv(g.M, P::BR);
-  g.steps = (int32_t)cdiv(g.x.len, kStepOf<typename P::type>);
+  g.steps = (int32_t)cdiv(cdiv(g.x.len, kStepOf<typename P::type>), g.slices);
+  if (g.slices == 1) g.part = nullptr;
   GATED_LAUNCH((gated_kernel<P, GRAD>), n, P::kThreads, g);
-  return ASTRA_OK;
+  return g.slices > 1 ? launch_join<typename P::type, GRAD>(g, g.part, st) : ASTRA_OK;
 }
+template <class T>
+int64_t gated_slices(int64_t M, int64_t F, int64_t D) {
+  typedef Small<T, false, false, true> S;
+  return slices_for(tiles<S>(F, M), kCus * S::GROUPS, cdiv(D, kStepOf<T>));
+}
+// `part` has room for the slices
 template <class T, bool GRAD>
-int launch_gated(const GatedArgs &g, hipStream_t st) {
+int launch_gated(GatedArgs &g, void *part, hipStream_t st) {
   typedef Large<T, false, false, true> L;
   typedef Small<T, false, false, true> S;
-  return larger<L, S>(GRAD ? g.Fp : g.F, g.M, g.x.len) ? launch_gated_tiles<L, GRAD>(g, st) : launch_gated_tiles<S, GRAD>(g, st);
+  g.slices = (int32_t)gated_slices<T>(g.M, g.F, g.x.len);
+  g.part = (float *)part;
+  return g.slices == 1 && larger<L, S>(GRAD ? g.Fp : g.F, g.M, g.x.len) ? launch_gated_tiles<L, GRAD>(g, st)
+                                                                       : launch_gated_tiles<S, GRAD>(g, st);
+}
+template <class T>
+size_t gated_part_bytes(const astra_gated_linear &f) {
+  const int64_t s = gated_slices<T>(f.rows, f.hidden, round_up(f.width, per16(f.type)));
+  return s > 1 ? (size_t)(s * 2 * f.rows * f.hidden) * sizeof(float) : 0;
 }
 
 // Two tiles a workgroup, which read x half as often, and eight wavefronts, where the weights are
@@ -838,25 +906,30 @@ int forward(const astra_gated_linear &f, hipStream_t st) {
     g.up = {f.up, f.up_stride, f.hidden, f.width};
     return launch_few<T>(g, st);
   }
-  const size_t need = copies_bytes(f);
+  const size_t need = copies_bytes(f) + gated_part_bytes<T>(f);
   if (need) ASTRA_SEQ_POINTER(f.workspace);
   ASTRA_ABI_CHECK(f.workspace_bytes, >=, need);
+  if (need && !aligned(f.workspace, 16)) return fail(ASTRA_ERR_INVALID_ARGUMENT, "astra_gated_linear_forward: the workspace starts on 16 bytes");
   char *ws = (char *)f.workspace;
   const Operands o = operands<T>(f, &ws, st);
   ASTRA_HIP_CHECK(rt_last_error(), "align_kernel launch");
   g.x = o.x;
   g.gate = o.gate;
   g.up = o.up;
-  return launch_gated<T, false>(g, st);
+  return launch_gated<T, false>(g, ws, st);
 }
 
 template <class P>
-int launch_product(ProductArgs &g, hipStream_t st) {
+int launch_product(ProductArgs &g, void *part, hipStream_t st) {
+  typedef typename P::type T;
   const int64_t n = tiles<P>(g.nl, g.nr) * g.slices;
   ASTRA_ABI_CHECK(n, <, 2147483648ll);
   g.tiles_l = (int32_t)cdiv(g.nl, P::BL);
   g.tiles_r = (int32_t)cdiv(g.nr, P::BR);
+  g.steps = (int32_t)cdiv(cdiv(g.left[0].len, kStepOf<T>), g.slices);
+  g.part = g.slices > 1 ? (float *)part : nullptr;
   GATED_LAUNCH(product_kernel<P>, n, P::kThreads, g);
+  if (g.part) GATED_LAUNCH(join_slices_kernel<T>, cdiv(g.nr * cdiv(g.nl, 4), 256), 256, g);
   return ASTRA_OK;
 }
 
@@ -876,18 +949,28 @@ Slices slices_of(const astra_gated_linear &f) {
   const int64_t most = cdiv(f.rows, kStepOf<T>) / 8;
   return {alone, want < most ? want : most > 1 ? most : 1};
 }
-template <class T>
-size_t part_bytes(const astra_gated_linear &f) {
-  const int64_t s = slices_of<T>(f).n;
-  return s > 1 ? (size_t)(s * 2 * padded_hidden(f) * f.width) * sizeof(float) : 0;
-}
-
 // With many rows the weights are turned for the inputs' gradient: products along the contraction are
 // a fifth faster, which 4,096 rows make more than the turning takes.
 bool turned(const astra_gated_linear &f) { return f.rows >= 4096; }
 template <class T>
 size_t turned_bytes(const astra_gated_linear &f) {
   return turned(f) ? (size_t)round_up(f.width * 2 * padded_hidden(f), 16) * sizeof(T) : 0;
+}
+
+// Slices of the inputs' gradient's contraction: of twice the hidden width if turned, else of each half.
+template <class T>
+int64_t dx_slices(const astra_gated_linear &f) {
+  typedef Small<T, false, false, false> S;
+  return slices_for(tiles<S>(f.width, f.rows), kCus * S::GROUPS, cdiv(padded_hidden(f) * (turned(f) ? 2 : 1), kStepOf<T>));
+}
+// What the slices of one product after the other need.
+template <class T>
+size_t part_bytes(const astra_gated_linear &f) {
+  const int64_t w = slices_of<T>(f).n, x = dx_slices<T>(f);
+  const size_t of_w = w > 1 ? (size_t)(w * 2 * padded_hidden(f) * f.width) * sizeof(float) : 0;
+  const size_t of_x = x > 1 ? (size_t)(x * f.rows * f.width) * sizeof(float) : 0;
+  const size_t of_h = f.projections ? 0 : gated_part_bytes<T>(f);
+  return std::max(std::max(of_w, of_x), of_h);
 }
 
 template <class T>
@@ -913,29 +996,27 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
   g.x = o.x;
   g.gate = o.gate;
   g.up = o.up;
-  if (f.rows && f.projections) {
-    int shift = 4;
-    while (shift < 8 && (int64_t(8) << shift) < Fp) ++shift;
-    GATED_LAUNCH(gated_slopes_kernel<T>, cdiv(f.rows, 256 >> shift), 256, g, shift);
-  } else if (f.rows) {
-    if (int rc = launch_gated<T, true>(g, st)) return rc;
+  char *const turn = ws, *const part = ws + turned_bytes<T>(f);
+  if (f.rows) {
+    g.slices = 1;
+    if (int rc = f.projections ? launch_join<T, true>(g, f.projections, st) : launch_gated<T, true>(g, part, st)) return rc;
   }
   if (b.dx && f.rows) {  // da Wg + db Wu
     ProductArgs p{};
     p.out[0] = b.dx;
     p.out_ld = p.nl = f.width;
     p.nr = p.split = p.rows = f.rows;
-    p.slices = 1;
+    p.slices = (int32_t)dx_slices<T>(f);
     if (turned(f)) {
       const dim3 grid((unsigned)cdiv(Fp, kTurn), (unsigned)cdiv(f.width, kTurn), 2);
-      hipLaunchKernelGGL(turn_kernel<T>, grid, dim3(256), 0, st, o.gate, o.up, (T *)ws, (int64_t)f.width, (int64_t)f.hidden, Fp);
+      hipLaunchKernelGGL(turn_kernel<T>, grid, dim3(256), 0, st, o.gate, o.up, (T *)turn, (int64_t)f.width, (int64_t)f.hidden, Fp);
       ASTRA_HIP_CHECK(rt_last_error(), "turn_kernel launch");
       p.pairs = 1;
-      p.left[0] = {ws, 2 * Fp, f.width, 2 * Fp};
+      p.left[0] = {turn, 2 * Fp, f.width, 2 * Fp};
       p.right[0] = {g.dab, 2 * Fp, f.rows, 2 * Fp};
       typedef Large<T, false, false, false> L;
       typedef Small<T, false, false, false> S;
-      if (int rc = larger<L, S>(p.nl, p.nr, 2 * Fp) ? launch_product<L>(p, st) : launch_product<S>(p, st)) return rc;
+      if (int rc = p.slices == 1 && larger<L, S>(p.nl, p.nr, 2 * Fp) ? launch_product<L>(p, part, st) : launch_product<S>(p, part, st)) return rc;
     } else {
       p.pairs = 2;
       for (int i = 0; i < 2; ++i) {
@@ -943,10 +1024,9 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
         p.left[i] = {w.p, w.ld, Dp, f.hidden};  // lines: columns of the weight
         p.right[i] = {(const T *)g.dab + i * Fp, 2 * Fp, f.rows, Fp};
       }
-      if (int rc = launch_product<Small<T, true, false, false>>(p, st)) return rc;
+      if (int rc = launch_product<Small<T, true, false, false>>(p, part, st)) return rc;
     }
   }
-  ws += turned_bytes<T>(f);
   if (b.dgate || b.dup) {
     const Slices s = slices_of<T>(f);
     ProductArgs p{};
@@ -961,16 +1041,13 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
     p.split = Fp;
     p.rows = f.hidden;
     p.slices = (int32_t)s.n;
-    p.part = s.n > 1 ? (float *)ws : nullptr;
-    p.steps = (int32_t)cdiv(cdiv(f.rows, kStepOf<T>), s.n);
     int rc = ASTRA_OK;
     if constexpr (sizeof(T) == 2) {
-      rc = s.alone ? launch_product<Alone>(p, st) : launch_product<Small<T, true, true, false>>(p, st);
+      rc = s.alone ? launch_product<Alone>(p, part, st) : launch_product<Small<T, true, true, false>>(p, part, st);
     } else {
-      rc = launch_product<Small<T, true, true, false>>(p, st);
+      rc = launch_product<Small<T, true, true, false>>(p, part, st);
     }
     if (rc) return rc;
-    if (p.part) GATED_LAUNCH(join_slices_kernel<T>, cdiv(p.nr * cdiv(p.nl, 4), 256), 256, p);
   }
   return ASTRA_OK;
 }
@@ -985,7 +1062,7 @@ extern "C" {
 int astra_gated_linear_workspace_size(const astra_gated_linear *f, size_t *bytes) {
   if (int rc = check(f)) return rc;
   ASTRA_SEQ_POINTER(bytes);
-  *bytes = few(*f) ? 0 : copies_bytes(*f);
+  *bytes = few(*f) ? 0 : copies_bytes(*f) + (f->type == ASTRA_SEQ_F32 ? gated_part_bytes<float>(*f) : gated_part_bytes<bf16>(*f));
   return ASTRA_OK;
 }
 
