@@ -645,11 +645,11 @@ __device__ __forceinline__ void store4(T *p, const f32x4 &x, int n) {
 }
 
 // Up to 16 MT rows of x: the weights are read once, each by the lanes that multiply with it, and
-// nothing is staged. A workgroup has NT tiles of 16 columns of the result, its NW wavefronts share the
+// nothing is staged. A workgroup has NT tiles of 16 columns of the result, its wavefronts share the
 // contraction; what the next step needs is on its way while the last is multiplied.
-template <class T, int MT, int NT, int NW>
-__global__ __launch_bounds__(64 * NW) void gated_few_kernel(GatedArgs g) {
-  constexpr int V = 16 / sizeof(T), kStepE = kStepOf<T>;
+template <class T, int MT, int NT>
+__global__ __launch_bounds__(256) void gated_few_kernel(GatedArgs g) {
+  constexpr int V = 16 / sizeof(T), kStepE = kStepOf<T>, NW = 4;
   __shared__ f32x4 sums[NW][NT * 2 * MT][64];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int i = lane % 16, q = lane / 16, K = (int)g.x.len;
@@ -880,21 +880,22 @@ size_t gated_part_bytes(const astra_gated_linear &f) {
   return s > 1 ? (size_t)(s * 2 * f.rows * f.hidden) * sizeof(float) : 0;
 }
 
-// Two tiles a workgroup, which read x half as often, and eight wavefronts, where the weights are
-// large enough to keep all CUs busy with them.
-template <class T, int MT>
-int launch_few_rows(const GatedArgs &g, hipStream_t st) {
-  if (g.F >= 32 * kCus && g.x.len >= 2048)
-    GATED_LAUNCH((gated_few_kernel<T, MT, 2, 8>), cdiv(g.F, 32), 512, g);
-  else
-    GATED_LAUNCH((gated_few_kernel<T, MT, 1, 4>), cdiv(g.F, 16), 256, g);
-  return ASTRA_OK;
-}
+// More than 16 rows are read half as often by two tiles a workgroup, which is worth it where the weights
+// are large enough to keep all CUs busy all the same.
 template <class T>
 int launch_few(const GatedArgs &g, hipStream_t st) {
-  if (g.M <= 16) return launch_few_rows<T, 1>(g, st);
-  if (g.M <= 32) return launch_few_rows<T, 2>(g, st);
-  return launch_few_rows<T, 4>(g, st);
+  const bool two = g.F >= 32 * kCus && g.x.len >= 2048;
+  if (g.M <= 16)
+    GATED_LAUNCH((gated_few_kernel<T, 1, 1>), cdiv(g.F, 16), 256, g);
+  else if (g.M <= 32 && two)
+    GATED_LAUNCH((gated_few_kernel<T, 2, 2>), cdiv(g.F, 32), 256, g);
+  else if (g.M <= 32)
+    GATED_LAUNCH((gated_few_kernel<T, 2, 1>), cdiv(g.F, 16), 256, g);
+  else if (two)
+    GATED_LAUNCH((gated_few_kernel<T, 4, 2>), cdiv(g.F, 32), 256, g);
+  else
+    GATED_LAUNCH((gated_few_kernel<T, 4, 1>), cdiv(g.F, 16), 256, g);
+  return ASTRA_OK;
 }
 
 template <class T>
