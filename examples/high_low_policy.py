@@ -4,11 +4,14 @@ whole games.
     python examples/high_low_policy.py --envs 256 --updates 3
 
 Every seat of every env is one row of the batch. Each block is ``join_norm`` -> projection ->
-``short_conv`` -> ``state_scan`` -> projection. While games are played, the blocks'
+``short_conv`` -> ``state_scan`` -> projection, and a feed-forward block follows it:
+``join_norm`` -> ``gated_linear`` -> projection. ``log_probs`` gives the log probabilities of
+the four parts of a move and their entropies. While games are played, the blocks'
 convolution windows and scan states are carried from move to move (``short_conv_step``,
 ``state_scan_step``); the update runs the same weights over the recorded observations at
 once, and its log probabilities start out as those the moves were drawn from. The update is
-plain policy gradient on the rewards since a seat's last action, with a baseline.
+plain policy gradient on the rewards since a seat's last action, with a baseline and a bonus
+for entropy.
 """
 import argparse
 import math
@@ -73,24 +76,41 @@ class Block(nn.Module):
         return self.out(y.flatten(-2)), gate
 
 
+class FeedForward(nn.Module):
+    """Width D to the hidden width F and back, position by position."""
+
+    def __init__(self, D, F):
+        super().__init__()
+        self.gate_weight = nn.Parameter(torch.randn(F, D) / math.sqrt(D))
+        self.up_weight = nn.Parameter(torch.randn(F, D) / math.sqrt(D))
+        self.out = nn.Linear(F, D, bias=False)
+        self.post_weight = nn.Parameter(torch.ones(D))
+        self.scale = nn.Parameter(torch.full((D,), 0.5))
+
+    def forward(self, n):
+        return self.out(seq.gated_linear(n, self.gate_weight, self.up_weight))
+
+
 class Policy(nn.Module):
     """Observation -> logits of the four parts of a move (bid and ask price, bid and ask size)."""
 
-    def __init__(self, observation, max_value, max_trade, D=128, blocks=2, H=4, P=32, N=32):
+    def __init__(self, observation, max_value, max_trade, D=128, blocks=2, H=4, P=32, N=32, F=None):
         super().__init__()
         self.sizes = [max_value, max_value, max_trade + 1, max_trade + 1]
         self.embed = nn.Linear(observation, D)
-        self.norms = nn.ParameterList([nn.Parameter(torch.ones(D)) for _ in range(blocks + 1)])
+        self.norms = nn.ParameterList([nn.Parameter(torch.ones(D)) for _ in range(2 * blocks + 1)])
         self.blocks = nn.ModuleList([Block(D, H, P, N) for _ in range(blocks)])
+        self.forwards = nn.ModuleList([FeedForward(D, F or 2 * D) for _ in range(blocks)])
         self.head = nn.Linear(D, sum(self.sizes))
 
     def _run(self, observation, mix):
         r = self.embed(observation)
         n = seq.rms_norm(r, self.norms[0])
-        for i, block in enumerate(self.blocks):
+        for i, (block, forward) in enumerate(zip(self.blocks, self.forwards)):
             u, gate = mix(i, block, n)
-            r, n = seq.join_norm(r, u, block.post_weight, self.norms[i + 1], gate=gate, scale=block.scale)
-        return self.head(n).split(self.sizes, dim=-1)
+            r, n = seq.join_norm(r, u, block.post_weight, self.norms[2 * i + 1], gate=gate, scale=block.scale)
+            r, n = seq.join_norm(r, forward(n), forward.post_weight, self.norms[2 * i + 2], scale=forward.scale)
+        return Moves(self.head(n), self.sizes)
 
     def forward(self, observations):
         """[batch, length, observation]."""
@@ -104,10 +124,26 @@ class Policy(nn.Module):
         return [b.new_state(batch, device, dtype) for b in self.blocks]
 
 
-def log_prob(logits, choice):
+class Moves:
+    """What a policy would do: logits [..., entries] of a move's parts, one behind the other."""
+
+    def __init__(self, logits, sizes):
+        self.logits, self.sizes = logits, sizes
+
+    def draw(self, generator):
+        """An entry of each part [batch, 4]."""
+        return torch.stack([torch.multinomial(torch.softmax(part, -1), 1, generator=generator).squeeze(1)
+                            for part in self.logits.split(self.sizes, dim=-1)], -1)
+
+    def judge(self, choice):
+        """Log probability and entropy of moves [..., 4], each the sum over their parts."""
+        log_prob, entropy = seq.log_probs(self.logits, choice, sizes=self.sizes)
+        return log_prob.sum(-1), entropy.sum(-1)
+
+
+def log_prob(moves, choice):
     """Sum over the parts of a move of the log probability of its choice [..., 4]."""
-    return sum(torch.log_softmax(part, -1).gather(-1, choice[..., i:i + 1]).squeeze(-1)
-               for i, part in enumerate(logits))
+    return moves.judge(choice)[0]
 
 
 def deal(game, generator, device):
@@ -146,11 +182,10 @@ def play(game, policy, generator, device):
                     state.fill_rewards_since_last_action(since, seat)
                     reward[:, seat, t - 1] = since
                 state.fill_observation_tensor(seen)
-                logits = policy.step(seen, states[seat])
-                choice = torch.stack([torch.multinomial(torch.softmax(part, -1), 1, generator=generator).squeeze(1)
-                                      for part in logits], -1)
+                moves = policy.step(seen, states[seat])
+                choice = moves.draw(generator)
                 obs[:, seat, t], choices[:, seat, t] = seen, choice
-                logp[:, seat, t] = log_prob(logits, choice)
+                logp[:, seat, t] = log_prob(moves, choice)
                 prices = choice[:, :2] + 1
                 state.apply_action(torch.cat([prices, choice[:, 2:]], -1).to(torch.int32).contiguous())
         final = torch.empty(n, players, device=device)
@@ -164,11 +199,11 @@ def update(policy, optimizer, obs, choices, reward):
     """One step of policy gradient over whole games; returns the loss and the new pass's log
     probabilities."""
     n, players, rounds, width = obs.shape
-    logits = policy(obs.reshape(n * players, rounds, width))
-    logp = log_prob(logits, choices.reshape(n * players, rounds, 4)).view(n, players, rounds)
+    moves = policy(obs.reshape(n * players, rounds, width))
+    logp, entropy = (v.view(n, players, rounds) for v in moves.judge(choices.reshape(n * players, rounds, 4)))
     togo = reward.flip(-1).cumsum(-1).flip(-1)
     advantage = (togo - togo.mean((0, 1))) / (togo.std() + 1e-6)
-    loss = -(advantage * logp).mean()
+    loss = -(advantage * logp + 0.01 * entropy).mean()
     optimizer.zero_grad(set_to_none=True)
     loss.backward()
     optimizer.step()
