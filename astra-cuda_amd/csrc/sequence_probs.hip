@@ -419,11 +419,12 @@ __device__ __forceinline__ Slopes slopes_of(const ProbArgs &a, int64_t unit, int
   if (!a.choice) s.c = INT32_MAX;
   return s;
 }
-// dl (1[c = i] - p) - dh p (l + H); an entry that is left out has p = 0, and l = -inf or worse
+// dl (1[c = i] - p) - dh p (l + H). (Far below the maximum p is zero before l + H is -1000, and l may
+// be -inf, which times zero would be NaN.)
 __device__ __forceinline__ float slope(const Slopes &s, float x, int i) {
   const float l = x - s.most - s.log_z, p = exp_of(l);
-  const float d = (i == s.c ? s.dl : 0.f) - p * fmaf(s.dh, l + s.entropy, s.dl);
-  return x == -INFINITY || s.c == -1 ? 0.f : p == 0.f ? (i == s.c ? s.dl : 0.f) : d;
+  const float d = (i == s.c ? s.dl : 0.f) - p * fmaf(s.dh, fmaxf(l + s.entropy, -1000.f), s.dl);
+  return x == -INFINITY || s.c == -1 ? 0.f : d;
 }
 
 // Entries i .. i + V - 1 of `size`, -inf for those left out.
@@ -457,6 +458,10 @@ __device__ __forceinline__ void store_entries(T *d, int i, int size, const float
   }
 }
 
+// n / d for quotients of up to 64 and d of up to 2^11: (n + 0.5) / d is at least 2^-12 away from every
+// whole number, and three roundings of 64 are 2^-16.
+__device__ __forceinline__ int quotient(int n, float inv_d) { return (int)(((float)n + 0.5f) * inv_d); }
+
 // A workgroup has block_rows rows, and what their parts' gradients need in LDS: first V entries of a part
 // to a lane, then the last size % V entries of the parts, one to a lane: neighbours in memory are
 // neighbours among the lanes.
@@ -473,15 +478,15 @@ __global__ __launch_bounds__(256) void narrow_backward_kernel(ProbArgs a) {
     full += (a.begin[p + 1] - a.begin[p]) / V;
     rest += (a.begin[p + 1] - a.begin[p]) % V;
   }
+  const float inv_parts = 1.f / a.parts, inv_full = full ? 1.f / full : 0.f, inv_rest = rest ? 1.f / rest : 0.f;
   for (int n = threadIdx.x; n < rows * a.parts; n += 256) {
-    const int local = n / a.parts, part = n - local * a.parts, begin = a.begin[part];
+    const int local = quotient(n, inv_parts), part = n - local * a.parts, begin = a.begin[part];
     of_unit[n] = slopes_of(a, first * a.parts + n, a.begin[part + 1] - begin, logits + local * a.stride + begin,
                            masks ? masks + local * a.mask_stride + begin : nullptr);
   }
   __syncthreads();
   for (int n = threadIdx.x; n < rows * full; n += 256) {
-    const int local = n / full;
-    const int v = n - local * full;
+    const int local = quotient(n, inv_full), v = n - local * full;
     int part = 0, begin = 0, i = 0;  // entry i of the part is entry `begin` of the row
     for (int p = 0, seen = 0; p < a.parts; ++p) {  // the part that has vector v of the row
       const int here = (a.begin[p + 1] - a.begin[p]) / V;
@@ -496,8 +501,7 @@ __global__ __launch_bounds__(256) void narrow_backward_kernel(ProbArgs a) {
     store_entries(out + (int64_t)local * a.W + begin, 0, V, x);
   }
   for (int n = threadIdx.x; n < rows * rest; n += 256) {
-    const int local = n / rest;
-    const int v = n - local * rest;
+    const int local = quotient(n, inv_rest), v = n - local * rest;
     int part = 0, at = 0, i = 0;
     for (int p = 0, seen = 0; p < a.parts; ++p) {
       const int size = a.begin[p + 1] - a.begin[p], here = size % V;
@@ -581,6 +585,7 @@ __device__ __forceinline__ uint64_t largest_of(const float (&v)[kVectors][V], in
   uint32_t bound = (uint32_t)(key_of(lane_max, 0) >> 32);
   sort(bound, lane);
   bound = __builtin_amdgcn_readlane(bound, top - 1);
+  const float least = bound ? value_of((uint64_t)bound << 32) : -INFINITY;
   uint64_t best = 0, last = 0;
   int have = 0;
   const auto take = [&](int n) __attribute__((always_inline)) {
@@ -598,8 +603,9 @@ __device__ __forceinline__ uint64_t largest_of(const float (&v)[kVectors][V], in
   for (int c = 0; c < kVectors; ++c)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+      if (!__ballot(v[c][j] >= least)) continue;
       const uint64_t key = key_of(v[c][j], first + (c * 256 + (int)threadIdx.x) * V + j);
-      const bool in = key > last && (uint32_t)(key >> 32) >= bound;
+      const bool in = key > last && v[c][j] >= least;
       const uint64_t who = __ballot(in);
       if (!who) continue;
       if (in) gather[have + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
