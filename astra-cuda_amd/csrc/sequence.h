@@ -165,6 +165,10 @@ inline bool aligned(const void *p, int64_t bytes) { return reinterpret_cast<uint
 
 constexpr int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Threads of a launch along one dimension: 32 bits count them, and what is beyond is dropped without an
+// error.
+constexpr int64_t kMostThreads = 4294967295ll;
+
 inline size_t elem_size(int32_t type) { return type == ASTRA_SEQ_BF16 ? 2 : 4; }
 
 }  // namespace astra_seq

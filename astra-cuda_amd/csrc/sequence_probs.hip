@@ -10,6 +10,7 @@
 // traffic where there are many, by latency where there are few. One pass: a thread keeps the
 // maximum, Z and the entropy's sum of what it has seen, and scales both when the maximum moves.
 // Sums are float32; m and log Z are kept apart, so that l is as exact as x is.
+#include <algorithm>
 #include <type_traits>
 
 #include "sequence.h"
@@ -37,6 +38,7 @@ struct ProbArgs {
   uint64_t *lists;     // and its largest entries
   int64_t R, stride, mask_stride;
   int32_t W, parts, top, wide_choice;
+  bool cut;                    // whether larger parts go through in pieces
   int32_t block_rows;          // rows of a workgroup that has all their parts
   int32_t begin[kParts + 1];   // of each part in a row
   int64_t block[kParts + 1];   // the first workgroup of each part in this launch
@@ -781,6 +783,7 @@ ProbArgs args_of(const astra_log_probs &f) {
   a.mask_stride = f.mask_stride;
   a.parts = f.parts;
   a.top = f.top;
+  a.cut = f.top > 0 || f.rows * f.parts < 512;
   a.wide_choice = f.choice_bytes == 8;
   for (int i = 0; i < f.parts; ++i) a.begin[i + 1] = a.begin[i] + f.sizes[i];
   a.W = a.begin[f.parts];
@@ -820,9 +823,7 @@ bool some_wide(const ProbArgs &a) {
   return false;
 }
 
-// Larger parts are cut into pieces where there are few rows or the largest entries are wanted.
-bool in_pieces(const ProbArgs &a) { return a.top > 0 || a.R * a.parts < 512; }
-int64_t all_pieces(ProbArgs &a) {
+int64_t all_pieces(ProbArgs &a) {  // (of the rows of a launch)
   return share(a, [&](int size) { return a.R * pieces_of(size); });
 }
 bool joins(const ProbArgs &a) {
@@ -830,15 +831,43 @@ bool joins(const ProbArgs &a) {
     if (pieces_of(a.begin[i + 1] - a.begin[i]) > 1) return true;
   return false;
 }
+// Rows that one launch of each kernel has room for: at most 1,024 threads a row, and 256 a span or piece.
+int64_t most_rows(const ProbArgs &a) {
+  int64_t blocks = 4;
+  for (int i = 0; i < a.parts; ++i) blocks += cdiv(a.begin[i + 1] - a.begin[i], kSpan);
+  return kMostThreads / (256 * blocks);
+}
+// `n` of the rows, from `first` on
+ProbArgs rows_of(ProbArgs a, int32_t type, int64_t first, int64_t n) {
+  const auto on = [&](auto &p, int64_t bytes_a_row) {
+    if (p) p = (std::decay_t<decltype(p)>)((uintptr_t)p + (uintptr_t)(first * bytes_a_row));
+  };
+  const int64_t e = (int64_t)elem_size(type), each = a.parts * (int64_t)sizeof(float);
+  on(a.logits, a.stride * e);
+  on(a.mask, a.mask_stride);
+  on(a.choice, a.parts * (a.wide_choice ? 8 : 4));
+  on(a.log_prob, each);
+  on(a.entropy, each);
+  on(a.stats, each * kStats);
+  on(a.top_log_prob, each * a.top);
+  on(a.top_index, a.parts * a.top * (int64_t)sizeof(int64_t));
+  on(a.dlog_prob, each);
+  on(a.dentropy, each);
+  on(a.dlogits, a.W * e);
+  a.R = n;
+  return a;
+}
+
 // the lists first, which are of 8 bytes
 size_t piece_bytes(ProbArgs a) {
-  return in_pieces(a) && joins(a) ? (size_t)all_pieces(a) * (3 * sizeof(float) + a.top * sizeof(uint64_t)) : 0;
+  a.R = std::min(a.R, most_rows(a));
+  return a.cut && joins(a) ? (size_t)all_pieces(a) * (3 * sizeof(float) + a.top * sizeof(uint64_t)) : 0;
 }
 
 #define PROBS_LAUNCH(kernel, blocks, threads)                                                          \
   do {                                                                                                 \
     const int64_t blocks_ = (blocks);                                                                  \
-    ASTRA_ABI_CHECK(blocks_, <, 2147483648ll);                                                         \
+    ASTRA_ABI_CHECK(blocks_ * threads, <=, kMostThreads);                                              \
     hipLaunchKernelGGL((kernel), dim3((unsigned)blocks_), dim3(threads), 0, st, a);                    \
     ASTRA_HIP_CHECK(rt_last_error(), #kernel " launch");                                               \
   } while (false)
@@ -847,7 +876,7 @@ template <class T, bool TOP>
 int forward_in_pieces(ProbArgs &a, hipStream_t st) {
   PROBS_LAUNCH((piece_kernel<T, TOP>), all_pieces(a), 256);
   if (!joins(a)) return ASTRA_OK;
-  ASTRA_ABI_CHECK(a.R, <, 2147483648ll);
+  ASTRA_ABI_CHECK(a.R * 64 * kJoinWaves, <=, kMostThreads);
   hipLaunchKernelGGL((join_pieces_kernel<T, TOP>), dim3((unsigned)a.R, (unsigned)a.parts), dim3(64 * kJoinWaves), 0, st, a);
   ASTRA_HIP_CHECK(rt_last_error(), "join_pieces_kernel launch");
   return ASTRA_OK;
@@ -855,6 +884,7 @@ int forward_in_pieces(ProbArgs &a, hipStream_t st) {
 
 template <class T>
 int forward(ProbArgs a, hipStream_t st) {
+  if (a.lists) a.pieces = (float *)(a.lists + all_pieces(a) * a.top);
   if (some_narrow(a)) {
     a.block_rows = rows_together(a);
     if (a.top) {
@@ -864,7 +894,7 @@ int forward(ProbArgs a, hipStream_t st) {
     }
   }
   if (!some_wide(a)) return ASTRA_OK;
-  if (in_pieces(a)) return a.top ? forward_in_pieces<T, true>(a, st) : forward_in_pieces<T, false>(a, st);
+  if (a.cut) return a.top ? forward_in_pieces<T, true>(a, st) : forward_in_pieces<T, false>(a, st);
   PROBS_LAUNCH(wide_forward_kernel<T>, share(a, [&](int) { return a.R; }), 256);
   return ASTRA_OK;
 }
@@ -912,7 +942,6 @@ int astra_log_probs_forward(const astra_log_probs *f, void *stream) {
     ASTRA_ABI_CHECK(f->workspace_bytes, >=, need);
     if (!aligned(f->workspace, 8)) return fail(ASTRA_ERR_INVALID_ARGUMENT, "astra_log_probs_forward: the workspace starts on 8 bytes");
     a.lists = (uint64_t *)f->workspace;
-    a.pieces = (float *)(a.lists + all_pieces(a) * a.top);
   }
   if (f->choice) ASTRA_SEQ_POINTER(f->log_prob);
   if (f->log_prob) ASTRA_SEQ_POINTER(f->choice);
@@ -920,7 +949,11 @@ int astra_log_probs_forward(const astra_log_probs *f, void *stream) {
     ASTRA_SEQ_POINTER(f->top_log_prob);
     ASTRA_SEQ_POINTER(f->top_index);
   }
-  return f->type == ASTRA_SEQ_F32 ? forward<float>(a, as_stream(stream)) : forward<bf16>(a, as_stream(stream));
+  for (int64_t r = 0, most = most_rows(a); r < f->rows; r += most) {
+    const ProbArgs some = rows_of(a, f->type, r, std::min(most, f->rows - r));
+    if (int rc = f->type == ASTRA_SEQ_F32 ? forward<float>(some, as_stream(stream)) : forward<bf16>(some, as_stream(stream))) return rc;
+  }
+  return ASTRA_OK;
 }
 
 int astra_log_probs_backward(const astra_log_probs_grad *g, void *stream) {
@@ -935,7 +968,11 @@ int astra_log_probs_backward(const astra_log_probs_grad *g, void *stream) {
   a.dlog_prob = g->dlog_prob;
   a.dentropy = g->dentropy;
   a.dlogits = g->dlogits;
-  return f.type == ASTRA_SEQ_F32 ? backward<float>(a, as_stream(stream)) : backward<bf16>(a, as_stream(stream));
+  for (int64_t r = 0, most = most_rows(a); r < f.rows; r += most) {
+    const ProbArgs some = rows_of(a, f.type, r, std::min(most, f.rows - r));
+    if (int rc = f.type == ASTRA_SEQ_F32 ? backward<float>(some, as_stream(stream)) : backward<bf16>(some, as_stream(stream))) return rc;
+  }
+  return ASTRA_OK;
 }
 
 }  // extern "C"

@@ -279,6 +279,37 @@ def test_many_entries():
     check(seq, big, torch.tensor([[29_999_999]], device=DEV), [30_000_001], None, 3, 7)
 
 
+def test_many_rows_of_larger_parts():
+    """More workgroups than one launch may have: a row of logits, or of pieces of one, for each. (One row
+    of memory serves all.)"""
+    from astra_cuda import sequence as seq
+    logits, choice, _ = make(14, 1, [1025], BF16)
+    R = 2 ** 24 + 5
+    want = part(logits, None, choice[:, 0], 0, None, None, BF16)
+    got = seq.log_probs(logits.expand(R, 1025), choice[:, 0].expand(R))
+    for v, k in zip(got, ("log_prob", "entropy")):
+        assert bool((v == v[0]).all())
+        within(v[:1], want[k], k)
+    logits, choice, _ = make(15, 1, [9000], BF16)
+    R = 2 ** 22 + 5
+    want = seq.log_probs(logits, choice[:, 0], top=1)
+    got = seq.log_probs(logits.expand(R, 9000), choice[:, 0].expand(R), top=1)
+    for v, w in zip(got, want):
+        assert bool((v == w).all())
+
+
+def test_gradient_of_many_rows_of_larger_parts():
+    from astra_cuda import sequence as seq
+    logits, choice, _ = make(16, 1, [1025], BF16)
+    R = 2 ** 24 + 5
+    x = logits.expand(R, 1025).detach().requires_grad_()
+    lp, h = seq.log_probs(x, choice[:, 0].expand(R))
+    d, = torch.autograd.grad([lp, h], x, [torch.ones_like(lp), torch.ones_like(h)])
+    one = part(logits, None, choice[:, 0], 0, torch.ones(1, device=DEV), torch.ones(1, device=DEV), BF16)
+    within(d[:1], one["dlogits"], "dlogits")
+    assert all(bool((d[i:i + 2 ** 20] == d[0]).all()) for i in range(0, R, 2 ** 20))
+
+
 def test_refusals():
     from astra_cuda import sequence as seq
     import torch.autograd.forward_ad as fwd
