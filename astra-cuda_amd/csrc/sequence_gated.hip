@@ -6,6 +6,8 @@
 //
 // All are matrix products out[r, l] = sum_k left[l, k] right[r, k] on the matrix cores, with
 // what surrounds them done on the accumulators.
+#include <algorithm>
+
 #include "sequence.h"
 
 #define ASTRA_SRC_NAME "sequence_gated.hip"
@@ -587,13 +589,14 @@ __global__ __launch_bounds__(256) void join_slices_kernel(ProductArgs g) {
 template <class T>
 __global__ __launch_bounds__(256) void align_kernel(const T *in, T *out, int64_t rows, int64_t width, int64_t ld, int64_t wide) {
   constexpr int V = 16 / sizeof(T);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = wide / V;
-  if (i >= rows * per) return;
-  const int64_t row = i / per, c = (i - row * per) * V;
-  float v[V];
+  const int64_t per = wide / V, n = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per, c = (i - row * per) * V;
+    float v[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) v[j] = c + j < width ? (float)in[row * ld + c + j] : 0.f;
-  Vec<T, V>::store(out + row * wide + c, v);
+    for (int j = 0; j < V; ++j) v[j] = c + j < width ? (float)in[row * ld + c + j] : 0.f;
+    Vec<T, V>::store(out + row * wide + c, v);
+  }
 }
 
 // [D, 2 Fp] from the weights [F, D]: row d is column d of gate, zeros up to Fp, and column d of up.
@@ -774,9 +777,9 @@ Operand operand(const astra_gated_linear &f, const void *p, int64_t stride, int6
   const int64_t wide = round_up(f.width, per16(f.type)), pieces = rows * (wide / per16(f.type));
   T *out = (T *)*ws;
   *ws += (size_t)(rows * wide) * sizeof(T);
+  const int64_t blocks = std::min(cdiv(pieces, 256), kMostThreads / 256);
   if (pieces)
-    hipLaunchKernelGGL(align_kernel<T>, dim3((unsigned)cdiv(pieces, 256)), dim3(256), 0, st, (const T *)p, out, rows,
-                       (int64_t)f.width, stride, wide);
+    hipLaunchKernelGGL(align_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, (const T *)p, out, rows, (int64_t)f.width, stride, wide);
   return {out, wide, rows, wide};
 }
 
@@ -851,7 +854,7 @@ template <class P, bool GRAD>
 int launch_gated_tiles(GatedArgs g, hipStream_t st) {
   const int64_t F = GRAD ? g.Fp : g.F;
   const int64_t n = tiles<P>(F, g.M) * g.slices;
-  ASTRA_ABI_CHECK(n, <, 2147483648ll);
+  ASTRA_ABI_CHECK(n * P::kThreads, <=, kMostThreads);
   g.tiles_l = (int32_t)cdiv(F, P::BLL);
   g.tiles_r = (int32_t)cdiv(g.M, P::BR);
   g.steps = (int32_t)cdiv(cdiv(g.x.len, kStepOf<typename P::type>), g.slices);
@@ -924,7 +927,7 @@ template <class P>
 int launch_product(ProductArgs &g, void *part, hipStream_t st) {
   typedef typename P::type T;
   const int64_t n = tiles<P>(g.nl, g.nr) * g.slices;
-  ASTRA_ABI_CHECK(n, <, 2147483648ll);
+  ASTRA_ABI_CHECK(n * P::kThreads, <=, kMostThreads);
   g.tiles_l = (int32_t)cdiv(g.nl, P::BL);
   g.tiles_r = (int32_t)cdiv(g.nr, P::BR);
   g.steps = (int32_t)cdiv(cdiv(g.left[0].len, kStepOf<T>), g.slices);

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from gated_util import BF16, DEV, F32, call, check, half_step, inputs
+from gated_util import BF16, DEV, F32, call, check, half_step, inputs, results, within
 
 pytestmark = pytest.mark.gpu
 
@@ -102,6 +102,32 @@ def test_gradients_that_are_asked_for(dtype, which):
     got = torch.autograd.grad(seq.gated_linear(*leaves), [leaves[i] for i in which], dh)
     for i, d in zip(which, got):
         assert torch.equal(d, want[("dx", "dgate", "dup")[i]])
+
+
+def test_copies_of_more_than_64_gib():
+    """Rows that do not start on 16 bytes, more than one launch has threads for. (One row serves all.)"""
+    from astra_cuda import sequence as seq
+    M, D, F = 2 ** 25 + 5, 1024, 8
+    x, wg, wu, dh = inputs(17, 1, D + 1, F, BF16)
+    x, wg, wu = x[:, 1:], wg[:, 1:], wu[:, 1:]
+    h = seq.gated_linear(x.expand(M, D), wg, wu)
+    assert bool((h == h[0]).all())
+    within(h[:1], results(x, wg, wu, dh, "silu")["h"], "h")
+
+
+def test_more_than_2_to_the_31_results():
+    """Of whose gradient the last rows alone are not zero."""
+    from astra_cuda import sequence as seq
+    M, D, F = 2_200_001, 8, 1000
+    _, wg, wu, _ = inputs(15, 1, D, F, BF16)
+    x = torch.randn(M, D, device=DEV).to(BF16)
+    dh = torch.zeros(M, F, device=DEV, dtype=BF16)
+    dh[-70:] = torch.randn(70, F, device=DEV).to(BF16)
+    got = call(seq, x, wg, wu, dh, "silu")
+    want = results(x[-70:], wg, wu, dh[-70:], "silu")
+    assert not bool(got["dx"][:-70].any())
+    for k in ("h", "dx", "dgate", "dup"):
+        within(got[k][-70:] if k in ("h", "dx") else got[k], want[k], k)
 
 
 def test_no_rows():
