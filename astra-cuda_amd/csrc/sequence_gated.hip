@@ -754,10 +754,11 @@ bool keeps(const astra_gated_linear &f) { return f.width >= (f.type == ASTRA_SEQ
 bool few(const astra_gated_linear &f) { return f.rows <= 64; }
 
 // Whether an operand is read as it lies, or copied to a workspace first. (256 rows of a tile have to
-// be within the 2 GB that one access can reach.)
+// be within the 2 GB that one access can reach, and what lies behind the last row in no row before it:
+// rows that overlap, or one for all, are copied.)
 bool direct(const astra_gated_linear &f, const void *p, int64_t stride) {
   const int64_t v = per16(f.type);
-  return aligned(p, 16) && stride % v == 0 && f.width % v == 0 && stride < (int64_t(1) << 20);
+  return aligned(p, 16) && stride % v == 0 && f.width % v == 0 && stride >= f.width && stride <= ASTRA_SEQ_MAX_LINEAR_WIDTH;
 }
 size_t copy_bytes(const astra_gated_linear &f, const void *p, int64_t stride, int64_t rows) {
   return direct(f, p, stride) ? 0 : (size_t)(rows * round_up(f.width, per16(f.type))) * elem_size(f.type);
