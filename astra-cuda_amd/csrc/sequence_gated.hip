@@ -751,6 +751,8 @@ int64_t padded_hidden(const astra_gated_linear &f) { return round_up(f.hidden, p
 // again, 4 D operations.
 bool keeps(const astra_gated_linear &f) { return f.width >= (f.type == ASTRA_SEQ_BF16 ? 1024 : 128); }
 
+float *kept(const astra_gated_linear &f) { return keeps(f) ? f.projections : nullptr; }
+
 bool few(const astra_gated_linear &f) { return f.rows <= 64; }
 
 // Whether an operand is read as it lies, or copied to a workspace first. (256 rows of a tile have to
@@ -793,7 +795,7 @@ Operands operands(const astra_gated_linear &f, char **ws, hipStream_t st) {
 GatedArgs args_of(const astra_gated_linear &f) {
   GatedArgs g{};
   g.h = f.h;
-  g.ab = f.projections;
+  g.ab = kept(f);
   g.M = f.rows;
   g.F = f.hidden;
   g.Fp = padded_hidden(f);
@@ -974,7 +976,7 @@ size_t part_bytes(const astra_gated_linear &f) {
   const int64_t w = slices_of<T>(f).n, x = dx_slices<T>(f);
   const size_t of_w = w > 1 ? (size_t)(w * 2 * padded_hidden(f) * f.width) * sizeof(float) : 0;
   const size_t of_x = x > 1 ? (size_t)(x * f.rows * f.width) * sizeof(float) : 0;
-  const size_t of_h = f.projections ? 0 : gated_part_bytes<T>(f);
+  const size_t of_h = kept(f) ? 0 : gated_part_bytes<T>(f);
   return std::max(std::max(of_w, of_x), of_h);
 }
 
@@ -1004,7 +1006,7 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
   char *const turn = ws, *const part = ws + turned_bytes<T>(f);
   if (f.rows) {
     g.slices = 1;
-    if (int rc = f.projections ? launch_join<T, true>(g, f.projections, st) : launch_gated<T, true>(g, part, st)) return rc;
+    if (int rc = kept(f) ? launch_join<T, true>(g, kept(f), st) : launch_gated<T, true>(g, part, st)) return rc;
   }
   if (b.dx && f.rows) {  // da Wg + db Wu
     ProductArgs p{};

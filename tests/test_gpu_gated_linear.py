@@ -119,6 +119,32 @@ def test_rows_that_overlap(dtype):
     assert all(torch.equal(got[k].nan_to_num(-1.0, -2.0), want[k].nan_to_num(-1.0, -2.0)) for k in want)
 
 
+def test_projections_that_are_not_wanted():
+    """The C entry writes as many floats as it says, none where that is none."""
+    import ctypes
+    from astra_cuda import _native
+    lib = _native.lib()
+    for M in (40, 300):
+        x, wg, wu, dh = inputs(14, M, 64, 128, BF16)
+        h, spare = torch.empty_like(dh), torch.full((2, M, 128), 7.0, device=DEV)
+        f = _native.GatedLinear(x=x.data_ptr(), gate=wg.data_ptr(), up=wu.data_ptr(), h=h.data_ptr(),
+                                projections=spare.data_ptr(), rows=M, x_stride=64, gate_stride=64, up_stride=64,
+                                width=64, hidden=128, type=1, activation=1)
+        n = ctypes.c_size_t(1)
+        assert lib.astra_gated_linear_projections(ctypes.addressof(f), ctypes.byref(n)) == 0 and n.value == 0
+        assert lib.astra_gated_linear_workspace_size(ctypes.addressof(f), ctypes.byref(n)) == 0 and n.value == 0
+        assert lib.astra_gated_linear_forward(ctypes.addressof(f), torch.cuda.current_stream().cuda_stream) == 0
+        grads = [torch.empty_like(v) for v in (x, wg, wu)]
+        b = _native.GatedLinearGrad(f=f, dh=dh.data_ptr(), dx=grads[0].data_ptr(), dgate=grads[1].data_ptr(), dup=grads[2].data_ptr())
+        assert lib.astra_gated_linear_grad_workspace_size(ctypes.addressof(f), ctypes.byref(n)) == 0
+        ws = torch.empty(n.value, dtype=torch.uint8, device=DEV)
+        b.workspace, b.workspace_bytes = ws.data_ptr(), n.value
+        assert lib.astra_gated_linear_backward(ctypes.addressof(b), torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert bool((spare == 7).all())
+        check(dict(zip(("h", "dx", "dgate", "dup"), (h, *grads))), x, wg, wu, dh, "silu")
+
+
 def test_copies_of_more_than_64_gib():
     """Rows that do not start on 16 bytes, more than one launch has threads for. (One row serves all.)"""
     from astra_cuda import sequence as seq
