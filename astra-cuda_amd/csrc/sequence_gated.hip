@@ -601,9 +601,8 @@ __global__ __launch_bounds__(256) void align_kernel(const T *in, T *out, int64_t
 
 // [D, 2 Fp] from the weights [F, D]: row d is column d of gate, zeros up to Fp, and column d of up.
 constexpr int kTurn = 64;
-template <class T>
-__global__ __launch_bounds__(256) void turn_kernel(Operand gate, Operand up, T *out, int64_t D, int64_t F, int64_t Fp) {
-  __shared__ T tile[kTurn][kTurn + 4];
+__global__ __launch_bounds__(256) void turn_kernel(Operand gate, Operand up, bf16 *out, int64_t D, int64_t F, int64_t Fp) {
+  __shared__ bf16 tile[kTurn][kTurn + 4];
   const Operand &w = blockIdx.z ? up : gate;
   const int64_t f0 = (int64_t)blockIdx.x * kTurn, d0 = (int64_t)blockIdx.y * kTurn;
   const int i = threadIdx.x / 16, j = threadIdx.x % 16 * 4;
@@ -611,9 +610,9 @@ __global__ __launch_bounds__(256) void turn_kernel(Operand gate, Operand up, T *
   for (int n = 0; n < kTurn; n += 16) {
     float v[4];
     const int64_t f = f0 + i + n;
-    Loose<T, 4>::load((const T *)w.p + f * w.ld + d0 + j, v, f < F ? (int)min((int64_t)4, D - d0 - j) : 0);
+    Loose<bf16, 4>::load((const bf16 *)w.p + f * w.ld + d0 + j, v, f < F ? (int)min((int64_t)4, D - d0 - j) : 0);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) tile[i + n][j + k] = (T)v[k];
+    for (int k = 0; k < 4; ++k) tile[i + n][j + k] = (bf16)v[k];
   }
   __syncthreads();
 #pragma unroll
@@ -622,7 +621,7 @@ __global__ __launch_bounds__(256) void turn_kernel(Operand gate, Operand up, T *
     float v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = (float)tile[j + k][i + n];
-    if (d < D) Loose<T, 4>::store(out + d * 2 * Fp + blockIdx.z * Fp + f0 + j, v, (int)min((int64_t)4, Fp - f0 - j));
+    if (d < D) Loose<bf16, 4>::store(out + d * 2 * Fp + blockIdx.z * Fp + f0 + j, v, (int)min((int64_t)4, Fp - f0 - j));
   }
 }
 
@@ -956,19 +955,21 @@ Slices slices_of(const astra_gated_linear &f) {
   const int64_t most = cdiv(f.rows, kStepOf<T>) / 8;
   return {alone, want < most ? want : most > 1 ? most : 1};
 }
-// With many rows the weights are turned for the inputs' gradient: products along the contraction are
-// a fifth faster, which 4,096 rows make more than the turning takes.
-bool turned(const astra_gated_linear &f) { return f.rows >= 4096; }
-template <class T>
+// With many rows, wide bf16 weights are turned for the inputs' gradient: lines along the contraction are
+// read from memory in fewer, longer pieces. Whole passes without and with it, us: 16,384 rows of 4,096
+// to 8,192 wide 5,296 / 4,429, 8,192 of 8,192 to 8,192 5,552 / 4,276, 8,192 of 2,048 to 8,192
+// 1,317 / 1,306, 8,192 of 1,024 to 4,096 447 / 441; but 4,096 of 2,048 to 8,192 739 / 770, 16,384 of
+// 256 to 1,024 101 / 106, and float 16,384 of 4,096 to 4,096 15,580 / 16,010.
+bool turned(const astra_gated_linear &f) { return f.type == ASTRA_SEQ_BF16 && f.rows >= 8192 && f.width >= 1024; }
 size_t turned_bytes(const astra_gated_linear &f) {
-  return turned(f) ? (size_t)round_up(f.width * 2 * padded_hidden(f), 16) * sizeof(T) : 0;
+  return turned(f) ? (size_t)round_up(f.width * 2 * padded_hidden(f), 16) * sizeof(bf16) : 0;
 }
 
-// Slices of the inputs' gradient's contraction: of twice the hidden width if turned, else of each half.
+// Slices of each half of the inputs' gradient's contraction. (Turned, there are tiles enough.)
 template <class T>
 int64_t dx_slices(const astra_gated_linear &f) {
-  typedef Small<T, false, false, false> S;
-  return slices_for(tiles<S>(f.width, f.rows), kCus * S::GROUPS, cdiv(padded_hidden(f) * (turned(f) ? 2 : 1), kStepOf<T>));
+  typedef Small<T, true, false, false> S;
+  return slices_for(tiles<S>(f.width, f.rows), kCus * S::GROUPS, cdiv(padded_hidden(f), kStepOf<T>));
 }
 // What the slices of one product after the other need.
 template <class T>
@@ -982,7 +983,7 @@ size_t part_bytes(const astra_gated_linear &f) {
 
 template <class T>
 size_t grad_bytes(const astra_gated_linear &f) {
-  return (size_t)(f.rows * 2 * padded_hidden(f)) * sizeof(T) + copies_bytes(f) + turned_bytes<T>(f) + part_bytes<T>(f);
+  return (size_t)(f.rows * 2 * padded_hidden(f)) * sizeof(T) + copies_bytes(f) + turned_bytes(f) + part_bytes<T>(f);
 }
 
 template <class T>
@@ -1003,7 +1004,7 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
   g.x = o.x;
   g.gate = o.gate;
   g.up = o.up;
-  char *const turn = ws, *const part = ws + turned_bytes<T>(f);
+  char *const turn = ws, *const part = ws + turned_bytes(f);
   if (f.rows) {
     g.slices = 1;
     if (int rc = kept(f) ? launch_join<T, true>(g, kept(f), st) : launch_gated<T, true>(g, part, st)) return rc;
@@ -1015,15 +1016,17 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
     p.nr = p.split = p.rows = f.rows;
     p.slices = (int32_t)dx_slices<T>(f);
     if (turned(f)) {
-      const dim3 grid((unsigned)cdiv(Fp, kTurn), (unsigned)cdiv(f.width, kTurn), 2);
-      hipLaunchKernelGGL(turn_kernel<T>, grid, dim3(256), 0, st, o.gate, o.up, (T *)turn, (int64_t)f.width, (int64_t)f.hidden, Fp);
-      ASTRA_HIP_CHECK(rt_last_error(), "turn_kernel launch");
-      p.pairs = 1;
-      p.left[0] = {turn, 2 * Fp, f.width, 2 * Fp};
-      p.right[0] = {g.dab, 2 * Fp, f.rows, 2 * Fp};
-      typedef Large<T, false, false, false> L;
-      typedef Small<T, false, false, false> S;
-      if (int rc = p.slices == 1 && larger<L, S>(p.nl, p.nr, 2 * Fp) ? launch_product<L>(p, part, st) : launch_product<S>(p, part, st)) return rc;
+      if constexpr (sizeof(T) == 2) {
+        const dim3 grid((unsigned)cdiv(Fp, kTurn), (unsigned)cdiv(f.width, kTurn), 2);
+        hipLaunchKernelGGL(turn_kernel, grid, dim3(256), 0, st, o.gate, o.up, (T *)turn, (int64_t)f.width, (int64_t)f.hidden, Fp);
+        ASTRA_HIP_CHECK(rt_last_error(), "turn_kernel launch");
+        p.pairs = 1;
+        p.left[0] = {turn, 2 * Fp, f.width, 2 * Fp};
+        p.right[0] = {g.dab, 2 * Fp, f.rows, 2 * Fp};
+        typedef Large<T, false, false, false> L;
+        typedef Small<T, false, false, false> S;
+        if (int rc = larger<L, S>(p.nl, p.nr, 2 * Fp) ? launch_product<L>(p, part, st) : launch_product<S>(p, part, st)) return rc;
+      }
     } else {
       p.pairs = 2;
       for (int i = 0; i < 2; ++i) {
