@@ -576,8 +576,11 @@ __global__ __launch_bounds__(256) void wide_forward_kernel(ProbArgs a) {
   if (threadIdx.x == 0) store_result(a, unit, c, x, mask, result_of(s));
 }
 
-// Few rows, or the largest entries wanted: a workgroup has kPiece entries in registers.
-constexpr int kVectors = 4, kPiece = 256 * V * kVectors;
+// Few rows of many entries, or the largest entries wanted: a workgroup has kPiece entries in registers.
+// In pieces and joined, or a workgroup a row, us: one row of 130,000 bf16 entries 6.9 / 25.9, of 50,000
+// 6.6 / 11.5, of 20,000 6.7 / 6.2, of 1,500 4.5 / 3.5; 256 rows 26 / 49, 15 / 22, 10.6 / 9.0, 5.0 / 4.0;
+// 511 rows of 50,000 22 / 24, 1,024 rows 37 / 27.
+constexpr int kVectors = 4, kPiece = 256 * V * kVectors, kCut = 4 * kPiece;
 __host__ __device__ inline int pieces_of(int size) { return (size + kPiece - 1) / kPiece; }
 
 // A wavefront's largest entries, sorted, of those in its lanes' registers. The top-th largest of
@@ -783,9 +786,13 @@ ProbArgs args_of(const astra_log_probs &f) {
   a.mask_stride = f.mask_stride;
   a.parts = f.parts;
   a.top = f.top;
-  a.cut = f.top > 0 || f.rows * f.parts < 512;
   a.wide_choice = f.choice_bytes == 8;
-  for (int i = 0; i < f.parts; ++i) a.begin[i + 1] = a.begin[i] + f.sizes[i];
+  int largest = 0;
+  for (int i = 0; i < f.parts; ++i) {
+    a.begin[i + 1] = a.begin[i] + f.sizes[i];
+    largest = std::max(largest, f.sizes[i]);
+  }
+  a.cut = f.top > 0 || (f.rows * f.parts < 512 && largest > kCut);
   a.W = a.begin[f.parts];
   return a;
 }
