@@ -23,7 +23,6 @@ namespace {
 constexpr int kParts = ASTRA_SEQ_MAX_PARTS;
 static_assert(ASTRA_SEQ_MAX_TOP <= kWave, "a lane for each of the largest");
 constexpr int V = 8;             // entries a lane takes at a time
-constexpr int kNarrow = 1024;    // parts up to here are a group of lanes' work, larger ones workgroups'
 constexpr int kStats = 3;        // m, log Z, H of a row and part
 
 struct ProbArgs {
@@ -38,6 +37,7 @@ struct ProbArgs {
   uint64_t *lists;     // and its largest entries
   int64_t R, stride, mask_stride;
   int32_t W, parts, top, wide_choice;
+  int32_t narrow;              // parts up to here are a group of lanes' work, larger ones workgroups'
   bool cut;                    // whether larger parts go through in pieces
   int32_t block_rows;          // rows of a workgroup that has all their parts
   int32_t begin[kParts + 1];   // of each part in a row
@@ -276,7 +276,7 @@ __device__ __forceinline__ float log_prob_of(int c, float x, const Result &r) {
   return c == -1 ? 0.f : c == INT32_MAX ? NAN : x - r.most - r.log_z;
 }
 
-// ------------------------------------------------------------- parts of up to 1,024 entries
+// ------------------------------------------------------------------------- smaller parts
 
 // A group of lanes has one part of one row in registers; results go to LDS, from where whole rows
 // of them are written.
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256) void narrow_forward_kernel(ProbArgs a) {
   const int rows = (int)min((int64_t)a.block_rows, a.R - first);
   for (int part = 0; part < a.parts; ++part) {
     const int size = a.begin[part + 1] - a.begin[part], turn = (wave + part) & 3;
-    if (size > kNarrow) continue;
+    if (size > a.narrow) continue;
     if (size <= V)
       narrow_part<T, 1, 1, TOP>(a, out, part, first, rows, turn);
     else if (size <= 2 * V)
@@ -384,14 +384,16 @@ __global__ __launch_bounds__(256) void narrow_forward_kernel(ProbArgs a) {
       narrow_part<T, 32, 1, TOP>(a, out, part, first, rows, turn);
     else if (size <= 64 * V)
       narrow_part<T, 64, 1, TOP>(a, out, part, first, rows, turn);
-    else
+    else if (TOP || size <= 128 * V)
       narrow_part<T, 64, 2, TOP>(a, out, part, first, rows, turn);
+    else if constexpr (!TOP)
+      narrow_part<T, 64, 4, TOP>(a, out, part, first, rows, turn);
   }
   __syncthreads();
   const int64_t at = first * a.parts;
   for (int n = threadIdx.x; n < rows * a.parts * kStats; n += 256) {
     const int unit = n / kStats, part_n = unit % a.parts;
-    if (a.begin[part_n + 1] - a.begin[part_n] > kNarrow) continue;
+    if (a.begin[part_n + 1] - a.begin[part_n] > a.narrow) continue;
     if (a.stats) a.stats[at * kStats + n] = out.stats[n];
     if (n == unit * kStats) {
       a.entropy[at + unit] = out.entropy[unit];
@@ -460,7 +462,7 @@ __device__ __forceinline__ void store_entries(T *d, int i, int size, const float
   }
 }
 
-// n / d for quotients of up to 64 and d of up to 2^11: (n + 0.5) / d is at least 2^-12 away from every
+// n / d for quotients of up to 64 and d of up to 2^12: (n + 0.5) / d is at least 2^-13 away from every
 // whole number, and three roundings of 64 are 2^-16.
 __device__ __forceinline__ int quotient(int n, float inv_d) { return (int)(((float)n + 0.5f) * inv_d); }
 
@@ -693,7 +695,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_pieces_kernel(ProbArgs a
   __shared__ uint64_t lists[TOP ? kJoinWaves : 1][64];
   const int part = blockIdx.y;
   const int begin = a.begin[part], size = a.begin[part + 1] - begin, pieces = pieces_of(size);
-  if (size <= kNarrow || pieces == 1) return;
+  if (pieces == 1) return;
   const int64_t row = blockIdx.x, unit = row * a.parts + part, at = a.block[part] + row * pieces;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   Seen s{-INFINITY, 0.f, 0.f};
@@ -792,12 +794,16 @@ ProbArgs args_of(const astra_log_probs &f) {
     a.begin[i + 1] = a.begin[i] + f.sizes[i];
     largest = std::max(largest, f.sizes[i]);
   }
+  // Lanes' work ends with its loads, a workgroup's with two barriers. Both, us, the former first: 81,920
+  // rows of 1,000 bf16 entries 51 / 95, of 1,500 73 / 136, of 2,048 81 / 106; of 1,000 floats 73 / 100, of
+  // 1,500 107 / 133, but with the gradient 338 / 312. 16,384 rows of 1,000 bf16 entries 15 / 21, 4,096
+  // 9.9 / 9.2, 1,024 6.6 / 5.9. (The largest entries are taken one by one there.)
+  a.narrow = f.top || f.type == ASTRA_SEQ_F32 ? 1024 : 2048;
+  if (!f.top && f.rows < 8192) a.narrow = 512;
   a.cut = f.top > 0 || (f.rows * f.parts < 512 && largest > kCut);
   a.W = a.begin[f.parts];
   return a;
 }
-
-bool narrow(int size) { return size <= kNarrow; }
 
 // Gives the workgroups of a launch to the larger parts, `each(size)` for one; how many there are.
 template <class Each>
@@ -806,7 +812,7 @@ int64_t share(ProbArgs &a, Each &&each) {
   for (int i = 0; i < a.parts; ++i) {
     const int size = a.begin[i + 1] - a.begin[i];
     a.block[i] = n;
-    if (!narrow(size)) n += each(size);
+    if (size > a.narrow) n += each(size);
   }
   for (int i = a.parts; i <= kParts; ++i) a.block[i] = n;
   return n;
@@ -821,12 +827,12 @@ int rows_together(const ProbArgs &a) {
 }
 bool some_narrow(const ProbArgs &a) {
   for (int i = 0; i < a.parts; ++i)
-    if (narrow(a.begin[i + 1] - a.begin[i])) return true;
+    if (a.begin[i + 1] - a.begin[i] <= a.narrow) return true;
   return false;
 }
 bool some_wide(const ProbArgs &a) {
   for (int i = 0; i < a.parts; ++i)
-    if (!narrow(a.begin[i + 1] - a.begin[i])) return true;
+    if (a.begin[i + 1] - a.begin[i] > a.narrow) return true;
   return false;
 }
 

@@ -41,7 +41,8 @@ def test_values_gradients_and_top(sizes, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("R,sizes", [(600, [1500]), (2000, [3001, 9]), (20_000, [127, 127, 6, 6]), (70_001, [5]), (513, [20_000])],
+@pytest.mark.parametrize("R,sizes", [(600, [1500]), (2000, [3001, 9]), (20_000, [127, 127, 6, 6]), (70_001, [5]), (513, [20_000]),
+                                      (8192, [1000, 513]), (8195, [2048, 600]), (9000, [1025]), (8193, [1500, 2049])],
                          ids=str)
 def test_many_rows(R, sizes, dtype):
     from astra_cuda import sequence as seq
