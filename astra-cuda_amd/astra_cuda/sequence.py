@@ -14,10 +14,10 @@ time in rollouts with a state of fixed size per env (include/sequence/astra_sequ
 ``log_probs``        log probability of a move, entropy and likeliest alternatives from logits
 ``short_conv_step``, ``state_scan_step``   one position, the state moved on in place
 
-All but the steps are differentiable in every floating point tensor they take, backwards and once: tensors with
-a forward-mode tangent are refused, and so is being part of a torch.jit trace. A step raises its
-state's version: a backward pass that had saved the state refuses to run, as after torch's own
-operations in place.
+All but the steps are differentiable in every floating point tensor they take, backwards and
+once: tensors with a forward-mode tangent are refused, and so is being part of a torch.jit
+trace. A step raises its state's version: a backward pass that had saved the state refuses to
+run, as after torch's own operations in place.
 
 Tensors are float32 or bfloat16 on one HIP device. Sums, states and norms are float32
 throughout, and each result is rounded to its type once; what is computed in between enters
@@ -129,7 +129,9 @@ def gated_linear(x, gate_weight, up_weight, *, activation="silu"):
     ``x`` ``[..., D]``, the weights ``[F, D]`` of x's type, as those of two ``nn.Linear``; returns
     ``[..., F]``. ``activation``: ``"silu"``, or ``"gelu"`` (v times the normal distribution function
     at v, by erf). Bfloat16 products are summed in float32 and the result is rounded once; the
-    gradients of the two projections are rounded to x's type before their own products.
+    gradients of the two projections are rounded to x's type before their own products. A forward
+    pass that is differentiated keeps its inputs, and from a width of 1,024 (float32: 128) on the
+    two projections in float32, 8 bytes an element of the result.
     """
     return (_ops or _compiled()).gated_linear(x, gate_weight, up_weight, activation)
 
@@ -145,8 +147,8 @@ def log_probs(logits, choice=None, *, sizes=None, mask=None, top=0):
     allowed; logits of -inf are not, either. ``top_log_prob`` and ``top_index`` ``[..., k]`` are the
     likeliest allowed entries, ties to the lower index, -inf and -1 where there are fewer.
 
-    A choice of -1 says that a part does not count (a game that is over): its logits are not read,
-    its log_prob, entropy and gradient are 0. The log probability of an entry that is left out is
+    A choice of -1 says that a part does not count (a game that is over): its logits may be
+    anything, its log_prob, entropy and gradient are 0. The log probability of an entry that is left out is
     -inf and has no gradient, that of a choice outside of its part is NaN. Where nothing is allowed
     the entropy is 0. An allowed NaN or infinity makes its part's log probabilities, entropy and
     gradient NaN. log_prob and entropy are float32 and differentiable in logits; the top ones are not.

@@ -5,7 +5,21 @@
 //   dx = da Wg + db Wu,  dWg = da^T x,  dWu = db^T x
 //
 // All are matrix products out[r, l] = sum_k left[l, k] right[r, k] on the matrix cores, with
-// what surrounds them done on the accumulators.
+// what surrounds them done on the accumulators: 4 M D F operations forwards, 8 M D F backwards, and 4 M D F
+// again where a and b are computed a second time. Sums are float32; h is rounded once, da and db are
+// rounded to x's type before their products, as the matrix cores take them (2^-8 of bf16 each, which
+// makes the gradients' error 1.4 times that of h).
+//
+// Measured (us; the card's large bf16 library product reaches 1,390 TFLOP/s, its float product 154,
+// its copies 4.8 TB/s):
+//   16,384 rows of 4,096 to 8,192, bf16   h 1,907 (1,150 TFLOP/s; 1,680 without keeping a and b), da and db
+//                                         350 (5.4 TB/s), weights turned 52, dx 1,956 (1,120), dWg and dWu 1,833 (1,200)
+//   81,920 rows of 256 to 1,024, bf16     h 125-135, da and db 208 (a and b again), dx 147, dWg and dWu 115 + 15
+//   30,000 rows of 256 to 683, float      h 229, da and db 77, dx 194, dWg and dWu 212 + 18
+//   one row of 256 to 1,024               3.5; of 4,096 to 8,192 30 (4.5 TB/s), 64 such rows 46 to 50
+// The matrix cores are busy 60% of the wide bf16 products' time at some 2.1 GHz, and their power holds the
+// clock there; 75% of the float products'. Rows of 256 have 4 steps: bound by the results' traffic (h alone is
+// 168 MB) and by how little of it overlaps with the products. Few rows are bound by the weights' traffic.
 #include <algorithm>
 
 #include "sequence.h"
@@ -18,9 +32,9 @@ namespace {
 // ------------------------------------------------------------------ tiles of a product
 //
 // A workgroup of WL x WR wavefronts has a tile of BL x BR results, a wavefront NL x NR of 16 x 16.
-// 128 bytes of the contraction at a time (64 bf16 or 32 floats) are brought straight into LDS, one
-// such step ahead of the products, which read them as fragments: lane i has 16 bytes of line
-// i % 16, the (i / 16)-th of its four.
+// 128 bytes of the contraction at a time (64 bf16 or 32 floats) are brought straight into LDS, which the
+// products read as fragments: lane i has 16 bytes of line i % 16, the (i / 16)-th of its four. (Products
+// of 32 x 32 are no faster: 1,710-1,780 TFLOP/s alone to 1,620-1,940.)
 //
 // An operand lies along the contraction (a line of the tile is 128 contiguous bytes) or across it
 // (TR: the tile is 64 or 32 rows of memory, a line is a column). Its memory starts on 16 bytes, as
@@ -766,11 +780,16 @@ int64_t per16(int32_t type) { return 16 / (int64_t)elem_size(type); }
 int64_t padded_hidden(const astra_gated_linear &f) { return round_up(f.hidden, per16(f.type)); }
 
 // Whether the backward call gets a and b, 16 bytes an element written and read, or computes them
-// again, 4 D operations.
+// again, 4 D operations. Again / kept, us, a training pass of 8,192 rows to four times the width: bf16 of 256
+// 112 / 115, of 512 228 / 250, of 1,024 622 / 607, of 2,048 2,060 / 1,827; float of 64 101 / 97, of 128
+// 138 / 130, of 256 355 / 318.
 bool keeps(const astra_gated_linear &f) { return f.width >= (f.type == ASTRA_SEQ_BF16 ? 1024 : 128); }
 
 float *kept(const astra_gated_linear &f) { return keeps(f) ? f.projections : nullptr; }
 
+// Rows that are read straight from memory rather than as tiles. Few rows' kernel / tiles, us: 64 bf16 rows of 256
+// to 1,024 10.5 / 8.8, of 1,024 to 4,096 13.5 / 18.3, of 4,096 to 8,192 51 / 58, 17 of them 41 / 49; float 10 / 23,
+// 22 / 32, 105 / 150, 77 / 146. Its registers hold 64 rows.
 bool few(const astra_gated_linear &f) { return f.rows <= 64; }
 
 // Whether an operand is read as it lies, or copied to a workspace first. (256 rows of a tile have to
@@ -822,7 +841,10 @@ GatedArgs args_of(const astra_gated_linear &f) {
 }
 
 // Tiles of 128 x 192 results, three workgroups to a CU, or 128 x 128, four; or 256 x 256 with a CU to
-// themselves.
+// themselves. Along the contraction several workgroups a CU are faster (us: 16,384 rows of 4,096 to 8,192 1,680,
+// 1,840, 1,740; 81,920 of 256 to 1,024 136, 123, 150). Across it (both operands of the weights' gradients), where
+// every fragment is two transposing reads, bf16 tiles are better large: 256 x 256 alone 1,690 and 113 us, 256 x 128
+// twice a CU 1,860 and 130, 128 x 128 four times 3,160 and 153; with floats 128 x 128 takes 209, 256 x 256 296.
 template <class T, bool LTR, bool RTR, bool HALVES>
 using Large = Product<T, LTR, RTR, 4, 6, HALVES, 3>;
 template <class T, bool LTR, bool RTR, bool HALVES>
@@ -841,7 +863,9 @@ int64_t room(int64_t nl, int64_t nr) {
   const int64_t n = tiles<P>(nl, nr), each = kCus * P::GROUPS;
   return (n < 3 * each ? round_up(n, each) : n) * P::BL * P::BR;
 }
-// Large tiles read less for each product, small ones overlap more of what is not products.
+// Large tiles read less for each product, small ones overlap more of what is not products. Large / small, us, 8,192
+// rows: of 256 to 4,096 59 / 58, of 512 to 4,096 82.8 / 82.1, of 1,024 134 / 137, of 2,048 248 / 255, of 4,096 to
+// 8,192 946 / 984; 3,000 of 1,024 to 5,000 70 / 74.
 template <class L, class S>
 bool larger(int64_t nl, int64_t nr, int64_t len) {
   return len >= 1024 && 9 * room<L>(nl, nr) <= 10 * room<S>(nl, nr);
@@ -856,7 +880,9 @@ bool larger(int64_t nl, int64_t nr, int64_t len) {
   } while (false)
 
 // Slices of a contraction of `steps` steps for `n` tiles of which the CUs hold `room` at a time: more of
-// them where there are less tiles than CUs, with 8 steps at least.
+// them where there are less tiles than CUs, with 8 steps at least. (Training passes without and with
+// slices, us: 183 float rows of 2,083 to 10,203 1,876 / 770, 237 of 224 to 6,808 943 / 130; one bf16 row of
+// 536 to 7,336 240 / 101.)
 int64_t slices_for(int64_t n, int64_t room, int64_t steps) {
   if (n < 1 || n >= kCus) return 1;
   const int64_t want = cdiv(room, n), most = steps / 8;
@@ -905,7 +931,8 @@ size_t gated_part_bytes(const astra_gated_linear &f) {
 }
 
 // More than 16 rows are read half as often by two tiles a workgroup, which is worth it where the weights
-// are large enough to keep all CUs busy all the same.
+// are large enough to keep all CUs busy all the same. One / two, us, 64 rows: of 4,096 to 8,192 61 / 50, of 2,048 to
+// 8,192 32 / 27, of 2,048 to 4,096 20 / 24, of 256 to 1,024 11 / 13. (16 rows of 4,096 to 8,192: 35 / 42.)
 template <class T>
 int launch_few(const GatedArgs &g, hipStream_t st) {
   const bool two = g.F >= 32 * kCus && g.x.len >= 2048;
@@ -968,7 +995,7 @@ template <class T>
 Slices slices_of(const astra_gated_linear &f) {
   const int64_t D = f.width, F2 = 2 * padded_hidden(f);
   typedef Small<T, true, true, false> S;
-  // float products take their time whatever the tiles are; of bf16 ones, small tiles ask for 1.4 times as much
+  // of bf16, tiles of 128 x 128 take 1.4 to 1.9 times as long for as many results, floats less (as above)
   const bool alone = f.type == ASTRA_SEQ_BF16 && 10 * tiles<Alone>(D, F2) * Alone::BL * Alone::BR <= 14 * tiles<S>(D, F2) * S::BL * S::BR;
   const int64_t want = alone ? cdiv(kCus, tiles<Alone>(D, F2)) : cdiv(kCus * S::GROUPS, tiles<S>(D, F2));
   const int64_t most = cdiv(f.rows, kStepOf<T>) / 8;

@@ -181,9 +181,10 @@ int astra_join_norm_backward(const astra_join_norm_grad *a, void *stream);
 
 /* Forward. x [M,D], gate and up [F,D] of `type` with row strides; h [M,F] contiguous.
  * activation: ASTRA_SEQ_SILU or ASTRA_SEQ_GELU. projections (may be NULL) keeps x gate^T and
- * x up^T for the backward call, astra_gated_linear_projections() floats: zero where the
- * backward call is faster without. The workspace holds aligned copies of operands whose rows
- * do not start on 16 bytes. */
+ * x up^T for the backward call, astra_gated_linear_projections() floats: zero, and not used,
+ * where the backward call is faster without. The workspace holds copies of operands whose rows
+ * do not start on 16 bytes or overlap, and partial sums where few rows' contraction is cut; up
+ * to 64 rows need none. It starts on 16 bytes. */
 typedef struct astra_gated_linear {
   const void *x, *gate, *up;
   void *h;
@@ -220,7 +221,7 @@ int astra_gated_linear_backward(const astra_gated_linear_grad *a, void *stream);
  * top_log_prob float and top_index int64 [R,parts,top] (top up to every part's size): the
  * likeliest entries, ties to the lower index, -inf and -1 where there are fewer. stats float
  * [R,parts,3] (may be NULL) is kept for the backward call.
- * A part that does not count is not read: its log_prob and entropy are 0, and there are no
+ * A part that does not count may hold anything: its log_prob and entropy are 0, and there are no
  * likeliest entries. The log probability of an entry that is left out is -inf, that of a choice
  * in no entry NaN; where nothing is allowed the entropy is 0. The workspace starts on 8 bytes. */
 typedef struct astra_log_probs {
