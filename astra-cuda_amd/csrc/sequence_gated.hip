@@ -617,19 +617,26 @@ __global__ __launch_bounds__(256) void join_slices_kernel(ProductArgs g) {
 
 // ---------------------------------------------------------------------- aligned copies
 
-// [rows, width] with rows of `ld` elements, any alignment, as rows of `wide` elements (a multiple of
-// 16 bytes) filled up with zeros.
+// Operands [rows, width] with rows of `ld` elements, any alignment, as rows of `pitch` elements filled up
+// with zeros. 2^shift threads a row.
+struct AlignArgs {
+  const void *in[3];
+  void *out[3];
+  int64_t rows[3], ld[3];
+  int32_t width, pitch;
+};
 template <class T>
-__global__ __launch_bounds__(256) void align_kernel(const T *in, T *out, int64_t rows, int64_t width, int64_t ld, int64_t wide) {
+__global__ __launch_bounds__(256) void align_kernel(AlignArgs a, int shift) {
   constexpr int V = 16 / sizeof(T);
-  const int64_t per = wide / V, n = rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / per, c = (i - row * per) * V;
-    float v[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = c + j < width ? (float)in[row * ld + c + j] : 0.f;
-    Vec<T, V>::store(out + row * wide + c, v);
-  }
+  const int which = blockIdx.y, each = 256 >> shift;
+  const T *in = (const T *)a.in[which];
+  T *out = (T *)a.out[which];
+  for (int64_t row = (int64_t)blockIdx.x * each + (threadIdx.x >> shift); row < a.rows[which]; row += (int64_t)gridDim.x * each)
+    for (int c = (threadIdx.x & ((1 << shift) - 1)) * V; c < a.pitch; c += V << shift) {
+      float v[V];
+      Loose<T, V>::load(in + row * a.ld[which] + c, v, a.width - c);
+      Vec<T, V>::store(out + row * a.pitch + c, v);
+    }
 }
 
 // [D, 2 Fp] from the weights [F, D]: row d is column d of gate, zeros up to Fp, and column d of up.
@@ -776,8 +783,9 @@ int check(const astra_gated_linear *f) {
 
 int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 int64_t per16(int32_t type) { return 16 / (int64_t)elem_size(type); }
-// rows of the hidden width in a workspace
-int64_t padded_hidden(const astra_gated_linear &f) { return round_up(f.hidden, per16(f.type)); }
+// Rows in a workspace start on the caches' lines of 128 bytes.
+int64_t pitch_of(int64_t width, int32_t type) { return round_up(width, kStep / (int64_t)elem_size(type)); }
+int64_t padded_hidden(const astra_gated_linear &f) { return pitch_of(f.hidden, f.type); }
 
 // Whether the backward call gets a and b, 16 bytes an element written and read, or computes them
 // again, 4 D operations. Again / kept, us, a training pass of 8,192 rows to four times the width: bf16 of 256
@@ -792,41 +800,52 @@ float *kept(const astra_gated_linear &f) { return keeps(f) ? f.projections : nul
 // 22 / 32, 105 / 150, 77 / 146. Its registers hold 64 rows.
 bool few(const astra_gated_linear &f) { return f.rows <= 64; }
 
-// Whether an operand is read as it lies, or copied to a workspace first. (256 rows of a tile have to
-// be within the 2 GB that one access can reach, and what lies behind the last row in no row before it:
-// rows that overlap, or one for all, are copied.)
-bool direct(const astra_gated_linear &f, const void *p, int64_t stride) {
-  const int64_t v = per16(f.type);
-  return aligned(p, 16) && stride % v == 0 && f.width % v == 0 && stride >= f.width && stride <= ASTRA_SEQ_MAX_LINEAR_WIDTH;
-}
-size_t copy_bytes(const astra_gated_linear &f, const void *p, int64_t stride, int64_t rows) {
-  return direct(f, p, stride) ? 0 : (size_t)(rows * round_up(f.width, per16(f.type))) * elem_size(f.type);
+// Whether bf16 rows that do not start on the caches' lines are copied to where they do: a step of such a row
+// is in two lines. As they lie / copied, us: 20,000 rows of 4,088 to 2,048 948 / 632, with the gradients
+// 2,182 / 1,972, of 1,000 to 2,731 293 / 257 and 1,188 / 1,097, to 1,100 126 / 114 and 524 / 496; 4,097 rows to
+// 2,731 70 / 70 and 320 / 313; but 20,000 rows to 520 65 / 70 and 292 / 297, 2,048 to 2,731 41 / 41 and 185 / 186,
+// 300 to 1,100 21 / 26. (Float products take longer than either.)
+bool lined(const astra_gated_linear &f) {
+  return f.type == ASTRA_SEQ_BF16 && f.rows >= 1024 && f.hidden >= 1024 && f.rows * f.hidden >= (int64_t(1) << 24);
 }
 
+// Whether an operand is read as it lies, or copied to a workspace first. (256 rows of a tile have to be
+// within the 2 GB that one access can reach, and what lies behind the last row in no row before it: rows
+// that overlap, or one for all, are copied.)
+bool direct(const astra_gated_linear &f, const void *p, int64_t stride) {
+  const int64_t v = per16(f.type);
+  if (lined(f) && (!aligned(p, kStep) || stride * (int64_t)elem_size(f.type) % kStep)) return false;
+  return aligned(p, 16) && stride % v == 0 && f.width % v == 0 && stride >= f.width && stride <= ASTRA_SEQ_MAX_LINEAR_WIDTH;
+}
 struct Operands {
   Operand x, gate, up;
 };
+// The operands, and what has to be copied first; the copies' bytes.
+size_t operands_of(const astra_gated_linear &f, char *ws, Operands *o, AlignArgs *a) {
+  const void *p[3] = {f.x, f.gate, f.up};
+  const int64_t ld[3] = {f.x_stride, f.gate_stride, f.up_stride}, rows[3] = {f.rows, f.hidden, f.hidden};
+  Operand *out[3] = {&o->x, &o->gate, &o->up};
+  *a = {};
+  a->width = f.width;
+  a->pitch = (int32_t)pitch_of(f.width, f.type);
+  size_t bytes = 0;
+  for (int i = 0; i < 3; ++i) {
+    *out[i] = {p[i], ld[i], rows[i], round_up(f.width, per16(f.type))};
+    if (direct(f, p[i], ld[i])) continue;
+    a->in[i] = p[i];
+    a->ld[i] = ld[i];
+    a->rows[i] = rows[i];
+    a->out[i] = ws + bytes;
+    out[i]->p = ws + bytes;
+    out[i]->ld = a->pitch;
+    bytes += (size_t)(rows[i] * a->pitch) * elem_size(f.type);
+  }
+  return bytes;
+}
 size_t copies_bytes(const astra_gated_linear &f) {
-  return copy_bytes(f, f.x, f.x_stride, f.rows) + copy_bytes(f, f.gate, f.gate_stride, f.hidden) +
-         copy_bytes(f, f.up, f.up_stride, f.hidden);
-}
-
-template <class T>
-Operand operand(const astra_gated_linear &f, const void *p, int64_t stride, int64_t rows, char **ws, hipStream_t st) {
-  if (direct(f, p, stride)) return {p, stride, rows, f.width};
-  const int64_t wide = round_up(f.width, per16(f.type)), pieces = rows * (wide / per16(f.type));
-  T *out = (T *)*ws;
-  *ws += (size_t)(rows * wide) * sizeof(T);
-  const int64_t blocks = std::min(cdiv(pieces, 256), kMostThreads / 256);
-  if (pieces)
-    hipLaunchKernelGGL(align_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, (const T *)p, out, rows, (int64_t)f.width, stride, wide);
-  return {out, wide, rows, wide};
-}
-
-template <class T>
-Operands operands(const astra_gated_linear &f, char **ws, hipStream_t st) {
-  return {operand<T>(f, f.x, f.x_stride, f.rows, ws, st), operand<T>(f, f.gate, f.gate_stride, f.hidden, ws, st),
-          operand<T>(f, f.up, f.up_stride, f.hidden, ws, st)};
+  Operands o;
+  AlignArgs a;
+  return operands_of(f, nullptr, &o, &a);
 }
 
 GatedArgs args_of(const astra_gated_linear &f) {
@@ -887,6 +906,20 @@ int64_t slices_for(int64_t n, int64_t room, int64_t steps) {
   if (n < 1 || n >= kCus) return 1;
   const int64_t want = cdiv(room, n), most = steps / 8;
   return want < most ? want : most > 1 ? most : 1;
+}
+
+template <class T>
+int operands(const astra_gated_linear &f, char **ws, Operands *o, hipStream_t st) {
+  AlignArgs a;
+  *ws += operands_of(f, *ws, o, &a);
+  const int64_t rows = std::max(std::max(a.rows[0], a.rows[1]), a.rows[2]);
+  if (!rows) return ASTRA_OK;
+  int shift = 0;
+  while (shift < 8 && ((int64_t)per16(f.type) << shift) < a.pitch) ++shift;
+  const dim3 grid((unsigned)std::min(cdiv(rows, 256 >> shift), int64_t(1) << 20), 3);
+  hipLaunchKernelGGL(align_kernel<T>, grid, dim3(256), 0, st, a, shift);
+  ASTRA_HIP_CHECK(rt_last_error(), "align_kernel launch");
+  return ASTRA_OK;
 }
 
 template <class T, bool GRAD>
@@ -963,8 +996,8 @@ int forward(const astra_gated_linear &f, hipStream_t st) {
   ASTRA_ABI_CHECK(f.workspace_bytes, >=, need);
   if (need && !aligned(f.workspace, 16)) return fail(ASTRA_ERR_INVALID_ARGUMENT, "astra_gated_linear_forward: the workspace starts on 16 bytes");
   char *ws = (char *)f.workspace;
-  const Operands o = operands<T>(f, &ws, st);
-  ASTRA_HIP_CHECK(rt_last_error(), "align_kernel launch");
+  Operands o;
+  if (int rc = operands<T>(f, &ws, &o, st)) return rc;
   g.x = o.x;
   g.gate = o.gate;
   g.up = o.up;
@@ -1045,8 +1078,8 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
   g.dab = ws;
   g.dh = b.dh;
   ws += (size_t)(f.rows * 2 * Fp) * sizeof(T);
-  const Operands o = operands<T>(f, &ws, st);
-  ASTRA_HIP_CHECK(rt_last_error(), "align_kernel launch");
+  Operands o;
+  if (int rc = operands<T>(f, &ws, &o, st)) return rc;
   g.x = o.x;
   g.gate = o.gate;
   g.up = o.up;

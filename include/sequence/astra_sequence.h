@@ -183,8 +183,8 @@ int astra_join_norm_backward(const astra_join_norm_grad *a, void *stream);
  * activation: ASTRA_SEQ_SILU or ASTRA_SEQ_GELU. projections (may be NULL) keeps x gate^T and
  * x up^T for the backward call, astra_gated_linear_projections() floats: zero, and not used,
  * where the backward call is faster without. The workspace holds copies of operands whose rows
- * do not start on 16 bytes or overlap, and partial sums where few rows' contraction is cut; up
- * to 64 rows need none. It starts on 16 bytes. */
+ * overlap or do not start on 16 bytes (many bf16 rows: 128), and partial sums where few rows'
+ * contraction is cut; up to 64 rows need none. It starts on 16 bytes. */
 typedef struct astra_gated_linear {
   const void *x, *gate, *up;
   void *h;

@@ -14,7 +14,7 @@ SIZES = [
     (1, 1, 1), (1, 256, 1024), (2, 7, 3), (15, 8, 16), (16, 32, 17), (17, 64, 64), (33, 128, 40), (64, 96, 130),
     (65, 64, 128), (127, 72, 129), (128, 128, 64), (129, 33, 65), (200, 520, 1000), (256, 64, 256), (257, 1000, 136),
     (1000, 136, 1111), (2049, 256, 512), (4100, 100, 4096), (20_000, 40, 72), (70_001, 24, 16), (513, 1031, 2050),
-    (8200, 1031, 72), (8193, 1024, 600),
+    (8200, 1031, 72), (8193, 1024, 600), (16_400, 136, 1032),
 ]
 
 
