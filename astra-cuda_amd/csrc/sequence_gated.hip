@@ -299,8 +299,10 @@ struct Product {
 };
 
 // Tile `n` of nl x nr, spread so that an XCD (workgroups are given to the eight in turn) works on
-// neighbouring tiles, kBand right tiles by all left ones: what they share stays in its L2.
-constexpr int kXcds = 8, kBand = 8;
+// neighbouring tiles, kBand right tiles by all left ones: what they share stays in its L2. Bands of 2, 4, 8 and
+// 12, us: a training pass of 16,384 rows of 4,096 to 8,192 5,940, 5,990, 6,100 and 6,700, of 8,192 of 8,192 5,980,
+// 6,020, 6,360, of 16,384 of 2,048 to 4,096 1,730, 1,670, 1,660.
+constexpr int kXcds = 8, kBand = 4;
 __device__ __forceinline__ void tile_of(uint32_t n, uint32_t nl, uint32_t nr, int *l, int *r) {
   const uint32_t total = nl * nr, each = total / kXcds, rest = total % kXcds;
   const uint32_t xcd = n % kXcds;
