@@ -12,11 +12,11 @@
 //
 // Measured (us; the card's large bf16 library product reaches 1,390 TFLOP/s, its float product 154,
 // its copies 4.8 TB/s):
-//   16,384 rows of 4,096 to 8,192, bf16   h 1,907 (1,150 TFLOP/s; 1,680 without keeping a and b), da and db
-//                                         350 (5.4 TB/s), weights turned 52, dx 1,956 (1,120), dWg and dWu 1,833 (1,200)
-//   81,920 rows of 256 to 1,024, bf16     h 125-135, da and db 208 (a and b again), dx 147, dWg and dWu 115 + 15
-//   30,000 rows of 256 to 683, float      h 229, da and db 77, dx 194, dWg and dWu 212 + 18
-//   one row of 256 to 1,024               3.5; of 4,096 to 8,192 30 (4.5 TB/s), 64 such rows 46 to 50
+//   16,384 rows of 4,096 to 8,192, bf16   h 1,890 (1,160 TFLOP/s), da and db 345 (5.4 TB/s), weights turned 52, dx 1,849
+//                                         (1,190), dWg and dWu 1,805 (1,220)
+//   81,920 rows of 256 to 1,024, bf16     h 133, da and db 204 (a and b again), dx 145, dWg and dWu 113 + 14
+//   30,000 rows of 256 to 683, float      h 225, da and db 74, dx 189, dWg and dWu 209 + 18
+//   one row of 256 to 1,024               3.5; of 4,096 to 8,192 33 (4.1 TB/s), 64 such rows 46 to 51
 // The matrix cores are busy 60% of the wide bf16 products' time at some 2.1 GHz, and their power holds the
 // clock there; 75% of the float products'. Rows of 256 have 4 steps: bound by the results' traffic (h alone is
 // 168 MB) and by how little of it overlaps with the products. Few rows are bound by the weights' traffic.
@@ -300,7 +300,7 @@ struct Product {
 
 // Tile `n` of nl x nr, spread so that an XCD (workgroups are given to the eight in turn) works on
 // neighbouring tiles, kBand right tiles by all left ones: what they share stays in its L2. Bands of 2, 4, 8 and
-// 12, us: a training pass of 16,384 rows of 4,096 to 8,192 5,940, 5,990, 6,100 and 6,700, of 8,192 of 8,192 5,980,
+// 12, us: a training pass of 16,384 rows of 4,096 to 8,192 5,940, 5,990, 6,100 and 6,650, of 8,192 of 8,192 5,980,
 // 6,020, 6,360, of 16,384 of 2,048 to 4,096 1,730, 1,670, 1,660.
 constexpr int kXcds = 8, kBand = 4;
 __device__ __forceinline__ void tile_of(uint32_t n, uint32_t nl, uint32_t nr, int *l, int *r) {
