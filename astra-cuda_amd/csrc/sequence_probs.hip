@@ -275,6 +275,49 @@ __device__ __forceinline__ void in_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// A wavefront's largest entries, sorted, of those in its lanes' registers. The top-th largest of
+// the lanes' maxima is a bound below them all: what reaches it (some 25 of 2,048 entries for the top
+// 20, if they are in no order) is gathered in LDS and sorted 64 at a time.
+// `from`: the indices of a lane's vectors.
+template <int C>
+__device__ __forceinline__ uint64_t largest_of(const float (&v)[C][V], const int (&from)[C], float lane_max, int top, uint64_t *gather, int lane) {
+  uint32_t bound = (uint32_t)(key_of(lane_max, 0) >> 32);
+  sort(bound, lane);
+  bound = __builtin_amdgcn_readlane(bound, top - 1);
+  const float least = bound ? value_of((uint64_t)bound << 32) : -INFINITY;
+  uint64_t best = 0, last = 0;
+  int have = 0;
+  const auto take = [&](int n) __attribute__((always_inline)) {
+    in_order();
+    uint64_t k = lane < n ? gather[lane] : 0;
+    const uint64_t rest = gather[64 + lane];
+    in_order();
+    gather[lane] = rest;
+    if (!__ballot(k > last)) return;
+    sort(k, lane);
+    best = joined(best, k, lane);
+    last = lane_of(best, top - 1);
+  };
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!__ballot(v[c][j] >= least)) continue;
+      const uint64_t key = key_of(v[c][j], from[c] + j);
+      const bool in = key > last && v[c][j] >= least;
+      const uint64_t who = __ballot(in);
+      if (!who) continue;
+      if (in) gather[have + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
+      have += __popcll(who);
+      if (have >= 64) {
+        take(64);
+        have -= 64;
+      }
+    }
+  if (have) take(have);
+  return best;
+}
+
 __device__ __forceinline__ void store_top(const ProbArgs &a, int64_t at, uint64_t key, const Result &r) {
   a.top_log_prob[at] = key ? value_of(key) - r.most - r.log_z : -INFINITY;
   a.top_index[at] = key ? index_of(key) : -1;
@@ -295,7 +338,7 @@ struct Out {
 };
 // One part of the workgroup's rows: G lanes a row, V entries each, C times.
 template <class T, int G, int C, bool TOP>
-__device__ void narrow_part(const ProbArgs &a, Out &out, int part, int64_t first, int rows, int turn) {
+__device__ void narrow_part(const ProbArgs &a, Out &out, uint64_t *gather, int part, int64_t first, int rows, int turn) {
   constexpr int kEach = kWave / G;
   const int begin = a.begin[part], size = a.begin[part + 1] - begin, lane = threadIdx.x % kWave, j = lane % G;
   const T *logits = (const T *)a.logits + first * a.stride + begin;
@@ -342,7 +385,15 @@ __device__ void narrow_part(const ProbArgs &a, Out &out, int part, int64_t first
       out.stats[n * kStats + 1] = r.log_z;
       out.stats[n * kStats + 2] = r.entropy;
     }
-    if constexpr (TOP) {  // the largest one after the other
+    // the largest one after the other, or by sorting (20,000 rows of 1,000, us: 3 of them 89, 5 116 / 95, 20
+    // 320 / 111, 64 915 / 185)
+    if (TOP && G == kWave && a.top > 4) {
+      int from[C];
+#pragma unroll
+      for (int k = 0; k < C; ++k) from[k] = e[k].from;
+      const uint64_t best = largest_of(v, from, most, a.top, gather, lane);
+      if (in && lane < a.top) store_top(a, unit * a.top + lane, best, r);
+    } else if constexpr (TOP) {
       uint32_t gone = 0;
       for (int t = 0; t < a.top; ++t) {
         uint64_t best = 0;
@@ -373,6 +424,7 @@ __device__ void narrow_part(const ProbArgs &a, Out &out, int part, int64_t first
 template <class T, bool TOP>
 __global__ __launch_bounds__(256) void narrow_forward_kernel(ProbArgs a) {
   __shared__ Out out;
+  __shared__ uint64_t gather[TOP ? 4 : 1][128];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t first = (int64_t)blockIdx.x * a.block_rows;
   const int rows = (int)min((int64_t)a.block_rows, a.R - first);
@@ -380,23 +432,23 @@ __global__ __launch_bounds__(256) void narrow_forward_kernel(ProbArgs a) {
     const int size = a.begin[part + 1] - a.begin[part], turn = (wave + part) & 3;
     if (size > a.narrow) continue;
     if (size <= V)
-      narrow_part<T, 1, 1, TOP>(a, out, part, first, rows, turn);
+      narrow_part<T, 1, 1, TOP>(a, out, gather[wave], part, first, rows, turn);
     else if (size <= 2 * V)
-      narrow_part<T, 2, 1, TOP>(a, out, part, first, rows, turn);
+      narrow_part<T, 2, 1, TOP>(a, out, gather[wave], part, first, rows, turn);
     else if (size <= 4 * V)
-      narrow_part<T, 4, 1, TOP>(a, out, part, first, rows, turn);
+      narrow_part<T, 4, 1, TOP>(a, out, gather[wave], part, first, rows, turn);
     else if (size <= 8 * V)
-      narrow_part<T, 8, 1, TOP>(a, out, part, first, rows, turn);
+      narrow_part<T, 8, 1, TOP>(a, out, gather[wave], part, first, rows, turn);
     else if (size <= 16 * V)
-      narrow_part<T, 16, 1, TOP>(a, out, part, first, rows, turn);
+      narrow_part<T, 16, 1, TOP>(a, out, gather[wave], part, first, rows, turn);
     else if (size <= 32 * V)
-      narrow_part<T, 32, 1, TOP>(a, out, part, first, rows, turn);
+      narrow_part<T, 32, 1, TOP>(a, out, gather[wave], part, first, rows, turn);
     else if (size <= 64 * V)
-      narrow_part<T, 64, 1, TOP>(a, out, part, first, rows, turn);
-    else if (TOP || size <= 128 * V)
-      narrow_part<T, 64, 2, TOP>(a, out, part, first, rows, turn);
-    else if constexpr (!TOP)
-      narrow_part<T, 64, 4, TOP>(a, out, part, first, rows, turn);
+      narrow_part<T, 64, 1, TOP>(a, out, gather[wave], part, first, rows, turn);
+    else if (size <= 128 * V)
+      narrow_part<T, 64, 2, TOP>(a, out, gather[wave], part, first, rows, turn);
+    else
+      narrow_part<T, 64, 4, TOP>(a, out, gather[wave], part, first, rows, turn);
   }
   __syncthreads();
   const int64_t at = first * a.parts;
@@ -594,47 +646,6 @@ __global__ __launch_bounds__(256) void wide_forward_kernel(ProbArgs a) {
 constexpr int kVectors = 4, kPiece = 256 * V * kVectors, kCut = 4 * kPiece;
 __host__ __device__ inline int pieces_of(int size) { return (size + kPiece - 1) / kPiece; }
 
-// A wavefront's largest entries, sorted, of those in its lanes' registers. The top-th largest of
-// the lanes' maxima is a bound below them all: what reaches it (some 25 of 2,048 entries for the top
-// 20, if they are in no order) is gathered in LDS and sorted 64 at a time.
-__device__ __forceinline__ uint64_t largest_of(const float (&v)[kVectors][V], int first, float lane_max, int top, uint64_t *gather, int lane) {
-  uint32_t bound = (uint32_t)(key_of(lane_max, 0) >> 32);
-  sort(bound, lane);
-  bound = __builtin_amdgcn_readlane(bound, top - 1);
-  const float least = bound ? value_of((uint64_t)bound << 32) : -INFINITY;
-  uint64_t best = 0, last = 0;
-  int have = 0;
-  const auto take = [&](int n) __attribute__((always_inline)) {
-    in_order();
-    uint64_t k = lane < n ? gather[lane] : 0;
-    const uint64_t rest = gather[64 + lane];
-    in_order();
-    gather[lane] = rest;
-    if (!__ballot(k > last)) return;
-    sort(k, lane);
-    best = joined(best, k, lane);
-    last = lane_of(best, top - 1);
-  };
-#pragma unroll
-  for (int c = 0; c < kVectors; ++c)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (!__ballot(v[c][j] >= least)) continue;
-      const uint64_t key = key_of(v[c][j], first + (c * 256 + (int)threadIdx.x) * V + j);
-      const bool in = key > last && v[c][j] >= least;
-      const uint64_t who = __ballot(in);
-      if (!who) continue;
-      if (in) gather[have + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
-      have += __popcll(who);
-      if (have >= 64) {
-        take(64);
-        have -= 64;
-      }
-    }
-  if (have) take(have);
-  return best;
-}
-
 // The lists of WAVES wavefronts, joined in pairs; the first wavefront has the result.
 template <int WAVES>
 __device__ __forceinline__ uint64_t join_lists(uint64_t best, uint64_t (*lists)[64], int wave, int lane) {
@@ -685,7 +696,10 @@ __global__ __launch_bounds__(256) void piece_kernel(ProbArgs a) {
     out[2] = s.s;
   }
   if constexpr (TOP) {
-    uint64_t best = largest_of(v, first, lane_max, a.top, gather[wave], lane);
+    int from[kVectors];
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) from[k] = first + (k * 256 + (int)threadIdx.x) * V;
+    uint64_t best = largest_of(v, from, lane_max, a.top, gather[wave], lane);
     best = join_lists<4>(best, lists, wave, lane);
     if (wave == 0 && lane < a.top) {
       if (pieces == 1)
@@ -807,9 +821,9 @@ ProbArgs args_of(const astra_log_probs &f) {
   // Lanes' work ends with its loads, a workgroup's with two barriers. Both, us, the former first: 81,920
   // rows of 1,000 bf16 entries 51 / 95, of 1,500 73 / 136, of 2,048 81 / 106; of 1,000 floats 73 / 100, of
   // 1,500 107 / 133, but with the gradient 338 / 312. 16,384 rows of 1,000 bf16 entries 15 / 21, 4,096
-  // 9.9 / 9.2, 1,024 6.6 / 5.9. (The largest entries are taken one by one there.)
-  a.narrow = f.top || f.type == ASTRA_SEQ_F32 ? 1024 : 2048;
-  if (!f.top && f.rows < 8192) a.narrow = 512;
+  // 9.9 / 9.2, 1,024 6.6 / 5.9. The 20 largest too: 20,000 rows of 1,000 111 / 159, of 2,000 143 / 161, 4,096 of
+  // 1,000 53 / 39.
+  a.narrow = f.rows < 8192 ? 512 : f.type == ASTRA_SEQ_F32 && !f.top ? 1024 : 2048;
   a.cut = f.top > 0 || (f.rows * f.parts < 512 && largest > kCut);
   a.W = a.begin[f.parts];
   return a;

@@ -55,6 +55,21 @@ def test_many_rows(R, sizes, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("top", [1, 4, 5, 33, 64])
+@pytest.mark.parametrize("n", [256, 257, 511, 700, 1024, 1025, 2000])
+def test_top_of_many_rows(n, top, dtype):
+    """Rows with many ties, few or no allowed entries, and choices that do not count among them."""
+    from astra_cuda import sequence as seq
+    R = 8200
+    logits, choice, mask = make(n + top, R, [n], dtype)
+    logits[::3] = logits[::3].round()
+    logits[5], mask[6], mask[7, 3:], choice[8] = 0.0, False, False, -1
+    check(seq, logits, choice, [n], mask, top, 9)
+    logits, choice, mask = make(n + top, R, [n, 300], dtype)
+    check(seq, logits, choice, [n, 300], None, top, 10)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("top", [1, 2, 20, 63, 64])
 @pytest.mark.parametrize("n", [64, 100, 513, 1024, 1025, 30_000, 131_072])
 def test_top_with_ties_and_orders(n, top, dtype):
