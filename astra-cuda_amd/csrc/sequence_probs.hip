@@ -820,10 +820,9 @@ ProbArgs args_of(const astra_log_probs &f) {
   }
   // Lanes' work ends with its loads, a workgroup's with two barriers. Both, us, the former first: 81,920
   // rows of 1,000 bf16 entries 51 / 95, of 1,500 73 / 136, of 2,048 81 / 106; of 1,000 floats 73 / 100, of
-  // 1,500 107 / 133, but with the gradient 338 / 312. 16,384 rows of 1,000 bf16 entries 15 / 21, 4,096
-  // 9.9 / 9.2, 1,024 6.6 / 5.9. The 20 largest too: 20,000 rows of 1,000 111 / 159, of 2,000 143 / 161, 4,096 of
-  // 1,000 53 / 39.
-  a.narrow = f.rows < 8192 ? 512 : f.type == ASTRA_SEQ_F32 && !f.top ? 1024 : 2048;
+  // 1,500 107 / 133, but with the gradient 338 / 312. 4,096 rows of 1,000 bf16 entries with the gradient 15 / 19, 512
+  // alike. The 20 largest: 20,000 rows of 1,000 111 / 159, of 2,000 143 / 161, 4,096 of 1,000 29 / 38.
+  a.narrow = f.rows < 512 && !f.top ? 512 : f.type == ASTRA_SEQ_F32 && !f.top ? 1024 : 2048;
   a.cut = f.top > 0 || (f.rows * f.parts < 512 && largest > kCut);
   a.W = a.begin[f.parts];
   return a;
@@ -842,13 +841,18 @@ int64_t share(ProbArgs &a, Each &&each) {
   return n;
 }
 
-// Rows of a workgroup that has all their smaller parts: few where there are few, so that all CUs
-// have some, and as many as LDS has room for. One / eight / these, us, with the gradient: parts of
-// 127, 127, 6, 6, 81,920 rows 381 / 77 / 56, 16,384 rows 83 / 25 / 25, 4,096 rows 28 / 20 / 22; one of 64,
-// 81,920 rows 233 / 41 / 20.
+// Rows of a workgroup that has all their smaller parts: enough for its four wavefronts where there are 512
+// such workgroups, and more of them, up to what LDS has room for, where there are many. One / eight / these,
+// us, with the gradient: parts of 127, 127, 6, 6, 81,920 rows 381 / 77 / 56, 16,384 rows 83 / 25 / 25; one of 64, 81,920
+// rows 233 / 41 / 20. More only with 4,096 workgroups / these: 7,235 rows of 64 18 / 9, of four parts 25 / 18, the
+// largest of 64 39 / 8.
 int rows_together(const ProbArgs &a) {
-  int n = 1;
-  while (2 * n * a.parts <= kUnits && 2 * n <= 64 && a.R >= 4096 * n) n *= 2;
+  int n = 1, lanes = 1;  // lanes: of the largest part
+  for (int i = 0; i < a.parts; ++i)
+    if (a.begin[i + 1] - a.begin[i] <= a.narrow)
+      while (lanes < kWave && lanes * V < a.begin[i + 1] - a.begin[i]) lanes *= 2;
+  const int busy = std::max(1, 4 * kWave / lanes / a.parts);
+  while (2 * n * a.parts <= kUnits && 2 * n <= 64 && a.R >= (n < busy ? 512 : 4096) * n) n *= 2;
   return n;
 }
 bool some_narrow(const ProbArgs &a) {
