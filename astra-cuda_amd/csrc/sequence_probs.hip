@@ -318,9 +318,12 @@ __device__ __forceinline__ uint64_t largest_of(const float (&v)[C][V], const int
   return best;
 }
 
+__device__ __forceinline__ void store_top(const ProbArgs &a, int64_t at, bool some, float x, int64_t index, const Result &r) {
+  a.top_log_prob[at] = some ? x - r.most - r.log_z : -INFINITY;
+  a.top_index[at] = some ? index : -1;
+}
 __device__ __forceinline__ void store_top(const ProbArgs &a, int64_t at, uint64_t key, const Result &r) {
-  a.top_log_prob[at] = key ? value_of(key) - r.most - r.log_z : -INFINITY;
-  a.top_index[at] = key ? index_of(key) : -1;
+  store_top(a, at, key != 0, value_of(key), index_of(key), r);
 }
 
 // The log probability of choice c, entry x.
@@ -385,44 +388,48 @@ __device__ void narrow_part(const ProbArgs &a, Out &out, uint64_t *gather, int p
       out.stats[n * kStats + 1] = r.log_z;
       out.stats[n * kStats + 2] = r.entropy;
     }
-    // the largest one after the other, or by sorting (20,000 rows of 1,000, us: 3 of them 89, 5 116 / 95, 20
-    // 320 / 111, 64 915 / 185)
-    if (TOP && G == kWave && a.top > 4) {
+    // the largest one after the other, or by sorting (20,000 rows of 1,000, us: 3 of them 34 / 42, 7 49 / 43, 20
+    // 99 / 48, 64 273 / 80; of 400 5 of them 27 / 32, 7 32 / 32; of 2,000 3 of them 50 / 54, 7 72 / 54)
+    if (TOP && G == kWave && a.top > 6) {
       int from[C];
 #pragma unroll
       for (int k = 0; k < C; ++k) from[k] = e[k].from;
       const uint64_t best = largest_of(v, from, most, a.top, gather, lane);
       if (in && lane < a.top) store_top(a, unit * a.top + lane, best, r);
     } else if constexpr (TOP) {
-      uint32_t gone = 0;
       for (int t = 0; t < a.top; ++t) {
-        uint64_t best = 0;
-        int which = 0;
+        float large = -INFINITY;
 #pragma unroll
         for (int k = 0; k < C; ++k)
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const uint64_t key = gone >> (k * V + i) & 1 ? 0 : key_of(v[k][i], e[k].from + i);
-            which = key > best ? k * V + i : which;
-            best = key > best ? key : best;
-          }
-        uint64_t all = best;
-        if constexpr (G >= 2) all = larger(all, across<1>(all, lane));
-        if constexpr (G >= 4) all = larger(all, across<2>(all, lane));
-        if constexpr (G >= 8) all = larger(all, across<4>(all, lane));
-        if constexpr (G >= 16) all = larger(all, across<8>(all, lane));
-        if constexpr (G >= 32) all = larger(all, across<16>(all, lane));
-        if constexpr (G >= 64) all = larger(all, across<32>(all, lane));
-        if (best == all) gone |= 1u << which;
-        if (in && j == 0) store_top(a, unit * a.top + t, all, r);
+          for (int i = 0; i < V; ++i) large = fmaxf(large, v[k][i]);
+        large = lanes_max<G>(large);
+        uint32_t index = ~0u;  // the first of them
+#pragma unroll
+        for (int k = C - 1; k >= 0; --k)
+#pragma unroll
+          for (int i = V - 1; i >= 0; --i) index = v[k][i] == large ? e[k].from + i : index;
+        if constexpr (G >= 2) index = min(index, across<1>(index, lane));
+        if constexpr (G >= 4) index = min(index, across<2>(index, lane));
+        if constexpr (G >= 8) index = min(index, across<4>(index, lane));
+        if constexpr (G >= 16) index = min(index, across<8>(index, lane));
+        if constexpr (G >= 32) index = min(index, across<16>(index, lane));
+        if constexpr (G >= 64) index = min(index, across<32>(index, lane));
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[k][i] = e[k].from + i == (int)index ? -INFINITY : v[k][i];
+        if (in && j == 0) store_top(a, unit * a.top + t, large > -INFINITY, large, index, r);
       }
     }
   }
 }
 
-// A workgroup has block_rows rows, its wavefronts take turns with them.
-template <class T, bool TOP>
-__global__ __launch_bounds__(256) void narrow_forward_kernel(ProbArgs a) {
+// A workgroup has block_rows rows, its wavefronts take turns with them. BIG: with parts of more than 512
+// entries, whose registers the others do without (168 and 72 with the largest: 81,920 rows of 400, the
+// likeliest, 71 and 43 us); three workgroups a CU, or four and 11 to 77 spilled (2,000 entries 113 and 128 us).
+template <class T, bool TOP, bool BIG>
+__global__ __launch_bounds__(256, BIG && TOP ? 3 : 1) void narrow_forward_kernel(ProbArgs a) {
   __shared__ Out out;
   __shared__ uint64_t gather[TOP ? 4 : 1][128];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -443,12 +450,14 @@ __global__ __launch_bounds__(256) void narrow_forward_kernel(ProbArgs a) {
       narrow_part<T, 16, 1, TOP>(a, out, gather[wave], part, first, rows, turn);
     else if (size <= 32 * V)
       narrow_part<T, 32, 1, TOP>(a, out, gather[wave], part, first, rows, turn);
-    else if (size <= 64 * V)
+    else if (!BIG || size <= 64 * V)
       narrow_part<T, 64, 1, TOP>(a, out, gather[wave], part, first, rows, turn);
-    else if (size <= 128 * V)
-      narrow_part<T, 64, 2, TOP>(a, out, gather[wave], part, first, rows, turn);
-    else
-      narrow_part<T, 64, 4, TOP>(a, out, gather[wave], part, first, rows, turn);
+    else if constexpr (BIG) {
+      if (size <= 128 * V)
+        narrow_part<T, 64, 2, TOP>(a, out, gather[wave], part, first, rows, turn);
+      else
+        narrow_part<T, 64, 4, TOP>(a, out, gather[wave], part, first, rows, turn);
+    }
   }
   __syncthreads();
   const int64_t at = first * a.parts;
@@ -821,7 +830,7 @@ ProbArgs args_of(const astra_log_probs &f) {
   // Lanes' work ends with its loads, a workgroup's with two barriers. Both, us, the former first: 81,920
   // rows of 1,000 bf16 entries 51 / 95, of 1,500 73 / 136, of 2,048 81 / 106; of 1,000 floats 73 / 100, of
   // 1,500 107 / 133, but with the gradient 338 / 312. 4,096 rows of 1,000 bf16 entries with the gradient 15 / 19, 512
-  // alike. The 20 largest: 20,000 rows of 1,000 111 / 159, of 2,000 143 / 161, 4,096 of 1,000 29 / 38.
+  // alike. The 20 largest: 20,000 rows of 1,000 48 / 159, of 2,000 61 / 161.
   a.narrow = f.rows < 512 && !f.top ? 512 : f.type == ASTRA_SEQ_F32 && !f.top ? 1024 : 2048;
   a.cut = f.top > 0 || (f.rows * f.parts < 512 && largest > kCut);
   a.W = a.begin[f.parts];
@@ -845,7 +854,7 @@ int64_t share(ProbArgs &a, Each &&each) {
 // such workgroups, and more of them, up to what LDS has room for, where there are many. One / eight / these,
 // us, with the gradient: parts of 127, 127, 6, 6, 81,920 rows 381 / 77 / 56, 16,384 rows 83 / 25 / 25; one of 64, 81,920
 // rows 233 / 41 / 20. More only with 4,096 workgroups / these: 7,235 rows of 64 18 / 9, of four parts 25 / 18, the
-// largest of 64 39 / 8.
+// likeliest of 64 39 / 8.
 int rows_together(const ProbArgs &a) {
   int n = 1, lanes = 1;  // lanes: of the largest part
   for (int i = 0; i < a.parts; ++i)
@@ -930,10 +939,20 @@ int forward(ProbArgs a, hipStream_t st) {
   if (a.lists) a.pieces = (float *)(a.lists + all_pieces(a) * a.top);
   if (some_narrow(a)) {
     a.block_rows = rows_together(a);
-    if (a.top) {
-      PROBS_LAUNCH((narrow_forward_kernel<T, true>), cdiv(a.R, a.block_rows), 256);
+    bool big = false;
+    for (int i = 0; i < a.parts; ++i) {
+      const int size = a.begin[i + 1] - a.begin[i];
+      big |= size > 64 * V && size <= a.narrow;
+    }
+    const int64_t blocks = cdiv(a.R, a.block_rows);
+    if (a.top && big) {
+      PROBS_LAUNCH((narrow_forward_kernel<T, true, true>), blocks, 256);
+    } else if (a.top) {
+      PROBS_LAUNCH((narrow_forward_kernel<T, true, false>), blocks, 256);
+    } else if (big) {
+      PROBS_LAUNCH((narrow_forward_kernel<T, false, true>), blocks, 256);
     } else {
-      PROBS_LAUNCH((narrow_forward_kernel<T, false>), cdiv(a.R, a.block_rows), 256);
+      PROBS_LAUNCH((narrow_forward_kernel<T, false, false>), blocks, 256);
     }
   }
   if (!some_wide(a)) return ASTRA_OK;
