@@ -115,3 +115,42 @@ def test_a_move_and_whole_games_agree():
     lp, h = seq.log_probs(logits, choice, sizes=SIZES, mask=allowed)
     parts = [seq.log_probs(logits[:, t], choice[:, t], sizes=SIZES, mask=allowed[:, t]) for t in range(12)]
     assert torch.equal(lp, torch.stack([p[0] for p in parts], 1)) and torch.equal(h, torch.stack([p[1] for p in parts], 1))
+
+
+def test_two_streams_and_two_graphs_at_once():
+    """Calls that use a workspace (copies, slices, pieces) side by side, eager and replayed, share none."""
+    from astra_cuda import sequence as seq
+    g = torch.Generator(device=DEV)
+    g.manual_seed(6)
+    def make():
+        x = torch.randn(300, 1003, generator=g, device=DEV).bfloat16().requires_grad_()
+        w = [(torch.randn(210, 1003, generator=g, device=DEV) / 30).bfloat16().requires_grad_() for _ in range(2)]
+        logits = torch.randn(5, 90_001, generator=g, device=DEV).requires_grad_()
+        choice = torch.randint(0, 90_001, (5,), generator=g, device=DEV)
+        return x, w, logits, choice, torch.randn(300, 210, generator=g, device=DEV).bfloat16(), torch.randn(5, generator=g, device=DEV)
+    def run(x, w, logits, choice, dh, dl):
+        h = seq.gated_linear(x, *w, activation="gelu")
+        lp, e, tl, ti = seq.log_probs(logits, choice, top=9)
+        return [h.detach(), lp.detach(), e.detach(), tl, ti, *torch.autograd.grad(h, (x, *w), dh), *torch.autograd.grad([lp, e], logits, [dl, dl])]
+    sets = [make(), make()]
+    want = [run(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        got = []
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                got.append(run(*s))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+    graphs, outs = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run(*s))
+    for _ in range(5):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(outs, want) for a, b in zip(x, y))
