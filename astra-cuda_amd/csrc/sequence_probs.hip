@@ -17,7 +17,7 @@
 //   81,920 rows of parts of 127, 127, 6, 6      31, 37: half of the vector units' time, and short of wavefronts
 //                                               (3.5 a SIMD) to cover the loads' latency with
 //   64 rows of parts of 10, 10, 3, 3            4: the launch
-//   64 rows of 131,072 bf16 entries, top 20     14 + 6; one row of 65,537 floats, top 5, 10 + 6: two launches and
+//   64 rows of 131,072 bf16 entries, top 20     14 + 6; one row of 65,537 floats, top 5, 8 + 6: two launches and
 //                                               the latency inside of them
 #include <algorithm>
 #include <type_traits>
@@ -47,7 +47,8 @@ struct ProbArgs {
   int64_t R, stride, mask_stride;
   int32_t W, parts, top, wide_choice;
   int32_t narrow;              // parts up to here are a group of lanes' work, larger ones workgroups'
-  bool cut;                    // whether larger parts go through in pieces
+  bool cut;                    // whether larger parts go through in pieces,
+  int32_t piece;               // of so many entries
   int32_t block_rows;          // rows of a workgroup that has all their parts
   int32_t begin[kParts + 1];   // of each part in a row
   int64_t block[kParts + 1];   // the first workgroup of each part in this launch
@@ -648,12 +649,14 @@ __global__ __launch_bounds__(256) void wide_forward_kernel(ProbArgs a) {
   if (threadIdx.x == 0) store_result(a, unit, c, x, mask, result_of(s));
 }
 
-// Few rows of many entries, or the largest entries wanted: a workgroup has kPiece entries in registers.
+// Few rows of many entries, or the largest entries wanted: a workgroup has a piece of 256 x 8 x N entries in
+// registers. N is 4, and 2 where that leaves CUs without one (one row of 65,537 floats, the 5 likeliest, 9.7 / 7.6 us,
+// but 64 rows of 131,072 14.9 / 18.5).
 // In pieces and joined, or a workgroup a row, us: one row of 130,000 bf16 entries 6.9 / 25.9, of 50,000
 // 6.6 / 11.5, of 20,000 6.7 / 6.2, of 1,500 4.5 / 3.5; 256 rows 26 / 49, 15 / 22, 10.6 / 9.0, 5.0 / 4.0;
 // 511 rows of 50,000 22 / 24, 1,024 rows 37 / 27.
-constexpr int kVectors = 4, kPiece = 256 * V * kVectors, kCut = 4 * kPiece;
-__host__ __device__ inline int pieces_of(int size) { return (size + kPiece - 1) / kPiece; }
+constexpr int kPiece = 256 * V * 4, kCut = 4 * kPiece;
+__host__ __device__ inline int pieces_of(const ProbArgs &a, int size) { return (size + a.piece - 1) / a.piece; }
 
 // The lists of WAVES wavefronts, joined in pairs; the first wavefront has the result.
 template <int WAVES>
@@ -669,30 +672,30 @@ __device__ __forceinline__ uint64_t join_lists(uint64_t best, uint64_t (*lists)[
   return best;
 }
 
-template <class T, bool TOP>
+template <class T, bool TOP, int N>
 __global__ __launch_bounds__(256) void piece_kernel(ProbArgs a) {
   __shared__ float lds[3][4];
   __shared__ uint64_t gather[TOP ? 4 : 1][128], lists[TOP ? 4 : 1][64];
   int64_t n;
   const int part = part_of(a, &n);
-  const int begin = a.begin[part], size = a.begin[part + 1] - begin, pieces = pieces_of(size);
+  const int begin = a.begin[part], size = a.begin[part + 1] - begin, pieces = pieces_of(a, size);
   const int64_t row = n / pieces, unit = row * a.parts + part;
-  const int first = (int)(n - row * pieces) * kPiece;
+  const int first = (int)(n - row * pieces) * (256 * V * N);
   const T *x = (const T *)a.logits + row * a.stride + begin;
   const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride + begin : nullptr;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int c = choice_of(a, unit, size);
-  float v[kVectors][V];
+  float v[N][V];
 #pragma unroll
-  for (int k = 0; k < kVectors; ++k) load_entries(x, mask, first + (k * 256 + (int)threadIdx.x) * V, c == -1 ? 0 : size, v[k]);
+  for (int k = 0; k < N; ++k) load_entries(x, mask, first + (k * 256 + (int)threadIdx.x) * V, c == -1 ? 0 : size, v[k]);
   float lane_max = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < kVectors; ++k)
+  for (int k = 0; k < N; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) lane_max = fmaxf(lane_max, v[k][j]);
   Seen s{block_max<4>(lane_max, lds[0]), 0.f, 0.f};
 #pragma unroll
-  for (int k = 0; k < kVectors; ++k) add(s, v[k]);
+  for (int k = 0; k < N; ++k) add(s, v[k]);
   s.z = block_sum<4>(s.z, lds[1]);
   s.s = block_sum<4>(s.s, lds[2]);
   const Result r = result_of(s);
@@ -705,9 +708,9 @@ __global__ __launch_bounds__(256) void piece_kernel(ProbArgs a) {
     out[2] = s.s;
   }
   if constexpr (TOP) {
-    int from[kVectors];
+    int from[N];
 #pragma unroll
-    for (int k = 0; k < kVectors; ++k) from[k] = first + (k * 256 + (int)threadIdx.x) * V;
+    for (int k = 0; k < N; ++k) from[k] = first + (k * 256 + (int)threadIdx.x) * V;
     uint64_t best = largest_of(v, from, lane_max, a.top, gather[wave], lane);
     best = join_lists<4>(best, lists, wave, lane);
     if (wave == 0 && lane < a.top) {
@@ -726,7 +729,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_pieces_kernel(ProbArgs a
   __shared__ float lds[3][kJoinWaves];
   __shared__ uint64_t lists[TOP ? kJoinWaves : 1][64];
   const int part = blockIdx.y;
-  const int begin = a.begin[part], size = a.begin[part + 1] - begin, pieces = pieces_of(size);
+  const int begin = a.begin[part], size = a.begin[part + 1] - begin, pieces = pieces_of(a, size);
   if (pieces == 1) return;
   const int64_t row = blockIdx.x, unit = row * a.parts + part, at = a.block[part] + row * pieces;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -834,6 +837,7 @@ ProbArgs args_of(const astra_log_probs &f) {
   a.narrow = f.rows < 512 && !f.top ? 512 : f.type == ASTRA_SEQ_F32 && !f.top ? 1024 : 2048;
   a.cut = f.top > 0 || (f.rows * f.parts < 512 && largest > kCut);
   a.W = a.begin[f.parts];
+  a.piece = f.rows < 256 && f.rows * cdiv(a.W, kPiece) < 256 ? kPiece / 2 : kPiece;
   return a;
 }
 
@@ -876,11 +880,11 @@ bool some_wide(const ProbArgs &a) {
 }
 
 int64_t all_pieces(ProbArgs &a) {  // (of the rows of a launch)
-  return share(a, [&](int size) { return a.R * pieces_of(size); });
+  return share(a, [&](int size) { return a.R * pieces_of(a, size); });
 }
 bool joins(const ProbArgs &a) {
   for (int i = 0; i < a.parts; ++i)
-    if (pieces_of(a.begin[i + 1] - a.begin[i]) > 1) return true;
+    if (pieces_of(a, a.begin[i + 1] - a.begin[i]) > 1) return true;
   return false;
 }
 // Rows that one launch of each kernel has room for: at most 1,024 threads a row, and 256 a span or piece.
@@ -926,7 +930,12 @@ size_t piece_bytes(ProbArgs a) {
 
 template <class T, bool TOP>
 int forward_in_pieces(ProbArgs &a, hipStream_t st) {
-  PROBS_LAUNCH((piece_kernel<T, TOP>), all_pieces(a), 256);
+  const int64_t pieces = all_pieces(a);
+  if (a.piece == kPiece) {
+    PROBS_LAUNCH((piece_kernel<T, TOP, 4>), pieces, 256);
+  } else {
+    PROBS_LAUNCH((piece_kernel<T, TOP, 2>), pieces, 256);
+  }
   if (!joins(a)) return ASTRA_OK;
   ASTRA_ABI_CHECK(a.R * 64 * kJoinWaves, <=, kMostThreads);
   hipLaunchKernelGGL((join_pieces_kernel<T, TOP>), dim3((unsigned)a.R, (unsigned)a.parts), dim3(64 * kJoinWaves), 0, st, a);

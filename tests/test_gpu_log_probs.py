@@ -308,10 +308,12 @@ def test_many_rows_of_larger_parts():
         within(v[:1], want[k], k)
     logits, choice, _ = make(15, 1, [9000], BF16)
     R = 2 ** 22 + 5
-    want = seq.log_probs(logits, choice[:, 0], top=1)
+    want = part(logits, None, choice[:, 0], 1, None, None, BF16)
     got = seq.log_probs(logits.expand(R, 9000), choice[:, 0].expand(R), top=1)
-    for v, w in zip(got, want):
-        assert bool((v == w).all())
+    for v, k in zip(got, ("log_prob", "entropy", "top_log_prob")):
+        assert bool((v == v[0]).all())
+        within(v[:1], want[k], k)
+    assert bool((got[3] == want["top_index"]).all())
 
 
 def test_gradient_of_many_rows_of_larger_parts():
