@@ -492,11 +492,9 @@ __global__ __launch_bounds__(P::kThreads, P::GROUPS * P::NW / 4) void gated_kern
 }
 
 // The results from a and b that are in memory: sums of slices, or what the forward call kept for the
-// gradient (one slice). 2^shift threads a row.
+// gradient (one slice). 2^shift threads a row; a launch has room for some of very many rows.
 template <class T, bool GRAD>
-__global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs g, const float *ab, int shift) {
-  const int64_t m = (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
-  if (m >= g.M) return;
+__device__ __forceinline__ void gated_join_row(const GatedArgs &g, const float *ab, int shift, int64_t m) {
   const int64_t size = g.M * g.F, row = m * g.F;
   const int F = (int)g.F, Fp = (int)g.Fp;
   for (int f = (threadIdx.x & ((1 << shift) - 1)) * 8; f < (GRAD ? Fp : F); f += 8 << shift) {
@@ -528,6 +526,12 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs g, const floa
       }
     }
   }
+}
+template <class T, bool GRAD>
+__global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs g, const float *ab, int shift) {
+  const int each = 256 >> shift;
+  for (int64_t m = (int64_t)blockIdx.x * each + (threadIdx.x >> shift); m < g.M; m += (int64_t)gridDim.x * each)
+    gated_join_row<T, GRAD>(g, ab, shift, m);
 }
 
 // ------------------------------------------------------------------- gradients' products
@@ -873,6 +877,8 @@ using Small = Product<T, LTR, RTR, 4, 4, HALVES, 4>;
 using Alone = Product<bf16, true, true, 8, 4, false, 1, 2, 4>;
 
 constexpr int64_t kCus = 256;
+// Workgroups of 256 threads that go on to further rows where there are more than these have.
+constexpr int64_t kMostLoopBlocks = int64_t(1) << 20;
 template <class P>
 int64_t tiles(int64_t nl, int64_t nr) {
   return cdiv(nl, P::BLL) * cdiv(nr, P::BR);
@@ -895,7 +901,7 @@ bool larger(int64_t nl, int64_t nr, int64_t len) {
 #define GATED_LAUNCH(kernel, blocks, threads, ...)                                                   \
   do {                                                                                               \
     const int64_t blocks_ = (blocks);                                                                \
-    ASTRA_ABI_CHECK(blocks_, <, 2147483648ll);                                                       \
+    ASTRA_ABI_CHECK(blocks_ * (threads), <=, kMostThreads);                                          \
     hipLaunchKernelGGL((kernel), dim3((unsigned)blocks_), dim3(threads), 0, st, __VA_ARGS__);        \
     ASTRA_HIP_CHECK(rt_last_error(), #kernel " launch");                                             \
   } while (false)
@@ -918,7 +924,7 @@ int operands(const astra_gated_linear &f, char **ws, Operands *o, hipStream_t st
   if (!rows) return ASTRA_OK;
   int shift = 0;
   while (shift < 8 && ((int64_t)per16(f.type) << shift) < a.pitch) ++shift;
-  const dim3 grid((unsigned)std::min(cdiv(rows, 256 >> shift), int64_t(1) << 20), 3);
+  const dim3 grid((unsigned)std::min(cdiv(rows, 256 >> shift), kMostLoopBlocks), 3);
   hipLaunchKernelGGL(align_kernel<T>, grid, dim3(256), 0, st, a, shift);
   ASTRA_HIP_CHECK(rt_last_error(), "align_kernel launch");
   return ASTRA_OK;
@@ -928,7 +934,7 @@ template <class T, bool GRAD>
 int launch_join(GatedArgs g, const float *ab, hipStream_t st) {
   int shift = 4;
   while (shift < 8 && (int64_t(8) << shift) < g.F) ++shift;
-  GATED_LAUNCH((gated_join_kernel<T, GRAD>), cdiv(g.M, 256 >> shift), 256, g, ab, shift);
+  GATED_LAUNCH((gated_join_kernel<T, GRAD>), std::min(cdiv(g.M, 256 >> shift), kMostLoopBlocks), 256, g, ab, shift);
   return ASTRA_OK;
 }
 
