@@ -169,6 +169,10 @@ constexpr int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // error.
 constexpr int64_t kMostThreads = 4294967295ll;
 
+// Rows of gated_linear and log_probs: more than memory has room for the results of, and few enough that
+// every size of an operand or workspace fits 64 bits.
+constexpr int64_t kMostRows = int64_t(1) << 38;
+
 inline size_t elem_size(int32_t type) { return type == ASTRA_SEQ_BF16 ? 2 : 4; }
 
 }  // namespace astra_seq

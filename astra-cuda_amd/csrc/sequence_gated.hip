@@ -775,6 +775,7 @@ int check(const astra_gated_linear *f) {
   ASTRA_SEQ_POINTER(f);
   ASTRA_SEQ_TYPE_CHECK(f->type);
   ASTRA_ABI_CHECK(f->rows, >=, 0);
+  ASTRA_ABI_CHECK(f->rows, <=, kMostRows);
   ASTRA_ABI_CHECK(f->width, >=, 1);
   ASTRA_ABI_CHECK(f->width, <=, ASTRA_SEQ_MAX_LINEAR_WIDTH);
   ASTRA_ABI_CHECK(f->hidden, >=, 1);

@@ -792,6 +792,7 @@ int check(const astra_log_probs *f) {
   ASTRA_SEQ_POINTER(f);
   ASTRA_SEQ_TYPE_CHECK(f->type);
   ASTRA_ABI_CHECK(f->rows, >=, 0);
+  ASTRA_ABI_CHECK(f->rows, <=, kMostRows);
   ASTRA_ABI_CHECK(f->parts, >=, 1);
   ASTRA_ABI_CHECK(f->parts, <=, ASTRA_SEQ_MAX_PARTS);
   ASTRA_ABI_CHECK(f->top, >=, 0);

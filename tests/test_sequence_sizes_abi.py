@@ -1,0 +1,38 @@
+"""Sizes that no launch or workspace has room for are refused by the sequence operators' C entries, on the
+CPU, before any device call."""
+import ctypes
+
+import pytest
+
+from test_gated_linear_abi import _gated
+from test_sequence_abi import _lib
+
+
+def _probs(**kw):
+    from astra_cuda import _native
+    f = dict(logits=4096, choice=8192, log_prob=4096, entropy=4096, stats=4096, rows=3, stride=15, parts=2, choice_bytes=8,
+             sizes=(10, 5))
+    f.update(kw)
+    f["sizes"] = (ctypes.c_int32 * 16)(*f["sizes"])
+    return _native.LogProbs(**f)
+
+
+@pytest.mark.parametrize("rows", [2 ** 38 + 1, 2 ** 43, 2 ** 62, 2 ** 63 - 1])
+@pytest.mark.parametrize("name,make", [("gated_linear", _gated), ("log_probs", _probs)])
+def test_more_rows_than_sizes_of_64_bits(name, make, rows):
+    lib = _lib()
+    from astra_cuda import _native
+    f = make(rows=rows)
+    n = ctypes.c_size_t(0)
+    assert getattr(lib, f"astra_{name}_workspace_size")(ctypes.addressof(f), ctypes.byref(n)) == 1
+    assert getattr(lib, f"astra_{name}_forward")(ctypes.addressof(f), None) == 1
+    if name == "gated_linear":
+        assert lib.astra_gated_linear_grad_workspace_size(ctypes.addressof(f), ctypes.byref(n)) == 1
+        assert lib.astra_gated_linear_projections(ctypes.addressof(f), ctypes.byref(n)) == 1
+        g = _native.GatedLinearGrad(f=f, dh=4096, dx=4096, workspace=4096, workspace_bytes=1 << 62)
+        assert lib.astra_gated_linear_backward(ctypes.addressof(g), None) == 1
+    else:
+        g = _native.LogProbsGrad(f=f, dlogits=4096)
+        assert lib.astra_log_probs_backward(ctypes.addressof(g), None) == 1
+    f = make(rows=2 ** 38)
+    assert getattr(lib, f"astra_{name}_workspace_size")(ctypes.addressof(f), ctypes.byref(n)) == 0
