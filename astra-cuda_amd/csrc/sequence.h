@@ -183,6 +183,9 @@ inline size_t elem_size(int32_t type) { return type == ASTRA_SEQ_BF16 ? 2 : 4; }
     ASTRA_ABI_CHECK(t, <=, ASTRA_SEQ_BF16);          \
   } while (false)
 
+// One dimension of a launch has room for these workgroups.
+#define ASTRA_SEQ_LAUNCH_CHECK(blocks, threads) ASTRA_ABI_CHECK(blocks, <=, astra_seq::kMostThreads / (threads))
+
 #define ASTRA_SEQ_POINTER(p)                                                                      \
   do {                                                                                            \
     if ((p) == nullptr)                                                                           \

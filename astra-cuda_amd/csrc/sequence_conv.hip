@@ -389,7 +389,7 @@ int forward(const astra_short_conv &f, hipStream_t st) {
   const int v = wide<T, kForward<T>>(a, {a.x, a.window, a.y, a.last}), taps = f.taps;
   set_runs(a, a.D / v);
   const int64_t blocks = cdiv(a.B * a.runs * (a.D / v), 256);
-  ASTRA_ABI_CHECK(blocks, <, 2147483648ll);
+  ASTRA_SEQ_LAUNCH_CHECK(blocks, 256);
   CONV_DISPATCH(T, conv_forward_kernel, kForward<T>, dim3((unsigned)blocks));
   ASTRA_HIP_CHECK(rt_last_error(), "conv_forward_kernel launch");
   return ASTRA_OK;
@@ -446,7 +446,7 @@ int step(const astra_short_conv_one &o, hipStream_t st) {
   a.silu = o.activation == ASTRA_SEQ_SILU;
   const int v = wide<T, kForward<T>>(a, {a.x, a.dwindow, a.y}), taps = o.taps;
   const int64_t blocks = cdiv(a.B * (a.D / v), 256);
-  ASTRA_ABI_CHECK(blocks, <, 2147483648ll);
+  ASTRA_SEQ_LAUNCH_CHECK(blocks, 256);
   CONV_DISPATCH(T, conv_step_kernel, kForward<T>, dim3((unsigned)blocks));
   ASTRA_HIP_CHECK(rt_last_error(), "conv_step_kernel launch");
   return ASTRA_OK;

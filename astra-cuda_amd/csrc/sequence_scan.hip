@@ -1799,7 +1799,7 @@ int allow_lds(size_t bytes) {
 
 #define SCAN_LAUNCH(kernel, blocks, threads, bytes)                                                    \
   do {                                                                                                 \
-    ASTRA_ABI_CHECK(blocks, <, 2147483648ll);                                                          \
+    ASTRA_SEQ_LAUNCH_CHECK(blocks, threads);                                                           \
     if (int rc = allow_lds<&kernel>(bytes)) return rc;                                                 \
     hipLaunchKernelGGL((kernel), dim3((unsigned)(blocks)), dim3(threads), bytes, st, a);               \
     ASTRA_HIP_CHECK(rt_last_error(), #kernel " launch");                                               \
@@ -1813,7 +1813,9 @@ int states(ScanArgs &a, hipStream_t st) {
   else
     SCAN_LAUNCH((scan_states_kernel<T, PT, NT, PW, REV, KEEP, false>), blocks, 256 * PW, (StatesLds<T, PT, NT>::bytes));
   if (KEEP) return ASTRA_OK;
-  hipLaunchKernelGGL(scan_carry_kernel<REV>, dim3((unsigned)cdiv(a.B * a.H * a.P * a.N, 256)), dim3(256), 0, st, a);
+  const int64_t carries = cdiv(a.B * a.H * a.P * a.N, 256);
+  ASTRA_SEQ_LAUNCH_CHECK(carries, 256);
+  hipLaunchKernelGGL(scan_carry_kernel<REV>, dim3((unsigned)carries), dim3(256), 0, st, a);
   ASTRA_HIP_CHECK(rt_last_error(), "scan_carry_kernel launch");
   return ASTRA_OK;
 }
@@ -1853,7 +1855,9 @@ int backward(ScanArgs &a, hipStream_t st) {
   else
     SCAN_LAUNCH((scan_grad_kernel<T, PT, NT, false, true>), blocks, 512, (GradLds<T, PT, NT, false>::bytes));
   if (a.slices > 1) {
-    hipLaunchKernelGGL(scan_join_slices_kernel<T>, dim3((unsigned)cdiv(2 * a.B * a.T * a.G * a.N, 256)), dim3(256), 0, st, a);
+    const int64_t joins = cdiv(2 * a.B * a.T * a.G * a.N, 256);
+    ASTRA_SEQ_LAUNCH_CHECK(joins, 256);
+    hipLaunchKernelGGL(scan_join_slices_kernel<T>, dim3((unsigned)joins), dim3(256), 0, st, a);
     ASTRA_HIP_CHECK(rt_last_error(), "scan_join_slices_kernel launch");
   }
   return ASTRA_OK;
@@ -1891,7 +1895,7 @@ int step(const StepArgs &a, bool wide, hipStream_t st) {
 #define STEP_LAUNCH(V, LPR, NJ)                                                                       \
   do {                                                                                                \
     const int64_t blocks = cdiv(a.B * a.H * cdiv(a.P, kStepRows / LPR), 4);                           \
-    ASTRA_ABI_CHECK(blocks, <, 2147483648ll);                                                         \
+    ASTRA_SEQ_LAUNCH_CHECK(blocks, 256);                                                              \
     hipLaunchKernelGGL((scan_step_kernel<T, V, LPR, NJ>), dim3((unsigned)blocks), dim3(256), 0, st, a); \
   } while (false)
   if (wide) {

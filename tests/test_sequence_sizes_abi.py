@@ -36,3 +36,37 @@ def test_more_rows_than_sizes_of_64_bits(name, make, rows):
         assert lib.astra_log_probs_backward(ctypes.addressof(g), None) == 1
     f = make(rows=2 ** 38)
     assert getattr(lib, f"astra_{name}_workspace_size")(ctypes.addressof(f), ctypes.byref(n)) == 0
+
+
+@pytest.mark.parametrize("type", [0, 1])
+@pytest.mark.parametrize("width,batch", [(1, 2 ** 32), (129, 2 ** 25), (1, 2 ** 39)])
+def test_convolutions_of_more_than_2_to_the_32_threads(type, width, batch):
+    from astra_cuda import _native
+    lib = _lib()
+    f = _native.ShortConv(x=4098, weight=4096, y=4098, last=4098, batch=batch, length=1, width=width, taps=3, type=type,
+                          x_stride_b=width, x_stride_t=width)
+    assert lib.astra_short_conv_forward(ctypes.addressof(f), None) == 1
+    assert "blocks" in _native.last_error()
+    o = _native.ShortConvOne(x=4098, weight=4096, window=4098, y=4098, batch=batch, width=width, taps=3, type=type,
+                             x_stride_b=width)
+    assert lib.astra_short_conv_step(ctypes.addressof(o), None) == 1
+    assert "blocks" in _native.last_error()
+
+
+@pytest.mark.parametrize("type", [0, 1])
+@pytest.mark.parametrize("batch", [2 ** 24, 2 ** 31])
+def test_scans_of_more_than_2_to_the_32_threads(type, batch):
+    """(16 heads of one feature and state each.)"""
+    from astra_cuda import _native
+    lib = _lib()
+    p = dict(x=4096, dt=4096, b=4096, c=4096, A=4096)
+    size = dict(batch=batch, heads=16, dim=1, groups=16, state=1, type=type)
+    f = _native.StateScan(**p, y=4096, length=1, **size)
+    assert lib.astra_state_scan_forward(ctypes.addressof(f), None) == 1
+    assert "blocks" in _native.last_error()
+    g = _native.StateScanGrad(f=f, dy=4096, dx=4096, ddt=4096, db=4096, dc=4096, workspace=4096, workspace_bytes=1 << 62)
+    assert lib.astra_state_scan_backward(ctypes.addressof(g), None) == 1
+    assert "blocks" in _native.last_error()
+    o = _native.StateScanOne(**p, h=4096, y=4096, **size)
+    assert lib.astra_state_scan_step(ctypes.addressof(o), None) == 1
+    assert "blocks" in _native.last_error()
