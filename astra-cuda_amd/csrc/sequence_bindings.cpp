@@ -117,6 +117,14 @@ void check_once() {
   if (at::GradMode::is_enabled()) fatal("sequence: the operators can be differentiated once only (create_graph)");
 }
 
+// Whether a pass asks for the gradients of a node's tensors, one after the other in the order that the
+// node took them (absent ones have no edge). One that requires a gradient need not be asked for.
+struct Asked {
+  AutogradContext *ctx;
+  size_t edge = 0;
+  bool operator()(const Tensor &input) { return input.defined() && ctx->needs_input_grad(edge++); }
+};
+
 Tensor undefined_or_contiguous(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
 
 // ------------------------------------------------------------------------ short_conv
@@ -170,8 +178,9 @@ struct ShortConv : torch::autograd::Function<ShortConv> {
     if (!dy.defined() && !dlast.defined()) return out;
     const c10::DeviceGuard guard(x.device());
     if (!dy.defined()) dy = at::zeros(x.sizes(), x.options());
+    Asked asked{ctx};
     for (int i = 0; i < 4; ++i)
-      if (saved[i].defined() && saved[i].requires_grad()) out[i] = empty(saved[i], saved[i].sizes(), saved[i].scalar_type());
+      if (asked(saved[i])) out[i] = empty(saved[i], saved[i].sizes(), saved[i].scalar_type());
     astra_short_conv_grad g{};
     g.f = conv_struct(x, weight, bias, window, lengths, ctx->saved_data["activation"].toInt());
     g.dy = ptr(dy);
@@ -350,9 +359,11 @@ struct StateScan : torch::autograd::Function<StateScan> {
     if (!dy.defined() && !dfinal.defined()) return out;
     const c10::DeviceGuard guard(x.device());
     if (!dy.defined()) dy = at::zeros(x.sizes(), x.options());
-    for (int i : {0, 1, 3, 4}) out[i] = empty(s[i], s[i].sizes(), s[i].scalar_type());
-    for (int i : {2, 5, 6, 7})
-      if (s[i].defined() && s[i].requires_grad()) out[i] = empty(s[i]);
+    Asked asked{ctx};
+    for (int i = 0; i < 8; ++i) {
+      const bool always = i == 0 || i == 1 || i == 3 || i == 4;  // (of x, dt, B and C)
+      if (asked(s[i]) || always) out[i] = empty(s[i], s[i].sizes(), s[i].scalar_type());
+    }
     astra_state_scan_grad g{};
     g.f = scan_struct(x, dt, A, b, c, D, dt_bias, initial, lengths);
     g.f.chunk_states = ptr<float>(states);
@@ -524,8 +535,9 @@ struct JoinNorm : torch::autograd::Function<JoinNorm> {
     const Tensor &residual = s[0];
     const c10::DeviceGuard guard(residual.device());
     const bool any = residual.size(0) > 0;
+    Asked asked{ctx};
     for (int i = 0; i < 6; ++i)
-      if (s[i].defined() && s[i].requires_grad()) {
+      if (asked(s[i])) {
         out[i] = empty(s[i], s[i].sizes(), s[i].scalar_type());
         if (!any) out[i].zero_();
       }
@@ -659,8 +671,9 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     const Tensor dh = undefined_or_contiguous(grads[0]);
     if (!dh.defined()) return out;
     const c10::DeviceGuard guard(x.device());
+    Asked asked{ctx};
     for (int i = 0; i < 3; ++i)
-      if (s[i].requires_grad()) out[i] = empty(s[i], s[i].sizes(), s[i].scalar_type());
+      if (asked(s[i])) out[i] = empty(s[i], s[i].sizes(), s[i].scalar_type());
     astra_gated_linear_grad g{};
     g.f = gated_struct(x, gate, up, s[3], ctx->saved_data["activation"].toInt());
     g.dh = ptr(dh);
