@@ -123,7 +123,7 @@ def rms_norm(x, weight, *, eps=1e-6):
     return (_ops or _compiled()).rms_norm(x, weight, eps)
 
 
-def gated_linear(x, gate_weight, up_weight, *, activation="silu"):
+def gated_linear(x, gate_weight, up_weight, *, activation="silu", recompute=False):
     """The gated feed-forward block before its way back: ``act(x gate_weight^T) * (x up_weight^T)``.
 
     ``x`` ``[..., D]``, the weights ``[F, D]`` of x's type, as those of two ``nn.Linear``; returns
@@ -131,9 +131,11 @@ def gated_linear(x, gate_weight, up_weight, *, activation="silu"):
     at v, by erf). Bfloat16 products are summed in float32 and the result is rounded once; the
     gradients of the two projections are rounded to x's type before their own products. A forward
     pass that is differentiated keeps its inputs, and from a width of 1,024 (float32: 128) on the
-    two projections in float32, 8 bytes an element of the result.
+    two projections in float32, 8 bytes an element of the result, because the backward pass is faster
+    with them; with ``recompute`` it keeps its inputs alone and the backward pass computes the
+    projections again, which is as exact.
     """
-    return (_ops or _compiled()).gated_linear(x, gate_weight, up_weight, activation)
+    return (_ops or _compiled()).gated_linear(x, gate_weight, up_weight, activation, recompute)
 
 
 def log_probs(logits, choice=None, *, sizes=None, mask=None, top=0):

@@ -656,9 +656,10 @@ Tensor gated_forward(const Tensor &x, const Tensor &gate, const Tensor &up, int6
 }
 
 struct GatedLinear : torch::autograd::Function<GatedLinear> {
-  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &gate, const Tensor &up, int64_t activation) {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &gate, const Tensor &up, int64_t activation,
+                        bool recompute) {
     Tensor projections;
-    const Tensor h = gated_forward(x, gate, up, activation, &projections);
+    const Tensor h = gated_forward(x, gate, up, activation, recompute ? nullptr : &projections);
     ctx->save_for_backward({x, gate, up, projections});
     ctx->saved_data["activation"] = activation;
     return h;
@@ -667,7 +668,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     check_once();
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &gate = s[1], &up = s[2];
-    variable_list out(4);
+    variable_list out(5);
     const Tensor dh = undefined_or_contiguous(grads[0]);
     if (!dh.defined()) return out;
     const c10::DeviceGuard guard(x.device());
@@ -688,7 +689,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
   }
 };
 
-Tensor gated_linear(const Tensor &x_, const Tensor &gate_, const Tensor &up_, const std::string &activation) {
+Tensor gated_linear(const Tensor &x_, const Tensor &gate_, const Tensor &up_, const std::string &activation, bool recompute) {
   calls_only("gated_linear", x_, gate_, up_);
   check_data("x", x_);
   need(x_.dim() >= 1 && x_.size(-1) >= 1, "x", "must have shape [..., width], got " + shape_text(x_.sizes()));
@@ -701,7 +702,7 @@ Tensor gated_linear(const Tensor &x_, const Tensor &gate_, const Tensor &up_, co
   need(activation == "silu" || activation == "gelu", "activation", "must be 'silu' or 'gelu', got '" + activation + "'");
   const int64_t act = activation == "silu" ? ASTRA_SEQ_SILU : ASTRA_SEQ_GELU;
   const Tensor x = flat(x_), gate = rows(gate_), up = rows(up_);
-  const Tensor h = with_grad({&x, &gate, &up}) ? GatedLinear::apply(x, gate, up, act) : gated_forward(x, gate, up, act, nullptr);
+  const Tensor h = with_grad({&x, &gate, &up}) ? GatedLinear::apply(x, gate, up, act, recompute) : gated_forward(x, gate, up, act, nullptr);
   if (x_.dim() == 2) return h;
   std::vector<int64_t> shape(x_.sizes().begin(), x_.sizes().end());
   shape.back() = F;
@@ -852,7 +853,8 @@ void bind_sequence(py::module_ &m) {
   s.def("join_norm", &join_norm, py::arg("residual"), py::arg("block"), py::arg("post_weight"), py::arg("next_weight"),
         py::arg("gate"), py::arg("scale"), py::arg("eps"));
   s.def("rms_norm", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("eps"));
-  s.def("gated_linear", &gated_linear, py::arg("x"), py::arg("gate_weight"), py::arg("up_weight"), py::arg("activation"));
+  s.def("gated_linear", &gated_linear, py::arg("x"), py::arg("gate_weight"), py::arg("up_weight"), py::arg("activation"),
+        py::arg("recompute"));
   s.def("log_probs", &log_probs, py::arg("logits"), py::arg("choice"), py::arg("sizes"), py::arg("mask"), py::arg("top"));
   s.attr("MAX_TAPS") = ASTRA_SEQ_MAX_TAPS;
   s.attr("MAX_STATE") = ASTRA_SEQ_MAX_STATE;
