@@ -689,7 +689,8 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
   }
 };
 
-Tensor gated_linear(const Tensor &x_, const Tensor &gate_, const Tensor &up_, const std::string &activation, bool recompute) {
+Tensor gated_linear(const Tensor &x_, const Tensor &gate_, const Tensor &up_, const std::string &activation, bool recompute,
+                    bool exact_gradients) {
   calls_only("gated_linear", x_, gate_, up_);
   check_data("x", x_);
   need(x_.dim() >= 1 && x_.size(-1) >= 1, "x", "must have shape [..., width], got " + shape_text(x_.sizes()));
@@ -700,7 +701,7 @@ Tensor gated_linear(const Tensor &x_, const Tensor &gate_, const Tensor &up_, co
   check_like("gate_weight", gate_, x_, {F, D});
   check_like("up_weight", up_, x_, {F, D});
   need(activation == "silu" || activation == "gelu", "activation", "must be 'silu' or 'gelu', got '" + activation + "'");
-  const int64_t act = activation == "silu" ? ASTRA_SEQ_SILU : ASTRA_SEQ_GELU;
+  const int64_t act = (activation == "silu" ? ASTRA_SEQ_SILU : ASTRA_SEQ_GELU) | (exact_gradients ? ASTRA_SEQ_EXACT_GRADIENTS : 0);
   const Tensor x = flat(x_), gate = rows(gate_), up = rows(up_);
   const Tensor h = with_grad({&x, &gate, &up}) ? GatedLinear::apply(x, gate, up, act, recompute) : gated_forward(x, gate, up, act, nullptr);
   if (x_.dim() == 2) return h;
@@ -854,7 +855,7 @@ void bind_sequence(py::module_ &m) {
         py::arg("gate"), py::arg("scale"), py::arg("eps"));
   s.def("rms_norm", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("eps"));
   s.def("gated_linear", &gated_linear, py::arg("x"), py::arg("gate_weight"), py::arg("up_weight"), py::arg("activation"),
-        py::arg("recompute"));
+        py::arg("recompute"), py::arg("exact_gradients"));
   s.def("log_probs", &log_probs, py::arg("logits"), py::arg("choice"), py::arg("sizes"), py::arg("mask"), py::arg("top"));
   s.attr("MAX_TAPS") = ASTRA_SEQ_MAX_TAPS;
   s.attr("MAX_STATE") = ASTRA_SEQ_MAX_STATE;

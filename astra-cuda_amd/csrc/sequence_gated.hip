@@ -7,8 +7,10 @@
 // All are matrix products out[r, l] = sum_k left[l, k] right[r, k] on the matrix cores, with
 // what surrounds them done on the accumulators: 4 M D F operations forwards, 8 M D F backwards, and 4 M D F
 // again where a and b are computed a second time. Sums are float32; h is rounded once, da and db are
-// rounded to x's type before their products, as the matrix cores take them (2^-8 of bf16 each, which
-// makes the gradients' error 1.4 times that of h).
+// rounded to x's type before their products, as the matrix cores take them (2^-9 of bf16 each, which
+// makes the gradients' error 1.4 times that of h), or to two bf16 numbers each where the caller asks
+// for exact gradients: 8 M D F operations more, whole passes of 81,920 rows of 256 to 1,024 850 us and
+// not 580, of 16,384 rows of 4,096 to 8,192 9,800 and not 6,030.
 //
 // Measured (us; the card's large bf16 library product reaches 1,390 TFLOP/s, its float product 154,
 // its copies 4.8 TB/s):
@@ -370,6 +372,7 @@ struct GatedArgs {
   void *h;                   // [M, F]
   float *ab;                 // [2, M, F] (may be NULL): a and b, for the gradients
   void *dab;                 // [M, 2 Fp]: da, db, zero from F to Fp
+  void *rest;                // [M, 2 Fp] (may be NULL): what they lose when they are rounded to bf16
   int64_t M, F, Fp;
   int32_t kind;
   float *part;  // [slices, 2, M, F] or NULL: partial sums of a and b instead of results
@@ -386,6 +389,26 @@ __device__ __forceinline__ void slopes(const GatedArgs &g, const float (&a)[8], 
     act_slope<T>(a[i], g.kind, &v, &s);
     da[i] = i < n ? dh[i] * b[i] * s : 0.f;
     db[i] = i < n ? dh[i] * v : 0.f;
+  }
+}
+
+// da and db of 8 elements of a row, n of them inside, and with REST what they lose if it is wanted.
+template <class T, bool REST>
+__device__ __forceinline__ void store_slopes(const GatedArgs &g, int64_t at, float (&da)[8], float (&db)[8], int n) {
+  T *p = (T *)g.dab + at;
+  Loose<T, 8>::store(p, da, n);
+  Loose<T, 8>::store(p + g.Fp, db, n);
+  if constexpr (REST && sizeof(T) == 2) {
+    if (!g.rest) return;
+    const auto lost = [](float v) __attribute__((always_inline)) {
+      const float kept = (float)(bf16)v;
+      return fabsf(kept) < INFINITY ? v - kept : 0.f;  // (an infinity is whole, and so is a NaN)
+    };
+#pragma unroll
+    for (int i = 0; i < 8; ++i) da[i] = lost(da[i]), db[i] = lost(db[i]);
+    p = (T *)g.rest + at;
+    Loose<T, 8>::store(p, da, n);
+    Loose<T, 8>::store(p + g.Fp, db, n);
   }
 }
 
@@ -473,9 +496,7 @@ __global__ __launch_bounds__(P::kThreads, P::GROUPS * P::NW / 4) void gated_kern
           Loose<T, 8>::load((const T *)g.dh + start + at, dh, n);
         }
         slopes<T>(g, a, b, dh, da, db, n);
-        T *p = (T *)g.dab + m0 * 2 * g.Fp + f0 + (m * 2 * Fp + f);
-        Loose<T, 8>::store(p, da, zeros - f);
-        Loose<T, 8>::store(p + Fp, db, zeros - f);
+        store_slopes<T, true>(g, m0 * 2 * g.Fp + f0 + (m * 2 * Fp + f), da, db, zeros - f);
       } else {
         if (n <= 0) continue;
         float h[8];
@@ -493,7 +514,8 @@ __global__ __launch_bounds__(P::kThreads, P::GROUPS * P::NW / 4) void gated_kern
 
 // The results from a and b that are in memory: sums of slices, or what the forward call kept for the
 // gradient (one slice). 2^shift threads a row; a launch has room for some of very many rows.
-template <class T, bool GRAD>
+// (REST has registers of its own: with them the other bf16 gradients would have 7 wavefronts a SIMD and not 8.)
+template <class T, bool GRAD, bool REST>
 __device__ __forceinline__ void gated_join_row(const GatedArgs &g, const float *ab, int shift, int64_t m) {
   const int64_t size = g.M * g.F, row = m * g.F;
   const int F = (int)g.F, Fp = (int)g.Fp;
@@ -512,9 +534,7 @@ __device__ __forceinline__ void gated_join_row(const GatedArgs &g, const float *
       float dh[8], da[8], db[8];
       Loose<T, 8>::load((const T *)g.dh + row + f, dh, F - f);
       slopes<T>(g, a, b, dh, da, db, F - f);
-      T *out = (T *)g.dab + m * 2 * g.Fp + f;
-      Loose<T, 8>::store(out, da, Fp - f);
-      Loose<T, 8>::store(out + Fp, db, Fp - f);
+      store_slopes<T, REST>(g, m * 2 * g.Fp + f, da, db, Fp - f);
     } else {
       float h[8];
 #pragma unroll
@@ -527,17 +547,17 @@ __device__ __forceinline__ void gated_join_row(const GatedArgs &g, const float *
     }
   }
 }
-template <class T, bool GRAD>
+template <class T, bool GRAD, bool REST>
 __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs g, const float *ab, int shift) {
   const int each = 256 >> shift;
   for (int64_t m = (int64_t)blockIdx.x * each + (threadIdx.x >> shift); m < g.M; m += (int64_t)gridDim.x * each)
-    gated_join_row<T, GRAD>(g, ab, shift, m);
+    gated_join_row<T, GRAD, REST>(g, ab, shift, m);
 }
 
 // ------------------------------------------------------------------- gradients' products
 
 struct ProductArgs {
-  Operand left[2], right[2];  // summed over both pairs where there are two
+  Operand left[4], right[4];  // summed over the pairs
   int32_t pairs;
   // results [r, l]: rows from `split` on are the second output's
   void *out[2];
@@ -783,10 +803,15 @@ int check(const astra_gated_linear *f) {
   ASTRA_ABI_CHECK(f->x_stride, >=, 0);
   ASTRA_ABI_CHECK(f->gate_stride, >=, 0);
   ASTRA_ABI_CHECK(f->up_stride, >=, 0);
-  if (f->activation != ASTRA_SEQ_SILU && f->activation != ASTRA_SEQ_GELU)
+  const int32_t kind = f->activation & ~ASTRA_SEQ_EXACT_GRADIENTS;
+  if (kind != ASTRA_SEQ_SILU && kind != ASTRA_SEQ_GELU)
     return fail(ASTRA_ERR_INVALID_ARGUMENT, "astra_gated_linear: the activation is ASTRA_SEQ_SILU or ASTRA_SEQ_GELU");
   return ASTRA_OK;
 }
+
+// Whether da and db enter their products as two bf16 numbers each, the second of which is what the first lost:
+// 2^-18 of them is left out, and not 2^-9. Twice the products.
+bool exact(const astra_gated_linear &f) { return f.type == ASTRA_SEQ_BF16 && (f.activation & ASTRA_SEQ_EXACT_GRADIENTS); }
 
 int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 int64_t per16(int32_t type) { return 16 / (int64_t)elem_size(type); }
@@ -795,9 +820,10 @@ int64_t pitch_of(int64_t width, int32_t type) { return round_up(width, kStep / (
 int64_t padded_hidden(const astra_gated_linear &f) { return pitch_of(f.hidden, f.type); }
 
 // Whether the backward call gets a and b, 16 bytes an element written and read, or computes them
-// again, 4 D operations. Again / kept, us, a training pass of 8,192 rows to four times the width: bf16 of 256
-// 112 / 115, of 512 228 / 250, of 1,024 622 / 607, of 2,048 2,060 / 1,827; float of 64 101 / 97, of 128
-// 138 / 130, of 256 355 / 318.
+// again, 4 D operations (and always if the caller has no projections). Again / kept, us, a training pass of 8,192
+// rows to four times the width: bf16 of 256 112 / 115, of 512 228 / 250, of 1,024 565 / 564, of 1,280 901 / 861, of
+// 1,536 1,271 / 1,153, of 2,048 1,920 / 1,694; 1,000 rows of 1,024 124 / 118, of 1,280 207 / 187; float of 64
+// 104 / 104, of 128 139 / 130, of 256 333 / 281.
 bool keeps(const astra_gated_linear &f) { return f.width >= (f.type == ASTRA_SEQ_BF16 ? 1024 : 128); }
 
 float *kept(const astra_gated_linear &f) { return keeps(f) ? f.projections : nullptr; }
@@ -862,7 +888,7 @@ GatedArgs args_of(const astra_gated_linear &f) {
   g.M = f.rows;
   g.F = f.hidden;
   g.Fp = padded_hidden(f);
-  g.kind = f.activation;
+  g.kind = f.activation & ~ASTRA_SEQ_EXACT_GRADIENTS;
   return g;
 }
 
@@ -935,7 +961,14 @@ template <class T, bool GRAD>
 int launch_join(GatedArgs g, const float *ab, hipStream_t st) {
   int shift = 4;
   while (shift < 8 && (int64_t(8) << shift) < g.F) ++shift;
-  GATED_LAUNCH((gated_join_kernel<T, GRAD>), std::min(cdiv(g.M, 256 >> shift), kMostLoopBlocks), 256, g, ab, shift);
+  const int64_t blocks = std::min(cdiv(g.M, 256 >> shift), kMostLoopBlocks);
+  if constexpr (GRAD && sizeof(T) == 2) {
+    if (g.rest) {
+      GATED_LAUNCH((gated_join_kernel<T, GRAD, true>), blocks, 256, g, ab, shift);
+      return ASTRA_OK;
+    }
+  }
+  GATED_LAUNCH((gated_join_kernel<T, GRAD, false>), blocks, 256, g, ab, shift);
   return ASTRA_OK;
 }
 
@@ -1070,8 +1103,12 @@ size_t part_bytes(const astra_gated_linear &f) {
 }
 
 template <class T>
+size_t dab_bytes(const astra_gated_linear &f) {
+  return (size_t)(f.rows * 2 * padded_hidden(f)) * sizeof(T);
+}
+template <class T>
 size_t grad_bytes(const astra_gated_linear &f) {
-  return (size_t)(f.rows * 2 * padded_hidden(f)) * sizeof(T) + copies_bytes(f) + turned_bytes(f) + part_bytes<T>(f);
+  return (exact(f) ? 2 : 1) * dab_bytes<T>(f) + copies_bytes(f) + turned_bytes(f) + part_bytes<T>(f);
 }
 
 template <class T>
@@ -1086,7 +1123,13 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
   const int64_t Fp = g.Fp, Dp = round_up(f.width, per16(f.type));
   g.dab = ws;
   g.dh = b.dh;
-  ws += (size_t)(f.rows * 2 * Fp) * sizeof(T);
+  ws += dab_bytes<T>(f);
+  if (exact(f)) {
+    g.rest = ws;
+    ws += dab_bytes<T>(f);
+  }
+  const T *const parts[2] = {(const T *)g.dab, (const T *)g.rest};  // of da and db
+  const int each = exact(f) ? 2 : 1;
   Operands o;
   if (int rc = operands<T>(f, &ws, &o, st)) return rc;
   g.x = o.x;
@@ -1108,19 +1151,21 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
         const dim3 grid((unsigned)cdiv(Fp, kTurn), (unsigned)cdiv(f.width, kTurn), 2);
         hipLaunchKernelGGL(turn_kernel, grid, dim3(256), 0, st, o.gate, o.up, (T *)turn, (int64_t)f.width, (int64_t)f.hidden, Fp);
         ASTRA_HIP_CHECK(rt_last_error(), "turn_kernel launch");
-        p.pairs = 1;
-        p.left[0] = {turn, 2 * Fp, f.width, 2 * Fp};
-        p.right[0] = {g.dab, 2 * Fp, f.rows, 2 * Fp};
+        p.pairs = each;
+        for (int i = 0; i < each; ++i) {
+          p.left[i] = {turn, 2 * Fp, f.width, 2 * Fp};
+          p.right[i] = {parts[i], 2 * Fp, f.rows, 2 * Fp};
+        }
         typedef Large<T, false, false, false> L;
         typedef Small<T, false, false, false> S;
         if (int rc = larger<L, S>(p.nl, p.nr, 2 * Fp) ? launch_product<L>(p, part, st) : launch_product<S>(p, part, st)) return rc;
       }
     } else {
-      p.pairs = 2;
-      for (int i = 0; i < 2; ++i) {
-        const Operand &w = i ? o.up : o.gate;
+      p.pairs = 2 * each;
+      for (int i = 0; i < p.pairs; ++i) {
+        const Operand &w = i % 2 ? o.up : o.gate;
         p.left[i] = {w.p, w.ld, Dp, f.hidden};  // lines: columns of the weight
-        p.right[i] = {(const T *)g.dab + i * Fp, 2 * Fp, f.rows, Fp};
+        p.right[i] = {parts[i / 2] + i % 2 * Fp, 2 * Fp, f.rows, Fp};
       }
       if (int rc = launch_product<Small<T, true, false, false>>(p, part, st)) return rc;
     }
@@ -1128,11 +1173,13 @@ int backward(const astra_gated_linear_grad &b, hipStream_t st) {
   if (b.dgate || b.dup) {
     const Slices s = slices_of<T>(f);
     ProductArgs p{};
-    p.pairs = 1;
+    p.pairs = each;
     // (one weight's gradient alone is the product with its half of the columns)
     p.nr = b.dgate && b.dup ? 2 * Fp : Fp;
-    p.left[0] = {o.x.p, o.x.ld, Dp, f.rows};
-    p.right[0] = {(const T *)g.dab + (b.dgate ? 0 : Fp), 2 * Fp, p.nr, f.rows};
+    for (int i = 0; i < each; ++i) {
+      p.left[i] = {o.x.p, o.x.ld, Dp, f.rows};
+      p.right[i] = {parts[i] + (b.dgate ? 0 : Fp), 2 * Fp, p.nr, f.rows};
+    }
     p.out[0] = b.dgate ? b.dgate : b.dup;
     p.out[1] = b.dup;
     p.out_ld = p.nl = f.width;

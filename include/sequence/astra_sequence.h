@@ -36,6 +36,7 @@ extern "C" {
 #define ASTRA_SEQ_LINEAR 0 /* short_conv's activation: none */
 #define ASTRA_SEQ_SILU 1
 #define ASTRA_SEQ_GELU 2 /* gated_linear: v times the normal distribution function at v */
+#define ASTRA_SEQ_EXACT_GRADIENTS 256 /* gated_linear, or'ed with the activation */
 
 #define ASTRA_SEQ_MAX_TAPS 4
 #define ASTRA_SEQ_MAX_STATE 128
@@ -199,7 +200,9 @@ int astra_gated_linear_workspace_size(const astra_gated_linear *f, size_t *bytes
 int astra_gated_linear_forward(const astra_gated_linear *f, void *stream);
 
 /* Backward: `f` as in the forward call, with the projections that it wrote or without (h and
- * f's workspace are not used). dh [M,F] contiguous; dx [M,D], dgate and dup [F,D], contiguous,
+ * f's workspace are not used). bf16 products take the gradients of the projections rounded to bf16;
+ * with ASTRA_SEQ_EXACT_GRADIENTS as two bf16 numbers each, which is as exact as 32 bits within the
+ * results' rounding, and twice the products. dh [M,F] contiguous; dx [M,D], dgate and dup [F,D], contiguous,
  * of `type`: each may be NULL if not wanted. The workspace starts on 16 bytes. */
 typedef struct astra_gated_linear_grad {
   astra_gated_linear f;
