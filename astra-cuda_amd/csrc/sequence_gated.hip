@@ -7,7 +7,7 @@
 // All are matrix products out[r, l] = sum_k left[l, k] right[r, k] on the matrix cores, with
 // what surrounds them done on the accumulators: 4 M D F operations forwards, 8 M D F backwards, and 4 M D F
 // again where a and b are computed a second time. Sums are float32; h is rounded once, da and db are
-// rounded to x's type before their products, as the matrix cores take them (2^-9 of bf16 each, which
+// rounded to x's type before their products, as the matrix cores take them (2^-8 of bf16 each, which
 // makes the gradients' error 1.4 times that of h), or to two bf16 numbers each where the caller asks
 // for exact gradients: 8 M D F operations more, whole passes of 81,920 rows of 256 to 1,024 850 us and
 // not 580, of 16,384 rows of 4,096 to 8,192 9,800 and not 6,030.
@@ -810,7 +810,7 @@ int check(const astra_gated_linear *f) {
 }
 
 // Whether da and db enter their products as two bf16 numbers each, the second of which is what the first lost:
-// 2^-18 of them is left out, and not 2^-9. Twice the products.
+// 2^-17 of them at most is left out, and not 2^-8. Twice the products.
 bool exact(const astra_gated_linear &f) { return f.type == ASTRA_SEQ_BF16 && (f.activation & ASTRA_SEQ_EXACT_GRADIENTS); }
 
 int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }

@@ -69,8 +69,8 @@ def test_recomputed_projections_in_a_graph():
 
 
 def exact_gradients(x, wg, wu, dh, kind):
-    """{name: (value, bound)} of the gradients in 64 bits, where da and db enter their products to 2^-17 (two
-    roundings to 2^-9 of what there is, and one step more) and not to 2^-8."""
+    """{name: (value, bound)} of the gradients in 64 bits, where da and db enter their products to 2^-17 and not
+    to 2^-8: of v in [1, 2) the first number loses at most 2^-8, half a step of which is at most 2^-17."""
     u, rest = half_step(x.dtype), 2.0 ** -17
     x, wg, wu, dh = (v.detach().double() for v in (x, wg, wu, dh))
     (M, D), F = x.shape, wg.shape[0]
@@ -109,7 +109,7 @@ def test_exact_gradients(M, D, F, kind):
         within(got[name], want[name], name)
         if got[name].numel() > 1000:
             # In the mean, of independent roundings: that of the result, and da's and db's 2^-17 (and float32
-            # sums of up to 2 M terms, which are some 2^-20 here) instead of 2^-9 from each.
+            # sums of up to 2 M terms, which are some 2^-20 here) instead of 2^-8 from each.
             off, least = ((v.double() - want[name][0]).norm() / want[name][0].norm()
                           for v in (got[name], want[name][0].to(BF16)))
             assert float(off) <= 1.02 * float(least), (name, float(off), float(least))

@@ -70,3 +70,23 @@ def test_scans_of_more_than_2_to_the_32_threads(type, batch):
     o = _native.StateScanOne(**p, h=4096, y=4096, **size)
     assert lib.astra_state_scan_step(ctypes.addressof(o), None) == 1
     assert "blocks" in _native.last_error()
+
+
+@pytest.mark.parametrize("activation", [256, 259, 1 | 128, 1 | 256 | 512, 2 | 1 << 30, -1])
+def test_gated_linear_flags(activation):
+    """Exact gradients go with an activation, and nothing else does."""
+    from astra_cuda import _native
+    lib, n = _lib(), ctypes.c_size_t(0)
+    f = _gated(activation=activation)
+    assert lib.astra_gated_linear_grad_workspace_size(ctypes.addressof(f), ctypes.byref(n)) == 1
+    assert "activation" in _native.last_error()
+    for kind in (1, 2):
+        assert lib.astra_gated_linear_grad_workspace_size(ctypes.addressof(_gated(activation=kind | 256)), ctypes.byref(n)) == 0
+    exact, flt = n.value, ctypes.c_size_t(0)
+    assert lib.astra_gated_linear_grad_workspace_size(ctypes.addressof(_gated(activation=1)), ctypes.byref(n)) == 0
+    assert exact == n.value + 500 * 2 * 128 * 2
+    sizes = []
+    for a in (1, 1 | 256):  # float gradients are no different
+        assert lib.astra_gated_linear_grad_workspace_size(ctypes.addressof(_gated(activation=a, type=0)), ctypes.byref(flt)) == 0
+        sizes.append(flt.value)
+    assert sizes[0] == sizes[1]
