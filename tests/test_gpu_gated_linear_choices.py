@@ -186,3 +186,50 @@ def test_exact_gradients_by_the_c_entry():
         within(h, results(x, wg, wu, dh, "silu")["h"], "h")
         for name, d in zip(("dx", "dgate", "dup"), grads):
             within(d, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("choice", [{"recompute": True}, {"exact_gradients": True}, {"recompute": True, "exact_gradients": True}], ids=str)
+def test_choices_with_no_rows_and_other_shapes(choice, dtype):
+    from astra_cuda import sequence as seq
+    x, wg, wu, dh = inputs(7, 0, 1032, 40, dtype)
+    got, _ = call(seq, x, wg, wu, dh, "silu", **choice)
+    assert got["dx"].shape == (0, 1032) and not got["dgate"].any() and not got["dup"].any()
+    x, wg, wu, dh = inputs(9, 96, 136, 72, dtype)
+    want, _ = call(seq, x, wg, wu, dh, "gelu", **choice)
+    # rows beside others, and with leading dimensions
+    wide = torch.full((96, 150), math.nan, device=DEV, dtype=dtype)
+    wide[:, 9:145] = x
+    got, _ = call(seq, wide[:, 9:145], wg, wu, dh, "gelu", **choice)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    got, _ = call(seq, x.view(4, 24, 136), wg, wu, dh.view(4, 24, 72), "gelu", **choice)
+    assert all(torch.equal(got[k].flatten(0, -2), want[k]) for k in want)
+
+
+def test_exact_gradients_in_two_graphs_and_beside_them():
+    """Two graphs of one pass each, replayed in turn on streams of their own while eager passes run."""
+    from astra_cuda import sequence as seq
+    sets = [inputs(50 + i, 8200, 1024, 200, BF16) for i in range(3)]
+    want = [call(seq, *s, "silu", exact_gradients=True)[0] for s in sets]
+    graphs = []
+    for i in range(2):
+        x, wg, wu, dh = (v.clone() for v in sets[i])
+        leaves = [v.requires_grad_() for v in (x, wg, wu)]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            h = seq.gated_linear(*leaves, exact_gradients=True)
+            got = [h, *torch.autograd.grad(h, leaves, dh)]
+        graphs.append((graph, (x, wg, wu, dh), got, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for turn in range(3):
+        for i, (graph, into, got, stream) in enumerate(graphs):
+            with torch.cuda.stream(stream), torch.no_grad():
+                for a, b in zip(into, sets[(turn + i) % 3]):
+                    a.copy_(b)
+                graph.replay()
+        eager = call(seq, *sets[turn], "silu", exact_gradients=True)[0]
+        torch.cuda.synchronize()
+        assert all(torch.equal(eager[k], want[turn][k]) for k in eager)
+        for i, (graph, into, got, stream) in enumerate(graphs):
+            assert all(torch.equal(a.detach(), b) for a, b in zip(got, want[(turn + i) % 3].values())), (turn, i)
