@@ -301,7 +301,10 @@ struct Product {
 };
 
 // Tile `n` of nl x nr, spread so that an XCD (workgroups are given to the eight in turn) works on
-// neighbouring tiles, kBand right tiles by all left ones: what they share stays in its L2. Bands of 2, 4, 8 and
+// neighbouring tiles, kBand right tiles by all left ones: what they share stays in its L2. (Of a product in slices
+// these are the tiles of one slice, all of which read the same part of the contraction. Where a slice has few tiles
+// they are on different XCDs, and each of those reads that part: the weights' gradients of 81,920 rows of 256 to
+// 1,024, 8 tiles a slice, read 671 MB where 378 would do.) Bands of 2, 4, 8 and
 // 12, us: a training pass of 16,384 rows of 4,096 to 8,192 5,940, 5,990, 6,100 and 6,650, of 8,192 of 8,192 5,980,
 // 6,020, 6,360, of 16,384 of 2,048 to 4,096 1,730, 1,670, 1,660.
 constexpr int kXcds = 8, kBand = 4;
