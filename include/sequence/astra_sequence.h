@@ -185,7 +185,7 @@ int astra_join_norm_backward(const astra_join_norm_grad *a, void *stream);
  * x up^T for the backward call, astra_gated_linear_projections() floats: zero, and not used,
  * where the backward call is faster without. The workspace holds copies of operands whose rows
  * overlap or do not start on 16 bytes (many bf16 rows: 128), and partial sums where few rows'
- * contraction is cut; up to 64 rows need none. It starts on 16 bytes. */
+ * contraction is cut; up to 64 rows need none. It starts on 16 bytes. Rows are 2^38 at most. */
 typedef struct astra_gated_linear {
   const void *x, *gate, *up;
   void *h;
@@ -226,7 +226,8 @@ int astra_gated_linear_backward(const astra_gated_linear_grad *a, void *stream);
  * [R,parts,3] (may be NULL) is kept for the backward call.
  * A part that does not count may hold anything: its log_prob and entropy are 0, and there are no
  * likeliest entries. The log probability of an entry that is left out is -inf, that of a choice
- * in no entry NaN; where nothing is allowed the entropy is 0. The workspace starts on 8 bytes. */
+ * in no entry NaN; where nothing is allowed the entropy is 0. The workspace starts on 8 bytes. Rows
+ * are 2^38 at most. */
 typedef struct astra_log_probs {
   const void *logits;
   const uint8_t *mask;
